@@ -412,6 +412,92 @@ int litnice_b200_latent_attention_host(int32_t engine, const float *q, const flo
  * and the device must stay usable. */
 int litnice_b200_selftest_wait_timeout(int32_t limit_us, int32_t *code, int32_t *detail, double *waited_us);
 
+/* ------------------------------------------------------------------------ */
+/* 4. Operators of a training step beside those of the table.                 */
+/*    Attention whose backward pass recomputes the probabilities (the table   */
+/*    keeps them: softmax_backward_causal_rows), a clipped policy loss beside  */
+/*    cross_entropy_mean, orthogonalised momentum beside adamw_step.           */
+/* ------------------------------------------------------------------------ */
+
+/* Tensors are the table's views (device 1, strides in bytes, any order and overlap for inputs) on the
+ * caller's device memory. dtype 0 is f32; these entries also take 2, bfloat16. Outputs may not
+ * overlap each other, themselves or inputs unless an entry says so. Every call only enqueues kernels on `stream` (a
+ * cudaStream_t of the current device, NULL: the default stream) and allocates nothing: it may be
+ * captured into a graph. Where an entry wants a workspace, it is device memory of the size that the
+ * _workspace function gives, on a 256-byte boundary, not shared by calls that may overlap on the GPU;
+ * what it holds before and after does not matter. Return 0 or a negative code, with text in
+ * litnice_b200_last_error(NULL) of the same thread; a refused call has enqueued nothing. No result
+ * depends on the order in which blocks finish. */
+#define LITNICE_B200_VIEW_F32 0u
+#define LITNICE_B200_VIEW_BF16 2u
+
+/* The stream on which a table instance issues its calls, those recorded so far issued: what the entries
+ * of this section then enqueue on it runs behind them and before later table calls. Ask again before
+ * each group of own calls (the table keeps copies of memory that it takes to be unchanged). */
+int litnice_b200_backend_stream(void *backend, void **stream);
+
+/* Row i of a stream has position first + i; it sees key j if j < m, j < lengths[stream], with causal
+ * j <= first + i, with window > 0 j > first + i - window. A row that sees no key has out 0 and lse
+ * -infinity and takes no part in any gradient. Keys and values at and behind lengths[stream] are not
+ * used, whatever they hold, and get gradients of zero. Rows of keys and values below it are taken to
+ * be finite: one that is not may reach rows that do not see it. */
+typedef struct litnice_b200_attention_options {
+  float scale;            /* of the scores, finite */
+  int32_t causal;
+  int32_t first;          /* >= 0 */
+  int32_t window;         /* 0: all */
+  const int32_t *lengths; /* device, [streams] (below 0 counts as 0, above m as m), or NULL: m */
+} litnice_b200_attention_options;
+
+/* q [streams, n, heads, dim], k and v [streams, m, groups, dim], out like q: one dtype, dim 1 .. 128,
+ * heads a multiple of groups (head h uses key head h * groups / heads). lse [streams, heads, n] f32
+ * dense: log of the sum of exp(scores). Scores, weights and sums in 32 bits; bfloat16 operands of
+ * dim % 8 == 0 whose rows lie on 16-byte boundaries run on the tensor cores, weights rounded to
+ * bfloat16 for their product with the values, others with 32-bit products. */
+int litnice_b200_attention_forward(LitniceView q, LitniceView k, LitniceView v,
+                                   const litnice_b200_attention_options *options, LitniceView out, float *lse, void *stream);
+/* Gradients of sum(out * dout) from what the forward call left in out and lse. dout and dq like q, dk and dv like k.
+ * Weights and their gradients are rounded to bfloat16 for their products where the forward call's are. */
+uint64_t litnice_b200_attention_backward_workspace(LitniceView q, LitniceView k);
+int litnice_b200_attention_backward(LitniceView dout, LitniceView q, LitniceView k, LitniceView v, LitniceView out,
+                                    const float *lse, const litnice_b200_attention_options *options, LitniceView dq,
+                                    LitniceView dk, LitniceView dv, void *workspace, uint64_t workspace_bytes, void *stream);
+
+/* logits [rows, vocab] f32 or bfloat16, columns contiguous; targets [rows]. With z = logits / temp,
+ * logp = z[target] - log sum exp z, r = exp(logp - old_logp), d = ref_logp - logp:
+ *   loss = sum_rows weight (-min(r advantage, clip(r, 1 - clip_low, 1 + clip_high) advantage)
+ *                           + kl_weight (exp d - d - 1)) / sum_rows weight
+ * and dlogits its gradient (NULL: not computed; logits itself: in place). weight NULL: all 1; ref_logp may be
+ * NULL if kl_weight is 0. loss: one float, logp [rows]. Rows of weight 0 are not read, their logp and gradient are 0;
+ * weights without a sum give loss 0. A target outside the vocabulary in a row of nonzero weight makes
+ * that row's logp and gradient, and the loss, NaN. */
+typedef struct litnice_b200_policy_options {
+  float temp;                /* > 0 */
+  float clip_low, clip_high; /* >= 0, clip_low <= 1 */
+  float kl_weight;
+} litnice_b200_policy_options;
+uint64_t litnice_b200_policy_loss_workspace(LitniceView logits);
+int litnice_b200_policy_loss(LitniceView logits, const int32_t *targets, const float *old_logp, const float *advantage,
+                             const float *ref_logp, const float *weight, const litnice_b200_policy_options *options,
+                             float *loss, float *logp, LitniceView dlogits, void *workspace, uint64_t workspace_bytes,
+                             void *stream);
+
+/* x, out [..., m, n] f32: every matrix U as X = U / (|U| + 1e-7) (Frobenius) followed by `steps` times
+ * X <- 3.4445 X + (-4.7750 A + 2.0315 A A) X, A = X X^T, in the smaller side's space: its singular
+ * vectors with values near 1. out may be x. */
+uint64_t litnice_b200_orthogonalise_workspace(LitniceView x);
+int litnice_b200_orthogonalise(LitniceView x, LitniceView out, int32_t steps, void *workspace, uint64_t workspace_bytes,
+                               void *stream);
+/* momentum <- mu momentum + grads, U = grads + mu momentum (nesterov) or momentum, X as above,
+ * params <- (1 - lr weight_decay) params - lr sqrt(max(1, m / n)) X; params and momentum like grads, changed in
+ * place. Workspace as for orthogonalise on grads. */
+typedef struct litnice_b200_muon_options {
+  float lr, mu, weight_decay;
+  int32_t nesterov, steps;
+} litnice_b200_muon_options;
+int litnice_b200_muon_step(LitniceView params, LitniceView grads, LitniceView momentum,
+                           const litnice_b200_muon_options *options, void *workspace, uint64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1453,3 +1453,19 @@ const BackendApiV1 kApi = {
 }  // namespace lb
 
 extern "C" const BackendApiV1 *litnice_backend_get_api(void) { return &lb::kApi; }
+
+extern "C" int litnice_b200_backend_stream(void *backend, void **stream) {
+  if (stream == nullptr) return LITNICE_B200_EINVAL;
+  *stream = nullptr;
+  try {
+    lb::Backend *b = lb::self(backend);  // issues what is recorded and drops the read-ahead copy
+    *stream = b->st;
+    return LITNICE_B200_OK;
+  } catch (const std::invalid_argument &e) {
+    lb::set_call_error(e.what());
+    return LITNICE_B200_EINVAL;
+  } catch (const std::exception &e) {
+    lb::set_call_error(e.what());
+    return LITNICE_B200_ECUDA;
+  }
+}

@@ -27,6 +27,9 @@ inline void cuda_check(cudaError_t e, const char *what, const char *file, int li
 #define LB_CUDA(expr) ::lb::cuda_check((expr), #expr, __FILE__, __LINE__)
 #define LB_LAUNCH_CHECK() ::lb::cuda_check(cudaGetLastError(), "kernel launch", __FILE__, __LINE__)
 
+// The text that litnice_b200_last_error(NULL) gives this thread: of calls that have no session (session.cu).
+void set_call_error(const char *text);
+
 // Error word written by kernels into host-mapped memory; the host reads it
 // after the next stream synchronisation. Kernels never trap.
 enum DevErrCode : int {

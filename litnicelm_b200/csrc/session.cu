@@ -2470,3 +2470,5 @@ static int projection_impl(int32_t engine, const float *a, int32_t m, int32_t k,
 }
 
 }  // extern "C"
+
+void lb::set_call_error(const char *text) { g_create_error = text; }

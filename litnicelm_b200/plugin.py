@@ -128,6 +128,9 @@ NATIVE_SYMBOLS = [
     "litnice_b200_gemv_noalloc",
     "litnice_b200_session_create_model", "litnice_b200_architectures", "litnice_b200_model_dims",
     "litnice_b200_extend", "litnice_b200_release",
+    "litnice_b200_backend_stream", "litnice_b200_attention_forward", "litnice_b200_attention_backward_workspace",
+    "litnice_b200_attention_backward", "litnice_b200_policy_loss_workspace", "litnice_b200_policy_loss",
+    "litnice_b200_orthogonalise_workspace", "litnice_b200_orthogonalise", "litnice_b200_muon_step",
 ]
 
 
@@ -306,6 +309,17 @@ class Backend:
         dt = np.float32 if t.dtype == 0 else np.int32
         return np.lib.stride_tricks.as_strided(host[t.ptr - buffer_ptr:].view(dt), shape=t.shape,
                                                strides=t.strides).copy()
+
+    def stream(self) -> int:
+        """The stream (cudaStream_t) of this instance, with the calls recorded so far issued on it: for operators of
+        ``litnicelm_b200.training`` between table calls. Ask again before each group of them."""
+        fn = self.lib.litnice_b200_backend_stream
+        fn.argtypes = [C.c_void_p, C.POINTER(C.c_void_p)]
+        st = C.c_void_p()
+        rc = fn(self.h, C.byref(st))
+        if rc != 0:
+            raise RuntimeError(f"litnice_b200_backend_stream failed with status {rc}")
+        return st.value or 0
 
     def call(self, name: str, *args):
         """Invoke a table entry; DevTensor arguments become view pointers."""

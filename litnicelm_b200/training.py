@@ -1,0 +1,233 @@
+"""Operators of a training step on torch tensors, beside those of the plugin table (section 4 of
+include/litnice_backend_b200.h; the kernels are in csrc/train_attention*.cu, csrc/policy_loss.cu and csrc/orthogonal*.cu).
+
+* ``attention_forward`` / ``attention_backward``: attention that keeps one number per row and computes the probabilities
+  again in its backward pass, instead of the table's softmax over kept scores.
+* ``policy_loss``: clipped policy loss with a KL term and the gradient of the logits, beside ``cross_entropy_mean``.
+* ``orthogonalise`` / ``muon_step``: orthogonalised momentum, beside ``adamw_step``.
+
+Tensors are CUDA tensors of one device; views of any strides are taken as they are. Work is enqueued on torch's current
+stream of that device, nothing is synchronised, and calls may be captured into a CUDA graph. Workspaces come from torch's allocator
+for the call. Tensors that another stream uses need its ordering, as everywhere in torch.
+
+The gradients are explicit, as in the table: nothing here joins torch's autograd, and tensors that would need it are refused
+while it records. There is no fallback: without the library or without a GPU every call raises.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+import struct
+from typing import Optional, Tuple
+
+import torch
+
+from .plugin import NativeError, load_library
+
+_VIEW = struct.Struct("<IIQI4x4q12q")  # BackendTensorView
+_KINDS = {torch.float32: 0, torch.int32: 1, torch.bfloat16: 2}
+
+
+class AttentionOptions(C.Structure):
+    _fields_ = [("scale", C.c_float), ("causal", C.c_int32), ("first", C.c_int32), ("window", C.c_int32),
+                ("lengths", C.c_void_p)]
+
+
+class PolicyOptions(C.Structure):
+    _fields_ = [("temp", C.c_float), ("clip_low", C.c_float), ("clip_high", C.c_float), ("kl_weight", C.c_float)]
+
+
+class MuonOptions(C.Structure):
+    _fields_ = [("lr", C.c_float), ("mu", C.c_float), ("weight_decay", C.c_float), ("nesterov", C.c_int32),
+                ("steps", C.c_int32)]
+
+
+_lib = None
+
+
+def _library():
+    global _lib
+    if _lib is None:
+        lib = load_library()
+        P, U = C.c_void_p, C.c_uint64
+        for name, args in (("attention_forward", [P] * 7), ("attention_backward", [P] * 11 + [U, P]),
+                           ("policy_loss", [P] * 11 + [U, P]), ("orthogonalise", [P, P, C.c_int32, P, U, P]),
+                           ("muon_step", [P] * 5 + [U, P])):
+            fn = getattr(lib, "litnice_b200_" + name)
+            fn.argtypes, fn.restype = args, C.c_int
+        for name, args in (("attention_backward", [P, P]), ("policy_loss", [P]), ("orthogonalise", [P])):
+            fn = getattr(lib, f"litnice_b200_{name}_workspace")
+            fn.argtypes, fn.restype = args, U
+        lib.litnice_b200_last_error.argtypes, lib.litnice_b200_last_error.restype = [P], C.c_char_p
+        _lib = lib
+    return _lib
+
+
+class _Call:
+    """Views of a call's tensors, checked to be CUDA tensors of one device that autograd does not record."""
+
+    def __init__(self, **tensors):
+        self.lib = _library()
+        recording = torch.is_grad_enabled()
+        device, at, raw = None, 0, bytearray(_VIEW.size * len(tensors))
+        self.offset = {}
+        for name, t in tensors.items():
+            if not isinstance(t, torch.Tensor):
+                raise TypeError(f"{name} is not a tensor")
+            if device is None:
+                device = t.device
+                if device.type != "cuda":
+                    raise ValueError(f"{name} is not a CUDA tensor")
+            elif t.device != device:
+                raise ValueError(f"{name} is on {t.device}, not on {device}")
+            if recording and t.requires_grad:
+                raise ValueError(f"{name} requires a gradient: the operators here have explicit backward calls "
+                                 "(use torch.no_grad() or detach())")
+            kind = _KINDS.get(t.dtype)
+            if kind is None:
+                raise TypeError(f"{name} has type {t.dtype}")
+            shape, rank, size = t.shape, t.dim(), t.element_size()
+            if rank > 6:
+                raise ValueError(f"{name} has {rank} axes")
+            strides = t.stride()
+            more = (0,) * (6 - rank)
+            _VIEW.pack_into(raw, at, 1, kind, t.data_ptr(), rank, shape[0] if rank else 0, shape[1] if rank > 1 else 0,
+                            strides[-2] * size if rank > 1 else 0, strides[-1] * size if rank else 0,
+                            *shape, *more, *[x * size for x in strides], *more)
+            self.offset[name] = at
+            at += _VIEW.size
+        self.device = device
+        self.raw = (C.c_char * len(raw)).from_buffer(raw)
+        self.base = C.addressof(self.raw)
+
+    def __getitem__(self, name):
+        return self.base + self.offset[name]
+
+    def workspace(self, nbytes: int) -> torch.Tensor:
+        if nbytes == 0:
+            raise self.error(-1)
+        return torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+
+    def error(self, rc: int) -> Exception:
+        text = self.lib.litnice_b200_last_error(None).decode()
+        return ValueError(text) if rc == -1 else NativeError(f"{text} ({rc})")
+
+    def __call__(self, fn, *args):
+        """The entry point on the current stream of the tensors' device."""
+        index = self.device.index
+        if index == torch.cuda.current_device():
+            rc = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+        else:
+            with torch.cuda.device(index):
+                rc = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+        if rc != 0:
+            raise self.error(rc)
+
+
+def _vector(t: Optional[torch.Tensor], name: str, count: int, dtype, device) -> Optional[int]:
+    """Address of a dense vector of `count` elements."""
+    if t is None:
+        return None
+    if t.dtype != dtype or t.shape != (count,) or (count > 1 and t.stride(0) != 1):
+        raise ValueError(f"{name} must be a dense {dtype} vector of {count} elements")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, not on {device}")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient: the operators here have explicit backward calls "
+                         "(use torch.no_grad() or detach())")
+    return t.data_ptr()
+
+
+def _options(call: _Call, q: torch.Tensor, scale, causal, first, window, lengths) -> AttentionOptions:
+    if q.dim() != 4:
+        raise ValueError("q must be [streams, rows, heads, dim]")
+    if not (0 <= first < 1 << 30 and 0 <= window < 1 << 30):
+        raise ValueError("first and window must be at least 0")
+    return AttentionOptions(1 / math.sqrt(max(1, q.shape[3])) if scale is None else scale, 1 if causal else 0, first, window,
+                            _vector(lengths, "lengths", q.shape[0], torch.int32, call.device))
+
+
+def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: Optional[float] = None, causal: bool = True,
+                      first: int = 0, window: int = 0, lengths: Optional[torch.Tensor] = None,
+                      out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(out [streams, n, heads, dim], lse [streams, heads, n]) of q [streams, n, heads, dim] over k and v [streams, m, groups, dim],
+    float32 or bfloat16, dim up to 128; query head h uses key head h * groups // heads.
+
+    Row i stands at position first + i and sees key j if j < m, j < lengths[stream], with ``causal`` j <= first + i, with a
+    ``window`` j > first + i - window. A row that sees no key has out 0 and lse -inf. scale: 1 / sqrt(dim) if None."""
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
+    call = _Call(q=q, k=k, v=v, out=out)
+    o = _options(call, q, scale, causal, first, window, lengths)
+    lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=q.device)
+    call(call.lib.litnice_b200_attention_forward, call["q"], call["k"], call["v"], C.addressof(o), call["out"], lse.data_ptr())
+    return out, lse
+
+
+def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
+                       lse: torch.Tensor, *, scale: Optional[float] = None, causal: bool = True, first: int = 0, window: int = 0,
+                       lengths: Optional[torch.Tensor] = None, dq: Optional[torch.Tensor] = None,
+                       dk: Optional[torch.Tensor] = None,
+                       dv: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(dq, dk, dv): gradients of sum(out * dout), from what ``attention_forward`` with the same options returned. Key heads
+    shared by query heads receive the sum over those. dq, dk and dv may be given, slices of one buffer for instance."""
+    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device) if dq is None else dq
+    dk = torch.empty(k.shape, dtype=k.dtype, device=k.device) if dk is None else dk
+    dv = torch.empty(v.shape, dtype=v.dtype, device=v.device) if dv is None else dv
+    call = _Call(dout=dout, q=q, k=k, v=v, out=out, dq=dq, dk=dk, dv=dv)
+    o = _options(call, q, scale, causal, first, window, lengths)
+    if lse.dtype != torch.float32 or lse.shape != (q.shape[0], q.shape[2], q.shape[1]) or not lse.is_contiguous() or \
+            lse.device != call.device:
+        raise ValueError("lse must be what attention_forward returned")
+    work = call.workspace(call.lib.litnice_b200_attention_backward_workspace(call["q"], call["k"]))
+    call(call.lib.litnice_b200_attention_backward, call["dout"], call["q"], call["k"], call["v"], call["out"], lse.data_ptr(),
+         C.addressof(o), call["dq"], call["dk"], call["dv"], work.data_ptr(), work.numel())
+    return dq, dk, dv
+
+
+def policy_loss(logits: torch.Tensor, targets: torch.Tensor, old_logp: torch.Tensor, advantage: torch.Tensor, *,
+                ref_logp: Optional[torch.Tensor] = None, weight: Optional[torch.Tensor] = None, temp: float = 1.0,
+                clip_low: float = 0.2, clip_high: float = 0.2, kl_weight: float = 0.0, gradient: bool = True,
+                dlogits: Optional[torch.Tensor] = None
+                ) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
+    """(loss, logp [rows], dlogits) of logits [rows, vocab], float32 or bfloat16 with contiguous columns.
+
+    With z = logits / temp, logp = log_softmax(z)[target], r = exp(logp - old_logp), d = ref_logp - logp:
+    loss = sum weight (-min(r advantage, clip(r, 1 - clip_low, 1 + clip_high) advantage) + kl_weight (exp d - d - 1)) / sum weight.
+    Rows of weight 0 are not read; their logp and gradient are 0. A target outside the vocabulary in another row gives NaN there
+    and in the loss. dlogits may be given, logits itself included; with ``gradient`` false it is None."""
+    if gradient and dlogits is None:
+        dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    call = _Call(logits=logits, dlogits=dlogits) if gradient else _Call(logits=logits)
+    if logits.dim() != 2:
+        raise ValueError("logits must be [rows, vocab]")
+    rows, dev = logits.shape[0], call.device
+    o = PolicyOptions(temp, clip_low, clip_high, kl_weight)
+    results = torch.empty(rows + 1, dtype=torch.float32, device=dev)
+    work = call.workspace(call.lib.litnice_b200_policy_loss_workspace(call["logits"]))
+    call(call.lib.litnice_b200_policy_loss, call["logits"], _vector(targets, "targets", rows, torch.int32, dev),
+         _vector(old_logp, "old_logp", rows, torch.float32, dev), _vector(advantage, "advantage", rows, torch.float32, dev),
+         _vector(ref_logp, "ref_logp", rows, torch.float32, dev), _vector(weight, "weight", rows, torch.float32, dev),
+         C.addressof(o), results.data_ptr() + 4 * rows, results.data_ptr(), call["dlogits"] if gradient else None,
+         work.data_ptr(), work.numel())
+    return results[rows], results[:rows], dlogits if gradient else None
+
+
+def orthogonalise(x: torch.Tensor, *, steps: int = 5, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Every matrix of x [..., m, n] float32 with its singular values driven towards 1: X = x / (|x| + 1e-7), then ``steps`` times
+    X <- 3.4445 X + (-4.7750 A + 2.0315 A A) X with A = X X^T (in the smaller side's space). out may be x."""
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
+    call = _Call(x=x, out=out)
+    work = call.workspace(call.lib.litnice_b200_orthogonalise_workspace(call["x"]))
+    call(call.lib.litnice_b200_orthogonalise, call["x"], call["out"], steps, work.data_ptr(), work.numel())
+    return out
+
+
+def muon_step(params: torch.Tensor, grads: torch.Tensor, momentum: torch.Tensor, lr: float, *, mu: float = 0.95,
+              weight_decay: float = 0.0, nesterov: bool = True, steps: int = 5) -> None:
+    """One optimiser step on matrices [..., m, n] float32, in place: momentum <- mu momentum + grads, U = grads + mu momentum (or
+    momentum without ``nesterov``), params <- (1 - lr weight_decay) params - lr sqrt(max(1, m / n)) orthogonalise(U)."""
+    call = _Call(params=params, grads=grads, momentum=momentum)
+    o = MuonOptions(lr, mu, weight_decay, 1 if nesterov else 0, steps)
+    work = call.workspace(call.lib.litnice_b200_orthogonalise_workspace(call["grads"]))
+    call(call.lib.litnice_b200_muon_step, call["params"], call["grads"], call["momentum"], C.addressof(o), work.data_ptr(),
+         work.numel())
