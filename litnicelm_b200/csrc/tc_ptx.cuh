@@ -95,6 +95,12 @@ __device__ __forceinline__ void tma_load_2d(unsigned dst, const CUtensorMap *map
       ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar)
       : "memory");
 }
+__device__ __forceinline__ void tma_load_4d(unsigned dst, const CUtensorMap *map, int x, int y, int z, int w, unsigned bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+      ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+      : "memory");
+}
 // Brings a tensor map into the descriptor cache ahead of its first use (the maps of operands
 // an earlier kernel writes are first used right after the wait for that kernel).
 __device__ __forceinline__ void tma_prefetch_map(const CUtensorMap *map) {

@@ -433,6 +433,7 @@ void backward(const TrainAttention &a, float *delta, cudaStream_t st) {
 }  // namespace
 
 void launch_train_attention_forward(const TrainAttention &a, cudaStream_t st) {
+  if (train_attention_tc_supports(a, false)) return launch_train_attention_forward_tc(a, st);
   const TaArgs g = ta_args(a, nullptr, a.n);
   if (a.bf16) {
     if (a.dim <= 32) forward<32, bf16>(g, st);
@@ -456,6 +457,7 @@ void launch_train_delta(const TrainAttention &a, float *delta, cudaStream_t st) 
 
 void launch_train_attention_backward(const TrainAttention &a, float *delta, cudaStream_t st) {
   launch_train_delta(a, delta, st);
+  if (train_attention_tc_supports(a, true)) return launch_train_attention_backward_tc(a, delta, st);
   if (a.bf16) {
     if (a.dim <= 32) backward<32, bf16>(a, delta, st);
     else if (a.dim <= 64) backward<64, bf16>(a, delta, st);

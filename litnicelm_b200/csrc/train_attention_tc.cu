@@ -1,0 +1,900 @@
+// Attention with its backward pass for training on the sm_100a tensor cores (tcgen05 + TMEM + TMA): bfloat16 operands, 32-bit
+// scores, weights' sums, statistics and accumulators. The mathematics is that of train_attention.cu.
+//
+// forward   one CTA per 128 rows of a head walks the tiles of 128 keys they see: S = Q K^T, four warps (a thread: a row) turn S
+//           into weights 2^(s - m), stored as bfloat16 over the scores' own columns of tensor memory, O += P V from there. The
+//           reference m follows a row's maximum only where that has grown by more than 2^8, so most tiles need no pass over O.
+//           Two CTAs share an SM: one's products run under the other's softmax.
+// dk, dv    one CTA per 128 keys of a key head walks the tiles of 128 rows that see them, through all query heads that share it:
+//           S^T = K Q^T, dP^T = V dO^T; eight warps (a thread: a key and half of the rows) make P^T and then dS^T = P^T (dP^T -
+//           delta), each over its source's columns; dV += P^T dO and dK += dS^T Q with A from tensor memory and B as it lies in
+//           shared memory, rows of k. While the warps work on P the pipe multiplies for dS of the tile before, and the
+//           other way round: dV(i), S(i+1) | dK(i), dP(i+1).
+// dq        one CTA per 128 rows of a head in the same way: S = Q K^T, dP = dO V^T, dQ += dS K.
+// The scores are computed once for each, so that no sum depends on the order in which CTAs finish.
+//
+// Rounding to bfloat16: P and dS for their products (the tensor cores take both operands of one type), relative 2^-8 a term,
+// of independent sign, as much as the operands themselves have been rounded by; the results.
+//
+// Warp 0 issues TMA, warp 1 owns tensor memory and issues the MMAs. Rows outside the tensors load as zeros; keys behind a
+// stream's length are cleared in shared memory where a product would multiply them by a weight of zero. Every wait is bounded;
+// one that runs out ends the CTA, whose results are then NaN. No clusters, no multicast.
+#include "train_ops.cuh"
+#include "gemm_tc.cuh"
+#include "tc_ptx.cuh"
+
+#include <cuda_bf16.h>
+
+namespace lb {
+
+namespace {
+
+typedef __nv_bfloat16 bf16;
+
+constexpr int TT_B = 128;
+constexpr int TT_SLAB = 128 * 128;  // 128 rows of 64 elements
+constexpr float TT_NEG = -1.0e30f, TT_SLACK = 8.f, TT_LOG2E = 1.4426950408889634f;
+constexpr int TT_FWD_THREADS = 192, TT_BWD_THREADS = 320;
+
+__device__ __forceinline__ float tt_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ unsigned tt_pack(float a, float b) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const unsigned *>(&v);
+}
+
+struct TtArgs {
+  int n, m, heads, groups, share, streams, dim, tiles;
+  TrainSpan span;
+  const int *lengths;
+  float scale, factor;   // factor = scale * log2(e)
+  float *lse;
+  float *delta;
+  HeadView o1, o2;       // out | dq | dk, dv
+  int vec;               // results' rows on 16-byte boundaries
+};
+
+struct TtPlace {
+  int tile, head, stream, keys;
+};
+__device__ __forceinline__ TtPlace tt_place(const TtArgs &a, int heads, bool last_first) {
+  const int each = heads * a.streams, b = (int)blockIdx.x;
+  const int t = b / each, rest = b - t * each;
+  TtPlace p;
+  p.tile = last_first ? a.tiles - 1 - t : t;
+  p.stream = rest / heads;
+  p.head = rest - p.stream * heads;
+  p.keys = a.lengths ? max(0, min(a.m, a.lengths[p.stream])) : a.m;
+  return p;
+}
+
+__device__ __forceinline__ void tt_alloc(volatile unsigned *holder, unsigned cols) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void *)holder)), "r"(cols)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+
+// One row's columns c0 .. c0 + 15 of a result, as bfloat16.
+__device__ __forceinline__ void tt_store16(bf16 *row, const TtArgs &a, int c0, const float (&x)[16]) {
+  if (a.vec && c0 + 16 <= a.dim) {
+    unsigned w[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = tt_pack(x[2 * j], x[2 * j + 1]);
+    *reinterpret_cast<uint4 *>(row + c0) = make_uint4(w[0], w[1], w[2], w[3]);
+    *reinterpret_cast<uint4 *>(row + c0 + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (c0 + j < a.dim) row[c0 + j] = __float2bfloat16_rn(x[j]);
+  }
+}
+
+// Accumulator columns [c0, c1) of this thread's lane times `factor` into its row of a result; NaN where the CTA gave up.
+__device__ __forceinline__ void tt_store_row(bf16 *row, bool live, const TtArgs &a, unsigned tmem, int c0, int c1, float factor,
+                                             bool zero, bool ok) {
+#pragma unroll 1
+  for (int c = c0; c < c1; c += 16) {
+    float x[16];
+    if (ok && !zero) {
+      unsigned r[16];
+      tc_ld16(tmem + (unsigned)c, r);
+      asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+      for (int j = 0; j < 16; ++j) x[j] = __uint_as_float(r[j]) * factor;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) x[j] = ok ? 0.f : NAN;
+    }
+    if (live) tt_store16(row, a, c, x);
+  }
+}
+
+// Rows `from` .. 127 of a tile of slabs, as zeros (by one warp; the tensor cores read them next).
+__device__ __forceinline__ void tt_clear_rows(unsigned char *tile, int slabs, int from, int lane) {
+  for (int s = 0; s < slabs; ++s)
+    for (int e = from * 8 + lane; e < 128 * 8; e += 32)
+      *reinterpret_cast<uint4 *>(tile + s * TT_SLAB + e * 16) = make_uint4(0u, 0u, 0u, 0u);
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncwarp();
+}
+
+// S (128 x 128) = rows of a . rows of b over dim, both with contiguous dim
+__device__ __forceinline__ void tt_mma_rows(unsigned d, unsigned a, unsigned b, int ksteps, unsigned idesc) {
+  for (int ks = 0; ks < ksteps; ++ks) {
+    const unsigned slab = (unsigned)((ks >> 2) * TT_SLAB);
+    const unsigned long long in = (unsigned long long)((ks & 3) * 2);
+    tc_mma_f16(d, umma_desc_k128(a + slab) + in, umma_desc_k128(b + slab) + in, idesc, ks ? 1u : 0u);
+  }
+}
+
+template <int D>
+__global__ void __launch_bounds__(TT_FWD_THREADS, 2)
+train_forward_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                        const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TtArgs a) {
+  constexpr int SLABS = D / 64, TILE = SLABS * TT_SLAB;
+  extern __shared__ unsigned char smem_raw[];
+  const unsigned base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  unsigned char *base_ptr = smem_raw + (base - smem_u32(smem_raw));
+  const unsigned q_off = base, k_off = base + TILE, v_off = base + 2 * TILE, bars = base + 3 * TILE;
+  const unsigned q_full = bars, k_full = bars + 8, v_full = bars + 16, k_free = bars + 24, s_full = bars + 32,
+                 p_ready = bars + 40, o_full = bars + 48;
+  volatile unsigned *tmem_holder = reinterpret_cast<volatile unsigned *>(base_ptr + 3 * TILE + 64);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(base_ptr + 3 * TILE + 68);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const TtPlace at = tt_place(a, a.heads, a.span.causal != 0);
+  const int r0 = at.tile * TT_B, r1 = min(r0 + TT_B, a.n), kh = at.head / a.share;
+  const int lo = a.span.lo(r0), end = a.span.end(r1 - 1, at.keys);
+  const int tiles = end > lo ? (end - lo + TT_B - 1) / TT_B : 0;
+
+  if (threadIdx.x == 0) {
+    for (unsigned bar : {q_full, k_full, v_full, k_free, s_full, o_full}) mbar_init(bar, 1);
+    mbar_init(p_ready, 4);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) tt_alloc(tmem_holder, 256u);
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const unsigned tmem_s = *tmem_holder, tmem_o = tmem_s + TT_B;
+
+  if (warp == 0) {
+    int k_loads = 0, v_loads = 0;
+    bool ok = true;
+    if (lane == 0 && tiles > 0) {
+      mbar_expect_tx(q_full, (unsigned)TILE);
+      for (int s = 0; s < SLABS; ++s) tma_load_4d(q_off + s * TT_SLAB, &map_q, s * 64, at.head, r0, at.stream, q_full);
+    }
+    for (int i = 0; i < tiles && ok; ++i) {
+      const int j0 = lo + i * TT_B;
+      if (i > 0) ok = mbar_wait(k_free, (unsigned)(i - 1) & 1u, abort_flag, nullptr, 71);
+      __syncwarp();
+      if (!ok) break;
+      if (lane == 0) {
+        mbar_expect_tx(k_full, (unsigned)TILE);
+        for (int s = 0; s < SLABS; ++s) tma_load_4d(k_off + s * TT_SLAB, &map_k, s * 64, kh, j0, at.stream, k_full);
+      }
+      ++k_loads;
+      if (i > 0) ok = mbar_wait(o_full, (unsigned)(i - 1) & 1u, abort_flag, nullptr, 72);  // P V has read the values
+      __syncwarp();
+      if (!ok) break;
+      if (lane == 0) {
+        mbar_expect_tx(v_full, (unsigned)TILE);
+        for (int s = 0; s < SLABS; ++s) tma_load_4d(v_off + s * TT_SLAB, &map_v, s * 64, kh, j0, at.stream, v_full);
+      }
+      ++v_loads;
+      __syncwarp();
+    }
+    if (*abort_flag && tiles > 0) {  // copies in flight must land before the shared memory goes away
+      const unsigned long long limit = global_timer() + WAIT_LIMIT_NS;
+      while (!mbar_try_wait(q_full, 0) && global_timer() < limit) {}
+      while (k_loads > 0 && !mbar_try_wait(k_full, (unsigned)(k_loads - 1) & 1u) && global_timer() < limit) {}
+      while (v_loads > 0 && !mbar_try_wait(v_full, (unsigned)(v_loads - 1) & 1u) && global_timer() < limit) {}
+    }
+  } else if (warp == 1) {
+    const int cols = (a.dim + 15) & ~15, ksteps = cols >> 4;
+    const unsigned idesc_s = umma_idesc_bf16(TT_B), idesc_o = umma_idesc_bf16(cols) | UMMA_B_MN_MAJOR;
+    bool ok = tiles > 0 ? mbar_wait_warp(q_full, 0, abort_flag, nullptr, 73) : true;
+    int i = 0;
+    for (; i < tiles && ok; ++i) {
+      ok = mbar_wait_warp(k_full, (unsigned)i & 1u, abort_flag, nullptr, 74);
+      if (!ok) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      if (lane == 0) {
+        tt_mma_rows(tmem_s, q_off, k_off, ksteps, idesc_s);
+        tc_commit(k_free);
+        tc_commit(s_full);
+      }
+      __syncwarp();
+      ok = mbar_wait_warp(v_full, (unsigned)i & 1u, abort_flag, nullptr, 75);
+      if (!ok) break;
+      const int have = at.keys - (lo + i * TT_B);
+      if (have < TT_B && at.keys < a.m) tt_clear_rows(base_ptr + 2 * TILE, SLABS, have, lane);
+      ok = mbar_wait_warp(p_ready, (unsigned)i & 1u, abort_flag, nullptr, 76);
+      if (!ok) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      if (lane == 0) {
+#pragma unroll
+        for (int ks = 0; ks < TT_B / 16; ++ks)
+          tc_mma_f16_ts(tmem_o, tmem_s + (unsigned)(ks * 8), umma_desc_mn128(v_off + (unsigned)(ks * 16 * 128), TT_SLAB), idesc_o,
+                        (i | ks) ? 1u : 0u);
+        tc_commit(o_full);
+      }
+      __syncwarp();
+    }
+    if (!ok) {  // a bounded chance for the tensor pipe to finish before tensor memory is freed
+      if (lane == 0) tc_commit(o_full);
+      __syncwarp();
+      const unsigned long long limit = global_timer() + WAIT_LIMIT_NS;
+      while (!mbar_try_wait(o_full, (unsigned)i & 1u) && global_timer() < limit) {}
+    }
+  } else {
+    const int q = warp & 3;
+    const unsigned lanes = (unsigned)(q * 32) << 16;
+    const int row = r0 + q * 32 + lane;
+    const int row_lo = a.span.lo(row), row_end = a.span.end(row, at.keys);
+    const int warp_lo = a.span.lo(r0 + q * 32 + 31), warp_end = a.span.end(r0 + q * 32, at.keys);
+    float m = TT_NEG, l = 0.f;
+    bool ok = true;
+    for (int i = 0; i < tiles && ok; ++i) {
+      const int j0 = lo + i * TT_B;
+      ok = mbar_wait_warp(s_full, (unsigned)i & 1u, abort_flag, nullptr, 77);
+      if (!ok) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const int c_lo = row_lo - j0, c_end = row_end - j0;  // keys j0 + c that this row sees
+      const bool inside = warp_lo <= j0 && warp_end >= j0 + TT_B;
+      float s[TT_B];
+      {
+        unsigned(&u)[4][32] = reinterpret_cast<unsigned(&)[4][32]>(s);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tc_ld32(tmem_s + lanes + (unsigned)(c * 32), u[c]);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+      }
+#pragma unroll
+      for (int j = 0; j < TT_B; ++j) s[j] *= a.factor;
+      if (!inside) {
+#pragma unroll
+        for (int j = 0; j < TT_B; ++j)
+          if (j >= c_end || j < c_lo) s[j] = 2.f * TT_NEG;  // weight zero against any reference
+      }
+      float mq[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+      for (int j = 4; j < TT_B; ++j) mq[j & 3] = fmaxf(mq[j & 3], s[j]);
+      const float mx = fmaxf(TT_NEG, fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3])));
+      const bool grow = mx > m + TT_SLACK;
+      const float keep = grow ? tt_exp2(m - mx) : 1.f;
+      if (grow) m = mx;
+      l *= keep;
+      if (i > 0) {
+        ok = mbar_wait_warp(o_full, (unsigned)(i - 1) & 1u, abort_flag, nullptr, 78);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll 1
+          for (int c0 = 0; c0 < a.dim; c0 += 16) {
+            unsigned r[16];
+            tc_ld16(tmem_o + lanes + (unsigned)c0, r);
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+            for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * keep);
+            tc_st16(tmem_o + lanes + (unsigned)c0, r);
+          }
+        }
+      }
+      float lq[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c0 = 0; c0 < TT_B; c0 += 32) {
+        unsigned pk[16];
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) {
+          const float e0 = tt_exp2(s[c0 + j] - m), e1 = tt_exp2(s[c0 + j + 1] - m);
+          lq[j & 2] += e0;
+          lq[(j & 2) + 1] += e1;
+          pk[j >> 1] = tt_pack(e0, e1);
+        }
+        tc_st16(tmem_s + lanes + (unsigned)(c0 >> 1), pk);  // over the scores, which this warp has read
+      }
+      l += (lq[0] + lq[1]) + (lq[2] + lq[3]);
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_ready);
+    }
+    if (ok && tiles > 0) ok = mbar_wait_warp(o_full, (unsigned)(tiles - 1) & 1u, abort_flag, nullptr, 79);
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const bool live = row < a.n, empty = row_end <= row_lo;
+    bf16 *o = reinterpret_cast<bf16 *>(a.o1.p) + at.stream * a.o1.s + (long long)row * a.o1.r + at.head * a.o1.h;
+    // a warp's rows are read together: a row without keys has factor 0 (its accumulator holds finite weights of nothing)
+    const float inv = empty ? 0.f : 1.0f / l;
+    tt_store_row(o, live, a, tmem_o + lanes, 0, (a.dim + 15) & ~15, inv, tiles == 0, ok);
+    if (live)
+      a.lse[((long long)at.stream * a.heads + at.head) * a.n + row] =
+          !ok ? NAN : empty ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+  }
+  __syncwarp();
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == 1) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_s), "r"(256u));
+  }
+}
+
+// Shared memory of the backward kernels: two resident tiles, two stages of two streamed tiles, statistics of the stages' rows.
+template <int D>
+struct TtBwd {
+  static constexpr int SLABS = D / 64, TILE = SLABS * TT_SLAB;
+  static constexpr int STAGE_OFF = 2 * TILE;
+  static constexpr int STAT_OFF = STAGE_OFF + 4 * TILE;  // [2][2][128] floats
+  static constexpr int BAR_OFF = STAT_OFF + 2 * 2 * 128 * 4;
+  static constexpr int TOTAL = BAR_OFF + 128 + 1024;
+  static_assert(TOTAL <= 227 * 1024, "");
+};
+
+template <int D>
+__global__ void __launch_bounds__(TT_BWD_THREADS, 1)
+train_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                    const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do,
+                    const __grid_constant__ TtArgs a) {
+  using L = TtBwd<D>;
+  constexpr int SLABS = L::SLABS, TILE = L::TILE;
+  extern __shared__ unsigned char smem_raw[];
+  const unsigned base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  unsigned char *base_ptr = smem_raw + (base - smem_u32(smem_raw));
+  const unsigned k_off = base, v_off = base + TILE, bars = base + L::BAR_OFF;
+  auto q_tile = [&](int s) { return base + (unsigned)(L::STAGE_OFF + s * 2 * TILE); };
+  auto do_tile = [&](int s) { return base + (unsigned)(L::STAGE_OFF + (s * 2 + 1) * TILE); };
+  float *stat = reinterpret_cast<float *>(base_ptr + L::STAT_OFF);
+  const unsigned kv_full = bars, s_full = bars + 8, p_ready = bars + 16, dp_full = bars + 24, ds_ready = bars + 32, done = bars + 40;
+  auto q_full = [&](int s) { return bars + 48u + 8u * s; };
+  auto q_empty = [&](int s) { return bars + 64u + 8u * s; };
+  auto stat_full = [&](int s) { return bars + 80u + 8u * s; };
+  volatile unsigned *tmem_holder = reinterpret_cast<volatile unsigned *>(base_ptr + L::BAR_OFF + 96);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(base_ptr + L::BAR_OFF + 100);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const TtPlace at = tt_place(a, a.groups, false);
+  const int j0 = at.tile * TT_B, j1 = min(j0 + TT_B, at.keys);
+  // rows that see a key of this tile: from lo on, to row_end
+  const int lo = a.span.causal ? max(0, j0 - a.span.first) / TT_B * TT_B : 0;
+  const long long past = a.span.window > 0 ? (long long)j1 - 1 + a.span.window - a.span.first : a.n;
+  const int row_end = past < a.n ? (int)max(past, 0LL) : a.n;
+  const int each = j0 < at.keys && row_end > lo ? (row_end - lo + TT_B - 1) / TT_B : 0;  // tiles per query head
+  const int tiles = each * a.share;
+
+  if (threadIdx.x == 0) {
+    for (unsigned bar : {kv_full, s_full, dp_full, done}) mbar_init(bar, 1);
+    mbar_init(p_ready, 8);
+    mbar_init(ds_ready, 8);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(q_full(s), 1);
+      mbar_init(q_empty(s), 1);
+      mbar_init(stat_full(s), 1);
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) tt_alloc(tmem_holder, 512u);
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const unsigned tmem_s = *tmem_holder, tmem_dp = tmem_s + 128, tmem_dv = tmem_s + 256, tmem_dk = tmem_dv + D;
+
+  if (warp == 0) {
+    int it = 0;
+    bool ok = true;
+    if (lane == 0 && tiles > 0) {
+      mbar_expect_tx(kv_full, 2u * TILE);
+      for (int s = 0; s < SLABS; ++s) {
+        tma_load_4d(k_off + s * TT_SLAB, &map_k, s * 64, at.head, j0, at.stream, kv_full);
+        tma_load_4d(v_off + s * TT_SLAB, &map_v, s * 64, at.head, j0, at.stream, kv_full);
+      }
+    }
+    for (int h = at.head * a.share; h < (at.head + 1) * a.share && ok; ++h) {
+      const long long stats = ((long long)at.stream * a.heads + h) * a.n;
+      for (int t = 0; t < each; ++t, ++it) {
+        const int st = it & 1, r0 = lo + t * TT_B;
+        ok = mbar_wait_warp(q_empty(st), ((unsigned)(it >> 1) & 1u) ^ 1u, abort_flag, nullptr, 81);
+        if (!ok) break;
+        if (lane == 0) {
+          mbar_expect_tx(q_full(st), 2u * TILE);
+          for (int s = 0; s < SLABS; ++s) {
+            tma_load_4d(q_tile(st) + s * TT_SLAB, &map_q, s * 64, h, r0, at.stream, q_full(st));
+            tma_load_4d(do_tile(st) + s * TT_SLAB, &map_do, s * 64, h, r0, at.stream, q_full(st));
+          }
+        }
+        // a row that does not exist or sees no key has no weights: 2^(s - infinity)
+#pragma unroll
+        for (int e = lane; e < TT_B; e += 32) {
+          const int row = r0 + e;
+          const float z = row < a.n ? a.lse[stats + row] : -INFINITY;
+          stat[st * 256 + e] = z == -INFINITY ? INFINITY : z * TT_LOG2E;
+          stat[st * 256 + 128 + e] = row < a.n ? a.delta[stats + row] : 0.f;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(stat_full(st));
+        __syncwarp();
+      }
+    }
+    if (*abort_flag && tiles > 0) {  // copies in flight must land before the shared memory goes away
+      const unsigned long long limit = global_timer() + WAIT_LIMIT_NS;
+      while (!mbar_try_wait(kv_full, 0) && global_timer() < limit) {}
+      for (int j = it > 2 ? it - 2 : 0; j < it; ++j)
+        while (!mbar_try_wait(q_full(j & 1), (unsigned)(j >> 1) & 1u) && global_timer() < limit) {}
+    }
+  } else if (warp == 1) {
+    const int cols = (a.dim + 15) & ~15, ksteps = cols >> 4;
+    const unsigned idesc_s = umma_idesc_bf16(TT_B), idesc_d = umma_idesc_bf16(cols) | UMMA_B_MN_MAJOR;
+    bool ok = true;
+    // rows of k of an A operand in tensor memory: each half of the warps has written its 64 over its own 64 columns
+    auto times = [&](unsigned d, unsigned w, unsigned b, bool more) {
+#pragma unroll
+      for (int ks = 0; ks < TT_B / 16; ++ks)
+        tc_mma_f16_ts(d, w + (unsigned)((ks >> 2) * 64 + (ks & 3) * 8), umma_desc_mn128(b + (unsigned)(ks * 16 * 128), TT_SLAB),
+                      idesc_d, more || ks ? 1u : 0u);
+    };
+    if (tiles > 0) {
+      ok = mbar_wait_warp(kv_full, 0, abort_flag, nullptr, 82) && mbar_wait_warp(q_full(0), 0, abort_flag, nullptr, 83);
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      if (ok && lane == 0) {
+        tt_mma_rows(tmem_s, k_off, q_tile(0), ksteps, idesc_s);
+        tc_commit(s_full);
+        tt_mma_rows(tmem_dp, v_off, do_tile(0), ksteps, idesc_s);
+        tc_commit(dp_full);
+      }
+      __syncwarp();
+    }
+    for (int i = 0; i < tiles && ok; ++i) {
+      const int st = i & 1, next = st ^ 1;
+      ok = mbar_wait_warp(p_ready, (unsigned)i & 1u, abort_flag, nullptr, 84);
+      if (!ok) break;
+      if (i + 1 < tiles) ok = mbar_wait_warp(q_full(next), (unsigned)((i + 1) >> 1) & 1u, abort_flag, nullptr, 85);
+      if (!ok) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      if (lane == 0) {
+        times(tmem_dv, tmem_s, do_tile(st), i > 0);
+        if (i + 1 < tiles) {
+          tt_mma_rows(tmem_s, k_off, q_tile(next), ksteps, idesc_s);
+          tc_commit(s_full);
+        }
+      }
+      __syncwarp();
+      ok = mbar_wait_warp(ds_ready, (unsigned)i & 1u, abort_flag, nullptr, 86);
+      if (!ok) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      if (lane == 0) {
+        times(tmem_dk, tmem_dp, q_tile(st), i > 0);
+        tc_commit(q_empty(st));
+        if (i + 1 < tiles) {
+          tt_mma_rows(tmem_dp, v_off, do_tile(next), ksteps, idesc_s);
+          tc_commit(dp_full);
+        }
+      }
+      __syncwarp();
+    }
+    if (tiles > 0 && lane == 0) tc_commit(done);
+    __syncwarp();
+    if (!ok) {  // a bounded chance for the tensor pipe to finish before tensor memory is freed
+      const unsigned long long limit = global_timer() + WAIT_LIMIT_NS;
+      while (!mbar_try_wait(done, 0) && global_timer() < limit) {}
+    }
+  } else {
+    const int q = warp & 3, half = (warp - 2) >> 2;
+    const unsigned lanes = (unsigned)(q * 32) << 16;
+    const int key = j0 + q * 32 + lane;
+    const bool key_live = key < at.keys;
+    bool ok = true;
+    for (int i = 0; i < tiles && ok; ++i) {
+      const int st = i & 1, r0 = lo + i % each * TT_B + half * 64;
+      // rows r0 + c that see this key: [c_lo, c_end)
+      const int c_lo = a.span.causal ? key - a.span.first - r0 : 0;
+      const long long pe = a.span.window > 0 ? (long long)key + a.span.window - a.span.first - r0 : 64;
+      const int c_end = !key_live ? 0 : pe < 64 ? (int)max(pe, 0LL) : 64;
+      const bool inside = __all_sync(0xffffffffu, c_lo <= 0 && c_end >= 64);
+      ok = mbar_wait_warp(stat_full(st), (unsigned)(i >> 1) & 1u, abort_flag, nullptr, 87) &&
+           mbar_wait_warp(s_full, (unsigned)i & 1u, abort_flag, nullptr, 88);
+      if (!ok) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      float p[64];
+      {
+        unsigned(&u)[2][32] = reinterpret_cast<unsigned(&)[2][32]>(p);
+        tc_ld32(tmem_s + lanes + (unsigned)(half * 64), u[0]);
+        tc_ld32(tmem_s + lanes + (unsigned)(half * 64 + 32), u[1]);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+      }
+      const float4 *z = reinterpret_cast<const float4 *>(stat + st * 256 + half * 64);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float4 v = z[j];
+        p[4 * j] = tt_exp2(fmaf(p[4 * j], a.factor, -v.x));
+        p[4 * j + 1] = tt_exp2(fmaf(p[4 * j + 1], a.factor, -v.y));
+        p[4 * j + 2] = tt_exp2(fmaf(p[4 * j + 2], a.factor, -v.z));
+        p[4 * j + 3] = tt_exp2(fmaf(p[4 * j + 3], a.factor, -v.w));
+      }
+      if (!inside) {
+#pragma unroll
+        for (int j = 0; j < 64; ++j)
+          if (j < c_lo || j >= c_end) p[j] = 0.f;
+      }
+#pragma unroll
+      for (int c = 0; c < 64; c += 32) {
+        unsigned w[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) w[j] = tt_pack(p[c + 2 * j], p[c + 2 * j + 1]);
+        tc_st16(tmem_s + lanes + (unsigned)(half * 64 + (c >> 1)), w);
+      }
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_ready);
+      ok = mbar_wait_warp(dp_full, (unsigned)i & 1u, abort_flag, nullptr, 89);
+      if (!ok) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const float4 *de = reinterpret_cast<const float4 *>(stat + st * 256 + 128 + half * 64);
+#pragma unroll
+      for (int c = 0; c < 64; c += 32) {
+        unsigned u[32], w[16];
+        tc_ld32(tmem_dp + lanes + (unsigned)(half * 64 + c), u);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+          const float4 v = de[(c + j) >> 2];
+          // (a weight of zero has no part even where the other factor is not finite)
+          const float x0 = (__uint_as_float(u[j]) - v.x) * p[c + j], x1 = (__uint_as_float(u[j + 1]) - v.y) * p[c + j + 1];
+          const float x2 = (__uint_as_float(u[j + 2]) - v.z) * p[c + j + 2], x3 = (__uint_as_float(u[j + 3]) - v.w) * p[c + j + 3];
+          w[j >> 1] = tt_pack(x0, x1);
+          w[(j >> 1) + 1] = tt_pack(x2, x3);
+        }
+        if (!key_live) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) w[j] = 0u;
+        }
+        tc_st16(tmem_dp + lanes + (unsigned)(half * 64 + (c >> 1)), w);
+      }
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(ds_ready);
+    }
+    if (ok && tiles > 0) ok = mbar_wait_warp(done, 0, abort_flag, nullptr, 90);
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const HeadView &o = half ? a.o2 : a.o1;  // one half of the warps stores dk, the other dv
+    bf16 *row = reinterpret_cast<bf16 *>(o.p) + at.stream * o.s + (long long)key * o.r + at.head * o.h;
+    tt_store_row(row, key < a.m, a, (half ? tmem_dv : tmem_dk) + lanes, 0, (a.dim + 15) & ~15, half ? 1.f : a.scale, tiles == 0,
+                 __all_sync(0xffffffffu, ok && !*abort_flag));
+  }
+  __syncwarp();
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == 1) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_s), "r"(512u));
+  }
+}
+
+template <int D>
+__global__ void __launch_bounds__(TT_BWD_THREADS, 1)
+train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                   const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do,
+                   const __grid_constant__ TtArgs a) {
+  using L = TtBwd<D>;
+  constexpr int SLABS = L::SLABS, TILE = L::TILE;
+  extern __shared__ unsigned char smem_raw[];
+  const unsigned base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  unsigned char *base_ptr = smem_raw + (base - smem_u32(smem_raw));
+  const unsigned q_off = base, do_off = base + TILE, bars = base + L::BAR_OFF;
+  auto k_tile = [&](int s) { return base + (unsigned)(L::STAGE_OFF + s * 2 * TILE); };
+  auto v_tile = [&](int s) { return base + (unsigned)(L::STAGE_OFF + (s * 2 + 1) * TILE); };
+  float *stat = reinterpret_cast<float *>(base_ptr + L::STAT_OFF);
+  const unsigned q_full = bars, s_full = bars + 8, s_free = bars + 16, dp_full = bars + 24, ds_ready = bars + 32, done = bars + 40;
+  auto k_full = [&](int s) { return bars + 48u + 8u * s; };
+  auto k_empty = [&](int s) { return bars + 64u + 8u * s; };
+  volatile unsigned *tmem_holder = reinterpret_cast<volatile unsigned *>(base_ptr + L::BAR_OFF + 96);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(base_ptr + L::BAR_OFF + 100);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const TtPlace at = tt_place(a, a.heads, a.span.causal != 0);
+  const int r0 = at.tile * TT_B, r1 = min(r0 + TT_B, a.n), kh = at.head / a.share;
+  const int lo = a.span.lo(r0), end = a.span.end(r1 - 1, at.keys);
+  const int tiles = end > lo ? (end - lo + TT_B - 1) / TT_B : 0;
+
+  if (threadIdx.x == 0) {
+    for (unsigned bar : {q_full, s_full, dp_full, done}) mbar_init(bar, 1);
+    mbar_init(s_free, 8);
+    mbar_init(ds_ready, 8);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(k_full(s), 1);
+      mbar_init(k_empty(s), 1);
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) tt_alloc(tmem_holder, 512u);
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const unsigned tmem_s = *tmem_holder, tmem_dp = tmem_s + 128, tmem_dq = tmem_s + 256;
+
+  if (warp == 0) {
+    int it = 0;
+    bool ok = true;
+    if (lane == 0 && tiles > 0) {
+      mbar_expect_tx(q_full, 2u * TILE);
+      for (int s = 0; s < SLABS; ++s) {
+        tma_load_4d(q_off + s * TT_SLAB, &map_q, s * 64, at.head, r0, at.stream, q_full);
+        tma_load_4d(do_off + s * TT_SLAB, &map_do, s * 64, at.head, r0, at.stream, q_full);
+      }
+    }
+    for (; it < tiles; ++it) {
+      const int st = it & 1, j0 = lo + it * TT_B;
+      ok = mbar_wait_warp(k_empty(st), ((unsigned)(it >> 1) & 1u) ^ 1u, abort_flag, nullptr, 91);
+      if (!ok) break;
+      if (lane == 0) {
+        mbar_expect_tx(k_full(st), 2u * TILE);
+        for (int s = 0; s < SLABS; ++s) {
+          tma_load_4d(k_tile(st) + s * TT_SLAB, &map_k, s * 64, kh, j0, at.stream, k_full(st));
+          tma_load_4d(v_tile(st) + s * TT_SLAB, &map_v, s * 64, kh, j0, at.stream, k_full(st));
+        }
+      }
+      __syncwarp();
+    }
+    if (*abort_flag && tiles > 0) {  // copies in flight must land before the shared memory goes away
+      const unsigned long long limit = global_timer() + WAIT_LIMIT_NS;
+      while (!mbar_try_wait(q_full, 0) && global_timer() < limit) {}
+      for (int j = it > 2 ? it - 2 : 0; j < it; ++j)
+        while (!mbar_try_wait(k_full(j & 1), (unsigned)(j >> 1) & 1u) && global_timer() < limit) {}
+    }
+  } else if (warp == 1) {
+    const int cols = (a.dim + 15) & ~15, ksteps = cols >> 4;
+    const unsigned idesc_s = umma_idesc_bf16(TT_B), idesc_d = umma_idesc_bf16(cols) | UMMA_B_MN_MAJOR;
+    // keys behind the stream's length must not meet the zeros of dS as anything but zeros
+    auto arrived = [&](int i) {
+      if (!mbar_wait_warp(k_full(i & 1), (unsigned)(i >> 1) & 1u, abort_flag, nullptr, 92)) return false;
+      const int have = at.keys - (lo + i * TT_B);
+      if (have < TT_B && at.keys < a.m) tt_clear_rows(base_ptr + (k_tile(i & 1) - base), SLABS, have, lane);
+      return true;
+    };
+    bool ok = true;
+    if (tiles > 0) {
+      ok = mbar_wait_warp(q_full, 0, abort_flag, nullptr, 93) && arrived(0);
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      if (ok && lane == 0) {
+        tt_mma_rows(tmem_s, q_off, k_tile(0), ksteps, idesc_s);
+        tc_commit(s_full);
+        tt_mma_rows(tmem_dp, do_off, v_tile(0), ksteps, idesc_s);
+        tc_commit(dp_full);
+      }
+      __syncwarp();
+    }
+    for (int i = 0; i < tiles && ok; ++i) {
+      const int st = i & 1, next = st ^ 1;
+      if (i + 1 < tiles) {
+        ok = mbar_wait_warp(s_free, (unsigned)i & 1u, abort_flag, nullptr, 94) && arrived(i + 1);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (lane == 0) {
+          tt_mma_rows(tmem_s, q_off, k_tile(next), ksteps, idesc_s);
+          tc_commit(s_full);
+        }
+        __syncwarp();
+      }
+      ok = mbar_wait_warp(ds_ready, (unsigned)i & 1u, abort_flag, nullptr, 95);
+      if (!ok) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      if (lane == 0) {
+#pragma unroll
+        for (int ks = 0; ks < TT_B / 16; ++ks)
+          tc_mma_f16_ts(tmem_dq, tmem_dp + (unsigned)((ks >> 2) * 64 + (ks & 3) * 8),
+                        umma_desc_mn128(k_tile(st) + (unsigned)(ks * 16 * 128), TT_SLAB), idesc_d, (i | ks) ? 1u : 0u);
+        tc_commit(k_empty(st));
+        if (i + 1 < tiles) {
+          tt_mma_rows(tmem_dp, do_off, v_tile(next), ksteps, idesc_s);
+          tc_commit(dp_full);
+        }
+      }
+      __syncwarp();
+    }
+    if (tiles > 0 && lane == 0) tc_commit(done);
+    __syncwarp();
+    if (!ok) {  // a bounded chance for the tensor pipe to finish before tensor memory is freed
+      const unsigned long long limit = global_timer() + WAIT_LIMIT_NS;
+      while (!mbar_try_wait(done, 0) && global_timer() < limit) {}
+    }
+  } else {
+    const int q = warp & 3, half = (warp - 2) >> 2;
+    const unsigned lanes = (unsigned)(q * 32) << 16;
+    const int row = r0 + q * 32 + lane;
+    const int row_lo = a.span.lo(row), row_end = a.span.end(row, at.keys);
+    const int warp_lo = a.span.lo(r0 + q * 32 + 31), warp_end = a.span.end(r0 + q * 32, at.keys);
+    const long long x = ((long long)at.stream * a.heads + at.head) * a.n + row;
+    const float z = row < a.n ? a.lse[x] : -INFINITY;
+    float delta = row < a.n ? a.delta[x] : 0.f;
+    const float lse = z == -INFINITY ? INFINITY : z * TT_LOG2E;  // a row that sees no key has no weights: 2^(s - infinity)
+    // dout . out is off by what out was rounded by, which counts in rows of few keys. Where all of a row's keys lie in this one
+    // tile, the same sum over keys, p dP, is at hand in 32 bits (the kernel of dk and dv then finds it in place of the other).
+    auto exact_delta = [&](const float (&p)[64], int half, int c_lo, int c_end) {
+      float t = 0.f;
+#pragma unroll
+      for (int c = 0; c < 64; c += 32) {
+        unsigned u[32];
+        tc_ld32(tmem_dp + lanes + (unsigned)(half * 64 + c), u);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (c + j >= c_lo && c + j < c_end) t = fmaf(p[c + j], __uint_as_float(u[j]), t);
+      }
+      float *both = stat + q * 32 + lane;
+      both[half * 128] = t;
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      t = both[0] + both[128];
+      if (half == 0 && row < a.n) a.delta[x] = t;
+      return t;
+    };
+    bool ok = true;
+    for (int i = 0; i < tiles && ok; ++i) {
+      const int j0 = lo + i * TT_B + half * 64;
+      const int c_lo = row_lo - j0, c_end = row_end - j0;
+      const bool inside = warp_lo <= j0 && warp_end >= j0 + 64;
+      ok = mbar_wait_warp(s_full, (unsigned)i & 1u, abort_flag, nullptr, 96);
+      if (!ok) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      float p[64];
+      {
+        unsigned(&u)[2][32] = reinterpret_cast<unsigned(&)[2][32]>(p);
+        tc_ld32(tmem_s + lanes + (unsigned)(half * 64), u[0]);
+        tc_ld32(tmem_s + lanes + (unsigned)(half * 64 + 32), u[1]);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(s_free);
+#pragma unroll
+      for (int j = 0; j < 64; ++j) p[j] = tt_exp2(fmaf(p[j], a.factor, -lse));
+      ok = mbar_wait_warp(dp_full, (unsigned)i & 1u, abort_flag, nullptr, 97);
+      if (!ok) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      if (!inside) {
+#pragma unroll
+        for (int j = 0; j < 64; ++j)
+          if (j < c_lo || j >= c_end) p[j] = 0.f;
+      }
+      if (tiles == 1) delta = exact_delta(p, half, c_lo, c_end);
+#pragma unroll
+      for (int c = 0; c < 64; c += 32) {
+        unsigned u[32], w[16];
+        tc_ld32(tmem_dp + lanes + (unsigned)(half * 64 + c), u);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+        for (int j = 0; j < 32; ++j) p[c + j] *= __uint_as_float(u[j]) - delta;
+        if (!inside) {  // (a weight of zero has no part even where the other factor is not finite)
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (c + j < c_lo || c + j >= c_end) p[c + j] = 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) w[j] = tt_pack(p[c + 2 * j], p[c + 2 * j + 1]);
+        tc_st16(tmem_dp + lanes + (unsigned)(half * 64 + (c >> 1)), w);
+      }
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(ds_ready);
+    }
+    if (ok && tiles > 0) ok = mbar_wait_warp(done, 0, abort_flag, nullptr, 98);
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    bf16 *o = reinterpret_cast<bf16 *>(a.o1.p) + at.stream * a.o1.s + (long long)row * a.o1.r + at.head * a.o1.h;
+    const int cols = (a.dim + 15) & ~15, mid = (cols / 2 + 15) & ~15;  // each half of the warps stores half of the columns
+    tt_store_row(o, row < a.n, a, tmem_dq + lanes, half ? mid : 0, half ? cols : mid, a.scale, tiles == 0, __all_sync(0xffffffffu, ok && !*abort_flag));
+  }
+  __syncwarp();
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == 1) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_s), "r"(512u));
+  }
+}
+
+// Whether TMA can address the rows: contiguous columns, 16-byte boundaries, strides that are no repetition.
+bool tt_addressable(const HeadView &x, long long streams, long long rows, long long heads) {
+  auto stride = [](long long s, long long extent) { return extent <= 1 || (s > 0 && s % 8 == 0 && s < (1ll << 38)); };
+  return x.c == 1 && reinterpret_cast<uintptr_t>(x.p) % 16 == 0 && stride(x.s, streams) && stride(x.r, rows) && stride(x.h, heads);
+}
+
+CUtensorMap tt_map(const HeadView &x, long long streams, long long rows, long long heads, int dim) {
+  CUtensorMap map;
+  auto bytes = [](long long s, long long extent) { return extent <= 1 ? 16ull : (unsigned long long)s * 2; };
+  const unsigned long long extent[4] = {(unsigned long long)dim, (unsigned long long)heads, (unsigned long long)rows,
+                                        (unsigned long long)streams};
+  const unsigned long long strides[3] = {bytes(x.h, heads), bytes(x.r, rows), bytes(x.s, streams)};
+  tc_make_map_heads(&map, x.p, extent, strides, TT_B);
+  return map;
+}
+
+bool tt_rows16(const HeadView &x) {
+  return x.c == 1 && reinterpret_cast<uintptr_t>(x.p) % 16 == 0 && x.s % 8 == 0 && x.r % 8 == 0 && x.h % 8 == 0;
+}
+
+TtArgs tt_args(const TrainAttention &a, int rows) {
+  TtArgs t{};
+  t.n = a.n;
+  t.m = a.m;
+  t.heads = a.heads;
+  t.groups = a.groups;
+  t.share = a.heads / a.groups;
+  t.streams = a.streams;
+  t.dim = a.dim;
+  t.tiles = (rows + TT_B - 1) / TT_B;
+  t.span = TrainSpan{a.first, a.window, a.causal};
+  t.lengths = a.lengths;
+  t.scale = a.scale;
+  t.factor = a.scale * TT_LOG2E;
+  t.lse = a.lse;
+  return t;
+}
+
+unsigned tt_grid(const TtArgs &t, int heads) {
+  const long long blocks = (long long)t.tiles * heads * t.streams;
+  if (blocks > 0x7fffffffLL) throw std::invalid_argument("attention: too many rows, heads and streams for one call");
+  return (unsigned)blocks;
+}
+
+template <int D>
+void forward(const TrainAttention &a, cudaStream_t st) {
+  TtArgs t = tt_args(a, a.n);
+  t.o1 = a.out;
+  t.vec = tt_rows16(a.out);
+  const size_t smem = 3 * (size_t)(D / 64) * TT_SLAB + 128 + 1024;
+  LB_CUDA(cudaFuncSetAttribute(train_forward_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  train_forward_tc_kernel<D><<<tt_grid(t, a.heads), TT_FWD_THREADS, smem, st>>>(
+      tt_map(a.q, a.streams, a.n, a.heads, a.dim), tt_map(a.k, a.streams, a.m, a.groups, a.dim),
+      tt_map(a.v, a.streams, a.m, a.groups, a.dim), t);
+  LB_LAUNCH_CHECK();
+}
+
+template <int D>
+void backward(const TrainAttention &a, float *delta, cudaStream_t st) {
+  const CUtensorMap mq = tt_map(a.q, a.streams, a.n, a.heads, a.dim), mk = tt_map(a.k, a.streams, a.m, a.groups, a.dim),
+                    mv = tt_map(a.v, a.streams, a.m, a.groups, a.dim), md = tt_map(a.dout, a.streams, a.n, a.heads, a.dim);
+  constexpr int smem = TtBwd<D>::TOTAL;
+  TtArgs t = tt_args(a, a.n);
+  t.delta = delta;
+  t.o1 = a.dq;
+  t.vec = tt_rows16(a.dq);
+  LB_CUDA(cudaFuncSetAttribute(train_dq_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  train_dq_tc_kernel<D><<<tt_grid(t, a.heads), TT_BWD_THREADS, smem, st>>>(mq, mk, mv, md, t);
+  LB_LAUNCH_CHECK();
+  t = tt_args(a, a.m);
+  t.delta = delta;
+  t.o1 = a.dk;
+  t.o2 = a.dv;
+  t.vec = tt_rows16(a.dk) && tt_rows16(a.dv);
+  LB_CUDA(cudaFuncSetAttribute(train_dkv_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  train_dkv_tc_kernel<D><<<tt_grid(t, a.groups), TT_BWD_THREADS, smem, st>>>(mq, mk, mv, md, t);
+  LB_LAUNCH_CHECK();
+}
+
+}  // namespace
+
+bool train_attention_tc_supports(const TrainAttention &a, bool backward) {
+  if (!a.bf16 || a.dim % 8 != 0) return false;
+  const long long s = a.streams;
+  return tt_addressable(a.q, s, a.n, a.heads) && tt_addressable(a.k, s, a.m, a.groups) && tt_addressable(a.v, s, a.m, a.groups) &&
+         (backward ? tt_addressable(a.dout, s, a.n, a.heads) && a.dq.c == 1 && a.dk.c == 1 && a.dv.c == 1 : a.out.c == 1);
+}
+
+void launch_train_attention_forward_tc(const TrainAttention &a, cudaStream_t st) {
+  if (a.dim <= 64) forward<64>(a, st);
+  else forward<128>(a, st);
+}
+
+void launch_train_attention_backward_tc(const TrainAttention &a, float *delta, cudaStream_t st) {
+  if (a.dim <= 64) backward<64>(a, delta, st);
+  else backward<128>(a, delta, st);
+}
+
+}  // namespace lb

@@ -39,6 +39,11 @@ void launch_train_attention_backward(const TrainAttention &a, float *delta, cuda
 // delta[s, h, i] = dout_i . out_i
 void launch_train_delta(const TrainAttention &a, float *delta, cudaStream_t st);
 
+// train_attention_tc.cu: bfloat16 on the tensor cores, where every operand can be addressed by TMA
+bool train_attention_tc_supports(const TrainAttention &a, bool backward);
+void launch_train_attention_forward_tc(const TrainAttention &a, cudaStream_t st);
+void launch_train_attention_backward_tc(const TrainAttention &a, float *delta, cudaStream_t st);
+
 struct PolicyLoss {
   const char *logits = nullptr;
   char *dlogits = nullptr;         // null: no gradient; may be logits
