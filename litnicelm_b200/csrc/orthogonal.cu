@@ -1,137 +1,549 @@
 // Orthogonalised momentum: the update of a weight matrix by the polynomial iteration
 //   X = U / (|U| + 1e-7),  X <- a X + (b A + c A^2) X,  A = X X^T,  (a, b, c) = (3.4445, -4.7750, 2.0315)
-// in the space of the matrix's smaller side, which drives its singular values towards 1; and the optimiser step with it,
+// in the space of the matrix's smaller side (X <- X (b A + c A^2) + a X with A = X^T X for a tall one), which drives its singular
+// values towards 1; and the optimiser step with it,
 //   momentum <- mu momentum + grad,  U = grad + mu momentum or momentum,
 //   params <- (1 - lr decay) params - lr sqrt(max(1, m / n)) X.
-// All matrices of a call have one shape and go through each step together. 32-bit products throughout.
+// All matrices of a call have one shape and go through each product together.
+//
+// Matrices live as pairs of fp16 values: z 2^e = hi + 2^-11 lo, 22 bits, with one exponent e per matrix, kind and step. It follows
+// from a bound on the singular values alone: those of X_k are at most min(1.25, rho a^k) where rho = |X_0| (the polynomial stays
+// below 1.21 on [0, 1.21] and below a s), so those of A at most its square and those of b A + c A^2 at most min(2.85, |b| of
+// that); no entry is larger, and e puts the bound at 2^13 to 2^14. A product is three: hi hi in one accumulator of tensor memory,
+// hi lo and lo hi in another; lo lo is below 2^-24 of a term and left out. The tensor pipe truncates when it adds, so chains in
+// tensor memory are 256 k long and are added in registers, rounded to nearest.
+//
+// One persistent kernel for the three products of a step, tiles of 128 x 128: warp 0 issues TMA (stages of 64 k: four tiles of 16
+// KB), warp 1 owns tensor memory and issues the MMAs, eight warps add finished chains (a thread: a row and half of the columns) and
+// store. Nothing is transposed in memory: an operand whose rows run along k is read as it lies (M or N contiguous). A and b A +
+// c A^2 are symmetric: tiles below the diagonal are multiplied, and stored on both sides.
+// Every wait is bounded; one that runs out ends the CTA, whose results are then NaN. No clusters, no multicast.
 #include "train_ops.cuh"
+#include "gemm_tc.cuh"
+#include "tc_ptx.cuh"
+
+#include <cuda_fp16.h>
 
 namespace lb {
 
 namespace {
 
 constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f, NS_EPS = 1e-7f;
-constexpr int NS_PARTS = 64;  // partial sums of a matrix's norm
+constexpr int NS_PARTS = 256;  // partial sums of a matrix's norm, at most
+constexpr int NS_THREADS = 320, NS_CHAIN = 4;
 
-struct NsWork {
-  double *parts;      // [count][NS_PARTS]
-  float *x, *y, *a, *b;
+struct Pair {
+  __half *hi, *lo;  // [count][rows][ld]
 };
 
-__device__ __forceinline__ float *element(const MatView &v, long long batch, long long r, long long c) {
-  return reinterpret_cast<float *>(v.data + batch_offset(v, batch) + r * v.rs + c * v.cs);
+struct NsWork {
+  double *parts;   // [count][NS_PARTS]
+  float *rho;      // [count]
+  Pair x[2], a, b;
+  long long ldx, ldp;
+};
+
+// Exponents of the pairs of X, A and b A + c A^2 in step k.
+__device__ __forceinline__ int ns_exponent(float bound) {
+  if (!(bound > 0.f)) return 0;
+  const int e = 13 - ilogbf(bound);
+  return e < 100 ? e : 100;
+}
+__device__ __forceinline__ float ns_bound_x(float rho, int k) {
+  float s = rho;
+  for (int i = 0; i < k; ++i) s *= 3.45f;
+  return fminf(1.25f, s);
+}
+__device__ __forceinline__ int ns_exp_x(float rho, int k) { return ns_exponent(ns_bound_x(rho, k)); }
+__device__ __forceinline__ int ns_exp_a(float rho, int k) {
+  const float s = ns_bound_x(rho, k);
+  return ns_exponent(s * s);
+}
+__device__ __forceinline__ int ns_exp_b(float rho, int k) {
+  const float s = ns_bound_x(rho, k);
+  return ns_exponent(fminf(2.85f, 4.8f * s * s));
 }
 
-// Momentum and the matrix to orthogonalise (in the orientation of x, whose rows are the smaller side), with partial sums of squares.
-__global__ void __launch_bounds__(256) muon_begin_kernel(const __grid_constant__ MuonStep g, NsWork w, int tall) {
-  const long long m = g.grads.rows, n = g.grads.cols, each = m * n, batch = blockIdx.y;
-  double sum = 0.0;
-  for (long long e = blockIdx.x * 256LL + threadIdx.x; e < each; e += 256LL * gridDim.x) {
-    const long long r = e / n, c = e - r * n;
-    const float grad = *element(g.grads, batch, r, c);
-    float u = grad;
-    if (g.step) {
-      float *mom = element(g.momentum, batch, r, c);
-      const float v = fmaf(g.mu, *mom, grad);
-      *mom = v;
-      u = g.nesterov ? fmaf(g.mu, v, grad) : v;
-    }
-    w.x[batch * each + (tall ? c * m + r : e)] = u;
-    sum += (double)u * (double)u;
+__device__ __forceinline__ void ns_split(float z, __half &hi, __half &lo) {  // z already scaled
+  hi = __float2half_rn(z);
+  lo = __float2half_rn((z - __half2float(hi)) * 2048.f);
+}
+__device__ __forceinline__ float ns_value(__half hi, __half lo) { return fmaf(__half2float(lo), 1.f / 2048.f, __half2float(hi)); }
+__device__ __forceinline__ float ns_pow2(int e) { return ldexpf(1.f, e); }
+
+// ---- momentum and norm, first pair, end ------------------------------------------------------------------------------------------
+
+__device__ __forceinline__ float *element(const MatView &v, long long batch_off, long long r, long long c) {
+  return reinterpret_cast<float *>(v.data + batch_off + r * v.rs + c * v.cs);
+}
+
+// Four elements of a row from column c on; `vec`: rows of the view on 16-byte boundaries. What lies behind the row is 0.
+__device__ __forceinline__ void load4(const MatView &v, long long off, long long r, long long c, bool vec, float (&x)[4]) {
+  const float *p = element(v, off, r, c);
+  if (vec && c + 4 <= v.cols) {
+    const float4 f = *reinterpret_cast<const float4 *>(p);
+    x[0] = f.x; x[1] = f.y; x[2] = f.z; x[3] = f.w;
+    return;
   }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) x[j] = c + j < v.cols ? *reinterpret_cast<const float *>(reinterpret_cast<const char *>(p) + j * v.cs) : 0.f;
+}
+__device__ __forceinline__ void store4(const MatView &v, long long off, long long r, long long c, bool vec, const float (&x)[4]) {
+  float *p = element(v, off, r, c);
+  if (vec && c + 4 <= v.cols) {
+    *reinterpret_cast<float4 *>(p) = make_float4(x[0], x[1], x[2], x[3]);
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (c + j < v.cols) *reinterpret_cast<float *>(reinterpret_cast<char *>(p) + j * v.cs) = x[j];
+}
+
+__device__ __forceinline__ double ns_block_sum(double s) {
   __shared__ double red[8];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = sum;
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int i = 1; i < 8; ++i) sum += red[i];
-    w.parts[batch * NS_PARTS + blockIdx.x] = sum;
-  }
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
+  __syncthreads();
+  s = red[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) s += red[i];
+  return s;
 }
 
-__global__ void __launch_bounds__(256) muon_scale_kernel(NsWork w, long long each) {
-  const long long batch = blockIdx.y;
+enum { VEC_G = 1, VEC_M = 2, VEC_P = 4 };
+
+__global__ void __launch_bounds__(256) muon_begin_kernel(const __grid_constant__ MuonStep g, NsWork w, unsigned vec) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const long long batch = blockIdx.y, quads = (g.grads.cols + 3) / 4, each = g.grads.rows * quads;
+  const long long go = batch_offset(g.grads, batch), mo = g.step ? batch_offset(g.momentum, batch) : 0;
   double sum = 0.0;
-  for (int i = 0; i < (int)gridDim.x; ++i) sum += w.parts[batch * NS_PARTS + i];
-  const float norm = (float)sqrt(sum) + NS_EPS;
-  for (long long e = blockIdx.x * 256LL + threadIdx.x; e < each; e += 256LL * gridDim.x) w.x[batch * each + e] /= norm;
-}
-
-// y = p x + q y
-__global__ void __launch_bounds__(256) muon_combine_kernel(float p, const float *x, float q, float *y, long long n) {
-  for (long long e = blockIdx.x * 256LL + threadIdx.x; e < n; e += 256LL * gridDim.x) y[e] = fmaf(q, y[e], p * x[e]);
-}
-
-__global__ void __launch_bounds__(256) muon_end_kernel(const __grid_constant__ MuonStep g, const float *x, int tall, float keep,
-                                                       float rate) {
-  const long long m = g.grads.rows, n = g.grads.cols, each = m * n, batch = blockIdx.y;
   for (long long e = blockIdx.x * 256LL + threadIdx.x; e < each; e += 256LL * gridDim.x) {
-    const long long r = e / n, c = e - r * n;
-    const float v = x[batch * each + (tall ? c * m + r : e)];
-    float *p = element(g.params, batch, r, c);
-    *p = g.step ? fmaf(-rate, v, *p * keep) : v;
+    const long long r = div_index(e, quads), c = (e - r * quads) * 4;
+    float u[4];
+    load4(g.grads, go, r, c, vec & VEC_G, u);
+    if (g.step) {
+      float m[4];
+      load4(g.momentum, mo, r, c, vec & VEC_M, m);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        m[j] = fmaf(g.mu, m[j], u[j]);
+        u[j] = g.nesterov ? fmaf(g.mu, m[j], u[j]) : m[j];
+      }
+      store4(g.momentum, mo, r, c, vec & VEC_M, m);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum += (double)u[j] * (double)u[j];
+  }
+  sum = ns_block_sum(sum);
+  if (threadIdx.x == 0) w.parts[batch * NS_PARTS + blockIdx.x] = sum;
+}
+
+__global__ void __launch_bounds__(256) muon_pair_kernel(const __grid_constant__ MuonStep g, NsWork w, unsigned vec, int parts) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const long long batch = blockIdx.y, quads = w.ldx / 4, each = g.grads.rows * quads;
+  const long long go = batch_offset(g.grads, batch), mo = g.step ? batch_offset(g.momentum, batch) : 0;
+  const double norm = sqrt(ns_block_sum((int)threadIdx.x < parts ? w.parts[batch * NS_PARTS + threadIdx.x] : 0.0));
+  const double inv = 1.0 / (norm + (double)NS_EPS);
+  const float rho = (float)(norm * inv);
+  if (blockIdx.x == 0 && threadIdx.x == 0) w.rho[batch] = rho;
+  const double scale = inv * (double)ns_pow2(ns_exp_x(rho, 0));
+  __half *hi = w.x[0].hi + batch * g.grads.rows * w.ldx, *lo = w.x[0].lo + batch * g.grads.rows * w.ldx;
+  for (long long e = blockIdx.x * 256LL + threadIdx.x; e < each; e += 256LL * gridDim.x) {
+    const long long r = div_index(e, quads), c = (e - r * quads) * 4;
+    float u[4] = {0.f, 0.f, 0.f, 0.f};
+    if (c < g.grads.cols) load4(g.grads, go, r, c, vec & VEC_G, u);
+    if (g.step && c < g.grads.cols) {
+      float m[4];
+      load4(g.momentum, mo, r, c, vec & VEC_M, m);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) u[j] = g.nesterov ? fmaf(g.mu, m[j], u[j]) : m[j];
+    }
+    __half h[4], l[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) ns_split((float)((double)u[j] * scale), h[j], l[j]);
+    *reinterpret_cast<uint2 *>(hi + r * w.ldx + c) = *reinterpret_cast<const uint2 *>(h);
+    *reinterpret_cast<uint2 *>(lo + r * w.ldx + c) = *reinterpret_cast<const uint2 *>(l);
   }
 }
 
-MatView dense(float *p, long long count, long long rows, long long cols) {
-  MatView v{};
-  v.data = reinterpret_cast<char *>(p);
-  v.nb = count > 1 ? 1 : 0;
-  v.bd[0] = count;
-  v.bs[0] = rows * cols * 4;
-  v.batch = count;
-  v.rows = rows;
-  v.cols = cols;
-  v.rs = cols * 4;
-  v.cs = 4;
-  return v;
+__global__ void __launch_bounds__(256) muon_end_kernel(const __grid_constant__ MuonStep g, NsWork w, unsigned vec, float keep,
+                                                       float rate) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const long long batch = blockIdx.y, quads = (g.grads.cols + 3) / 4, each = g.grads.rows * quads;
+  const long long po = batch_offset(g.params, batch);
+  const Pair x = w.x[g.steps & 1];
+  const __half *hi = x.hi + batch * g.grads.rows * w.ldx, *lo = x.lo + batch * g.grads.rows * w.ldx;
+  const float scale = ns_pow2(-ns_exp_x(w.rho[batch], g.steps));
+  for (long long e = blockIdx.x * 256LL + threadIdx.x; e < each; e += 256LL * gridDim.x) {
+    const long long r = div_index(e, quads), c = (e - r * quads) * 4;
+    __half h[4], l[4];
+    *reinterpret_cast<uint2 *>(h) = *reinterpret_cast<const uint2 *>(hi + r * w.ldx + c);
+    *reinterpret_cast<uint2 *>(l) = *reinterpret_cast<const uint2 *>(lo + r * w.ldx + c);
+    float v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = ns_value(h[j], l[j]) * scale;
+    if (g.step) {
+      float p[4];
+      load4(g.params, po, r, c, vec & VEC_P, p);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = fmaf(-rate, v[j], p[j] * keep);
+    }
+    store4(g.params, po, r, c, vec & VEC_P, v);
+  }
 }
 
-MatView turned(MatView v) {
-  std::swap(v.rows, v.cols);
-  std::swap(v.rs, v.cs);
-  return v;
+// ---- the products of a step -------------------------------------------------------------------------------------------------------
+
+// GRAM: A = X X^T or X^T X; POLY: B = b A + c A A; APPLY: X' = a X + B X or a X + X B
+enum NsOp { GRAM, POLY, APPLY };
+
+struct NsProduct {
+  Pair out, add;         // result; the matrix that is added (A for POLY, X for APPLY)
+  long long out_ld;
+  int m, n, k;           // sizes of the product
+  int m_tiles, n_tiles, tiles;  // tiles of all matrices
+  int step;
+  const float *rho;
+};
+
+template <bool A_MN, bool B_MN>
+struct NsSmem {
+  static constexpr int STAGES = 3, TILE = 16384, STAGE = 4 * TILE;
+  static constexpr int BAR_OFF = STAGES * STAGE;
+  static constexpr int TOTAL = BAR_OFF + 128 + 1024;
+};
+
+constexpr unsigned UMMA_A_MN_MAJOR = 1u << 15;
+
+template <NsOp OP, bool A_MN, bool B_MN>
+__global__ void __launch_bounds__(NS_THREADS, 1)
+ns_product_kernel(const __grid_constant__ CUtensorMap map_ah, const __grid_constant__ CUtensorMap map_al,
+                  const __grid_constant__ CUtensorMap map_bh, const __grid_constant__ CUtensorMap map_bl,
+                  const __grid_constant__ NsProduct g) {
+  using L = NsSmem<A_MN, B_MN>;
+  constexpr int S = L::STAGES;
+  constexpr bool SYM = OP != APPLY;
+  extern __shared__ unsigned char smem_raw[];
+  const unsigned base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  unsigned char *base_ptr = smem_raw + (base - smem_u32(smem_raw));
+  const unsigned bars = base + L::BAR_OFF;
+  auto full = [&](int s) { return bars + 8u * s; };
+  auto empty = [&](int s) { return bars + 8u * (S + s); };
+  auto chain_full = [&](int b) { return bars + 8u * (2 * S + b); };
+  auto chain_empty = [&](int b) { return bars + 8u * (2 * S + 2 + b); };
+  const unsigned done = bars + 8u * (2 * S + 4);
+  volatile unsigned *tmem_holder = reinterpret_cast<volatile unsigned *>(base_ptr + L::BAR_OFF + 96);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(base_ptr + L::BAR_OFF + 100);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int kblocks = (g.k + 63) / 64, chains = (kblocks + NS_CHAIN - 1) / NS_CHAIN;
+  auto place = [&](int tile, int &batch, int &mt, int &nt) {
+    const int per = SYM ? g.m_tiles * (g.m_tiles + 1) / 2 : g.m_tiles * g.n_tiles;
+    batch = tile / per;
+    const int rest = tile - batch * per;
+    if (SYM) {  // row mt has the tiles 0 .. mt
+      mt = (int)((sqrtf(8.f * rest + 1.f) - 1.f) * 0.5f);
+      while (mt * (mt + 1) / 2 > rest) --mt;
+      while ((mt + 1) * (mt + 2) / 2 <= rest) ++mt;
+      nt = rest - mt * (mt + 1) / 2;
+    } else {
+      mt = rest % g.m_tiles;
+      nt = rest / g.m_tiles;
+    }
+  };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(chain_full(b), 1);
+      mbar_init(chain_empty(b), 8);
+    }
+    mbar_init(done, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void *)tmem_holder)),
+                 "r"(512u)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const unsigned tmem = *tmem_holder;
+  pdl_launch_dependents();  // behind the allocation: a dependent's CTA must not take tensor memory first
+  pdl_wait();
+
+  if (warp == 0) {
+    int it = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; tile < g.tiles && ok; tile += gridDim.x) {
+      int batch, mt, nt;
+      place(tile, batch, mt, nt);
+      for (int kb = 0; kb < kblocks; ++kb, ++it) {
+        const int s = it % S;
+        ok = mbar_wait_warp(empty(s), ((unsigned)(it / S) & 1u) ^ 1u, abort_flag, nullptr, 61);
+        if (!ok) break;
+        if (lane == 0) {
+          const unsigned st = base + (unsigned)(s * L::STAGE), bar = full(s);
+          mbar_expect_tx(bar, (unsigned)L::STAGE);
+          auto load = [&](unsigned to, const CUtensorMap *map, bool mn, int at) {
+            if (mn) {  // rows of k, two slabs of 64 columns
+              tma_load_4d(to, map, at * 128, 0, kb * 64, batch, bar);
+              tma_load_4d(to + 8192, map, at * 128 + 64, 0, kb * 64, batch, bar);
+            } else {
+              tma_load_4d(to, map, kb * 64, 0, at * 128, batch, bar);
+            }
+          };
+          load(st, &map_ah, A_MN, mt);
+          load(st + L::TILE, &map_al, A_MN, mt);
+          load(st + 2 * L::TILE, &map_bh, B_MN, nt);
+          load(st + 3 * L::TILE, &map_bl, B_MN, nt);
+        }
+        __syncwarp();
+      }
+    }
+    if (*abort_flag) {  // copies in flight must land before the shared memory goes away
+      const unsigned long long limit = global_timer() + WAIT_LIMIT_NS;
+      for (int j = it > S ? it - S : 0; j < it; ++j)
+        while (!mbar_try_wait(full(j % S), (unsigned)(j / S) & 1u) && global_timer() < limit) {}
+    }
+  } else if (warp == 1) {
+    constexpr unsigned idesc = umma_idesc_f16(128) | (A_MN ? UMMA_A_MN_MAJOR : 0u) | (B_MN ? UMMA_B_MN_MAJOR : 0u);
+    int it = 0, chain = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; tile < g.tiles && ok; tile += gridDim.x) {
+      for (int kb = 0; kb < kblocks; ++kb, ++it) {
+        const int s = it % S, buf = chain & 1;
+        if (kb % NS_CHAIN == 0)
+          ok = mbar_wait_warp(chain_empty(buf), ((unsigned)(chain >> 1) & 1u) ^ 1u, abort_flag, nullptr, 62);
+        if (ok) ok = mbar_wait_warp(full(s), (unsigned)(it / S) & 1u, abort_flag, nullptr, 63);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const bool last = kb + 1 == kblocks || (kb + 1) % NS_CHAIN == 0;
+        if (lane == 0) {
+          const unsigned st = base + (unsigned)(s * L::STAGE), d = tmem + (unsigned)(buf * 256);
+          auto desc = [&](int t, bool mn, int ks) {
+            const unsigned p = st + (unsigned)(t * L::TILE);
+            return mn ? umma_desc_mn128(p + (unsigned)(ks * 2048), 8192u) : umma_desc_k128(p) + (unsigned long long)(ks * 2);
+          };
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks) {
+            const unsigned more = (kb % NS_CHAIN) | ks ? 1u : 0u;
+            const unsigned long long ah = desc(0, A_MN, ks), al = desc(1, A_MN, ks), bh = desc(2, B_MN, ks), bl = desc(3, B_MN, ks);
+            tc_mma_f16(d, ah, bh, idesc, more);
+            tc_mma_f16(d + 128, ah, bl, idesc, more);
+            tc_mma_f16(d + 128, al, bh, idesc, 1u);
+          }
+          tc_commit(empty(s));
+          if (last) tc_commit(chain_full(buf));
+        }
+        __syncwarp();
+        if (last) ++chain;
+      }
+    }
+    if (!ok) {  // what was issued ends, within the limit, before the shared memory goes away
+      if (lane == 0) tc_commit(done);
+      __syncwarp();
+      const unsigned long long limit = global_timer() + WAIT_LIMIT_NS;
+      while (!mbar_try_wait(done, 0u) && global_timer() < limit) {}
+    }
+  } else {
+    const int q = warp & 3, half = (warp - 2) >> 2;
+    int chain = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; tile < g.tiles; tile += gridDim.x) {
+      float acc[64];
+#pragma unroll
+      for (int j = 0; j < 64; ++j) acc[j] = 0.f;
+      for (int c = 0; c < chains && ok; ++c, ++chain) {
+        const int buf = chain & 1;
+        ok = mbar_wait_warp(chain_full(buf), (unsigned)(chain >> 1) & 1u, abort_flag, nullptr, 64);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+        for (int c0 = 0; c0 < 64; c0 += 32) {
+          unsigned r[32], t[32];
+          const unsigned at = tmem + ((unsigned)(q * 32) << 16) + (unsigned)(buf * 256 + half * 64 + c0);
+          tc_ld32(at, r);
+          tc_ld32(at + 128, t);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            acc[c0 + j] += fmaf(__uint_as_float(t[j]), 1.f / 2048.f, __uint_as_float(r[j]));
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(chain_empty(buf));
+      }
+      int batch, mt, nt;
+      place(tile, batch, mt, nt);
+      const float rho = g.rho[batch];
+      const int ex = ns_exp_x(rho, g.step), ea = ns_exp_a(rho, g.step), eb = ns_exp_b(rho, g.step);
+      // acc = the product times 2^(sum of the operands' exponents); out = (p add + q product) 2^(its exponent)
+      const int e_in = OP == GRAM ? 2 * ex : OP == POLY ? 2 * ea : eb + ex;
+      const int e_out = OP == GRAM ? ea : OP == POLY ? eb : ns_exp_x(rho, g.step + 1);
+      const int e_add = OP == POLY ? ea : ex;
+      const float f_add = OP == POLY ? NS_B : NS_A;
+      // exponents of up to 200 in two factors each
+      const float f_in = (OP == POLY ? NS_C : 1.f) * ns_pow2(-(e_in / 2)), f_in2 = ns_pow2(-(e_in - e_in / 2));
+      const float s_add = f_add * ns_pow2(-e_add), s_out = ns_pow2(e_out);
+      const int row = mt * 128 + q * 32 + lane;
+      const long long at = (long long)batch * g.m * g.out_ld + (long long)row * g.out_ld;
+      const bool mirror = SYM && mt != nt;
+#pragma unroll
+      for (int c0 = 0; c0 < 64; c0 += 8) {
+        const int col = nt * 128 + half * 64 + c0;
+        if (col >= g.n) continue;
+        __half h[8], l[8];
+        if (OP != GRAM && row < g.m) {
+          *reinterpret_cast<uint4 *>(h) = *reinterpret_cast<const uint4 *>(g.add.hi + at + col);
+          *reinterpret_cast<uint4 *>(l) = *reinterpret_cast<const uint4 *>(g.add.lo + at + col);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          float v = acc[c0 + j] * f_in * f_in2;
+          if (OP != GRAM) v = fmaf(ns_value(h[j], l[j]), s_add, v);
+          ns_split(ok ? v * s_out : NAN, h[j], l[j]);
+        }
+        if (row < g.m) {
+          *reinterpret_cast<uint4 *>(g.out.hi + at + col) = *reinterpret_cast<const uint4 *>(h);
+          *reinterpret_cast<uint4 *>(g.out.lo + at + col) = *reinterpret_cast<const uint4 *>(l);
+          if (mirror) {
+            const long long to = (long long)batch * g.m * g.out_ld + (long long)col * g.out_ld + row;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (col + j < g.n) {
+                g.out.hi[to + j * g.out_ld] = h[j];
+                g.out.lo[to + j * g.out_ld] = l[j];
+              }
+          }
+        }
+      }
+    }
+  }
+  __syncwarp();
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == 1) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+  }
 }
 
-unsigned blocks(long long n) { return (unsigned)((n + 255) / 256 < 148 * 8 ? (n + 255) / 256 : 148 * 8); }
+struct Operand {
+  Pair p;
+  long long rows, cols, ld;
+};
+
+CUtensorMap ns_map(const __half *p, const Operand &o, long long count, bool mn) {
+  CUtensorMap map;
+  const unsigned long long extent[4] = {(unsigned long long)o.cols, 1, (unsigned long long)o.rows, (unsigned long long)count};
+  const unsigned long long strides[3] = {16, (unsigned long long)o.ld * 2, (unsigned long long)(o.rows * o.ld) * 2};
+  tc_make_map_heads(&map, p, extent, strides, mn ? 64 : 128);
+  return map;
+}
+
+template <NsOp OP, bool A_MN, bool B_MN>
+void product(const Operand &a, const Operand &b, NsProduct g, long long count, cudaStream_t st) {
+  g.m_tiles = (g.m + 127) / 128;
+  g.n_tiles = (g.n + 127) / 128;
+  const long long per = OP == APPLY ? (long long)g.m_tiles * g.n_tiles : (long long)g.m_tiles * (g.m_tiles + 1) / 2;
+  if (per * count > 0x3fffffffLL) throw std::invalid_argument("too many matrices of this size for one call");
+  g.tiles = (int)(per * count);
+  using L = NsSmem<A_MN, B_MN>;
+  LB_CUDA(cudaFuncSetAttribute(ns_product_kernel<OP, A_MN, B_MN>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL));
+  launch_pdl(ns_product_kernel<OP, A_MN, B_MN>, dim3((unsigned)(g.tiles < 148 ? g.tiles : 148)), dim3(NS_THREADS), L::TOTAL, st, true,
+             ns_map(a.p.hi, a, count, A_MN), ns_map(a.p.lo, a, count, A_MN), ns_map(b.p.hi, b, count, B_MN),
+             ns_map(b.p.lo, b, count, B_MN), g);
+}
+
+bool rows16(const MatView &v) {
+  if (v.cs != 4 || v.rs % 16 || reinterpret_cast<uintptr_t>(v.data) % 16) return false;
+  for (int i = 0; i < v.nb; ++i)
+    if (v.bs[i] % 16) return false;
+  return true;
+}
+
+size_t up(size_t bytes) { return (bytes + 255) / 256 * 256; }
+
+// The workspace's parts; its size.
+size_t ns_layout(long long count, long long m, long long n, char *p, NsWork *w) {
+  const long long small = m < n ? m : n;
+  const long long ldx = (n + 7) / 8 * 8, ldp = (small + 7) / 8 * 8;
+  char *const begin = p;
+  auto take = [&](size_t bytes) {
+    char *at = p;
+    p += up(bytes);
+    return at;
+  };
+  NsWork k;
+  k.ldx = ldx;
+  k.ldp = ldp;
+  k.parts = reinterpret_cast<double *>(take((size_t)count * NS_PARTS * 8));
+  k.rho = reinterpret_cast<float *>(take((size_t)count * 4));
+  for (Pair *x : {&k.x[0], &k.x[1]}) {
+    x->hi = reinterpret_cast<__half *>(take((size_t)count * m * ldx * 2));
+    x->lo = reinterpret_cast<__half *>(take((size_t)count * m * ldx * 2));
+  }
+  for (Pair *x : {&k.a, &k.b}) {
+    x->hi = reinterpret_cast<__half *>(take((size_t)count * small * ldp * 2));
+    x->lo = reinterpret_cast<__half *>(take((size_t)count * small * ldp * 2));
+  }
+  if (w) *w = k;
+  return (size_t)(p - begin);
+}
 
 }  // namespace
 
-size_t muon_workspace_bytes(long long count, long long m, long long n) {
-  const long long p = m < n ? m : n;
-  return 256 + (size_t)count * (NS_PARTS * 8 + 2 * (size_t)m * n * 4 + 2 * (size_t)p * p * 4);
-}
+size_t muon_workspace_bytes(long long count, long long m, long long n) { return ns_layout(count, m, n, nullptr, nullptr); }
 
 void launch_muon(const MuonStep &g, void *workspace, cudaStream_t st) {
-  const long long m = g.grads.rows, n = g.grads.cols, count = g.grads.batch, each = m * n;
-  const int tall = m > n;
-  const long long p = tall ? n : m, q = tall ? m : n;
-  NsWork w{};
-  w.parts = static_cast<double *>(workspace);
-  w.x = reinterpret_cast<float *>(w.parts + count * NS_PARTS);
-  w.y = w.x + count * each;
-  w.a = w.y + count * each;
-  w.b = w.a + count * p * p;
-  const dim3 grid((unsigned)((each + 255) / 256 < NS_PARTS ? (each + 255) / 256 : NS_PARTS), (unsigned)count);
-  muon_begin_kernel<<<grid, 256, 0, st>>>(g, w, tall);
-  LB_LAUNCH_CHECK();
-  muon_scale_kernel<<<grid, 256, 0, st>>>(w, each);
-  LB_LAUNCH_CHECK();
+  const long long m = g.grads.rows, n = g.grads.cols, count = g.grads.batch;
+  const bool tall = m > n;
+  const int p = (int)(tall ? n : m);
+  NsWork w;
+  ns_layout(count, m, n, static_cast<char *>(workspace), &w);
+  const unsigned vec = (rows16(g.grads) ? VEC_G : 0) | (g.step && rows16(g.momentum) ? VEC_M : 0) | (rows16(g.params) ? VEC_P : 0);
+  const long long quads = m * ((n + 3) / 4), blocks = (quads + 255) / 256;
+  const unsigned parts = (unsigned)(blocks < NS_PARTS ? blocks : NS_PARTS);
+  const dim3 grid(parts, (unsigned)count), wide((unsigned)(blocks < 1184 ? blocks : 1184), (unsigned)count);
+  launch_pdl(muon_begin_kernel, grid, dim3(256), 0, st, true, g, w, vec);
+  launch_pdl(muon_pair_kernel, wide, dim3(256), 0, st, true, g, w, vec, (int)parts);
   for (int i = 0; i < g.steps; ++i) {
-    const MatView x = dense(w.x, count, p, q), a = dense(w.a, count, p, p), b = dense(w.b, count, p, p);
-    launch_gemm_simt(x, turned(x), a, p, p, q, GemmEpilogue{}, st);
-    launch_gemm_simt(a, a, b, p, p, p, GemmEpilogue{}, st);
-    muon_combine_kernel<<<blocks(count * p * p), 256, 0, st>>>(NS_B, w.a, NS_C, w.b, count * p * p);
-    LB_LAUNCH_CHECK();
-    launch_gemm_simt(b, x, dense(w.y, count, p, q), p, q, p, GemmEpilogue{}, st);
-    muon_combine_kernel<<<blocks(count * each), 256, 0, st>>>(NS_A, w.x, 1.f, w.y, count * each);
-    LB_LAUNCH_CHECK();
-    std::swap(w.x, w.y);
+    const Operand x{w.x[i & 1], m, n, w.ldx}, a{w.a, p, p, w.ldp}, b{w.b, p, p, w.ldp};
+    NsProduct f{};
+    f.step = i;
+    f.rho = w.rho;
+    f.out = w.a;
+    f.out_ld = w.ldp;
+    f.m = f.n = p;
+    f.k = (int)(tall ? m : n);
+    if (tall) product<GRAM, true, true>(x, x, f, count, st);
+    else product<GRAM, false, false>(x, x, f, count, st);
+    f.out = w.b;
+    f.add = w.a;
+    f.k = p;
+    product<POLY, false, false>(a, a, f, count, st);
+    f.out = w.x[(i + 1) & 1];
+    f.add = w.x[i & 1];
+    f.out_ld = w.ldx;
+    f.m = (int)m;
+    f.n = (int)n;
+    if (tall) product<APPLY, false, false>(x, b, f, count, st);
+    else product<APPLY, false, true>(b, x, f, count, st);
   }
   const float rate = g.lr * sqrtf(m > n ? (float)m / (float)n : 1.f);
-  muon_end_kernel<<<grid, 256, 0, st>>>(g, w.x, tall, 1.f - g.lr * g.weight_decay, rate);
-  LB_LAUNCH_CHECK();
+  launch_pdl(muon_end_kernel, wide, dim3(256), 0, st, true, g, w, vec, 1.f - g.lr * g.weight_decay, rate);
 }
 
 }  // namespace lb
