@@ -665,16 +665,16 @@ void tc_make_map_bf16(CUtensorMap *map, const void *base, unsigned long long row
 }
 
 void tc_make_map_heads(CUtensorMap *map, const void *base, const unsigned long long (&extent)[4],
-                       const unsigned long long (&stride_bytes)[3], unsigned box_rows) {
+                       const unsigned long long (&stride_bytes)[3], unsigned box_rows, unsigned box_cols) {
   EncodeTiledFn fn = encode_tiled_fn();
   if (fn == nullptr) throw std::runtime_error("litnice_b200: cuTensorMapEncodeTiled is not available");
   const cuuint64_t dims[4] = {extent[0], extent[1], extent[2], extent[3]};
   const cuuint64_t strides[3] = {stride_bytes[0], stride_bytes[1], stride_bytes[2]};
-  const cuuint32_t box[4] = {64, 1, box_rows, 1};
+  const cuuint32_t box[4] = {box_cols, 1, box_rows, 1};
   const cuuint32_t estr[4] = {1, 1, 1, 1};
   const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(base), dims, strides, box, estr,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, box_cols == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     throw std::runtime_error("litnice_b200: cuTensorMapEncodeTiled failed with code " + std::to_string((int)r));
 }

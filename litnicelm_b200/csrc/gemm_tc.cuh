@@ -113,9 +113,10 @@ void tc_make_map_plain(CUtensorMap *map, const float *base, unsigned long long r
 void tc_make_map_bf16(CUtensorMap *map, const void *base, unsigned long long rows, unsigned long long cols,
                       unsigned long long ld, unsigned box_rows);
 // bfloat16 elements [extent 3, 2, 1, 0] with contiguous innermost axis, byte strides of the outer three (multiples of 16) in
-// the order of extents 1, 2, 3; boxes of 64 elements by box_rows of extent 2, 128-byte swizzle.
+// the order of extents 1, 2, 3; boxes of 64 or 32 elements by box_rows of extent 2, swizzled over their rows' length. (Elements
+// of any 16-bit type: what lies outside reads as zero bits.)
 void tc_make_map_heads(CUtensorMap *map, const void *base, const unsigned long long (&extent)[4],
-                       const unsigned long long (&stride_bytes)[3], unsigned box_rows);
+                       const unsigned long long (&stride_bytes)[3], unsigned box_rows, unsigned box_cols = 64);
 void tc_make_store_map(CUtensorMap *map, void *base, bool half, unsigned long long rows, unsigned long long cols,
                        unsigned long long ld, unsigned box_cols);
 

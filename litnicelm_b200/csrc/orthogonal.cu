@@ -6,17 +6,21 @@
 //   params <- (1 - lr decay) params - lr sqrt(max(1, m / n)) X.
 // All matrices of a call have one shape and go through each product together.
 //
+// The polynomial as a square, b A + c A^2 + a = c (A + b / 2c)^2 + (a - b^2 / 4c): a step is three products without any added
+// matrix,  S = X X^T + b / 2c,  B = c S S + (a - b^2 / 4c),  X <- B X,  the constants on the diagonal; nothing cancels in B.
+//
 // Matrices live as pairs of fp16 values: z 2^e = hi + 2^-11 lo, 22 bits, with one exponent e per matrix, kind and step. It follows
 // from a bound on the singular values alone: those of X_k are at most min(1.25, rho a^k) where rho = |X_0| (the polynomial stays
-// below 1.21 on [0, 1.21] and below a s), so those of A at most its square and those of b A + c A^2 at most min(2.85, |b| of
-// that); no entry is larger, and e puts the bound at 2^13 to 2^14. A product is three: hi hi in one accumulator of tensor memory,
-// hi lo and lo hi in another; lo lo is below 2^-24 of a term and left out. The tensor pipe truncates when it adds, so chains in
-// tensor memory are 256 k long and are added in registers, rounded to nearest.
+// below 1.21 on [0, 1.21] and below a s), those of S at most 1.2, of B 3.45. No entry is larger, and e puts the bound at 2^13 to
+// 2^14. A product is three: hi hi in one accumulator of tensor memory, hi lo and lo hi in another; lo lo is below 2^-24 of a
+// term and left out. The tensor pipe truncates when it adds, so chains in tensor memory are NS_CHAIN blocks of 64 k long and are
+// added in registers, rounded to nearest.
 //
 // One persistent kernel for the three products of a step, tiles of 128 x 128: warp 0 issues TMA (stages of 64 k: four tiles of 16
 // KB), warp 1 owns tensor memory and issues the MMAs, eight warps add finished chains (a thread: a row and half of the columns) and
-// store. Nothing is transposed in memory: an operand whose rows run along k is read as it lies (M or N contiguous). A and b A +
-// c A^2 are symmetric: tiles below the diagonal are multiplied, and stored on both sides.
+// store through patches of shared memory that TMA carries out. Nothing is transposed in memory: an operand whose rows run along k
+// is read as it lies (M or N contiguous). S and B are symmetric: tiles up to the diagonal are multiplied, and stored on both
+// sides of it.
 // Every wait is bounded; one that runs out ends the CTA, whose results are then NaN. No clusters, no multicast.
 #include "train_ops.cuh"
 #include "gemm_tc.cuh"
@@ -28,9 +32,9 @@ namespace lb {
 
 namespace {
 
-constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f, NS_EPS = 1e-7f;
+constexpr float NS_C = 2.0315f, NS_EPS = 1e-7f;
 constexpr int NS_PARTS = 256;  // partial sums of a matrix's norm, at most
-constexpr int NS_THREADS = 320, NS_CHAIN = 4;
+constexpr int NS_THREADS = 320, NS_CHAIN = 1;
 
 struct Pair {
   __half *hi, *lo;  // [count][rows][ld]
@@ -39,29 +43,21 @@ struct Pair {
 struct NsWork {
   double *parts;   // [count][NS_PARTS]
   float *rho;      // [count]
-  Pair x[2], a, b;
+  Pair x[2], s, b;
   long long ldx, ldp;
 };
 
-// Exponents of the pairs of X, A and b A + c A^2 in step k.
-__device__ __forceinline__ int ns_exponent(float bound) {
-  if (!(bound > 0.f)) return 0;
-  const int e = 13 - ilogbf(bound);
-  return e < 100 ? e : 100;
-}
-__device__ __forceinline__ float ns_bound_x(float rho, int k) {
+constexpr float NS_SHIFT = (float)(-4.7750 / (2 * 2.0315)), NS_REST = (float)(3.4445 - 4.7750 * 4.7750 / (4 * 2.0315));
+constexpr int NS_EXP_S = 13, NS_EXP_B = 12;
+
+// The exponent of X_k's pair.
+__device__ __forceinline__ int ns_exp_x(float rho, int k) {
   float s = rho;
   for (int i = 0; i < k; ++i) s *= 3.45f;
-  return fminf(1.25f, s);
-}
-__device__ __forceinline__ int ns_exp_x(float rho, int k) { return ns_exponent(ns_bound_x(rho, k)); }
-__device__ __forceinline__ int ns_exp_a(float rho, int k) {
-  const float s = ns_bound_x(rho, k);
-  return ns_exponent(s * s);
-}
-__device__ __forceinline__ int ns_exp_b(float rho, int k) {
-  const float s = ns_bound_x(rho, k);
-  return ns_exponent(fminf(2.85f, 4.8f * s * s));
+  s = fminf(1.25f, s);
+  if (!(s > 0.f)) return 0;
+  const int e = 13 - ilogbf(s);
+  return e < 100 ? e : 100;
 }
 
 __device__ __forceinline__ void ns_split(float z, __half &hi, __half &lo) {  // z already scaled
@@ -199,12 +195,10 @@ __global__ void __launch_bounds__(256) muon_end_kernel(const __grid_constant__ M
 
 // ---- the products of a step -------------------------------------------------------------------------------------------------------
 
-// GRAM: A = X X^T or X^T X; POLY: B = b A + c A A; APPLY: X' = a X + B X or a X + X B
+// GRAM: S = X X^T + b / 2c (or X^T X); POLY: B = c S S + (a - b^2 / 4c); APPLY: X' = B X (or X B)
 enum NsOp { GRAM, POLY, APPLY };
 
 struct NsProduct {
-  Pair out, add;         // result; the matrix that is added (A for POLY, X for APPLY)
-  long long out_ld;
   int m, n, k;           // sizes of the product
   int m_tiles, n_tiles, tiles;  // tiles of all matrices
   int step;
@@ -214,8 +208,10 @@ struct NsProduct {
 template <bool A_MN, bool B_MN>
 struct NsSmem {
   static constexpr int STAGES = 3, TILE = 16384, STAGE = 4 * TILE;
-  static constexpr int BAR_OFF = STAGES * STAGE;
+  static constexpr int PATCH_OFF = STAGES * STAGE, PATCH = 4096;  // 32 x 32 elements of hi and of lo, per storing warp
+  static constexpr int BAR_OFF = PATCH_OFF + 8 * PATCH;
   static constexpr int TOTAL = BAR_OFF + 128 + 1024;
+  static_assert(TOTAL <= 227 * 1024, "");
 };
 
 constexpr unsigned UMMA_A_MN_MAJOR = 1u << 15;
@@ -224,6 +220,7 @@ template <NsOp OP, bool A_MN, bool B_MN>
 __global__ void __launch_bounds__(NS_THREADS, 1)
 ns_product_kernel(const __grid_constant__ CUtensorMap map_ah, const __grid_constant__ CUtensorMap map_al,
                   const __grid_constant__ CUtensorMap map_bh, const __grid_constant__ CUtensorMap map_bl,
+                  const __grid_constant__ CUtensorMap map_oh, const __grid_constant__ CUtensorMap map_ol,
                   const __grid_constant__ NsProduct g) {
   using L = NsSmem<A_MN, B_MN>;
   constexpr int S = L::STAGES;
@@ -359,6 +356,8 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_ah, const __grid_const
     }
   } else {
     const int q = warp & 3, half = (warp - 2) >> 2;
+    unsigned char *patch = base_ptr + L::PATCH_OFF + (warp - 2) * L::PATCH;
+    const unsigned patch_u = base + (unsigned)(L::PATCH_OFF + (warp - 2) * L::PATCH);
     int chain = 0;
     bool ok = true;
     for (int tile = blockIdx.x; tile < g.tiles; tile += gridDim.x) {
@@ -387,49 +386,67 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_ah, const __grid_const
       }
       int batch, mt, nt;
       place(tile, batch, mt, nt);
-      const float rho = g.rho[batch];
-      const int ex = ns_exp_x(rho, g.step), ea = ns_exp_a(rho, g.step), eb = ns_exp_b(rho, g.step);
-      // acc = the product times 2^(sum of the operands' exponents); out = (p add + q product) 2^(its exponent)
-      const int e_in = OP == GRAM ? 2 * ex : OP == POLY ? 2 * ea : eb + ex;
-      const int e_out = OP == GRAM ? ea : OP == POLY ? eb : ns_exp_x(rho, g.step + 1);
-      const int e_add = OP == POLY ? ea : ex;
-      const float f_add = OP == POLY ? NS_B : NS_A;
-      // exponents of up to 200 in two factors each
-      const float f_in = (OP == POLY ? NS_C : 1.f) * ns_pow2(-(e_in / 2)), f_in2 = ns_pow2(-(e_in - e_in / 2));
-      const float s_add = f_add * ns_pow2(-e_add), s_out = ns_pow2(e_out);
-      const int row = mt * 128 + q * 32 + lane;
-      const long long at = (long long)batch * g.m * g.out_ld + (long long)row * g.out_ld;
-      const bool mirror = SYM && mt != nt;
+      // acc = the product times 2^(sum of the operands' exponents), which may reach 200: two factors
+      const float rho = OP == POLY ? 0.f : g.rho[batch];
+      const int ex = OP == POLY ? 0 : ns_exp_x(rho, g.step);
+      const int e_in = OP == GRAM ? 2 * ex : OP == POLY ? 2 * NS_EXP_S : NS_EXP_B + ex;
+      const int e_out = OP == GRAM ? NS_EXP_S : OP == POLY ? NS_EXP_B : ns_exp_x(rho, g.step + 1);
+      const float f1 = (OP == POLY ? NS_C : 1.f) * ns_pow2(-(e_in / 2)), f2 = ns_pow2(e_out - (e_in - e_in / 2));
+      const float diagonal = (OP == GRAM ? NS_SHIFT : NS_REST) * ns_pow2(e_out);
+      const int row0 = mt * 128 + q * 32;
 #pragma unroll
-      for (int c0 = 0; c0 < 64; c0 += 8) {
+      for (int c0 = 0; c0 < 64; c0 += 32) {
         const int col = nt * 128 + half * 64 + c0;
-        if (col >= g.n) continue;
-        __half h[8], l[8];
-        if (OP != GRAM && row < g.m) {
-          *reinterpret_cast<uint4 *>(h) = *reinterpret_cast<const uint4 *>(g.add.hi + at + col);
-          *reinterpret_cast<uint4 *>(l) = *reinterpret_cast<const uint4 *>(g.add.lo + at + col);
-        }
+        if (col >= g.n || row0 >= g.m) continue;
+        unsigned h[16], l[16];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          float v = acc[c0 + j] * f_in * f_in2;
-          if (OP != GRAM) v = fmaf(ns_value(h[j], l[j]), s_add, v);
-          ns_split(ok ? v * s_out : NAN, h[j], l[j]);
-        }
-        if (row < g.m) {
-          *reinterpret_cast<uint4 *>(g.out.hi + at + col) = *reinterpret_cast<const uint4 *>(h);
-          *reinterpret_cast<uint4 *>(g.out.lo + at + col) = *reinterpret_cast<const uint4 *>(l);
-          if (mirror) {
-            const long long to = (long long)batch * g.m * g.out_ld + (long long)col * g.out_ld + row;
+        for (int j = 0; j < 32; j += 2) {
+          __half2 hh, ll;
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              if (col + j < g.n) {
-                g.out.hi[to + j * g.out_ld] = h[j];
-                g.out.lo[to + j * g.out_ld] = l[j];
-              }
+          for (int e = 0; e < 2; ++e) {
+            float v = acc[c0 + j + e] * f1 * f2;
+            if (SYM && row0 + lane == col + j + e) v += diagonal;
+            if (!ok) v = NAN;
+            __half x, y;
+            ns_split(v, x, y);
+            if (e) hh.y = x, ll.y = y;
+            else hh.x = x, ll.x = y;
           }
+          h[j >> 1] = *reinterpret_cast<const unsigned *>(&hh);
+          l[j >> 1] = *reinterpret_cast<const unsigned *>(&ll);
+        }
+        if (lane == 0) bulk_wait_read<0>();
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int to = lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4);
+          *reinterpret_cast<uint4 *>(patch + to) = make_uint4(h[4 * j], h[4 * j + 1], h[4 * j + 2], h[4 * j + 3]);
+          *reinterpret_cast<uint4 *>(patch + 2048 + to) = make_uint4(l[4 * j], l[4 * j + 1], l[4 * j + 2], l[4 * j + 3]);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_4d(&map_oh, patch_u, col, 0, row0, batch);
+          tma_store_4d(&map_ol, patch_u + 2048, col, 0, row0, batch);
+        }
+        if (!SYM || mt == nt) continue;
+        if (lane == 0) bulk_wait_read<0>();
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {  // the same turned: row j is column col + j
+          const int to = j * 64 + (((lane >> 3) ^ ((j >> 1) & 3)) << 4) + (lane & 7) * 2;
+          *reinterpret_cast<unsigned short *>(patch + to) = (unsigned short)(h[j >> 1] >> (16 * (j & 1)));
+          *reinterpret_cast<unsigned short *>(patch + 2048 + to) = (unsigned short)(l[j >> 1] >> (16 * (j & 1)));
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_4d(&map_oh, patch_u, row0, 0, col, batch);
+          tma_store_4d(&map_ol, patch_u + 2048, row0, 0, col, batch);
         }
       }
     }
+    if (lane == 0) bulk_wait_all();  // the stores are part of the grid's results
   }
   __syncwarp();
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -445,16 +462,24 @@ struct Operand {
   long long rows, cols, ld;
 };
 
-CUtensorMap ns_map(const __half *p, const Operand &o, long long count, bool mn) {
+CUtensorMap ns_map(const __half *p, const Operand &o, long long count, bool mn, bool result = false) {
   CUtensorMap map;
   const unsigned long long extent[4] = {(unsigned long long)o.cols, 1, (unsigned long long)o.rows, (unsigned long long)count};
   const unsigned long long strides[3] = {16, (unsigned long long)o.ld * 2, (unsigned long long)(o.rows * o.ld) * 2};
-  tc_make_map_heads(&map, p, extent, strides, mn ? 64 : 128);
+  if (result) tc_make_map_heads(&map, p, extent, strides, 32, 32);
+  else tc_make_map_heads(&map, p, extent, strides, mn ? 64 : 128);
   return map;
 }
 
 template <NsOp OP, bool A_MN, bool B_MN>
-void product(const Operand &a, const Operand &b, NsProduct g, long long count, cudaStream_t st) {
+void product(const Operand &a, const Operand &b, const Operand &out, int k, int step, const float *rho, long long count,
+             cudaStream_t st) {
+  NsProduct g{};
+  g.m = (int)out.rows;
+  g.n = (int)out.cols;
+  g.k = k;
+  g.step = step;
+  g.rho = rho;
   g.m_tiles = (g.m + 127) / 128;
   g.n_tiles = (g.n + 127) / 128;
   const long long per = OP == APPLY ? (long long)g.m_tiles * g.n_tiles : (long long)g.m_tiles * (g.m_tiles + 1) / 2;
@@ -464,7 +489,7 @@ void product(const Operand &a, const Operand &b, NsProduct g, long long count, c
   LB_CUDA(cudaFuncSetAttribute(ns_product_kernel<OP, A_MN, B_MN>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL));
   launch_pdl(ns_product_kernel<OP, A_MN, B_MN>, dim3((unsigned)(g.tiles < 148 ? g.tiles : 148)), dim3(NS_THREADS), L::TOTAL, st, true,
              ns_map(a.p.hi, a, count, A_MN), ns_map(a.p.lo, a, count, A_MN), ns_map(b.p.hi, b, count, B_MN),
-             ns_map(b.p.lo, b, count, B_MN), g);
+             ns_map(b.p.lo, b, count, B_MN), ns_map(out.p.hi, out, count, false, true), ns_map(out.p.lo, out, count, false, true), g);
 }
 
 bool rows16(const MatView &v) {
@@ -495,7 +520,7 @@ size_t ns_layout(long long count, long long m, long long n, char *p, NsWork *w) 
     x->hi = reinterpret_cast<__half *>(take((size_t)count * m * ldx * 2));
     x->lo = reinterpret_cast<__half *>(take((size_t)count * m * ldx * 2));
   }
-  for (Pair *x : {&k.a, &k.b}) {
+  for (Pair *x : {&k.s, &k.b}) {
     x->hi = reinterpret_cast<__half *>(take((size_t)count * small * ldp * 2));
     x->lo = reinterpret_cast<__half *>(take((size_t)count * small * ldp * 2));
   }
@@ -520,27 +545,12 @@ void launch_muon(const MuonStep &g, void *workspace, cudaStream_t st) {
   launch_pdl(muon_begin_kernel, grid, dim3(256), 0, st, true, g, w, vec);
   launch_pdl(muon_pair_kernel, wide, dim3(256), 0, st, true, g, w, vec, (int)parts);
   for (int i = 0; i < g.steps; ++i) {
-    const Operand x{w.x[i & 1], m, n, w.ldx}, a{w.a, p, p, w.ldp}, b{w.b, p, p, w.ldp};
-    NsProduct f{};
-    f.step = i;
-    f.rho = w.rho;
-    f.out = w.a;
-    f.out_ld = w.ldp;
-    f.m = f.n = p;
-    f.k = (int)(tall ? m : n);
-    if (tall) product<GRAM, true, true>(x, x, f, count, st);
-    else product<GRAM, false, false>(x, x, f, count, st);
-    f.out = w.b;
-    f.add = w.a;
-    f.k = p;
-    product<POLY, false, false>(a, a, f, count, st);
-    f.out = w.x[(i + 1) & 1];
-    f.add = w.x[i & 1];
-    f.out_ld = w.ldx;
-    f.m = (int)m;
-    f.n = (int)n;
-    if (tall) product<APPLY, false, false>(x, b, f, count, st);
-    else product<APPLY, false, true>(b, x, f, count, st);
+    const Operand x{w.x[i & 1], m, n, w.ldx}, y{w.x[(i + 1) & 1], m, n, w.ldx}, a{w.s, p, p, w.ldp}, b{w.b, p, p, w.ldp};
+    if (tall) product<GRAM, true, true>(x, x, a, (int)m, i, w.rho, count, st);
+    else product<GRAM, false, false>(x, x, a, (int)n, i, w.rho, count, st);
+    product<POLY, false, false>(a, a, b, p, i, w.rho, count, st);
+    if (tall) product<APPLY, false, false>(x, b, y, p, i, w.rho, count, st);
+    else product<APPLY, false, true>(b, x, y, p, i, w.rho, count, st);
   }
   const float rate = g.lr * sqrtf(m > n ? (float)m / (float)n : 1.f);
   launch_pdl(muon_end_kernel, wide, dim3(256), 0, st, true, g, w, vec, 1.f - g.lr * g.weight_decay, rate);

@@ -115,6 +115,12 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap *map, unsigned sr
                : "memory");
   asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap *map, unsigned src, int x, int y, int z, int w) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3, %4}], [%5];"
+               ::"l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(src)
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
 __device__ __forceinline__ void tma_add_2d(const CUtensorMap *map, unsigned src, int x, int y) {
   asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%1, %2}], [%3];"
                ::"l"(map), "r"(x), "r"(y), "r"(src)
