@@ -6,20 +6,21 @@
 //   params <- (1 - lr decay) params - lr sqrt(max(1, m / n)) X.
 // All matrices of a call have one shape and go through each product together.
 //
-// The polynomial as a square, b A + c A^2 + a = c (A + b / 2c)^2 + (a - b^2 / 4c): a step is three products without any added
-// matrix,  S = X X^T + b / 2c,  B = c S S + (a - b^2 / 4c),  X <- B X,  the constants on the diagonal; nothing cancels in B.
+// A step is three products: A = X X^T, B = b A + c A A, X <- a X + B X. The matrix that is added is the first term of the sum that a
+// thread keeps in registers, so nothing of it is lost to the tensor pipe's truncation (with a on B's diagonal instead the result
+// of two steps was 13 times as far from 64 bits as by 32-bit products; so 2).
 //
 // Matrices live as pairs of fp16 values: z 2^e = hi + 2^-11 lo, 22 bits, with one exponent e per matrix, kind and step. It follows
 // from a bound on the singular values alone: those of X_k are at most min(1.25, rho a^k) where rho = |X_0| (the polynomial stays
-// below 1.21 on [0, 1.21] and below a s), those of S at most 1.2, of B 3.45. No entry is larger, and e puts the bound at 2^13 to
-// 2^14. A product is three: hi hi in one accumulator of tensor memory, hi lo and lo hi in another; lo lo is below 2^-24 of a
-// term and left out. The tensor pipe truncates when it adds, so chains in tensor memory are NS_CHAIN blocks of 64 k long and are
-// added in registers, rounded to nearest.
+// below 1.21 on [0, 1.21] and below a s), those of A at most its square, of B min(2.85, |b| of that). No entry is larger, and e puts
+// the bound at 2^13 to 2^14. A product is three: hi hi in one accumulator of tensor memory, hi lo and lo hi in another; lo lo is below 2^-24 of a
+// term and left out. The tensor pipe truncates when it adds, so chains in tensor memory are 64 k long and are added in
+// registers, rounded to nearest.
 //
 // One persistent kernel for the three products of a step, tiles of 128 x 128: warp 0 issues TMA (stages of 64 k: four tiles of 16
 // KB), warp 1 owns tensor memory and issues the MMAs, eight warps add finished chains (a thread: a row and half of the columns) and
 // store through patches of shared memory that TMA carries out. Nothing is transposed in memory: an operand whose rows run along k
-// is read as it lies (M or N contiguous). S and B are symmetric: tiles up to the diagonal are multiplied, and stored on both
+// is read as it lies (M or N contiguous). A and B are symmetric: tiles up to the diagonal are multiplied, and stored on both
 // sides of it.
 // Every wait is bounded; one that runs out ends the CTA, whose results are then NaN. No clusters, no multicast.
 #include "train_ops.cuh"
@@ -32,9 +33,10 @@ namespace lb {
 
 namespace {
 
-constexpr float NS_C = 2.0315f, NS_EPS = 1e-7f;
+constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f, NS_EPS = 1e-7f;
 constexpr int NS_PARTS = 256;  // partial sums of a matrix's norm, at most
-constexpr int NS_THREADS = 320, NS_CHAIN = 1;
+constexpr int NS_THREADS = 320;
+constexpr double NS_PAIR_COST = 1.4;
 
 struct Pair {
   __half *hi, *lo;  // [count][rows][ld]
@@ -43,21 +45,28 @@ struct Pair {
 struct NsWork {
   double *parts;   // [count][NS_PARTS]
   float *rho;      // [count]
-  Pair x[2], s, b;
+  Pair x[2], a, b;
   long long ldx, ldp;
 };
 
-constexpr float NS_SHIFT = (float)(-4.7750 / (2 * 2.0315)), NS_REST = (float)(3.4445 - 4.7750 * 4.7750 / (4 * 2.0315));
-constexpr int NS_EXP_S = 13, NS_EXP_B = 12;
-
-// The exponent of X_k's pair.
-__device__ __forceinline__ int ns_exp_x(float rho, int k) {
-  float s = rho;
-  for (int i = 0; i < k; ++i) s *= 3.45f;
-  s = fminf(1.25f, s);
-  if (!(s > 0.f)) return 0;
-  const int e = 13 - ilogbf(s);
+// Exponents of the pairs of X, A and B in step k.
+__device__ __forceinline__ int ns_exponent(float bound) {
+  if (!(bound > 0.f)) return 0;
+  const int e = 13 - ilogbf(bound);
   return e < 100 ? e : 100;
+}
+__device__ __forceinline__ float ns_bound(float rho, int k) {
+  for (int i = 0; i < k; ++i) rho *= 3.45f;
+  return fminf(1.25f, rho);
+}
+__device__ __forceinline__ int ns_exp_x(float rho, int k) { return ns_exponent(ns_bound(rho, k)); }
+__device__ __forceinline__ int ns_exp_a(float rho, int k) {
+  const float s = ns_bound(rho, k);
+  return ns_exponent(s * s);
+}
+__device__ __forceinline__ int ns_exp_b(float rho, int k) {
+  const float s = ns_bound(rho, k);
+  return ns_exponent(fminf(2.85f, 4.8f * s * s));
 }
 
 __device__ __forceinline__ void ns_split(float z, __half &hi, __half &lo) {  // z already scaled
@@ -195,17 +204,19 @@ __global__ void __launch_bounds__(256) muon_end_kernel(const __grid_constant__ M
 
 // ---- the products of a step -------------------------------------------------------------------------------------------------------
 
-// GRAM: S = X X^T + b / 2c (or X^T X); POLY: B = c S S + (a - b^2 / 4c); APPLY: X' = B X (or X B)
+// GRAM: A = X X^T or X^T X; POLY: B = b A + c A A; APPLY: X' = a X + B X or a X + X B
 enum NsOp { GRAM, POLY, APPLY };
 
 struct NsProduct {
+  Pair add;              // A for POLY, X for APPLY
+  long long ld;          // of it and of the result
   int m, n, k;           // sizes of the product
   int m_tiles, n_tiles, tiles;  // tiles of all matrices
   int step;
   const float *rho;
 };
 
-template <bool A_MN, bool B_MN>
+template <bool PAIR>
 struct NsSmem {
   static constexpr int STAGES = 3, TILE = 16384, STAGE = 4 * TILE;
   static constexpr int PATCH_OFF = STAGES * STAGE, PATCH = 4096;  // 32 x 32 elements of hi and of lo, per storing warp
@@ -216,15 +227,48 @@ struct NsSmem {
 
 constexpr unsigned UMMA_A_MN_MAJOR = 1u << 15;
 
-template <NsOp OP, bool A_MN, bool B_MN>
+// Instructions of a pair of CTAs: the even one's thread issues them for both, operands at the same places of both shared memories
+// (of the right operand each CTA holds half of the rows), rows 128 .. 255 of the result in the odd one's tensor memory.
+template <bool PAIR>
+__device__ __forceinline__ void ns_load(unsigned to, const CUtensorMap *map, int x, int z, int w, unsigned bar) {
+  if constexpr (PAIR)
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4, %5}], "
+        "[%6];" ::"r"(to), "l"(map), "r"(x), "r"(0), "r"(z), "r"(w), "r"(bar)
+        : "memory");
+  else tma_load_4d(to, map, x, 0, z, w, bar);
+}
+template <bool PAIR>
+__device__ __forceinline__ void ns_mma(unsigned d, unsigned long long a, unsigned long long b, unsigned idesc, unsigned more) {
+  if constexpr (PAIR)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(more)
+        : "memory");
+  else tc_mma_f16(d, a, b, idesc, more);
+}
+template <bool PAIR>
+__device__ __forceinline__ void ns_commit(unsigned bar) {  // of a pair: the barrier at this place in both CTAs
+  if constexpr (PAIR)
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                 ::"r"(bar), "h"((unsigned short)3)
+                 : "memory");
+  else tc_commit(bar);
+}
+
+template <NsOp OP, bool A_MN, bool B_MN, bool PAIR>
 __global__ void __launch_bounds__(NS_THREADS, 1)
 ns_product_kernel(const __grid_constant__ CUtensorMap map_ah, const __grid_constant__ CUtensorMap map_al,
                   const __grid_constant__ CUtensorMap map_bh, const __grid_constant__ CUtensorMap map_bl,
                   const __grid_constant__ CUtensorMap map_oh, const __grid_constant__ CUtensorMap map_ol,
                   const __grid_constant__ NsProduct g) {
-  using L = NsSmem<A_MN, B_MN>;
-  constexpr int S = L::STAGES;
+  using L = NsSmem<PAIR>;
+  constexpr int S = L::STAGES, CTAS = PAIR ? 2 : 1, T = 128 * CTAS;  // tiles of T x T by CTAS CTAs, each 128 rows in HALVES pieces
+  constexpr int HALVES = CTAS;
   constexpr bool SYM = OP != APPLY;
+  const int rank = PAIR ? (int)blockIdx.x & 1 : 0, cta = (int)blockIdx.x / CTAS, ctas = (int)gridDim.x / CTAS;
   extern __shared__ unsigned char smem_raw[];
   const unsigned base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char *base_ptr = smem_raw + (base - smem_u32(smem_raw));
@@ -237,7 +281,7 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_ah, const __grid_const
   volatile unsigned *tmem_holder = reinterpret_cast<volatile unsigned *>(base_ptr + L::BAR_OFF + 96);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(base_ptr + L::BAR_OFF + 100);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int kblocks = (g.k + 63) / 64, chains = (kblocks + NS_CHAIN - 1) / NS_CHAIN;
+  const int kblocks = (g.k + 63) / 64;
   auto place = [&](int tile, int &batch, int &mt, int &nt) {
     const int per = SYM ? g.m_tiles * (g.m_tiles + 1) / 2 : g.m_tiles * g.n_tiles;
     batch = tile / per;
@@ -260,21 +304,31 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_ah, const __grid_const
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(chain_full(b), 1);
-      mbar_init(chain_empty(b), 8);
+      mbar_init(chain_empty(b), 8 * CTAS);
     }
     mbar_init(done, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
+  if (warp == 0 && lane == 0)
+    for (const CUtensorMap *map : {&map_ah, &map_al, &map_bh, &map_bl, &map_oh, &map_ol}) tma_prefetch_map(map);
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void *)tmem_holder)),
-                 "r"(512u)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    if constexpr (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void *)tmem_holder)),
+                   "r"(512u)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void *)tmem_holder)),
+                   "r"(512u)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
+  if constexpr (PAIR) cluster_sync_all();  // both CTAs' barriers are there
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const unsigned tmem = *tmem_holder;
   pdl_launch_dependents();  // behind the allocation: a dependent's CTA must not take tensor memory first
@@ -283,7 +337,7 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_ah, const __grid_const
   if (warp == 0) {
     int it = 0;
     bool ok = true;
-    for (int tile = blockIdx.x; tile < g.tiles && ok; tile += gridDim.x) {
+    for (int tile = cta; tile < g.tiles && ok; tile += ctas) {
       int batch, mt, nt;
       place(tile, batch, mt, nt);
       for (int kb = 0; kb < kblocks; ++kb, ++it) {
@@ -291,65 +345,74 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_ah, const __grid_const
         ok = mbar_wait_warp(empty(s), ((unsigned)(it / S) & 1u) ^ 1u, abort_flag, nullptr, 61);
         if (!ok) break;
         if (lane == 0) {
-          const unsigned st = base + (unsigned)(s * L::STAGE), bar = full(s);
-          mbar_expect_tx(bar, (unsigned)L::STAGE);
-          auto load = [&](unsigned to, const CUtensorMap *map, bool mn, int at) {
+          const unsigned st = base + (unsigned)(s * L::STAGE);
+          // (of a pair, the even one's barrier counts both CTAs' bytes)
+          if (rank == 0) mbar_expect_tx(full(s), (unsigned)(CTAS * L::STAGE));
+          const unsigned bar = PAIR ? cluster_map(full(s), 0) : full(s);
+          auto load = [&](unsigned to, const CUtensorMap *map, bool mn, int r0, int r1) {  // 64 rows from r0 on, and from r1 on
             if (mn) {  // rows of k, two slabs of 64 columns
-              tma_load_4d(to, map, at * 128, 0, kb * 64, batch, bar);
-              tma_load_4d(to + 8192, map, at * 128 + 64, 0, kb * 64, batch, bar);
+              ns_load<PAIR>(to, map, r0, kb * 64, batch, bar);
+              ns_load<PAIR>(to + 8192, map, r1, kb * 64, batch, bar);
             } else {
-              tma_load_4d(to, map, kb * 64, 0, at * 128, batch, bar);
+              ns_load<PAIR>(to, map, kb * 64, r0, batch, bar);
+              ns_load<PAIR>(to + 8192, map, kb * 64, r1, batch, bar);
             }
           };
-          load(st, &map_ah, A_MN, mt);
-          load(st + L::TILE, &map_al, A_MN, mt);
-          load(st + 2 * L::TILE, &map_bh, B_MN, nt);
-          load(st + 3 * L::TILE, &map_bl, B_MN, nt);
+          const int m0 = mt * T + rank * 128, n0 = nt * T + rank * 64, n1 = PAIR ? n0 + 128 : n0 + 64;
+          load(st, &map_ah, A_MN, m0, m0 + 64);
+          load(st + L::TILE, &map_al, A_MN, m0, m0 + 64);
+          load(st + 2 * L::TILE, &map_bh, B_MN, n0, n1);
+          load(st + 3 * L::TILE, &map_bl, B_MN, n0, n1);
         }
         __syncwarp();
       }
     }
-    if (*abort_flag) {  // copies in flight must land before the shared memory goes away
+    if (PAIR && *abort_flag) {  // copies in flight must land (only the even CTA's barriers know: a millisecond is ample)
+      const unsigned long long limit = global_timer() + 1000000ull;
+      while (global_timer() < limit) {}
+    } else if (*abort_flag) {  // copies in flight must land before the shared memory goes away
       const unsigned long long limit = global_timer() + WAIT_LIMIT_NS;
       for (int j = it > S ? it - S : 0; j < it; ++j)
         while (!mbar_try_wait(full(j % S), (unsigned)(j / S) & 1u) && global_timer() < limit) {}
     }
   } else if (warp == 1) {
-    constexpr unsigned idesc = umma_idesc_f16(128) | (A_MN ? UMMA_A_MN_MAJOR : 0u) | (B_MN ? UMMA_B_MN_MAJOR : 0u);
+    constexpr unsigned idesc = (umma_idesc_f16(128) + (PAIR ? (unsigned)(TC_BM >> 4) << 24 : 0u)) |
+                               (A_MN ? UMMA_A_MN_MAJOR : 0u) | (B_MN ? UMMA_B_MN_MAJOR : 0u);
     int it = 0, chain = 0;
     bool ok = true;
-    for (int tile = blockIdx.x; tile < g.tiles && ok; tile += gridDim.x) {
-      for (int kb = 0; kb < kblocks; ++kb, ++it) {
-        const int s = it % S, buf = chain & 1;
-        if (kb % NS_CHAIN == 0)
-          ok = mbar_wait_warp(chain_empty(buf), ((unsigned)(chain >> 1) & 1u) ^ 1u, abort_flag, nullptr, 62);
-        if (ok) ok = mbar_wait_warp(full(s), (unsigned)(it / S) & 1u, abort_flag, nullptr, 63);
-        if (!ok) break;
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const bool last = kb + 1 == kblocks || (kb + 1) % NS_CHAIN == 0;
-        if (lane == 0) {
-          const unsigned st = base + (unsigned)(s * L::STAGE), d = tmem + (unsigned)(buf * 256);
-          auto desc = [&](int t, bool mn, int ks) {
-            const unsigned p = st + (unsigned)(t * L::TILE);
-            return mn ? umma_desc_mn128(p + (unsigned)(ks * 2048), 8192u) : umma_desc_k128(p) + (unsigned long long)(ks * 2);
-          };
+    for (int tile = rank == 0 ? cta : g.tiles; tile < g.tiles && ok; tile += ctas) {
+      for (int kb = 0; kb < kblocks && ok; ++kb, ++it) {
+        const int s = it % S;
+        ok = mbar_wait_warp(full(s), (unsigned)(it / S) & 1u, abort_flag, nullptr, 63);
 #pragma unroll
-          for (int ks = 0; ks < 4; ++ks) {
-            const unsigned more = (kb % NS_CHAIN) | ks ? 1u : 0u;
-            const unsigned long long ah = desc(0, A_MN, ks), al = desc(1, A_MN, ks), bh = desc(2, B_MN, ks), bl = desc(3, B_MN, ks);
-            tc_mma_f16(d, ah, bh, idesc, more);
-            tc_mma_f16(d + 128, ah, bl, idesc, more);
-            tc_mma_f16(d + 128, al, bh, idesc, 1u);
+        for (int h = 0; h < HALVES; ++h, ++chain) {
+          const int buf = chain & 1;
+          if (ok) ok = mbar_wait_warp(chain_empty(buf), ((unsigned)(chain >> 1) & 1u) ^ 1u, abort_flag, nullptr, 62);
+          if (!ok) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          if (lane == 0) {
+            const unsigned st = base + (unsigned)(s * L::STAGE), d = tmem + (unsigned)(buf * 256);
+            auto desc = [&](int t, bool mn, int ks) {
+              const unsigned p = st + (unsigned)(t * L::TILE + (t >= 2 ? h * 8192 : 0));
+              return mn ? umma_desc_mn128(p + (unsigned)(ks * 2048), 8192u) : umma_desc_k128(p) + (unsigned long long)(ks * 2);
+            };
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) {
+              const unsigned more = ks ? 1u : 0u;
+              const unsigned long long ah = desc(0, A_MN, ks), al = desc(1, A_MN, ks), bh = desc(2, B_MN, ks), bl = desc(3, B_MN, ks);
+              ns_mma<PAIR>(d, ah, bh, idesc, more);
+              ns_mma<PAIR>(d + 128, ah, bl, idesc, more);
+              ns_mma<PAIR>(d + 128, al, bh, idesc, 1u);
+            }
+            if (h == HALVES - 1) ns_commit<PAIR>(empty(s));
+            ns_commit<PAIR>(chain_full(buf));
           }
-          tc_commit(empty(s));
-          if (last) tc_commit(chain_full(buf));
+          __syncwarp();
         }
-        __syncwarp();
-        if (last) ++chain;
       }
     }
     if (!ok) {  // what was issued ends, within the limit, before the shared memory goes away
-      if (lane == 0) tc_commit(done);
+      if (lane == 0) ns_commit<PAIR>(done);
       __syncwarp();
       const unsigned long long limit = global_timer() + WAIT_LIMIT_NS;
       while (!mbar_try_wait(done, 0u) && global_timer() < limit) {}
@@ -360,43 +423,100 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_ah, const __grid_const
     const unsigned patch_u = base + (unsigned)(L::PATCH_OFF + (warp - 2) * L::PATCH);
     int chain = 0;
     bool ok = true;
-    for (int tile = blockIdx.x; tile < g.tiles; tile += gridDim.x) {
-      float acc[64];
-#pragma unroll
-      for (int j = 0; j < 64; ++j) acc[j] = 0.f;
-      for (int c = 0; c < chains && ok; ++c, ++chain) {
-        const int buf = chain & 1;
-        ok = mbar_wait_warp(chain_full(buf), (unsigned)(chain >> 1) & 1u, abort_flag, nullptr, 64);
-        if (!ok) break;
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll
-        for (int c0 = 0; c0 < 64; c0 += 32) {
-          unsigned r[32], t[32];
-          const unsigned at = tmem + ((unsigned)(q * 32) << 16) + (unsigned)(buf * 256 + half * 64 + c0);
-          tc_ld32(at, r);
-          tc_ld32(at + 128, t);
-          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            acc[c0 + j] += fmaf(__uint_as_float(t[j]), 1.f / 2048.f, __uint_as_float(r[j]));
-        }
-        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(chain_empty(buf));
-      }
+    for (int tile = cta; tile < g.tiles; tile += ctas) {
       int batch, mt, nt;
       place(tile, batch, mt, nt);
+      const float rho = g.rho[batch];
       // acc = the product times 2^(sum of the operands' exponents), which may reach 200: two factors
-      const float rho = OP == POLY ? 0.f : g.rho[batch];
-      const int ex = OP == POLY ? 0 : ns_exp_x(rho, g.step);
-      const int e_in = OP == GRAM ? 2 * ex : OP == POLY ? 2 * NS_EXP_S : NS_EXP_B + ex;
-      const int e_out = OP == GRAM ? NS_EXP_S : OP == POLY ? NS_EXP_B : ns_exp_x(rho, g.step + 1);
+      const int ex = ns_exp_x(rho, g.step), ea = ns_exp_a(rho, g.step), eb = ns_exp_b(rho, g.step);
+      const int e_in = OP == GRAM ? 2 * ex : OP == POLY ? 2 * ea : eb + ex;
+      const int e_out = OP == GRAM ? ea : OP == POLY ? eb : ns_exp_x(rho, g.step + 1);
       const float f1 = (OP == POLY ? NS_C : 1.f) * ns_pow2(-(e_in / 2)), f2 = ns_pow2(e_out - (e_in - e_in / 2));
-      const float diagonal = (OP == GRAM ? NS_SHIFT : NS_REST) * ns_pow2(e_out);
-      const int row0 = mt * 128 + q * 32;
+      const int row0 = mt * T + rank * 128 + q * 32;
+      float acc[HALVES][64];
 #pragma unroll
-      for (int c0 = 0; c0 < 64; c0 += 32) {
-        const int col = nt * 128 + half * 64 + c0;
+      for (int h = 0; h < HALVES; ++h)
+#pragma unroll
+        for (int j = 0; j < 64; ++j) acc[h][j] = 0.f;
+      if (OP != GRAM) {  // whole rows' 128 bytes at a time through the patch
+        const float f_add = OP == POLY ? NS_B / NS_C * ns_pow2(ea) : NS_A * ns_pow2(eb);
+        if (lane == 0) bulk_wait_read<0>();
+        __syncwarp();
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h) {
+          const int col0 = nt * T + h * 128 + half * 64;
+          if (row0 >= g.m || col0 >= g.n) continue;
+#pragma unroll
+          for (int lo = 0; lo < 2; ++lo) {
+            const __half *from = (lo ? g.add.lo : g.add.hi) + ((long long)batch * g.m + row0) * g.ld + col0 + (lane & 7) * 8;
+            const bool in = col0 + (lane & 7) * 8 < g.n;
+            uint4 u[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int r = i * 4 + (lane >> 3);
+              u[i] = in && row0 + r < g.m ? *reinterpret_cast<const uint4 *>(from + r * g.ld) : make_uint4(0u, 0u, 0u, 0u);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int r = i * 4 + (lane >> 3);
+              *reinterpret_cast<uint4 *>(patch + r * 128 + (((lane & 7) ^ (r & 7)) << 4)) = u[i];
+            }
+            __syncwarp();
+            const float f = lo ? f_add / 2048.f : f_add;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const uint4 v = *reinterpret_cast<const uint4 *>(patch + lane * 128 + ((i ^ (lane & 7)) << 4));
+              const __half2 *z = reinterpret_cast<const __half2 *>(&v);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const float2 w = __half22float2(z[j]);
+                acc[h][i * 8 + 2 * j] = fmaf(w.x, f, acc[h][i * 8 + 2 * j]);
+                acc[h][i * 8 + 2 * j + 1] = fmaf(w.y, f, acc[h][i * 8 + 2 * j + 1]);
+              }
+            }
+            __syncwarp();
+          }
+        }
+      }
+      for (int kb = 0; kb < kblocks && ok; ++kb) {
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h, ++chain) {
+          const int buf = chain & 1;
+          if (ok) ok = mbar_wait_warp(chain_full(buf), (unsigned)(chain >> 1) & 1u, abort_flag, nullptr, 64);
+          if (!ok) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          constexpr int C = PAIR ? 16 : 32;  // columns at a time: registers
+#pragma unroll
+          for (int c0 = 0; c0 < 64; c0 += C) {
+            unsigned r[C], t[C];
+            const unsigned at = tmem + ((unsigned)(q * 32) << 16) + (unsigned)(buf * 256 + half * 64 + c0);
+            if constexpr (PAIR) {
+              tc_ld16(at, r);
+              tc_ld16(at + 128, t);
+            } else {
+              tc_ld32(at, r);
+              tc_ld32(at + 128, t);
+            }
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+            for (int j = 0; j < C; ++j)
+              acc[h][c0 + j] += fmaf(__uint_as_float(t[j]), 1.f / 2048.f, __uint_as_float(r[j]));
+          }
+          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) {
+            if constexpr (PAIR)
+              asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_map(chain_empty(buf), 0))
+                           : "memory");
+            else mbar_arrive(chain_empty(buf));
+          }
+        }
+      }
+#pragma unroll
+      for (int piece = 0; piece < 2 * HALVES; ++piece) {
+        const int c0 = piece * 32 % 64;
+        const float(&part)[64] = acc[piece / 2];
+        const int col = nt * T + piece / 2 * 128 + half * 64 + c0;
         if (col >= g.n || row0 >= g.m) continue;
         unsigned h[16], l[16];
 #pragma unroll
@@ -404,8 +524,7 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_ah, const __grid_const
           __half2 hh, ll;
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float v = acc[c0 + j + e] * f1 * f2;
-            if (SYM && row0 + lane == col + j + e) v += diagonal;
+            float v = part[c0 + j + e] * f1 * f2;
             if (!ok) v = NAN;
             __half x, y;
             ns_split(v, x, y);
@@ -451,9 +570,11 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_ah, const __grid_const
   __syncwarp();
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
+  if constexpr (PAIR) cluster_sync_all();  // nothing of the pair's is on its way to the other CTA
   if (warp == 1) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+    if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
   }
 }
 
@@ -462,34 +583,48 @@ struct Operand {
   long long rows, cols, ld;
 };
 
-CUtensorMap ns_map(const __half *p, const Operand &o, long long count, bool mn, bool result = false) {
+CUtensorMap ns_map(const __half *p, const Operand &o, long long count, bool result = false) {
   CUtensorMap map;
   const unsigned long long extent[4] = {(unsigned long long)o.cols, 1, (unsigned long long)o.rows, (unsigned long long)count};
   const unsigned long long strides[3] = {16, (unsigned long long)o.ld * 2, (unsigned long long)(o.rows * o.ld) * 2};
   if (result) tc_make_map_heads(&map, p, extent, strides, 32, 32);
-  else tc_make_map_heads(&map, p, extent, strides, mn ? 64 : 128);
+  else tc_make_map_heads(&map, p, extent, strides, 64);
   return map;
 }
 
+template <NsOp OP, bool A_MN, bool B_MN, bool PAIR>
+void launch_product(const Operand &a, const Operand &b, const Operand &out, NsProduct g, long long count, cudaStream_t st) {
+  constexpr int CTAS = PAIR ? 2 : 1, T = 128 * CTAS;
+  g.m_tiles = (g.m + T - 1) / T;
+  g.n_tiles = (g.n + T - 1) / T;
+  const long long per = OP == APPLY ? (long long)g.m_tiles * g.n_tiles : (long long)g.m_tiles * (g.m_tiles + 1) / 2;
+  if (per * count > 0x3fffffffLL) throw std::invalid_argument("too many matrices of this size for one call");
+  g.tiles = (int)(per * count);
+  using L = NsSmem<PAIR>;
+  LB_CUDA(cudaFuncSetAttribute(ns_product_kernel<OP, A_MN, B_MN, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL));
+  const int ctas = g.tiles < 148 / CTAS ? g.tiles : 148 / CTAS;
+  launch_pdl_cluster_x(ns_product_kernel<OP, A_MN, B_MN, PAIR>, dim3((unsigned)(ctas * CTAS)), dim3(NS_THREADS), L::TOTAL, st, true,
+                       (unsigned)CTAS, ns_map(a.p.hi, a, count), ns_map(a.p.lo, a, count), ns_map(b.p.hi, b, count),
+                       ns_map(b.p.lo, b, count), ns_map(out.p.hi, out, count, true), ns_map(out.p.lo, out, count, true), g);
+}
+
 template <NsOp OP, bool A_MN, bool B_MN>
-void product(const Operand &a, const Operand &b, const Operand &out, int k, int step, const float *rho, long long count,
-             cudaStream_t st) {
+void product(const Operand &a, const Operand &b, const Operand &out, int k, const Pair &add, int step, const float *rho,
+             long long count, cudaStream_t st) {
   NsProduct g{};
+  g.add = add;
+  g.ld = out.ld;
   g.m = (int)out.rows;
   g.n = (int)out.cols;
   g.k = k;
   g.step = step;
   g.rho = rho;
-  g.m_tiles = (g.m + 127) / 128;
-  g.n_tiles = (g.n + 127) / 128;
-  const long long per = OP == APPLY ? (long long)g.m_tiles * g.n_tiles : (long long)g.m_tiles * (g.m_tiles + 1) / 2;
-  if (per * count > 0x3fffffffLL) throw std::invalid_argument("too many matrices of this size for one call");
-  g.tiles = (int)(per * count);
-  using L = NsSmem<A_MN, B_MN>;
-  LB_CUDA(cudaFuncSetAttribute(ns_product_kernel<OP, A_MN, B_MN>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL));
-  launch_pdl(ns_product_kernel<OP, A_MN, B_MN>, dim3((unsigned)(g.tiles < 148 ? g.tiles : 148)), dim3(NS_THREADS), L::TOTAL, st, true,
-             ns_map(a.p.hi, a, count, A_MN), ns_map(a.p.lo, a, count, A_MN), ns_map(b.p.hi, b, count, B_MN),
-             ns_map(b.p.lo, b, count, B_MN), ns_map(out.p.hi, out, count, false, true), ns_map(out.p.lo, out, count, false, true), g);
+  auto turns = [&](long long t, long long at_once) {
+    const long long mt = (g.m + t - 1) / t, nt = (g.n + t - 1) / t, tiles = (OP == APPLY ? mt * nt : mt * (mt + 1) / 2) * count;
+    return (tiles + at_once - 1) / at_once;
+  };
+  if (NS_PAIR_COST * turns(256, 74) < turns(128, 148)) launch_product<OP, A_MN, B_MN, true>(a, b, out, g, count, st);
+  else launch_product<OP, A_MN, B_MN, false>(a, b, out, g, count, st);
 }
 
 bool rows16(const MatView &v) {
@@ -520,7 +655,7 @@ size_t ns_layout(long long count, long long m, long long n, char *p, NsWork *w) 
     x->hi = reinterpret_cast<__half *>(take((size_t)count * m * ldx * 2));
     x->lo = reinterpret_cast<__half *>(take((size_t)count * m * ldx * 2));
   }
-  for (Pair *x : {&k.s, &k.b}) {
+  for (Pair *x : {&k.a, &k.b}) {
     x->hi = reinterpret_cast<__half *>(take((size_t)count * small * ldp * 2));
     x->lo = reinterpret_cast<__half *>(take((size_t)count * small * ldp * 2));
   }
@@ -534,6 +669,7 @@ size_t muon_workspace_bytes(long long count, long long m, long long n) { return 
 
 void launch_muon(const MuonStep &g, void *workspace, cudaStream_t st) {
   const long long m = g.grads.rows, n = g.grads.cols, count = g.grads.batch;
+  if (muon_small_supports(m, n)) return launch_muon_small(g, st);
   const bool tall = m > n;
   const int p = (int)(tall ? n : m);
   NsWork w;
@@ -545,12 +681,12 @@ void launch_muon(const MuonStep &g, void *workspace, cudaStream_t st) {
   launch_pdl(muon_begin_kernel, grid, dim3(256), 0, st, true, g, w, vec);
   launch_pdl(muon_pair_kernel, wide, dim3(256), 0, st, true, g, w, vec, (int)parts);
   for (int i = 0; i < g.steps; ++i) {
-    const Operand x{w.x[i & 1], m, n, w.ldx}, y{w.x[(i + 1) & 1], m, n, w.ldx}, a{w.s, p, p, w.ldp}, b{w.b, p, p, w.ldp};
-    if (tall) product<GRAM, true, true>(x, x, a, (int)m, i, w.rho, count, st);
-    else product<GRAM, false, false>(x, x, a, (int)n, i, w.rho, count, st);
-    product<POLY, false, false>(a, a, b, p, i, w.rho, count, st);
-    if (tall) product<APPLY, false, false>(x, b, y, p, i, w.rho, count, st);
-    else product<APPLY, false, true>(b, x, y, p, i, w.rho, count, st);
+    const Operand x{w.x[i & 1], m, n, w.ldx}, y{w.x[(i + 1) & 1], m, n, w.ldx}, a{w.a, p, p, w.ldp}, b{w.b, p, p, w.ldp};
+    if (tall) product<GRAM, true, true>(x, x, a, (int)m, Pair{}, i, w.rho, count, st);
+    else product<GRAM, false, false>(x, x, a, (int)n, Pair{}, i, w.rho, count, st);
+    product<POLY, false, false>(a, a, b, p, a.p, i, w.rho, count, st);
+    if (tall) product<APPLY, false, false>(x, b, y, p, x.p, i, w.rho, count, st);
+    else product<APPLY, false, true>(b, x, y, p, x.p, i, w.rho, count, st);
   }
   const float rate = g.lr * sqrtf(m > n ? (float)m / (float)n : 1.f);
   launch_pdl(muon_end_kernel, wide, dim3(256), 0, st, true, g, w, vec, 1.f - g.lr * g.weight_decay, rate);

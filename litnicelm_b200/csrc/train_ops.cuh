@@ -65,5 +65,8 @@ struct MuonStep {
 };
 size_t muon_workspace_bytes(long long count, long long m, long long n);
 void launch_muon(const MuonStep &a, void *workspace, cudaStream_t st);
+// orthogonal_small.cu: small matrices in one launch
+bool muon_small_supports(long long m, long long n);
+void launch_muon_small(const MuonStep &a, cudaStream_t st);
 
 }  // namespace lb
