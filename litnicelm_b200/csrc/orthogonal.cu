@@ -13,8 +13,8 @@
 // Matrices live as pairs of fp16 values: z 2^e = hi + 2^-11 lo, 22 bits, with one exponent e per matrix, kind and step. It follows
 // from a bound on the singular values alone: those of X_k are at most min(1.25, rho a^k) where rho = |X_0| (the polynomial stays
 // below 1.21 on [0, 1.21] and below a s), those of A at most its square, of B min(2.85, |b| of that). No entry is larger, and e puts
-// the bound at 2^13 to 2^14. A product is three: hi hi in one accumulator of tensor memory, hi lo and lo hi in another; lo lo is below 2^-24 of a
-// term and left out. The tensor pipe truncates when it adds, so chains in tensor memory are 64 k long and are added in
+// the bound at 2^13 to 2^14. A product is three: hi lo and lo hi, then, scaled by 2^-11 in the instruction that starts it, hi hi on top; lo lo is below
+// 2^-22 of a term, mostly far below, and left out. The tensor pipe truncates when it adds, so chains in tensor memory are 64 k long and are added in
 // registers, rounded to nearest.
 //
 // One persistent kernel for the three products of a step, tiles of 128 x 128: warp 0 issues TMA (stages of 64 k: four tiles of 16
@@ -36,7 +36,6 @@ namespace {
 constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f, NS_EPS = 1e-7f;
 constexpr int NS_PARTS = 256;  // partial sums of a matrix's norm, at most
 constexpr int NS_THREADS = 320;
-constexpr double NS_PAIR_COST = 1.4;
 
 struct Pair {
   __half *hi, *lo;  // [count][rows][ld]
@@ -72,6 +71,14 @@ __device__ __forceinline__ int ns_exp_b(float rho, int k) {
 __device__ __forceinline__ void ns_split(float z, __half &hi, __half &lo) {  // z already scaled
   hi = __float2half_rn(z);
   lo = __float2half_rn((z - __half2float(hi)) * 2048.f);
+}
+// Two at once: a conversion of two values costs what one does.
+__device__ __forceinline__ void ns_split2(float a, float b, unsigned &hi, unsigned &lo) {
+  const __half2 h = __floats2half2_rn(a, b);
+  const float2 f = __half22float2(h);
+  const __half2 l = __floats2half2_rn((a - f.x) * 2048.f, (b - f.y) * 2048.f);
+  hi = *reinterpret_cast<const unsigned *>(&h);
+  lo = *reinterpret_cast<const unsigned *>(&l);
 }
 __device__ __forceinline__ float ns_value(__half hi, __half lo) { return fmaf(__half2float(lo), 1.f / 2048.f, __half2float(hi)); }
 __device__ __forceinline__ float ns_pow2(int e) { return ldexpf(1.f, e); }
@@ -238,16 +245,24 @@ __device__ __forceinline__ void ns_load(unsigned to, const CUtensorMap *map, int
         : "memory");
   else tma_load_4d(to, map, x, 0, z, w, bar);
 }
+// D = A B, D += A B, or D = 2^-11 D + A B.
+enum NsStart { NS_NEW, NS_ADD, NS_SCALED };
 template <bool PAIR>
-__device__ __forceinline__ void ns_mma(unsigned d, unsigned long long a, unsigned long long b, unsigned idesc, unsigned more) {
-  if constexpr (PAIR)
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(more)
-        : "memory");
-  else tc_mma_f16(d, a, b, idesc, more);
+__device__ __forceinline__ void ns_mma(unsigned d, unsigned long long a, unsigned long long b, unsigned idesc, NsStart how) {
+#define NS_MMA(group, scale)                                           \
+  asm volatile("{\n\t.reg .pred p;\n\t"                                \
+               "setp.ne.b32 p, %4, 0;\n\t"                             \
+               "tcgen05.mma.cta_group::" group ".kind::f16 [%0], %1, %2, %3, p" scale ";\n\t}" \
+               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(how == NS_NEW ? 0u : 1u)              \
+               : "memory")
+  if (how == NS_SCALED) {
+    if constexpr (PAIR) NS_MMA("2", ", 11");
+    else NS_MMA("1", ", 11");
+  } else {
+    if constexpr (PAIR) NS_MMA("2", "");
+    else NS_MMA("1", "");
+  }
+#undef NS_MMA
 }
 template <bool PAIR>
 __device__ __forceinline__ void ns_commit(unsigned bar) {  // of a pair: the barrier at this place in both CTAs
@@ -266,7 +281,7 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_ah, const __grid_const
                   const __grid_constant__ NsProduct g) {
   using L = NsSmem<PAIR>;
   constexpr int S = L::STAGES, CTAS = PAIR ? 2 : 1, T = 128 * CTAS;  // tiles of T x T by CTAS CTAs, each 128 rows in HALVES pieces
-  constexpr int HALVES = CTAS;
+  constexpr int CHAINS = 4 / CTAS, COLS = 64 * CTAS;  // chains in flight, T columns of tensor memory each; columns of a thread
   constexpr bool SYM = OP != APPLY;
   const int rank = PAIR ? (int)blockIdx.x & 1 : 0, cta = (int)blockIdx.x / CTAS, ctas = (int)gridDim.x / CTAS;
   extern __shared__ unsigned char smem_raw[];
@@ -276,10 +291,10 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_ah, const __grid_const
   auto full = [&](int s) { return bars + 8u * s; };
   auto empty = [&](int s) { return bars + 8u * (S + s); };
   auto chain_full = [&](int b) { return bars + 8u * (2 * S + b); };
-  auto chain_empty = [&](int b) { return bars + 8u * (2 * S + 2 + b); };
-  const unsigned done = bars + 8u * (2 * S + 4);
-  volatile unsigned *tmem_holder = reinterpret_cast<volatile unsigned *>(base_ptr + L::BAR_OFF + 96);
-  volatile int *abort_flag = reinterpret_cast<volatile int *>(base_ptr + L::BAR_OFF + 100);
+  auto chain_empty = [&](int b) { return bars + 8u * (2 * S + CHAINS + b); };
+  const unsigned done = bars + 8u * (2 * S + 2 * CHAINS);
+  volatile unsigned *tmem_holder = reinterpret_cast<volatile unsigned *>(base_ptr + L::BAR_OFF + 120);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(base_ptr + L::BAR_OFF + 124);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int kblocks = (g.k + 63) / 64;
   auto place = [&](int tile, int &batch, int &mt, int &nt) {
@@ -302,7 +317,7 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_ah, const __grid_const
       mbar_init(full(s), 1);
       mbar_init(empty(s), 1);
     }
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < CHAINS; ++b) {
       mbar_init(chain_full(b), 1);
       mbar_init(chain_empty(b), 8 * CTAS);
     }
@@ -331,7 +346,6 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_ah, const __grid_const
   if constexpr (PAIR) cluster_sync_all();  // both CTAs' barriers are there
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const unsigned tmem = *tmem_holder;
-  pdl_launch_dependents();  // behind the allocation: a dependent's CTA must not take tensor memory first
   pdl_wait();
 
   if (warp == 0) {
@@ -349,20 +363,19 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_ah, const __grid_const
           // (of a pair, the even one's barrier counts both CTAs' bytes)
           if (rank == 0) mbar_expect_tx(full(s), (unsigned)(CTAS * L::STAGE));
           const unsigned bar = PAIR ? cluster_map(full(s), 0) : full(s);
-          auto load = [&](unsigned to, const CUtensorMap *map, bool mn, int r0, int r1) {  // 64 rows from r0 on, and from r1 on
+          auto load = [&](unsigned to, const CUtensorMap *map, bool mn, int r0) {
             if (mn) {  // rows of k, two slabs of 64 columns
               ns_load<PAIR>(to, map, r0, kb * 64, batch, bar);
-              ns_load<PAIR>(to + 8192, map, r1, kb * 64, batch, bar);
+              ns_load<PAIR>(to + 8192, map, r0 + 64, kb * 64, batch, bar);
             } else {
               ns_load<PAIR>(to, map, kb * 64, r0, batch, bar);
-              ns_load<PAIR>(to + 8192, map, kb * 64, r1, batch, bar);
             }
           };
-          const int m0 = mt * T + rank * 128, n0 = nt * T + rank * 64, n1 = PAIR ? n0 + 128 : n0 + 64;
-          load(st, &map_ah, A_MN, m0, m0 + 64);
-          load(st + L::TILE, &map_al, A_MN, m0, m0 + 64);
-          load(st + 2 * L::TILE, &map_bh, B_MN, n0, n1);
-          load(st + 3 * L::TILE, &map_bl, B_MN, n0, n1);
+          const int m0 = mt * T + rank * 128, n0 = nt * T + rank * 128;
+          load(st, &map_ah, A_MN, m0);
+          load(st + L::TILE, &map_al, A_MN, m0);
+          load(st + 2 * L::TILE, &map_bh, B_MN, n0);
+          load(st + 3 * L::TILE, &map_bl, B_MN, n0);
         }
         __syncwarp();
       }
@@ -376,39 +389,35 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_ah, const __grid_const
         while (!mbar_try_wait(full(j % S), (unsigned)(j / S) & 1u) && global_timer() < limit) {}
     }
   } else if (warp == 1) {
-    constexpr unsigned idesc = (umma_idesc_f16(128) + (PAIR ? (unsigned)(TC_BM >> 4) << 24 : 0u)) |
+    constexpr unsigned idesc = (umma_idesc_f16(T) + (PAIR ? (unsigned)(TC_BM >> 4) << 24 : 0u)) |
                                (A_MN ? UMMA_A_MN_MAJOR : 0u) | (B_MN ? UMMA_B_MN_MAJOR : 0u);
-    int it = 0, chain = 0;
+    int it = 0;
     bool ok = true;
     for (int tile = rank == 0 ? cta : g.tiles; tile < g.tiles && ok; tile += ctas) {
-      for (int kb = 0; kb < kblocks && ok; ++kb, ++it) {
-        const int s = it % S;
-        ok = mbar_wait_warp(full(s), (unsigned)(it / S) & 1u, abort_flag, nullptr, 63);
+      for (int kb = 0; kb < kblocks; ++kb, ++it) {
+        const int s = it % S, buf = it % CHAINS;
+        ok = mbar_wait_warp(full(s), (unsigned)(it / S) & 1u, abort_flag, nullptr, 63) &&
+             mbar_wait_warp(chain_empty(buf), ((unsigned)(it / CHAINS) & 1u) ^ 1u, abort_flag, nullptr, 62);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (lane == 0) {
+          const unsigned st = base + (unsigned)(s * L::STAGE), d = tmem + (unsigned)(buf * T);
+          auto desc = [&](int t, bool mn, int ks) {
+            const unsigned p = st + (unsigned)(t * L::TILE);
+            return mn ? umma_desc_mn128(p + (unsigned)(ks * 2048), 8192u) : umma_desc_k128(p) + (unsigned long long)(ks * 2);
+          };
 #pragma unroll
-        for (int h = 0; h < HALVES; ++h, ++chain) {
-          const int buf = chain & 1;
-          if (ok) ok = mbar_wait_warp(chain_empty(buf), ((unsigned)(chain >> 1) & 1u) ^ 1u, abort_flag, nullptr, 62);
-          if (!ok) break;
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          if (lane == 0) {
-            const unsigned st = base + (unsigned)(s * L::STAGE), d = tmem + (unsigned)(buf * 256);
-            auto desc = [&](int t, bool mn, int ks) {
-              const unsigned p = st + (unsigned)(t * L::TILE + (t >= 2 ? h * 8192 : 0));
-              return mn ? umma_desc_mn128(p + (unsigned)(ks * 2048), 8192u) : umma_desc_k128(p) + (unsigned long long)(ks * 2);
-            };
-#pragma unroll
-            for (int ks = 0; ks < 4; ++ks) {
-              const unsigned more = ks ? 1u : 0u;
-              const unsigned long long ah = desc(0, A_MN, ks), al = desc(1, A_MN, ks), bh = desc(2, B_MN, ks), bl = desc(3, B_MN, ks);
-              ns_mma<PAIR>(d, ah, bh, idesc, more);
-              ns_mma<PAIR>(d + 128, ah, bl, idesc, more);
-              ns_mma<PAIR>(d + 128, al, bh, idesc, 1u);
-            }
-            if (h == HALVES - 1) ns_commit<PAIR>(empty(s));
-            ns_commit<PAIR>(chain_full(buf));
+          for (int ks = 0; ks < 4; ++ks) {
+            ns_mma<PAIR>(d, desc(0, A_MN, ks), desc(3, B_MN, ks), idesc, ks ? NS_ADD : NS_NEW);
+            ns_mma<PAIR>(d, desc(1, A_MN, ks), desc(2, B_MN, ks), idesc, NS_ADD);
           }
-          __syncwarp();
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks)
+            ns_mma<PAIR>(d, desc(0, A_MN, ks), desc(2, B_MN, ks), idesc, ks ? NS_ADD : NS_SCALED);
+          ns_commit<PAIR>(empty(s));
+          ns_commit<PAIR>(chain_full(buf));
         }
+        __syncwarp();
       }
     }
     if (!ok) {  // what was issued ends, within the limit, before the shared memory goes away
@@ -421,45 +430,48 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_ah, const __grid_const
     const int q = warp & 3, half = (warp - 2) >> 2;
     unsigned char *patch = base_ptr + L::PATCH_OFF + (warp - 2) * L::PATCH;
     const unsigned patch_u = base + (unsigned)(L::PATCH_OFF + (warp - 2) * L::PATCH);
-    int chain = 0;
+    int it = 0;
     bool ok = true;
     for (int tile = cta; tile < g.tiles; tile += ctas) {
       int batch, mt, nt;
       place(tile, batch, mt, nt);
       const float rho = g.rho[batch];
-      // acc = the product times 2^(sum of the operands' exponents), which may reach 200: two factors
-      const int ex = ns_exp_x(rho, g.step), ea = ns_exp_a(rho, g.step), eb = ns_exp_b(rho, g.step);
-      const int e_in = OP == GRAM ? 2 * ex : OP == POLY ? 2 * ea : eb + ex;
-      const int e_out = OP == GRAM ? ea : OP == POLY ? eb : ns_exp_x(rho, g.step + 1);
-      const float f1 = (OP == POLY ? NS_C : 1.f) * ns_pow2(-(e_in / 2)), f2 = ns_pow2(e_out - (e_in - e_in / 2));
       const int row0 = mt * T + rank * 128 + q * 32;
-      float acc[HALVES][64];
+      float acc[COLS];
+      int ex, ea, eb;
+      auto exponents = [&]() {
+        ex = ns_exp_x(rho, g.step);
+        ea = ns_exp_a(rho, g.step);
+        eb = ns_exp_b(rho, g.step);
+      };
+      if (OP == GRAM) {
+        exponents();
 #pragma unroll
-      for (int h = 0; h < HALVES; ++h)
-#pragma unroll
-        for (int j = 0; j < 64; ++j) acc[h][j] = 0.f;
-      if (OP != GRAM) {  // whole rows' 128 bytes at a time through the patch
-        const float f_add = OP == POLY ? NS_B / NS_C * ns_pow2(ea) : NS_A * ns_pow2(eb);
+        for (int j = 0; j < COLS; ++j) acc[j] = 0.f;
+      } else {  // the added matrix, whole rows' 128 bytes at a time through the patch; all loads of 64 columns in flight
         if (lane == 0) bulk_wait_read<0>();
         __syncwarp();
 #pragma unroll
-        for (int h = 0; h < HALVES; ++h) {
-          const int col0 = nt * T + h * 128 + half * 64;
-          if (row0 >= g.m || col0 >= g.n) continue;
+        for (int c0 = 0; c0 < COLS; c0 += 64) {
+          const int col0 = nt * T + half * COLS + c0;
+          const long long from = ((long long)batch * g.m + row0) * g.ld + col0 + (lane & 7) * 8;
+          const bool in = col0 + (lane & 7) * 8 < g.n;
+          uint4 u[2][8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int r = i * 4 + (lane >> 3);
+            const bool there = in && row0 + r < g.m;
+            u[0][i] = there ? *reinterpret_cast<const uint4 *>(g.add.hi + from + r * g.ld) : make_uint4(0u, 0u, 0u, 0u);
+            u[1][i] = there ? *reinterpret_cast<const uint4 *>(g.add.lo + from + r * g.ld) : make_uint4(0u, 0u, 0u, 0u);
+          }
+          if (c0 == 0) exponents();
+          const float f_add = OP == POLY ? NS_B / NS_C * ns_pow2(ea) : NS_A * ns_pow2(eb);
 #pragma unroll
           for (int lo = 0; lo < 2; ++lo) {
-            const __half *from = (lo ? g.add.lo : g.add.hi) + ((long long)batch * g.m + row0) * g.ld + col0 + (lane & 7) * 8;
-            const bool in = col0 + (lane & 7) * 8 < g.n;
-            uint4 u[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
               const int r = i * 4 + (lane >> 3);
-              u[i] = in && row0 + r < g.m ? *reinterpret_cast<const uint4 *>(from + r * g.ld) : make_uint4(0u, 0u, 0u, 0u);
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int r = i * 4 + (lane >> 3);
-              *reinterpret_cast<uint4 *>(patch + r * 128 + (((lane & 7) ^ (r & 7)) << 4)) = u[i];
+              *reinterpret_cast<uint4 *>(patch + r * 128 + (((lane & 7) ^ (r & 7)) << 4)) = u[lo][i];
             }
             __syncwarp();
             const float f = lo ? f_add / 2048.f : f_add;
@@ -470,70 +482,49 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_ah, const __grid_const
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
                 const float2 w = __half22float2(z[j]);
-                acc[h][i * 8 + 2 * j] = fmaf(w.x, f, acc[h][i * 8 + 2 * j]);
-                acc[h][i * 8 + 2 * j + 1] = fmaf(w.y, f, acc[h][i * 8 + 2 * j + 1]);
+                const int at = c0 + i * 8 + 2 * j;
+                acc[at] = lo ? fmaf(w.x, f, acc[at]) : w.x * f;
+                acc[at + 1] = lo ? fmaf(w.y, f, acc[at + 1]) : w.y * f;
               }
             }
             __syncwarp();
           }
         }
       }
-      for (int kb = 0; kb < kblocks && ok; ++kb) {
+      // acc = the product times 2^(sum of the operands' exponents), which may reach 200: two factors
+      const int e_in = OP == GRAM ? 2 * ex : OP == POLY ? 2 * ea : eb + ex;
+      const int e_out = OP == GRAM ? ea : OP == POLY ? eb : ns_exp_x(rho, g.step + 1);
+      const float f2 = ns_pow2(e_out - (e_in - e_in / 2));
+      for (int kb = 0; kb < kblocks && ok; ++kb, ++it) {
+        const int buf = it % CHAINS;
+        ok = mbar_wait_warp(chain_full(buf), (unsigned)(it / CHAINS) & 1u, abort_flag, nullptr, 64);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
-        for (int h = 0; h < HALVES; ++h, ++chain) {
-          const int buf = chain & 1;
-          if (ok) ok = mbar_wait_warp(chain_full(buf), (unsigned)(chain >> 1) & 1u, abort_flag, nullptr, 64);
-          if (!ok) break;
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          constexpr int C = PAIR ? 16 : 32;  // columns at a time: registers
+        for (int c0 = 0; c0 < COLS; c0 += 32) {
+          unsigned r[32];
+          tc_ld32(tmem + ((unsigned)(q * 32) << 16) + (unsigned)(buf * T + half * COLS + c0), r);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-          for (int c0 = 0; c0 < 64; c0 += C) {
-            unsigned r[C], t[C];
-            const unsigned at = tmem + ((unsigned)(q * 32) << 16) + (unsigned)(buf * 256 + half * 64 + c0);
-            if constexpr (PAIR) {
-              tc_ld16(at, r);
-              tc_ld16(at + 128, t);
-            } else {
-              tc_ld32(at, r);
-              tc_ld32(at + 128, t);
-            }
-            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-            for (int j = 0; j < C; ++j)
-              acc[h][c0 + j] += fmaf(__uint_as_float(t[j]), 1.f / 2048.f, __uint_as_float(r[j]));
-          }
-          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-          __syncwarp();
-          if (lane == 0) {
-            if constexpr (PAIR)
-              asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_map(chain_empty(buf), 0))
-                           : "memory");
-            else mbar_arrive(chain_empty(buf));
-          }
+          for (int j = 0; j < 32; ++j) acc[c0 + j] += __uint_as_float(r[j]);
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (PAIR)
+            asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_map(chain_empty(buf), 0))
+                         : "memory");
+          else mbar_arrive(chain_empty(buf));
         }
       }
+      const float f1 = ok ? (OP == POLY ? NS_C : 1.f) * ns_pow2(-(e_in / 2)) : NAN;
 #pragma unroll
-      for (int piece = 0; piece < 2 * HALVES; ++piece) {
-        const int c0 = piece * 32 % 64;
-        const float(&part)[64] = acc[piece / 2];
-        const int col = nt * T + piece / 2 * 128 + half * 64 + c0;
+      for (int c0 = 0; c0 < COLS; c0 += 32) {
+        const int col = nt * T + half * COLS + c0;
         if (col >= g.n || row0 >= g.m) continue;
         unsigned h[16], l[16];
 #pragma unroll
-        for (int j = 0; j < 32; j += 2) {
-          __half2 hh, ll;
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float v = part[c0 + j + e] * f1 * f2;
-            if (!ok) v = NAN;
-            __half x, y;
-            ns_split(v, x, y);
-            if (e) hh.y = x, ll.y = y;
-            else hh.x = x, ll.x = y;
-          }
-          h[j >> 1] = *reinterpret_cast<const unsigned *>(&hh);
-          l[j >> 1] = *reinterpret_cast<const unsigned *>(&ll);
-        }
+        for (int j = 0; j < 32; j += 2) ns_split2(acc[c0 + j] * f1 * f2, acc[c0 + j + 1] * f1 * f2, h[j >> 1], l[j >> 1]);
         if (lane == 0) bulk_wait_read<0>();
         __syncwarp();
 #pragma unroll
@@ -568,6 +559,7 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_ah, const __grid_const
     if (lane == 0) bulk_wait_all();  // the stores are part of the grid's results
   }
   __syncwarp();
+  pdl_launch_dependents();  // here and not at the start: a step of 256 x 256 takes 23.9 us so, 26.7 with waiting CTAs around
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   if constexpr (PAIR) cluster_sync_all();  // nothing of the pair's is on its way to the other CTA
@@ -583,12 +575,12 @@ struct Operand {
   long long rows, cols, ld;
 };
 
-CUtensorMap ns_map(const __half *p, const Operand &o, long long count, bool result = false) {
+CUtensorMap ns_map(const __half *p, const Operand &o, long long count, bool mn, bool result = false) {
   CUtensorMap map;
   const unsigned long long extent[4] = {(unsigned long long)o.cols, 1, (unsigned long long)o.rows, (unsigned long long)count};
   const unsigned long long strides[3] = {16, (unsigned long long)o.ld * 2, (unsigned long long)(o.rows * o.ld) * 2};
   if (result) tc_make_map_heads(&map, p, extent, strides, 32, 32);
-  else tc_make_map_heads(&map, p, extent, strides, 64);
+  else tc_make_map_heads(&map, p, extent, strides, mn ? 64 : 128);
   return map;
 }
 
@@ -604,8 +596,9 @@ void launch_product(const Operand &a, const Operand &b, const Operand &out, NsPr
   LB_CUDA(cudaFuncSetAttribute(ns_product_kernel<OP, A_MN, B_MN, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL));
   const int ctas = g.tiles < 148 / CTAS ? g.tiles : 148 / CTAS;
   launch_pdl_cluster_x(ns_product_kernel<OP, A_MN, B_MN, PAIR>, dim3((unsigned)(ctas * CTAS)), dim3(NS_THREADS), L::TOTAL, st, true,
-                       (unsigned)CTAS, ns_map(a.p.hi, a, count), ns_map(a.p.lo, a, count), ns_map(b.p.hi, b, count),
-                       ns_map(b.p.lo, b, count), ns_map(out.p.hi, out, count, true), ns_map(out.p.lo, out, count, true), g);
+                       (unsigned)CTAS, ns_map(a.p.hi, a, count, A_MN), ns_map(a.p.lo, a, count, A_MN), ns_map(b.p.hi, b, count, B_MN),
+                       ns_map(b.p.lo, b, count, B_MN), ns_map(out.p.hi, out, count, false, true),
+                       ns_map(out.p.lo, out, count, false, true), g);
 }
 
 template <NsOp OP, bool A_MN, bool B_MN>
@@ -619,11 +612,20 @@ void product(const Operand &a, const Operand &b, const Operand &out, int k, cons
   g.k = k;
   g.step = step;
   g.rho = rho;
-  auto turns = [&](long long t, long long at_once) {
+  // us of the longest CTA: a turn's blocks of 64 k and what surrounds them, and a launch. A CTA's 64 KB of operands a block come at
+  // 50 bytes a clock (0.69 us, of which 0.4 are products), a little slower with all SMs at it; a pair's CTAs take the same for twice
+  // the result (1.07 us, the tensor pipe 0.8) and longer before and behind it. Four matrices of 4096 x 1024, a step: A 60 us by single
+  // CTAs, 80 by pairs (80 of 148 SMs); X 116 and 103. Six of 512 x 2048: X 32 and 39.
+  const double kb = (k + 63) / 64;
+  auto turns = [&](long long t, long long at_once, double &busy) {
     const long long mt = (g.m + t - 1) / t, nt = (g.n + t - 1) / t, tiles = (OP == APPLY ? mt * nt : mt * (mt + 1) / 2) * count;
-    return (tiles + at_once - 1) / at_once;
+    busy = tiles < at_once ? (double)tiles / at_once : 1.0;
+    return (double)((tiles + at_once - 1) / at_once);
   };
-  if (NS_PAIR_COST * turns(256, 74) < turns(128, 148)) launch_product<OP, A_MN, B_MN, true>(a, b, out, g, count, st);
+  double busy = 0;
+  const double pair = turns(256, 74, busy) * (kb * 1.07 + 9) + 3.5;
+  const double one = turns(128, 148, busy) * (kb * (busy > 0.8 ? 0.86 * busy : 0.69) + 2.5) + 2.5;
+  if (pair < one) launch_product<OP, A_MN, B_MN, true>(a, b, out, g, count, st);
   else launch_product<OP, A_MN, B_MN, false>(a, b, out, g, count, st);
 }
 
