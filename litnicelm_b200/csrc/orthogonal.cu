@@ -34,8 +34,9 @@ namespace lb {
 namespace {
 
 constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f, NS_EPS = 1e-7f;
+constexpr double NS_SPLIT = 2.0;
 constexpr int NS_PARTS = 256;  // partial sums of a matrix's norm, at most
-constexpr int NS_THREADS = 320;
+constexpr int NS_THREADS = 320, NS_LD = 132;  // floats between rows of a finished range of k
 
 struct Pair {
   __half *hi, *lo;  // [count][rows][ld]
@@ -215,11 +216,12 @@ __global__ void __launch_bounds__(256) muon_end_kernel(const __grid_constant__ M
 enum NsOp { GRAM, POLY, APPLY };
 
 struct NsProduct {
-  Pair add;              // A for POLY, X for APPLY
+  Pair add, out;         // A for POLY, X for APPLY; the result
   long long ld;          // of it and of the result
   int m, n, k;           // sizes of the product
   int m_tiles, n_tiles, tiles;  // tiles of all matrices
   int step;
+  int splits;            // CTAs of a cluster that share a tile's range of k (SPLIT)
   const float *rho;
 };
 
@@ -273,7 +275,7 @@ __device__ __forceinline__ void ns_commit(unsigned bar) {  // of a pair: the bar
   else tc_commit(bar);
 }
 
-template <NsOp OP, bool A_MN, bool B_MN, bool PAIR>
+template <NsOp OP, bool A_MN, bool B_MN, bool PAIR, bool SPLIT>
 __global__ void __launch_bounds__(NS_THREADS, 1)
 ns_product_kernel(const __grid_constant__ CUtensorMap map_ah, const __grid_constant__ CUtensorMap map_al,
                   const __grid_constant__ CUtensorMap map_bh, const __grid_constant__ CUtensorMap map_bl,
@@ -283,7 +285,10 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_ah, const __grid_const
   constexpr int S = L::STAGES, CTAS = PAIR ? 2 : 1, T = 128 * CTAS;  // tiles of T x T by CTAS CTAs, each 128 rows in HALVES pieces
   constexpr int CHAINS = 4 / CTAS, COLS = 64 * CTAS;  // chains in flight, T columns of tensor memory each; columns of a thread
   constexpr bool SYM = OP != APPLY;
-  const int rank = PAIR ? (int)blockIdx.x & 1 : 0, cta = (int)blockIdx.x / CTAS, ctas = (int)gridDim.x / CTAS;
+  static_assert(!(PAIR && SPLIT), "");
+  const int rank = PAIR ? (int)blockIdx.x & 1 : 0;
+  const int share = SPLIT ? (int)blockIdx.x % g.splits : 0, per_tile = SPLIT ? g.splits : CTAS;
+  const int cta = (int)blockIdx.x / per_tile, ctas = (int)gridDim.x / per_tile;
   extern __shared__ unsigned char smem_raw[];
   const unsigned base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char *base_ptr = smem_raw + (base - smem_u32(smem_raw));
@@ -296,7 +301,8 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_ah, const __grid_const
   volatile unsigned *tmem_holder = reinterpret_cast<volatile unsigned *>(base_ptr + L::BAR_OFF + 120);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(base_ptr + L::BAR_OFF + 124);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int kblocks = (g.k + 63) / 64;
+  const int all_blocks = (g.k + 63) / 64, each = SPLIT ? (all_blocks + g.splits - 1) / g.splits : all_blocks;
+  const int kb0 = min(all_blocks, share * each), kblocks = min(all_blocks, kb0 + each) - kb0;  // of this CTA
   auto place = [&](int tile, int &batch, int &mt, int &nt) {
     const int per = SYM ? g.m_tiles * (g.m_tiles + 1) / 2 : g.m_tiles * g.n_tiles;
     batch = tile / per;
@@ -364,11 +370,12 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_ah, const __grid_const
           if (rank == 0) mbar_expect_tx(full(s), (unsigned)(CTAS * L::STAGE));
           const unsigned bar = PAIR ? cluster_map(full(s), 0) : full(s);
           auto load = [&](unsigned to, const CUtensorMap *map, bool mn, int r0) {
+            const int k0 = (kb0 + kb) * 64;
             if (mn) {  // rows of k, two slabs of 64 columns
-              ns_load<PAIR>(to, map, r0, kb * 64, batch, bar);
-              ns_load<PAIR>(to + 8192, map, r0 + 64, kb * 64, batch, bar);
+              ns_load<PAIR>(to, map, r0, k0, batch, bar);
+              ns_load<PAIR>(to + 8192, map, r0 + 64, k0, batch, bar);
             } else {
-              ns_load<PAIR>(to, map, kb * 64, r0, batch, bar);
+              ns_load<PAIR>(to, map, k0, r0, batch, bar);
             }
           };
           const int m0 = mt * T + rank * 128, n0 = nt * T + rank * 128;
@@ -444,7 +451,7 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_ah, const __grid_const
         ea = ns_exp_a(rho, g.step);
         eb = ns_exp_b(rho, g.step);
       };
-      if (OP == GRAM) {
+      if (OP == GRAM || share > 0) {
         exponents();
 #pragma unroll
         for (int j = 0; j < COLS; ++j) acc[j] = 0.f;
@@ -518,6 +525,13 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_ah, const __grid_const
         }
       }
       const float f1 = ok ? (OP == POLY ? NS_C : 1.f) * ns_pow2(-(e_in / 2)) : NAN;
+      if constexpr (SPLIT) {  // every product has been read: this range's sums may lie over the stages
+        float *sums = reinterpret_cast<float *>(base_ptr) + (q * 32 + lane) * NS_LD + half * COLS;
+#pragma unroll
+        for (int j = 0; j < COLS; j += 4)
+          *reinterpret_cast<float4 *>(sums + j) = make_float4(acc[j] * f1 * f2, acc[j + 1] * f1 * f2, acc[j + 2] * f1 * f2, acc[j + 3] * f1 * f2);
+        break;
+      } else {
 #pragma unroll
       for (int c0 = 0; c0 < COLS; c0 += 32) {
         const int col = nt * T + half * COLS + c0;
@@ -555,8 +569,56 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_ah, const __grid_const
           tma_store_4d(&map_ol, patch_u + 2048, row0, 0, col, batch);
         }
       }
+      }
     }
     if (lane == 0) bulk_wait_all();  // the stores are part of the grid's results
+  }
+  if constexpr (SPLIT) {  // one tile, its ranges of k over the CTAs of the cluster: each stores a share of the rows
+    __syncwarp();
+    cluster_sync_all();
+    int batch, mt, nt;
+    place(cta, batch, mt, nt);
+    const int rows = 128 / g.splits, r0 = share * rows;
+    float *whole = reinterpret_cast<float *>(base_ptr + 128 * NS_LD * 4);  // [rows][NS_LD]
+    for (int e = threadIdx.x; e < rows * 32; e += NS_THREADS) {
+      const int r = e / 32, c = e % 32 * 4;
+      const unsigned from = base + (unsigned)((r0 + r) * NS_LD + c) * 4u;
+      float4 v = ld_cluster_f4(cluster_map(from, 0u));
+      for (int i = 1; i < g.splits; ++i) {
+        const float4 w = ld_cluster_f4(cluster_map(from, (unsigned)i));
+        v = make_float4(v.x + w.x, v.y + w.y, v.z + w.z, v.w + w.w);
+      }
+      *reinterpret_cast<float4 *>(whole + r * NS_LD + c) = v;
+    }
+    __syncthreads();
+    auto store8 = [&](int row, int col, const float (&v)[8]) {  // columns col .. col + 7 of a row of the result
+      unsigned h[4], l[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) ns_split2(v[2 * j], v[2 * j + 1], h[j], l[j]);
+      const long long to = ((long long)batch * g.m + row) * g.ld + col;
+      *reinterpret_cast<uint4 *>(g.out.hi + to) = make_uint4(h[0], h[1], h[2], h[3]);
+      *reinterpret_cast<uint4 *>(g.out.lo + to) = make_uint4(l[0], l[1], l[2], l[3]);
+    };
+    for (int e = threadIdx.x; e < rows * 16; e += NS_THREADS) {
+      const int r = e / 16, c = e % 16 * 8, row = mt * 128 + r0 + r, col = nt * 128 + c;
+      if (row >= g.m || col >= g.n) continue;
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = whole[r * NS_LD + c + j];
+      store8(row, col, v);
+    }
+    if (SYM && mt != nt) {
+      for (int e = threadIdx.x; e < rows * 16; e += NS_THREADS) {  // a column, eight rows (those behind the matrix are its padding)
+        const int c = e % 128, r = e / 128 * 8, row = nt * 128 + c, col = mt * 128 + r0 + r;
+        if (row >= g.n || col >= g.m) continue;
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = whole[(r + j) * NS_LD + c];
+        store8(row, col, v);
+      }
+    }
+    __syncwarp();
+    cluster_sync_all();  // no peer reads these sums any more
   }
   __syncwarp();
   pdl_launch_dependents();  // here and not at the start: a step of 256 x 256 takes 23.9 us so, 26.7 with waiting CTAs around
@@ -584,7 +646,7 @@ CUtensorMap ns_map(const __half *p, const Operand &o, long long count, bool mn, 
   return map;
 }
 
-template <NsOp OP, bool A_MN, bool B_MN, bool PAIR>
+template <NsOp OP, bool A_MN, bool B_MN, bool PAIR, bool SPLIT>
 void launch_product(const Operand &a, const Operand &b, const Operand &out, NsProduct g, long long count, cudaStream_t st) {
   constexpr int CTAS = PAIR ? 2 : 1, T = 128 * CTAS;
   g.m_tiles = (g.m + T - 1) / T;
@@ -593,10 +655,10 @@ void launch_product(const Operand &a, const Operand &b, const Operand &out, NsPr
   if (per * count > 0x3fffffffLL) throw std::invalid_argument("too many matrices of this size for one call");
   g.tiles = (int)(per * count);
   using L = NsSmem<PAIR>;
-  LB_CUDA(cudaFuncSetAttribute(ns_product_kernel<OP, A_MN, B_MN, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL));
-  const int ctas = g.tiles < 148 / CTAS ? g.tiles : 148 / CTAS;
-  launch_pdl_cluster_x(ns_product_kernel<OP, A_MN, B_MN, PAIR>, dim3((unsigned)(ctas * CTAS)), dim3(NS_THREADS), L::TOTAL, st, true,
-                       (unsigned)CTAS, ns_map(a.p.hi, a, count, A_MN), ns_map(a.p.lo, a, count, A_MN), ns_map(b.p.hi, b, count, B_MN),
+  LB_CUDA(cudaFuncSetAttribute(ns_product_kernel<OP, A_MN, B_MN, PAIR, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL));
+  const int per_tile = SPLIT ? g.splits : CTAS, ctas = SPLIT || g.tiles < 148 / CTAS ? g.tiles : 148 / CTAS;
+  launch_pdl_cluster_x(ns_product_kernel<OP, A_MN, B_MN, PAIR, SPLIT>, dim3((unsigned)(ctas * per_tile)), dim3(NS_THREADS), L::TOTAL, st,
+                       true, (unsigned)per_tile, ns_map(a.p.hi, a, count, A_MN), ns_map(a.p.lo, a, count, A_MN), ns_map(b.p.hi, b, count, B_MN),
                        ns_map(b.p.lo, b, count, B_MN), ns_map(out.p.hi, out, count, false, true),
                        ns_map(out.p.lo, out, count, false, true), g);
 }
@@ -606,6 +668,8 @@ void product(const Operand &a, const Operand &b, const Operand &out, int k, cons
              long long count, cudaStream_t st) {
   NsProduct g{};
   g.add = add;
+  g.out = out.p;
+  g.splits = 1;
   g.ld = out.ld;
   g.m = (int)out.rows;
   g.n = (int)out.cols;
@@ -625,8 +689,21 @@ void product(const Operand &a, const Operand &b, const Operand &out, int k, cons
   double busy = 0;
   const double pair = turns(256, 74, busy) * (kb * 1.07 + 9) + 3.5;
   const double one = turns(128, 148, busy) * (kb * (busy > 0.8 ? 0.86 * busy : 0.69) + 2.5) + 2.5;
-  if (pair < one) launch_product<OP, A_MN, B_MN, true>(a, b, out, g, count, st);
-  else launch_product<OP, A_MN, B_MN, false>(a, b, out, g, count, st);
+  // Few tiles: a tile's k over the CTAs of a cluster, joined over distributed shared memory.
+  const long long mt = (g.m + 127) / 128, nt = (g.n + 127) / 128, tiles = (OP == APPLY ? mt * nt : mt * (mt + 1) / 2) * count;
+  const int *fit = tc_cluster_capacity();
+  double least = one < pair ? one : pair;
+  for (int s = 2; s <= 8; s *= 2) {
+    if (tiles * s > 148 || tiles > fit[s] || kb < s) break;
+    const double t = ceil(kb / s) * 0.69 + NS_SPLIT + 2.5 + 2.5;
+    if (t < least) {
+      least = t;
+      g.splits = s;
+    }
+  }
+  if (g.splits > 1) launch_product<OP, A_MN, B_MN, false, true>(a, b, out, g, count, st);
+  else if (pair < one) launch_product<OP, A_MN, B_MN, true, false>(a, b, out, g, count, st);
+  else launch_product<OP, A_MN, B_MN, false, false>(a, b, out, g, count, st);
 }
 
 bool rows16(const MatView &v) {
