@@ -451,11 +451,14 @@ typedef struct litnice_b200_attention_options {
 
 /* q [streams, n, heads, dim], k and v [streams, m, groups, dim], out like q: one dtype, dim 1 .. 128,
  * heads a multiple of groups (head h uses key head h * groups / heads). lse [streams, heads, n] f32
- * dense: log of the sum of exp(scores). Scores, weights and sums in 32 bits; bfloat16 operands of
+ * dense: log of the sum of exp(scores). Scores, weights and sums in 32 bits. bfloat16 operands of
  * dim % 8 == 0 whose rows lie on 16-byte boundaries run on the tensor cores, weights rounded to
- * bfloat16 for their product with the values, others with 32-bit products. */
+ * bfloat16 for their product with the values; f32 operands of dim up to 64 run there in parts that
+ * keep their 24 bits; others run with 32-bit products. */
+uint64_t litnice_b200_attention_forward_workspace(LitniceView q, LitniceView k);
 int litnice_b200_attention_forward(LitniceView q, LitniceView k, LitniceView v,
-                                   const litnice_b200_attention_options *options, LitniceView out, float *lse, void *stream);
+                                   const litnice_b200_attention_options *options, LitniceView out, float *lse,
+                                   void *workspace, uint64_t workspace_bytes, void *stream);
 /* Gradients of sum(out * dout) from what the forward call left in out and lse. dout and dq like q, dk and dv like k.
  * Weights and their gradients are rounded to bfloat16 for their products where the forward call's are. */
 uint64_t litnice_b200_attention_backward_workspace(LitniceView q, LitniceView k);

@@ -134,8 +134,15 @@ TrainAttention attention_args(LitniceView q, LitniceView k, LitniceView v, const
   return a;
 }
 
-uint64_t backward_workspace(LitniceView q, LitniceView) {
-  return 256 + ((uint64_t)q->dims[0] * (uint64_t)q->dims[1] * (uint64_t)q->dims[2] * 4 + 255) / 256 * 256;
+// Bytes in front of the operands' parts: delta of a backward pass.
+uint64_t delta_bytes(LitniceView q) { return ((uint64_t)q->dims[0] * (uint64_t)q->dims[1] * (uint64_t)q->dims[2] * 4 + 255) / 256 * 256; }
+
+uint64_t attention_workspace(LitniceView q, LitniceView k, bool backward) {
+  if (k->dims[0] != q->dims[0]) bad("k has another number of streams than q");
+  uint64_t need = 256 + (backward ? delta_bytes(q) : 0);
+  if (train_attention_f32_supports(q->dtype == LITNICE_B200_VIEW_BF16, q->dims[3]))
+    need += train_attention_f32_workspace(q->dims[0], q->dims[1], k->dims[1], q->dims[2], k->dims[2], backward);
+  return need;
 }
 
 void muon_sizes(LitniceView t) {
@@ -157,17 +164,28 @@ uint64_t muon_workspace(LitniceView t) {
 extern "C" {
 
 int litnice_b200_attention_forward(LitniceView q, LitniceView k, LitniceView v, const litnice_b200_attention_options *options,
-                                   LitniceView out, float *lse, void *stream) {
+                                   LitniceView out, float *lse, void *workspace, uint64_t workspace_bytes, void *stream) {
   return guarded("attention_forward", [&] {
     TrainAttention a = attention_args(q, k, v, options);
     check_tensor(out, "out", 4, true);
     check_like(out, q, "out", "q");
     check_result(out, "out");
     check_floats(lse, "lse");
+    check_workspace(workspace, workspace_bytes, attention_workspace(q, k, false));
     a.out = head_view(out);
     a.lse = lse;
-    launch_train_attention_forward(a, static_cast<cudaStream_t>(stream));
+    launch_train_attention_forward(a, workspace, static_cast<cudaStream_t>(stream));
   });
+}
+
+uint64_t litnice_b200_attention_forward_workspace(LitniceView q, LitniceView k) {
+  uint64_t need = 0;
+  guarded("attention_forward_workspace", [&] {
+    check_tensor(q, "q", 4, true);
+    check_tensor(k, "k", 4, true);
+    need = attention_workspace(q, k, false);
+  });
+  return need;
 }
 
 uint64_t litnice_b200_attention_backward_workspace(LitniceView q, LitniceView k) {
@@ -175,7 +193,7 @@ uint64_t litnice_b200_attention_backward_workspace(LitniceView q, LitniceView k)
   guarded("attention_backward_workspace", [&] {
     check_tensor(q, "q", 4, true);
     check_tensor(k, "k", 4, true);
-    need = backward_workspace(q, k);
+    need = attention_workspace(q, k, true);
   });
   return need;
 }
@@ -199,14 +217,15 @@ int litnice_b200_attention_backward(LitniceView dout, LitniceView q, LitniceView
     check_result(dk, "dk");
     check_result(dv, "dv");
     check_floats(lse, "lse");
-    check_workspace(workspace, workspace_bytes, backward_workspace(q, k));
+    check_workspace(workspace, workspace_bytes, attention_workspace(q, k, true));
     a.dout = head_view(dout);
     a.out = head_view(out);
     a.dq = head_view(dq);
     a.dk = head_view(dk);
     a.dv = head_view(dv);
     a.lse = const_cast<float *>(lse);
-    launch_train_attention_backward(a, static_cast<float *>(workspace), static_cast<cudaStream_t>(stream));
+    launch_train_attention_backward(a, static_cast<float *>(workspace), static_cast<char *>(workspace) + delta_bytes(q),
+                                    static_cast<cudaStream_t>(stream));
   });
 }
 

@@ -432,7 +432,8 @@ void backward(const TrainAttention &a, float *delta, cudaStream_t st) {
 
 }  // namespace
 
-void launch_train_attention_forward(const TrainAttention &a, cudaStream_t st) {
+void launch_train_attention_forward(const TrainAttention &a, void *work, cudaStream_t st) {
+  if (train_attention_f32_supports(a.bf16, a.dim)) return launch_train_attention_forward_f32(a, work, st);
   if (train_attention_tc_supports(a, false)) return launch_train_attention_forward_tc(a, st);
   const TaArgs g = ta_args(a, nullptr, a.n);
   if (a.bf16) {
@@ -440,13 +441,11 @@ void launch_train_attention_forward(const TrainAttention &a, cudaStream_t st) {
     else if (a.dim <= 64) forward<64, bf16>(g, st);
     else forward<128, bf16>(g, st);
   } else {
-    if (a.dim <= 32) forward<32, float>(g, st);
-    else if (a.dim <= 64) forward<64, float>(g, st);
-    else forward<128, float>(g, st);
+    forward<128, float>(g, st);
   }
 }
 
-void launch_train_delta(const TrainAttention &a, float *delta, cudaStream_t st) {
+static void launch_train_delta(const TrainAttention &a, float *delta, cudaStream_t st) {
   const TaArgs g = ta_args(a, delta, a.n);
   const long long rows = (long long)a.streams * a.heads * a.n;
   if ((rows + 7) / 8 > 0x7fffffffLL) throw std::invalid_argument("attention: too many rows, heads and streams for one call");
@@ -455,7 +454,8 @@ void launch_train_delta(const TrainAttention &a, float *delta, cudaStream_t st) 
   LB_LAUNCH_CHECK();
 }
 
-void launch_train_attention_backward(const TrainAttention &a, float *delta, cudaStream_t st) {
+void launch_train_attention_backward(const TrainAttention &a, float *delta, void *work, cudaStream_t st) {
+  if (train_attention_f32_supports(a.bf16, a.dim)) return launch_train_attention_backward_f32(a, delta, work, st);
   launch_train_delta(a, delta, st);
   if (train_attention_tc_supports(a, true)) return launch_train_attention_backward_tc(a, delta, st);
   if (a.bf16) {
@@ -463,9 +463,7 @@ void launch_train_attention_backward(const TrainAttention &a, float *delta, cuda
     else if (a.dim <= 64) backward<64, bf16>(a, delta, st);
     else backward<128, bf16>(a, delta, st);
   } else {
-    if (a.dim <= 32) backward<32, float>(a, delta, st);
-    else if (a.dim <= 64) backward<64, float>(a, delta, st);
-    else backward<128, float>(a, delta, st);
+    backward<128, float>(a, delta, st);
   }
 }
 

@@ -19,63 +19,13 @@
 // Warp 0 issues TMA, warp 1 owns tensor memory and issues the MMAs. Rows outside the tensors load as zeros; keys behind a
 // stream's length are cleared in shared memory where a product would multiply them by a weight of zero. Every wait is bounded;
 // one that runs out ends the CTA, whose results are then NaN. No clusters, no multicast.
-#include "train_ops.cuh"
-#include "gemm_tc.cuh"
-#include "tc_ptx.cuh"
-
-#include <cuda_bf16.h>
+#include "train_attention_tc.cuh"
 
 namespace lb {
 
 namespace {
 
-typedef __nv_bfloat16 bf16;
-
-constexpr int TT_B = 128;
-constexpr int TT_SLAB = 128 * 128;  // 128 rows of 64 elements
-constexpr float TT_NEG = -1.0e30f, TT_SLACK = 8.f, TT_LOG2E = 1.4426950408889634f;
 constexpr int TT_FWD_THREADS = 192, TT_BWD_THREADS = 320;
-
-__device__ __forceinline__ float tt_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ unsigned tt_pack(float a, float b) {
-  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<const unsigned *>(&v);
-}
-
-struct TtArgs {
-  int n, m, heads, groups, share, streams, dim, tiles;
-  TrainSpan span;
-  const int *lengths;
-  float scale, factor;   // factor = scale * log2(e)
-  float *lse;
-  float *delta;
-  HeadView o1, o2;       // out | dq | dk, dv
-  int vec;               // results' rows on 16-byte boundaries
-};
-
-struct TtPlace {
-  int tile, head, stream, keys;
-};
-__device__ __forceinline__ TtPlace tt_place(const TtArgs &a, int heads, bool last_first) {
-  const int each = heads * a.streams, b = (int)blockIdx.x;
-  const int t = b / each, rest = b - t * each;
-  TtPlace p;
-  p.tile = last_first ? a.tiles - 1 - t : t;
-  p.stream = rest / heads;
-  p.head = rest - p.stream * heads;
-  p.keys = a.lengths ? max(0, min(a.m, a.lengths[p.stream])) : a.m;
-  return p;
-}
-
-__device__ __forceinline__ void tt_alloc(volatile unsigned *holder, unsigned cols) {
-  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void *)holder)), "r"(cols)
-               : "memory");
-  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-}
 
 // One row's columns c0 .. c0 + 15 of a result, as bfloat16.
 __device__ __forceinline__ void tt_store16(bf16 *row, const TtArgs &a, int c0, const float (&x)[16]) {
@@ -593,8 +543,9 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
   const unsigned q_full = bars, s_full = bars + 8, s_free = bars + 16, dp_full = bars + 24, ds_ready = bars + 32, done = bars + 40;
   auto k_full = [&](int s) { return bars + 48u + 8u * s; };
   auto k_empty = [&](int s) { return bars + 64u + 8u * s; };
-  volatile unsigned *tmem_holder = reinterpret_cast<volatile unsigned *>(base_ptr + L::BAR_OFF + 96);
-  volatile int *abort_flag = reinterpret_cast<volatile int *>(base_ptr + L::BAR_OFF + 100);
+  auto halves = [&](int q) { return bars + 80u + 8u * q; };  // of the two warps that share 32 rows
+  volatile unsigned *tmem_holder = reinterpret_cast<volatile unsigned *>(base_ptr + L::BAR_OFF + 112);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(base_ptr + L::BAR_OFF + 116);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const TtPlace at = tt_place(a, a.heads, a.span.causal != 0);
   const int r0 = at.tile * TT_B, r1 = min(r0 + TT_B, a.n), kh = at.head / a.share;
@@ -605,6 +556,7 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     for (unsigned bar : {q_full, s_full, dp_full, done}) mbar_init(bar, 1);
     mbar_init(s_free, 8);
     mbar_init(ds_ready, 8);
+    for (int q = 0; q < 4; ++q) mbar_init(halves(q), 2);
     for (int s = 0; s < 2; ++s) {
       mbar_init(k_full(s), 1);
       mbar_init(k_empty(s), 1);
@@ -729,7 +681,9 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       }
       float *both = stat + q * 32 + lane;
       both[half * 128] = t;
-      asm volatile("bar.sync 1, 256;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(halves(q));
+      if (!mbar_wait_warp(halves(q), 0, abort_flag, nullptr, 99)) return NAN;
       t = both[0] + both[128];
       if (half == 0 && row < a.n) a.delta[x] = t;
       return t;
@@ -817,30 +771,6 @@ CUtensorMap tt_map(const HeadView &x, long long streams, long long rows, long lo
 
 bool tt_rows16(const HeadView &x) {
   return x.c == 1 && reinterpret_cast<uintptr_t>(x.p) % 16 == 0 && x.s % 8 == 0 && x.r % 8 == 0 && x.h % 8 == 0;
-}
-
-TtArgs tt_args(const TrainAttention &a, int rows) {
-  TtArgs t{};
-  t.n = a.n;
-  t.m = a.m;
-  t.heads = a.heads;
-  t.groups = a.groups;
-  t.share = a.heads / a.groups;
-  t.streams = a.streams;
-  t.dim = a.dim;
-  t.tiles = (rows + TT_B - 1) / TT_B;
-  t.span = TrainSpan{a.first, a.window, a.causal};
-  t.lengths = a.lengths;
-  t.scale = a.scale;
-  t.factor = a.scale * TT_LOG2E;
-  t.lse = a.lse;
-  return t;
-}
-
-unsigned tt_grid(const TtArgs &t, int heads) {
-  const long long blocks = (long long)t.tiles * heads * t.streams;
-  if (blocks > 0x7fffffffLL) throw std::invalid_argument("attention: too many rows, heads and streams for one call");
-  return (unsigned)blocks;
 }
 
 template <int D>

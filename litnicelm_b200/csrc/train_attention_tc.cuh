@@ -1,0 +1,89 @@
+// What the tensor-core kernels of the training attention share (train_attention_tc.cu in bfloat16, train_attention_f32.cu in 32
+// bits): arguments, which tile a CTA has, small helpers.
+#pragma once
+
+#include "train_ops.cuh"
+#include "gemm_tc.cuh"
+#include "tc_ptx.cuh"
+
+#include <cuda_bf16.h>
+
+namespace lb {
+
+namespace {
+
+typedef __nv_bfloat16 bf16;
+
+constexpr int TT_B = 128;
+constexpr int TT_SLAB = 128 * 128;  // 128 rows of 64 elements
+constexpr float TT_NEG = -1.0e30f, TT_SLACK = 8.f, TT_LOG2E = 1.4426950408889634f;
+
+__device__ __forceinline__ float tt_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ unsigned tt_pack(float a, float b) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const unsigned *>(&v);
+}
+
+struct TtArgs {
+  int n, m, heads, groups, share, streams, dim, tiles;
+  TrainSpan span;
+  const int *lengths;
+  float scale, factor;   // factor = scale * log2(e)
+  float *lse;
+  float *delta;
+  HeadView o1, o2;       // out | dq | dk, dv
+  int vec;               // results' rows on 16-byte boundaries
+};
+
+struct TtPlace {
+  int tile, head, stream, keys;
+};
+__device__ __forceinline__ TtPlace tt_place(const TtArgs &a, int heads, bool last_first) {
+  const int each = heads * a.streams, b = (int)blockIdx.x;
+  const int t = b / each, rest = b - t * each;
+  TtPlace p;
+  p.tile = last_first ? a.tiles - 1 - t : t;
+  p.stream = rest / heads;
+  p.head = rest - p.stream * heads;
+  p.keys = a.lengths ? max(0, min(a.m, a.lengths[p.stream])) : a.m;
+  return p;
+}
+
+__device__ __forceinline__ void tt_alloc(volatile unsigned *holder, unsigned cols) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void *)holder)), "r"(cols)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+
+
+TtArgs tt_args(const TrainAttention &a, int rows) {
+  TtArgs t{};
+  t.n = a.n;
+  t.m = a.m;
+  t.heads = a.heads;
+  t.groups = a.groups;
+  t.share = a.heads / a.groups;
+  t.streams = a.streams;
+  t.dim = a.dim;
+  t.tiles = (rows + TT_B - 1) / TT_B;
+  t.span = TrainSpan{a.first, a.window, a.causal};
+  t.lengths = a.lengths;
+  t.scale = a.scale;
+  t.factor = a.scale * TT_LOG2E;
+  t.lse = a.lse;
+  return t;
+}
+
+unsigned tt_grid(const TtArgs &t, int heads) {
+  const long long blocks = (long long)t.tiles * heads * t.streams;
+  if (blocks > 0x7fffffffLL) throw std::invalid_argument("attention: too many rows, heads and streams for one call");
+  return (unsigned)blocks;
+}
+
+}  // namespace
+
+}  // namespace lb

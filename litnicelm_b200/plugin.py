@@ -128,7 +128,8 @@ NATIVE_SYMBOLS = [
     "litnice_b200_gemv_noalloc",
     "litnice_b200_session_create_model", "litnice_b200_architectures", "litnice_b200_model_dims",
     "litnice_b200_extend", "litnice_b200_release",
-    "litnice_b200_backend_stream", "litnice_b200_attention_forward", "litnice_b200_attention_backward_workspace",
+    "litnice_b200_backend_stream", "litnice_b200_attention_forward_workspace", "litnice_b200_attention_forward",
+    "litnice_b200_attention_backward_workspace",
     "litnice_b200_attention_backward", "litnice_b200_policy_loss_workspace", "litnice_b200_policy_loss",
     "litnice_b200_orthogonalise_workspace", "litnice_b200_orthogonalise", "litnice_b200_muon_step",
 ]

@@ -50,12 +50,12 @@ def _library():
     if _lib is None:
         lib = load_library()
         P, U = C.c_void_p, C.c_uint64
-        for name, args in (("attention_forward", [P] * 7), ("attention_backward", [P] * 11 + [U, P]),
+        for name, args in (("attention_forward", [P] * 7 + [U, P]), ("attention_backward", [P] * 11 + [U, P]),
                            ("policy_loss", [P] * 11 + [U, P]), ("orthogonalise", [P, P, C.c_int32, P, U, P]),
                            ("muon_step", [P] * 5 + [U, P])):
             fn = getattr(lib, "litnice_b200_" + name)
             fn.argtypes, fn.restype = args, C.c_int
-        for name, args in (("attention_backward", [P, P]), ("policy_loss", [P]), ("orthogonalise", [P])):
+        for name, args in (("attention_forward", [P, P]), ("attention_backward", [P, P]), ("policy_loss", [P]), ("orthogonalise", [P])):
             fn = getattr(lib, f"litnice_b200_{name}_workspace")
             fn.argtypes, fn.restype = args, U
         lib.litnice_b200_last_error.argtypes, lib.litnice_b200_last_error.restype = [P], C.c_char_p
@@ -159,7 +159,9 @@ def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scal
     call = _Call(q=q, k=k, v=v, out=out)
     o = _options(call, q, scale, causal, first, window, lengths)
     lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=q.device)
-    call(call.lib.litnice_b200_attention_forward, call["q"], call["k"], call["v"], C.addressof(o), call["out"], lse.data_ptr())
+    work = call.workspace(call.lib.litnice_b200_attention_forward_workspace(call["q"], call["k"]))
+    call(call.lib.litnice_b200_attention_forward, call["q"], call["k"], call["v"], C.addressof(o), call["out"], lse.data_ptr(),
+         work.data_ptr(), work.numel())
     return out, lse
 
 

@@ -39,13 +39,14 @@ def ref(t):
     return None if t is None else C.addressof(t)
 
 
-def forward(lib, q=None, k=None, v=None, out=None, lse=BASE, options=True, **o):
+def forward(lib, q=None, k=None, v=None, out=None, lse=BASE, options=True, work=BASE, size=1 << 30, **o):
     q = q or view((2, 8, 4, 16))
     k = k or view((2, 8, 2, 16))
     v = v or view((2, 8, 2, 16))
     out = out or view((2, 8, 4, 16), q.dtype)
     opts = training.AttentionOptions(o.get("scale", 0.25), 1, o.get("first", 0), o.get("window", 0), o.get("lengths"))
-    return lib.litnice_b200_attention_forward(ref(q), ref(k), ref(v), ref(opts) if options else None, ref(out), lse, None)
+    return lib.litnice_b200_attention_forward(ref(q), ref(k), ref(v), ref(opts) if options else None, ref(out), lse, work,
+                                              size, None)
 
 
 @pytest.mark.parametrize("more,why", [
@@ -76,6 +77,9 @@ def forward(lib, q=None, k=None, v=None, out=None, lse=BASE, options=True, **o):
     (dict(first=(1 << 30) - 4), "first"),
     (dict(window=-1), "window"),
     (dict(lengths=BASE + 2), "lengths"),
+    (dict(work=None), "null workspace"),
+    (dict(work=BASE + 128), "256-byte"),
+    (dict(size=0), "needed"),
 ], ids=lambda x: x if isinstance(x, str) else "")
 def test_attention_forward_refuses(lib, more, why):
     assert forward(lib, **more) == EINVAL
@@ -86,10 +90,11 @@ def test_attention_null_views(lib):
     o = training.AttentionOptions(1.0, 1, 0, 0, None)
     q = view((1, 1, 1, 4))
     for at in (0, 1, 2, 4):
-        args = [ref(q), ref(q), ref(q), ref(o), ref(q), BASE, None]
+        args = [ref(q), ref(q), ref(q), ref(o), ref(q), BASE, BASE, 1 << 30, None]
         args[at] = None
         assert lib.litnice_b200_attention_forward(*args) == EINVAL and "null view" in text(lib)
     assert lib.litnice_b200_attention_backward_workspace(None, None) == 0
+    assert lib.litnice_b200_attention_forward_workspace(ref(q), ref(view((2, 1, 1, 4)))) == 0 and "streams" in text(lib)
 
 
 def test_attention_backward_refuses(lib):
