@@ -4,6 +4,7 @@
 
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 #include <stdexcept>
 #include <string>
@@ -25,6 +26,20 @@ inline void cuda_check(cudaError_t e, const char *what, const char *file, int li
   }
 }
 #define LB_CUDA(expr) ::lb::cuda_check((expr), #expr, __FILE__, __LINE__)
+// cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) once per device: it costs as much host time as
+// a quarter of a launch.
+struct SharedMemoryOnce {
+  std::atomic<uint64_t> done{0};
+  template <typename K>
+  void set(K *kernel, int bytes) {
+    int dev = 0;
+    LB_CUDA(cudaGetDevice(&dev));
+    const uint64_t bit = 1ull << (dev & 63);
+    if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return;
+    LB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    done.fetch_or(bit, std::memory_order_relaxed);
+  }
+};
 #define LB_LAUNCH_CHECK() ::lb::cuda_check(cudaGetLastError(), "kernel launch", __FILE__, __LINE__)
 
 // The text that litnice_b200_last_error(NULL) gives this thread: of calls that have no session (session.cu).

@@ -655,7 +655,8 @@ void launch_product(const Operand &a, const Operand &b, const Operand &out, NsPr
   if (per * count > 0x3fffffffLL) throw std::invalid_argument("too many matrices of this size for one call");
   g.tiles = (int)(per * count);
   using L = NsSmem<PAIR>;
-  LB_CUDA(cudaFuncSetAttribute(ns_product_kernel<OP, A_MN, B_MN, PAIR, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL));
+  static SharedMemoryOnce once;
+  once.set(ns_product_kernel<OP, A_MN, B_MN, PAIR, SPLIT>, L::TOTAL);
   const int per_tile = SPLIT ? g.splits : CTAS, ctas = SPLIT || g.tiles < 148 / CTAS ? g.tiles : 148 / CTAS;
   launch_pdl_cluster_x(ns_product_kernel<OP, A_MN, B_MN, PAIR, SPLIT>, dim3((unsigned)(ctas * per_tile)), dim3(NS_THREADS), L::TOTAL, st,
                        true, (unsigned)per_tile, ns_map(a.p.hi, a, count, A_MN), ns_map(a.p.lo, a, count, A_MN), ns_map(b.p.hi, b, count, B_MN),

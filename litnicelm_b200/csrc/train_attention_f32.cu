@@ -816,7 +816,8 @@ void launch_train_attention_forward_f32(const TrainAttention &a, void *work, cud
   TtArgs t = tt_args(a, a.n);
   t.o1 = a.out;
   t.vec = rows16(a.out);
-  LB_CUDA(cudaFuncSetAttribute(train_forward_f32_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TF_FWD_SMEM));
+  static SharedMemoryOnce once;
+  once.set(train_forward_f32_kernel, TF_FWD_SMEM);
   launch_pdl(train_forward_f32_kernel, dim3(tt_grid(t, a.heads)), dim3(TF_THREADS), TF_FWD_SMEM, st, true, part_map(p[0]), part_map(p[1]),
              part_map(p[2]), t);
 }
@@ -830,13 +831,15 @@ void launch_train_attention_backward_f32(const TrainAttention &a, float *delta, 
   t.o1 = a.dk;
   t.o2 = a.dv;
   t.vec = rows16(a.dk) && rows16(a.dv);
-  LB_CUDA(cudaFuncSetAttribute(train_dkv_f32_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TF_SMEM));
+  static SharedMemoryOnce once_dkv;
+  once_dkv.set(train_dkv_f32_kernel, TF_SMEM);
   launch_pdl(train_dkv_f32_kernel, dim3(tt_grid(t, a.groups)), dim3(TF_THREADS), TF_SMEM, st, true, mq, mk, mv, md, t);
   t = tt_args(a, a.n);
   t.delta = delta;
   t.o1 = a.dq;
   t.vec = rows16(a.dq);
-  LB_CUDA(cudaFuncSetAttribute(train_dq_f32_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TF_SMEM));
+  static SharedMemoryOnce once_dq;
+  once_dq.set(train_dq_f32_kernel, TF_SMEM);
   launch_pdl(train_dq_f32_kernel, dim3(tt_grid(t, a.heads)), dim3(TF_THREADS), TF_SMEM, st, true, mq, mk, mv, md, t);
 }
 

@@ -779,7 +779,8 @@ void forward(const TrainAttention &a, cudaStream_t st) {
   t.o1 = a.out;
   t.vec = tt_rows16(a.out);
   const size_t smem = 3 * (size_t)(D / 64) * TT_SLAB + 128 + 1024;
-  LB_CUDA(cudaFuncSetAttribute(train_forward_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  static SharedMemoryOnce once;
+  once.set(train_forward_tc_kernel<D>, (int)smem);
   train_forward_tc_kernel<D><<<tt_grid(t, a.heads), TT_FWD_THREADS, smem, st>>>(
       tt_map(a.q, a.streams, a.n, a.heads, a.dim), tt_map(a.k, a.streams, a.m, a.groups, a.dim),
       tt_map(a.v, a.streams, a.m, a.groups, a.dim), t);
@@ -795,7 +796,8 @@ void backward(const TrainAttention &a, float *delta, cudaStream_t st) {
   t.delta = delta;
   t.o1 = a.dq;
   t.vec = tt_rows16(a.dq);
-  LB_CUDA(cudaFuncSetAttribute(train_dq_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  static SharedMemoryOnce once_dq;
+  once_dq.set(train_dq_tc_kernel<D>, smem);
   train_dq_tc_kernel<D><<<tt_grid(t, a.heads), TT_BWD_THREADS, smem, st>>>(mq, mk, mv, md, t);
   LB_LAUNCH_CHECK();
   t = tt_args(a, a.m);
@@ -803,7 +805,8 @@ void backward(const TrainAttention &a, float *delta, cudaStream_t st) {
   t.o1 = a.dk;
   t.o2 = a.dv;
   t.vec = tt_rows16(a.dk) && tt_rows16(a.dv);
-  LB_CUDA(cudaFuncSetAttribute(train_dkv_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  static SharedMemoryOnce once_dkv;
+  once_dkv.set(train_dkv_tc_kernel<D>, smem);
   train_dkv_tc_kernel<D><<<tt_grid(t, a.groups), TT_BWD_THREADS, smem, st>>>(mq, mk, mv, md, t);
   LB_LAUNCH_CHECK();
 }

@@ -43,6 +43,12 @@ class MuonOptions(C.Structure):
 
 
 _lib = None
+_GRAD_REFUSED = " requires a gradient: the operators here have explicit backward calls (use torch.no_grad() or detach())"
+_PAD = tuple((0,) * (6 - rank) for rank in range(7))
+# what torch.cuda.current_stream(index).cuda_stream and torch.cuda.current_device() say, without the objects around it: a
+# quarter of the host's time in a small call
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _library():
@@ -55,7 +61,8 @@ def _library():
                            ("muon_step", [P] * 5 + [U, P])):
             fn = getattr(lib, "litnice_b200_" + name)
             fn.argtypes, fn.restype = args, C.c_int
-        for name, args in (("attention_forward", [P, P]), ("attention_backward", [P, P]), ("policy_loss", [P]), ("orthogonalise", [P])):
+        for name, args in (("attention_forward", [P, P]), ("attention_backward", [P, P]), ("policy_loss", [P]),
+                           ("orthogonalise", [P])):
             fn = getattr(lib, f"litnice_b200_{name}_workspace")
             fn.argtypes, fn.restype = args, U
         lib.litnice_b200_last_error.argtypes, lib.litnice_b200_last_error.restype = [P], C.c_char_p
@@ -63,88 +70,86 @@ def _library():
     return _lib
 
 
-class _Call:
-    """Views of a call's tensors, checked to be CUDA tensors of one device that autograd does not record."""
+def _error(rc: int) -> Exception:
+    text = _library().litnice_b200_last_error(None).decode()
+    return ValueError(text) if rc == -1 else NativeError(f"{text} ({rc})")
 
-    def __init__(self, **tensors):
-        self.lib = _library()
-        recording = torch.is_grad_enabled()
-        device, at, raw = None, 0, bytearray(_VIEW.size * len(tensors))
-        self.offset = {}
-        for name, t in tensors.items():
-            if not isinstance(t, torch.Tensor):
-                raise TypeError(f"{name} is not a tensor")
-            if device is None:
-                device = t.device
-                if device.type != "cuda":
-                    raise ValueError(f"{name} is not a CUDA tensor")
-            elif t.device != device:
-                raise ValueError(f"{name} is on {t.device}, not on {device}")
-            if recording and t.requires_grad:
-                raise ValueError(f"{name} requires a gradient: the operators here have explicit backward calls "
-                                 "(use torch.no_grad() or detach())")
-            kind = _KINDS.get(t.dtype)
-            if kind is None:
-                raise TypeError(f"{name} has type {t.dtype}")
-            shape, rank, size = t.shape, t.dim(), t.element_size()
-            if rank > 6:
-                raise ValueError(f"{name} has {rank} axes")
-            strides = t.stride()
-            more = (0,) * (6 - rank)
-            _VIEW.pack_into(raw, at, 1, kind, t.data_ptr(), rank, shape[0] if rank else 0, shape[1] if rank > 1 else 0,
-                            strides[-2] * size if rank > 1 else 0, strides[-1] * size if rank else 0,
-                            *shape, *more, *[x * size for x in strides], *more)
-            self.offset[name] = at
-            at += _VIEW.size
-        self.device = device
-        self.raw = (C.c_char * len(raw)).from_buffer(raw)
-        self.base = C.addressof(self.raw)
 
-    def __getitem__(self, name):
-        return self.base + self.offset[name]
+def _tensor(t, name: str):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} is not a tensor")
 
-    def workspace(self, nbytes: int) -> torch.Tensor:
-        if nbytes == 0:
-            raise self.error(-1)
-        return torch.empty(nbytes, dtype=torch.uint8, device=self.device)
 
-    def error(self, rc: int) -> Exception:
-        text = self.lib.litnice_b200_last_error(None).decode()
-        return ValueError(text) if rc == -1 else NativeError(f"{text} ({rc})")
+def _views(names, tensors):
+    """(addresses of the tensors' views, the memory that holds them), checked to be CUDA tensors of one device that autograd does
+    not record."""
+    recording = torch.is_grad_enabled()
+    device, at, raw = None, 0, bytearray(152 * len(tensors))
+    for name, t in zip(names, tensors):
+        _tensor(t, name)
+        if device is None:
+            device = t.device
+            if device.type != "cuda":
+                raise ValueError(f"{name} is not a CUDA tensor")
+        elif t.device != device:
+            raise ValueError(f"{name} is on {t.device}, not on {device}")
+        if recording and t.requires_grad:
+            raise ValueError(name + _GRAD_REFUSED)
+        kind = _KINDS.get(t.dtype)
+        if kind is None:
+            raise TypeError(f"{name} has type {t.dtype}")
+        shape, size = t.shape, t.element_size()
+        rank = len(shape)
+        if rank > 6:
+            raise ValueError(f"{name} has {rank} axes")
+        more = _PAD[rank]
+        # (rows, cols and their strides repeat the axes; these entries read the axes)
+        _VIEW.pack_into(raw, at, 1, kind, t.data_ptr(), rank, 0, 0, 0, 0, *shape, *more, *[x * size for x in t.stride()], *more)
+        at += 152
+    held = (C.c_char * at).from_buffer(raw)
+    base = C.addressof(held)
+    return range(base, base + at, 152), held
 
-    def __call__(self, fn, *args):
-        """The entry point on the current stream of the tensors' device."""
-        index = self.device.index
-        if index == torch.cuda.current_device():
-            rc = fn(*args, torch.cuda.current_stream(index).cuda_stream)
-        else:
-            with torch.cuda.device(index):
-                rc = fn(*args, torch.cuda.current_stream(index).cuda_stream)
-        if rc != 0:
-            raise self.error(rc)
+
+def _run(device: torch.device, fn, *args):
+    """The entry point on the current stream of the tensors' device."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc != 0:
+        raise _error(rc)
+
+
+def _workspace(nbytes: int, device) -> torch.Tensor:
+    if nbytes == 0:
+        raise _error(-1)
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 
 def _vector(t: Optional[torch.Tensor], name: str, count: int, dtype, device) -> Optional[int]:
     """Address of a dense vector of `count` elements."""
     if t is None:
         return None
+    _tensor(t, name)
     if t.dtype != dtype or t.shape != (count,) or (count > 1 and t.stride(0) != 1):
         raise ValueError(f"{name} must be a dense {dtype} vector of {count} elements")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, not on {device}")
     if t.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{name} requires a gradient: the operators here have explicit backward calls "
-                         "(use torch.no_grad() or detach())")
+        raise ValueError(name + _GRAD_REFUSED)
     return t.data_ptr()
 
 
-def _options(call: _Call, q: torch.Tensor, scale, causal, first, window, lengths) -> AttentionOptions:
+def _options(q: torch.Tensor, scale, causal, first, window, lengths) -> AttentionOptions:
     if q.dim() != 4:
         raise ValueError("q must be [streams, rows, heads, dim]")
     if not (0 <= first < 1 << 30 and 0 <= window < 1 << 30):
         raise ValueError("first and window must be at least 0")
     return AttentionOptions(1 / math.sqrt(max(1, q.shape[3])) if scale is None else scale, 1 if causal else 0, first, window,
-                            _vector(lengths, "lengths", q.shape[0], torch.int32, call.device))
+                            _vector(lengths, "lengths", q.shape[0], torch.int32, q.device))
 
 
 def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: Optional[float] = None, causal: bool = True,
@@ -155,13 +160,15 @@ def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scal
 
     Row i stands at position first + i and sees key j if j < m, j < lengths[stream], with ``causal`` j <= first + i, with a
     ``window`` j > first + i - window. A row that sees no key has out 0 and lse -inf. scale: 1 / sqrt(dim) if None."""
+    _tensor(q, "q")
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
-    call = _Call(q=q, k=k, v=v, out=out)
-    o = _options(call, q, scale, causal, first, window, lengths)
-    lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=q.device)
-    work = call.workspace(call.lib.litnice_b200_attention_forward_workspace(call["q"], call["k"]))
-    call(call.lib.litnice_b200_attention_forward, call["q"], call["k"], call["v"], C.addressof(o), call["out"], lse.data_ptr(),
-         work.data_ptr(), work.numel())
+    (vq, vk, vv, vo), held = _views(("q", "k", "v", "out"), (q, k, v, out))
+    o = _options(q, scale, causal, first, window, lengths)
+    streams, n, heads = q.shape[:3]
+    lse = torch.empty((streams, heads, n), dtype=torch.float32, device=q.device)
+    lib = _library()
+    work = _workspace(lib.litnice_b200_attention_forward_workspace(vq, vk), q.device)
+    _run(q.device, lib.litnice_b200_attention_forward, vq, vk, vv, C.addressof(o), vo, lse.data_ptr(), work.data_ptr(), work.numel())
     return out, lse
 
 
@@ -172,17 +179,20 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
                        dv: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(dq, dk, dv): gradients of sum(out * dout), from what ``attention_forward`` with the same options returned. Key heads
     shared by query heads receive the sum over those. dq, dk and dv may be given, slices of one buffer for instance."""
+    for t, name in ((q, "q"), (k, "k"), (v, "v"), (lse, "lse")):
+        _tensor(t, name)
     dq = torch.empty(q.shape, dtype=q.dtype, device=q.device) if dq is None else dq
     dk = torch.empty(k.shape, dtype=k.dtype, device=k.device) if dk is None else dk
     dv = torch.empty(v.shape, dtype=v.dtype, device=v.device) if dv is None else dv
-    call = _Call(dout=dout, q=q, k=k, v=v, out=out, dq=dq, dk=dk, dv=dv)
-    o = _options(call, q, scale, causal, first, window, lengths)
-    if lse.dtype != torch.float32 or lse.shape != (q.shape[0], q.shape[2], q.shape[1]) or not lse.is_contiguous() or \
-            lse.device != call.device:
+    (vd, vq, vk, vv, vo, wq, wk, wv), held = _views(("dout", "q", "k", "v", "out", "dq", "dk", "dv"), (dout, q, k, v, out, dq, dk, dv))
+    o = _options(q, scale, causal, first, window, lengths)
+    streams, n, heads = q.shape[:3]
+    if lse.dtype != torch.float32 or lse.shape != (streams, heads, n) or not lse.is_contiguous() or lse.device != q.device:
         raise ValueError("lse must be what attention_forward returned")
-    work = call.workspace(call.lib.litnice_b200_attention_backward_workspace(call["q"], call["k"]))
-    call(call.lib.litnice_b200_attention_backward, call["dout"], call["q"], call["k"], call["v"], call["out"], lse.data_ptr(),
-         C.addressof(o), call["dq"], call["dk"], call["dv"], work.data_ptr(), work.numel())
+    lib = _library()
+    work = _workspace(lib.litnice_b200_attention_backward_workspace(vq, vk), q.device)
+    _run(q.device, lib.litnice_b200_attention_backward, vd, vq, vk, vv, vo, lse.data_ptr(), C.addressof(o), wq, wk, wv,
+         work.data_ptr(), work.numel())
     return dq, dk, dv
 
 
@@ -197,30 +207,36 @@ def policy_loss(logits: torch.Tensor, targets: torch.Tensor, old_logp: torch.Ten
     loss = sum weight (-min(r advantage, clip(r, 1 - clip_low, 1 + clip_high) advantage) + kl_weight (exp d - d - 1)) / sum weight.
     Rows of weight 0 are not read; their logp and gradient are 0. A target outside the vocabulary in another row gives NaN there
     and in the loss. dlogits may be given, logits itself included; with ``gradient`` false it is None."""
-    if gradient and dlogits is None:
-        dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    call = _Call(logits=logits, dlogits=dlogits) if gradient else _Call(logits=logits)
+    _tensor(logits, "logits")
     if logits.dim() != 2:
         raise ValueError("logits must be [rows, vocab]")
-    rows, dev = logits.shape[0], call.device
+    rows, dev = logits.shape[0], logits.device
+    if gradient:
+        dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=dev) if dlogits is None else dlogits
+        (vz, vd), held = _views(("logits", "dlogits"), (logits, dlogits))
+    else:
+        (vz,), held = _views(("logits",), (logits,))
+        vd = dlogits = None
     o = PolicyOptions(temp, clip_low, clip_high, kl_weight)
-    results = torch.empty(rows + 1, dtype=torch.float32, device=dev)
-    work = call.workspace(call.lib.litnice_b200_policy_loss_workspace(call["logits"]))
-    call(call.lib.litnice_b200_policy_loss, call["logits"], _vector(targets, "targets", rows, torch.int32, dev),
+    loss, logp = torch.empty((), dtype=torch.float32, device=dev), torch.empty(rows, dtype=torch.float32, device=dev)
+    lib = _library()
+    work = _workspace(lib.litnice_b200_policy_loss_workspace(vz), dev)
+    _run(dev, lib.litnice_b200_policy_loss, vz, _vector(targets, "targets", rows, torch.int32, dev),
          _vector(old_logp, "old_logp", rows, torch.float32, dev), _vector(advantage, "advantage", rows, torch.float32, dev),
          _vector(ref_logp, "ref_logp", rows, torch.float32, dev), _vector(weight, "weight", rows, torch.float32, dev),
-         C.addressof(o), results.data_ptr() + 4 * rows, results.data_ptr(), call["dlogits"] if gradient else None,
-         work.data_ptr(), work.numel())
-    return results[rows], results[:rows], dlogits if gradient else None
+         C.addressof(o), loss.data_ptr(), logp.data_ptr(), vd, work.data_ptr(), work.numel())
+    return loss, logp, dlogits
 
 
 def orthogonalise(x: torch.Tensor, *, steps: int = 5, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Every matrix of x [..., m, n] float32 with its singular values driven towards 1: X = x / (|x| + 1e-7), then ``steps`` times
     X <- 3.4445 X + (-4.7750 A + 2.0315 A A) X with A = X X^T (in the smaller side's space). out may be x."""
+    _tensor(x, "x")
     out = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
-    call = _Call(x=x, out=out)
-    work = call.workspace(call.lib.litnice_b200_orthogonalise_workspace(call["x"]))
-    call(call.lib.litnice_b200_orthogonalise, call["x"], call["out"], steps, work.data_ptr(), work.numel())
+    (vx, vo), held = _views(("x", "out"), (x, out))
+    lib = _library()
+    work = _workspace(lib.litnice_b200_orthogonalise_workspace(vx), x.device)
+    _run(x.device, lib.litnice_b200_orthogonalise, vx, vo, steps, work.data_ptr(), work.numel())
     return out
 
 
@@ -228,8 +244,8 @@ def muon_step(params: torch.Tensor, grads: torch.Tensor, momentum: torch.Tensor,
               weight_decay: float = 0.0, nesterov: bool = True, steps: int = 5) -> None:
     """One optimiser step on matrices [..., m, n] float32, in place: momentum <- mu momentum + grads, U = grads + mu momentum (or
     momentum without ``nesterov``), params <- (1 - lr weight_decay) params - lr sqrt(max(1, m / n)) orthogonalise(U)."""
-    call = _Call(params=params, grads=grads, momentum=momentum)
+    (vp, vg, vm), held = _views(("params", "grads", "momentum"), (params, grads, momentum))
     o = MuonOptions(lr, mu, weight_decay, 1 if nesterov else 0, steps)
-    work = call.workspace(call.lib.litnice_b200_orthogonalise_workspace(call["grads"]))
-    call(call.lib.litnice_b200_muon_step, call["params"], call["grads"], call["momentum"], C.addressof(o), work.data_ptr(),
-         work.numel())
+    lib = _library()
+    work = _workspace(lib.litnice_b200_orthogonalise_workspace(vg), grads.device)
+    _run(grads.device, lib.litnice_b200_muon_step, vp, vg, vm, C.addressof(o), work.data_ptr(), work.numel())
