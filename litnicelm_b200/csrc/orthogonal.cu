@@ -409,18 +409,17 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_ah, const __grid_const
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         if (lane == 0) {
           const unsigned st = base + (unsigned)(s * L::STAGE), d = tmem + (unsigned)(buf * T);
-          auto desc = [&](int t, bool mn, int ks) {
-            const unsigned p = st + (unsigned)(t * L::TILE);
-            return mn ? umma_desc_mn128(p + (unsigned)(ks * 2048), 8192u) : umma_desc_k128(p) + (unsigned long long)(ks * 2);
-          };
+          const unsigned long long a0 = A_MN ? umma_desc_mn128(st, 8192u) : umma_desc_k128(st);
+          const unsigned long long b0 = B_MN ? umma_desc_mn128(st + 2 * L::TILE, 8192u) : umma_desc_k128(st + 2 * L::TILE);
+          auto a = [&](int part, int ks) { return a0 + (unsigned long long)(part * (L::TILE >> 4) + ks * (A_MN ? 2048 >> 4 : 2)); };
+          auto b = [&](int part, int ks) { return b0 + (unsigned long long)(part * (L::TILE >> 4) + ks * (B_MN ? 2048 >> 4 : 2)); };
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks) {
-            ns_mma<PAIR>(d, desc(0, A_MN, ks), desc(3, B_MN, ks), idesc, ks ? NS_ADD : NS_NEW);
-            ns_mma<PAIR>(d, desc(1, A_MN, ks), desc(2, B_MN, ks), idesc, NS_ADD);
+            ns_mma<PAIR>(d, a(0, ks), b(1, ks), idesc, ks ? NS_ADD : NS_NEW);
+            ns_mma<PAIR>(d, a(1, ks), b(0, ks), idesc, NS_ADD);
           }
 #pragma unroll
-          for (int ks = 0; ks < 4; ++ks)
-            ns_mma<PAIR>(d, desc(0, A_MN, ks), desc(2, B_MN, ks), idesc, ks ? NS_ADD : NS_SCALED);
+          for (int ks = 0; ks < 4; ++ks) ns_mma<PAIR>(d, a(0, ks), b(0, ks), idesc, ks ? NS_ADD : NS_SCALED);
           ns_commit<PAIR>(empty(s));
           ns_commit<PAIR>(chain_full(buf));
         }

@@ -56,7 +56,7 @@ struct TaArgs {
   int tiles;        // of 64 rows (or keys) per head
   unsigned vec;     // bit per view: rows can be read four elements at a time
 };
-enum { VQ = 1, VK = 2, VV = 4, VDO = 8 };
+enum { VQ = 1, VK = 2, VV = 4, VDO = 8, VO = 16 };
 
 // Rows r0 .. r0 + 63 of a head into shared memory, those from `end` on and the columns behind dim as zeros.
 template <int D, typename T>
@@ -248,21 +248,30 @@ train_attention_forward_kernel(const __grid_constant__ TaArgs g) {
   store_tile<D, T>(a.out, at.stream * a.out.s + at.head * a.out.h, r0, a.n, a.dim, o, inv);
 }
 
+// A row by 16 lanes, eight elements each at a time.
 template <typename T>
 __global__ void __launch_bounds__(256) train_delta_kernel(const __grid_constant__ TaArgs g) {
   const TrainAttention &a = g.a;
-  const long long row = blockIdx.x * 8LL + (threadIdx.x >> 5);  // in the order of delta
-  if (row >= (long long)a.streams * a.heads * a.n) return;
-  const int lane = threadIdx.x & 31;
-  const int i = (int)(row % a.n), h = (int)(row / a.n % a.heads);
-  const long long s = row / a.n / a.heads;
+  // rows in the order of memory as layers leave it, [streams, n, heads]: neighbours of a warp read on
+  const long long rows = (long long)a.streams * a.heads * a.n, mine = blockIdx.x * 16LL + (threadIdx.x >> 4);
+  const long long at = mine < rows ? mine : rows - 1;
+  const int lane = threadIdx.x & 15;
+  const long long si = at / a.heads, s = si / a.n;
+  const int h = (int)(at - si * a.heads), i = (int)(si - s * a.n);
   const T *x = reinterpret_cast<const T *>(a.out.p) + s * a.out.s + (long long)i * a.out.r + h * a.out.h;
   const T *y = reinterpret_cast<const T *>(a.dout.p) + s * a.dout.s + (long long)i * a.dout.r + h * a.dout.h;
   float t = 0.f;
-  for (int c = lane; c < a.dim; c += 32) t = fmaf(to_float(x[c * a.out.c]), to_float(y[c * a.dout.c]), t);
+  for (int c = lane * 8; c < a.dim; c += 128) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-  if (lane == 0) g.delta[row] = t;
+    for (int e = 0; e < 8; e += 4) {
+      const float4 u = load4<T>(x + (c + e) * a.out.c, a.out.c, a.dim - c - e, g.vec & VO);
+      const float4 v = load4<T>(y + (c + e) * a.dout.c, a.dout.c, a.dim - c - e, g.vec & VDO);
+      t = fmaf(u.x, v.x, fmaf(u.y, v.y, fmaf(u.z, v.z, fmaf(u.w, v.w, t))));
+    }
+  }
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+  if (lane == 0 && mine < rows) g.delta[(s * a.heads + h) * a.n + i] = t;
 }
 
 template <int D, typename T>
@@ -401,7 +410,7 @@ TaArgs ta_args(const TrainAttention &a, float *delta, int rows) {
   g.delta = delta;
   g.tiles = (rows + TA_B - 1) / TA_B;
   g.vec = (rows_vec(a.q, a.bf16) ? VQ : 0) | (rows_vec(a.k, a.bf16) ? VK : 0) | (rows_vec(a.v, a.bf16) ? VV : 0) |
-          (a.dout.p && rows_vec(a.dout, a.bf16) ? VDO : 0);
+          (a.dout.p && rows_vec(a.dout, a.bf16) ? VDO : 0) | (a.out.p && rows_vec(a.out, a.bf16) ? VO : 0);
   return g;
 }
 
@@ -448,9 +457,9 @@ void launch_train_attention_forward(const TrainAttention &a, void *work, cudaStr
 static void launch_train_delta(const TrainAttention &a, float *delta, cudaStream_t st) {
   const TaArgs g = ta_args(a, delta, a.n);
   const long long rows = (long long)a.streams * a.heads * a.n;
-  if ((rows + 7) / 8 > 0x7fffffffLL) throw std::invalid_argument("attention: too many rows, heads and streams for one call");
-  if (a.bf16) train_delta_kernel<bf16><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(g);
-  else train_delta_kernel<float><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(g);
+  if ((rows + 15) / 16 > 0x7fffffffLL) throw std::invalid_argument("attention: too many rows, heads and streams for one call");
+  if (a.bf16) train_delta_kernel<bf16><<<(unsigned)((rows + 15) / 16), 256, 0, st>>>(g);
+  else train_delta_kernel<float><<<(unsigned)((rows + 15) / 16), 256, 0, st>>>(g);
   LB_LAUNCH_CHECK();
 }
 

@@ -94,19 +94,23 @@ __global__ void __launch_bounds__(256) train_split_kernel(const __grid_constant_
 
 // Parts of the two operands of a product, in the order of their size.
 
-// The product of rows of a and rows of b over the (up to 64) dimensions.
-__device__ __forceinline__ void tf_mma_rows(unsigned d, unsigned a, unsigned b, int ksteps, unsigned idesc) {
+// The product of rows of a and rows of b over the (up to 64) dimensions, smallest parts first. (Descriptors differ by constants:
+// see tt_mma_rows in train_attention_tc.cu.)
+__device__ __forceinline__ void tf_mma_rows(unsigned d, unsigned a, unsigned b, unsigned idesc) {
+  const unsigned long long da = umma_desc_k128(a), db = umma_desc_k128(b);
 #pragma unroll
   for (int p = 0; p < 6; ++p) {
     const int pa = p == 0 ? 0 : p == 1 ? 2 : p == 2 ? 1 : p == 3 ? 0 : p == 4 ? 1 : 0;
     const int pb = p == 0 ? 2 : p == 1 ? 0 : p == 2 ? 1 : p == 3 ? 1 : p == 4 ? 0 : 0;
-    const unsigned long long da = umma_desc_k128(a + pa * TF_PART), db = umma_desc_k128(b + pb * TF_PART);
-    for (int ks = 0; ks < ksteps; ++ks)
-      tc_mma_f16(d, da + (unsigned long long)(ks * 2), db + (unsigned long long)(ks * 2), idesc, (p | ks) ? 1u : 0u);
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks)
+      tc_mma_f16(d, da + (unsigned long long)(pa * (TF_PART >> 4) + ks * 2), db + (unsigned long long)(pb * (TF_PART >> 4) + ks * 2), idesc,
+                 (p | ks) ? 1u : 0u);
   }
 }
 // Weights in tensor memory (parts where tf_store_parts puts them) by rows of b.
 __device__ __forceinline__ void tf_mma_weights(unsigned d, unsigned w, unsigned b, unsigned idesc) {
+  const unsigned long long db = umma_desc_mn128(b, TT_SLAB);
 #pragma unroll
   for (int p = 0; p < 6; ++p) {
     const int pa = p == 0 ? 0 : p == 1 ? 2 : p == 2 ? 1 : p == 3 ? 0 : p == 4 ? 1 : 0;
@@ -114,7 +118,7 @@ __device__ __forceinline__ void tf_mma_weights(unsigned d, unsigned w, unsigned 
 #pragma unroll
     for (int ks = 0; ks < TT_B / 16; ++ks) {
       const unsigned at = pa == 2 ? 128u + (unsigned)(ks * 8) : (unsigned)((ks >> 2) * 64 + pa * 32 + (ks & 3) * 8);
-      tc_mma_f16_ts(d, w + at, umma_desc_mn128(b + (unsigned)(pb * TF_PART + ks * 16 * 128), TT_SLAB), idesc, (p | ks) ? 1u : 0u);
+      tc_mma_f16_ts(d, w + at, db + (unsigned long long)((pb * TF_PART + ks * 16 * 128) >> 4), idesc, (p | ks) ? 1u : 0u);
     }
   }
 }
@@ -245,7 +249,7 @@ train_forward_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       while (v_loads > 0 && !mbar_try_wait(v_full, (unsigned)(v_loads - 1) & 1u) && global_timer() < limit) {}
     }
   } else if (warp == 1) {
-    const int cols = (a.dim + 15) & ~15, ksteps = cols >> 4;
+    const int cols = (a.dim + 15) & ~15;
     const unsigned idesc_s = umma_idesc_bf16(TT_B), idesc_o = umma_idesc_bf16(cols) | UMMA_B_MN_MAJOR;
     bool ok = tiles > 0 ? TF_WAIT(q_full, 0, 103) : true;
     int i = 0;
@@ -254,7 +258,7 @@ train_forward_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       if (!ok) break;
       TF_AFTER();
       if (lane == 0) {
-        tf_mma_rows(tmem_s, q_off, k_off, ksteps, idesc_s);
+        tf_mma_rows(tmem_s, q_off, k_off, idesc_s);
         tc_commit(s_full);
       }
       __syncwarp();
@@ -444,7 +448,7 @@ train_dkv_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       while (it > 0 && !mbar_try_wait(do_full, (unsigned)(it - 1) & 1u) && global_timer() < limit) {}
     }
   } else if (warp == 1) {
-    const int cols = (a.dim + 15) & ~15, ksteps = cols >> 4;
+    const int cols = (a.dim + 15) & ~15;
     const unsigned idesc_s = umma_idesc_bf16(TT_B), idesc_d = umma_idesc_bf16(cols) | UMMA_B_MN_MAJOR;
     bool ok = tiles > 0 ? TF_WAIT(kv_full, 0, 112) : true;
     int i = 0;
@@ -453,14 +457,14 @@ train_dkv_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       if (!ok) break;
       TF_AFTER();
       if (lane == 0) {
-        tf_mma_rows(tmem_s, k_off, q_off, ksteps, idesc_s);
+        tf_mma_rows(tmem_s, k_off, q_off, idesc_s);
         tc_commit(s_full);
       }
       __syncwarp();
       ok = TF_WAIT(do_full, i, 114);
       if (!ok) break;
       if (lane == 0) {
-        tf_mma_rows(tmem_dp, v_off, do_off, ksteps, idesc_s);
+        tf_mma_rows(tmem_dp, v_off, do_off, idesc_s);
         tc_commit(dp_full);
       }
       __syncwarp();
@@ -650,7 +654,7 @@ train_dq_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       while (k_loads > 0 && !mbar_try_wait(k_full, (unsigned)(k_loads - 1) & 1u) && global_timer() < limit) {}
     }
   } else if (warp == 1) {
-    const int cols = (a.dim + 15) & ~15, ksteps = cols >> 4;
+    const int cols = (a.dim + 15) & ~15;
     const unsigned idesc_s = umma_idesc_bf16(TT_B), idesc_d = umma_idesc_bf16(cols) | UMMA_B_MN_MAJOR;
     bool ok = tiles > 0 ? TF_WAIT(q_full, 0, 133) : true;
     int i = 0;
@@ -660,14 +664,14 @@ train_dq_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       TF_AFTER();
       // (over dP and its parts: dS k of the tile before has read them, in the order of issue; over S: read before ds_ready)
       if (lane == 0) {
-        tf_mma_rows(tmem_dp, do_off, v_off, ksteps, idesc_s);
+        tf_mma_rows(tmem_dp, do_off, v_off, idesc_s);
         tc_commit(dp_full);
       }
       __syncwarp();
       ok = TF_WAIT(k_full, i, 135);
       if (!ok) break;
       if (lane == 0) {
-        tf_mma_rows(tmem_s, q_off, k_off, ksteps, idesc_s);
+        tf_mma_rows(tmem_s, q_off, k_off, idesc_s);
         tc_commit(s_full);
       }
       __syncwarp();

@@ -71,14 +71,28 @@ __device__ __forceinline__ void tt_clear_rows(unsigned char *tile, int slabs, in
   __syncwarp();
 }
 
-// S (128 x 128) = rows of a . rows of b over dim, both with contiguous dim
-__device__ __forceinline__ void tt_mma_rows(unsigned d, unsigned a, unsigned b, int ksteps, unsigned idesc) {
-  for (int ks = 0; ks < ksteps; ++ks) {
-    const unsigned slab = (unsigned)((ks >> 2) * TT_SLAB);
-    const unsigned long long in = (unsigned long long)((ks & 3) * 2);
-    tc_mma_f16(d, umma_desc_k128(a + slab) + in, umma_desc_k128(b + slab) + in, idesc, ks ? 1u : 0u);
+// S (128 x 128) = rows of a . rows of b over dim, both with contiguous dim. The loops that issue products are unrolled, with
+// descriptors that differ by constants: with a loop over the steps that dim needs, each instruction's descriptors took the one
+// issuing thread about 130 clocks, twice what the tensor pipe takes for the product.
+template <int D>
+__device__ __forceinline__ void tt_mma_rows(unsigned d, unsigned long long a, unsigned long long b, unsigned idesc) {
+#pragma unroll
+  for (int ks = 0; ks < D / 16; ++ks) {
+    const unsigned long long at = (unsigned long long)((ks >> 2) * (TT_SLAB >> 4) + (ks & 3) * 2);
+    tc_mma_f16(d, a + at, b + at, idesc, ks ? 1u : 0u);
   }
 }
+// d (+)= weights in tensor memory (columns from w on; HALVES: two groups of 32, 64 apart) . rows of b, 128 of k
+template <bool HALVES>
+__device__ __forceinline__ void tt_mma_weights(unsigned d, unsigned w, unsigned long long b, unsigned idesc, bool more) {
+#pragma unroll
+  for (int ks = 0; ks < TT_B / 16; ++ks)
+    tc_mma_f16_ts(d, w + (unsigned)(HALVES ? (ks >> 2) * 64 + (ks & 3) * 8 : ks * 8), b + (unsigned long long)(ks * (16 * 128 >> 4)),
+                  idesc, ks ? 1u : (unsigned)more);
+}
+// Descriptors of a tile: rows along k, and rows of k.
+__device__ __forceinline__ unsigned long long tt_rows(unsigned tile) { return umma_desc_k128(tile); }
+__device__ __forceinline__ unsigned long long tt_cols(unsigned tile) { return umma_desc_mn128(tile, TT_SLAB); }
 
 template <int D>
 __global__ void __launch_bounds__(TT_FWD_THREADS, 2)
@@ -146,7 +160,8 @@ train_forward_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       while (v_loads > 0 && !mbar_try_wait(v_full, (unsigned)(v_loads - 1) & 1u) && global_timer() < limit) {}
     }
   } else if (warp == 1) {
-    const int cols = (a.dim + 15) & ~15, ksteps = cols >> 4;
+    const int cols = (a.dim + 15) & ~15;
+    const unsigned long long q_rows = tt_rows(q_off), k_rows = tt_rows(k_off), v_cols = tt_cols(v_off);
     const unsigned idesc_s = umma_idesc_bf16(TT_B), idesc_o = umma_idesc_bf16(cols) | UMMA_B_MN_MAJOR;
     bool ok = tiles > 0 ? mbar_wait_warp(q_full, 0, abort_flag, nullptr, 73) : true;
     int i = 0;
@@ -155,7 +170,7 @@ train_forward_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       if (lane == 0) {
-        tt_mma_rows(tmem_s, q_off, k_off, ksteps, idesc_s);
+        tt_mma_rows<D>(tmem_s, q_rows, k_rows, idesc_s);
         tc_commit(k_free);
         tc_commit(s_full);
       }
@@ -168,10 +183,7 @@ train_forward_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       if (lane == 0) {
-#pragma unroll
-        for (int ks = 0; ks < TT_B / 16; ++ks)
-          tc_mma_f16_ts(tmem_o, tmem_s + (unsigned)(ks * 8), umma_desc_mn128(v_off + (unsigned)(ks * 16 * 128), TT_SLAB), idesc_o,
-                        (i | ks) ? 1u : 0u);
+        tt_mma_weights<false>(tmem_o, tmem_s, v_cols, idesc_o, i > 0);
         tc_commit(o_full);
       }
       __syncwarp();
@@ -377,23 +389,25 @@ train_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         while (!mbar_try_wait(q_full(j & 1), (unsigned)(j >> 1) & 1u) && global_timer() < limit) {}
     }
   } else if (warp == 1) {
-    const int cols = (a.dim + 15) & ~15, ksteps = cols >> 4;
+    const int cols = (a.dim + 15) & ~15;
+    const unsigned long long k_rows = tt_rows(k_off), v_rows = tt_rows(v_off);
+    unsigned long long q_rows[2], do_rows[2], q_cols[2], do_cols[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      q_rows[s] = tt_rows(q_tile(s));
+      do_rows[s] = tt_rows(do_tile(s));
+      q_cols[s] = tt_cols(q_tile(s));
+      do_cols[s] = tt_cols(do_tile(s));
+    }
     const unsigned idesc_s = umma_idesc_bf16(TT_B), idesc_d = umma_idesc_bf16(cols) | UMMA_B_MN_MAJOR;
     bool ok = true;
-    // rows of k of an A operand in tensor memory: each half of the warps has written its 64 over its own 64 columns
-    auto times = [&](unsigned d, unsigned w, unsigned b, bool more) {
-#pragma unroll
-      for (int ks = 0; ks < TT_B / 16; ++ks)
-        tc_mma_f16_ts(d, w + (unsigned)((ks >> 2) * 64 + (ks & 3) * 8), umma_desc_mn128(b + (unsigned)(ks * 16 * 128), TT_SLAB),
-                      idesc_d, more || ks ? 1u : 0u);
-    };
     if (tiles > 0) {
       ok = mbar_wait_warp(kv_full, 0, abort_flag, nullptr, 82) && mbar_wait_warp(q_full(0), 0, abort_flag, nullptr, 83);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       if (ok && lane == 0) {
-        tt_mma_rows(tmem_s, k_off, q_tile(0), ksteps, idesc_s);
+        tt_mma_rows<D>(tmem_s, k_rows, q_rows[0], idesc_s);
         tc_commit(s_full);
-        tt_mma_rows(tmem_dp, v_off, do_tile(0), ksteps, idesc_s);
+        tt_mma_rows<D>(tmem_dp, v_rows, do_rows[0], idesc_s);
         tc_commit(dp_full);
       }
       __syncwarp();
@@ -406,9 +420,9 @@ train_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       if (lane == 0) {
-        times(tmem_dv, tmem_s, do_tile(st), i > 0);
+        tt_mma_weights<true>(tmem_dv, tmem_s, st ? do_cols[1] : do_cols[0], idesc_d, i > 0);
         if (i + 1 < tiles) {
-          tt_mma_rows(tmem_s, k_off, q_tile(next), ksteps, idesc_s);
+          tt_mma_rows<D>(tmem_s, k_rows, next ? q_rows[1] : q_rows[0], idesc_s);
           tc_commit(s_full);
         }
       }
@@ -417,10 +431,10 @@ train_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       if (lane == 0) {
-        times(tmem_dk, tmem_dp, q_tile(st), i > 0);
+        tt_mma_weights<true>(tmem_dk, tmem_dp, st ? q_cols[1] : q_cols[0], idesc_d, i > 0);
         tc_commit(q_empty(st));
         if (i + 1 < tiles) {
-          tt_mma_rows(tmem_dp, v_off, do_tile(next), ksteps, idesc_s);
+          tt_mma_rows<D>(tmem_dp, v_rows, next ? do_rows[1] : do_rows[0], idesc_s);
           tc_commit(dp_full);
         }
       }
@@ -601,7 +615,15 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         while (!mbar_try_wait(k_full(j & 1), (unsigned)(j >> 1) & 1u) && global_timer() < limit) {}
     }
   } else if (warp == 1) {
-    const int cols = (a.dim + 15) & ~15, ksteps = cols >> 4;
+    const int cols = (a.dim + 15) & ~15;
+    const unsigned long long q_rows = tt_rows(q_off), do_rows = tt_rows(do_off);
+    unsigned long long k_rows[2], v_rows[2], k_cols[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      k_rows[s] = tt_rows(k_tile(s));
+      v_rows[s] = tt_rows(v_tile(s));
+      k_cols[s] = tt_cols(k_tile(s));
+    }
     const unsigned idesc_s = umma_idesc_bf16(TT_B), idesc_d = umma_idesc_bf16(cols) | UMMA_B_MN_MAJOR;
     // keys behind the stream's length must not meet the zeros of dS as anything but zeros
     auto arrived = [&](int i) {
@@ -615,9 +637,9 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       ok = mbar_wait_warp(q_full, 0, abort_flag, nullptr, 93) && arrived(0);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       if (ok && lane == 0) {
-        tt_mma_rows(tmem_s, q_off, k_tile(0), ksteps, idesc_s);
+        tt_mma_rows<D>(tmem_s, q_rows, k_rows[0], idesc_s);
         tc_commit(s_full);
-        tt_mma_rows(tmem_dp, do_off, v_tile(0), ksteps, idesc_s);
+        tt_mma_rows<D>(tmem_dp, do_rows, v_rows[0], idesc_s);
         tc_commit(dp_full);
       }
       __syncwarp();
@@ -629,7 +651,7 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         if (lane == 0) {
-          tt_mma_rows(tmem_s, q_off, k_tile(next), ksteps, idesc_s);
+          tt_mma_rows<D>(tmem_s, q_rows, next ? k_rows[1] : k_rows[0], idesc_s);
           tc_commit(s_full);
         }
         __syncwarp();
@@ -638,13 +660,10 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       if (lane == 0) {
-#pragma unroll
-        for (int ks = 0; ks < TT_B / 16; ++ks)
-          tc_mma_f16_ts(tmem_dq, tmem_dp + (unsigned)((ks >> 2) * 64 + (ks & 3) * 8),
-                        umma_desc_mn128(k_tile(st) + (unsigned)(ks * 16 * 128), TT_SLAB), idesc_d, (i | ks) ? 1u : 0u);
+        tt_mma_weights<true>(tmem_dq, tmem_dp, st ? k_cols[1] : k_cols[0], idesc_d, i > 0);
         tc_commit(k_empty(st));
         if (i + 1 < tiles) {
-          tt_mma_rows(tmem_dp, do_off, v_tile(next), ksteps, idesc_s);
+          tt_mma_rows<D>(tmem_dp, do_rows, next ? v_rows[1] : v_rows[0], idesc_s);
           tc_commit(dp_full);
         }
       }
