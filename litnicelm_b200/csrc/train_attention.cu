@@ -248,29 +248,27 @@ train_attention_forward_kernel(const __grid_constant__ TaArgs g) {
   store_tile<D, T>(a.out, at.stream * a.out.s + at.head * a.out.h, r0, a.n, a.dim, o, inv);
 }
 
-// A row by 16 lanes, eight elements each at a time.
-template <typename T>
+// A row by LANES lanes, eight elements each.
+template <int LANES, typename T>
 __global__ void __launch_bounds__(256) train_delta_kernel(const __grid_constant__ TaArgs g) {
   const TrainAttention &a = g.a;
   // rows in the order of memory as layers leave it, [streams, n, heads]: neighbours of a warp read on
-  const long long rows = (long long)a.streams * a.heads * a.n, mine = blockIdx.x * 16LL + (threadIdx.x >> 4);
+  const long long rows = (long long)a.streams * a.heads * a.n, mine = blockIdx.x * (256LL / LANES) + threadIdx.x / LANES;
   const long long at = mine < rows ? mine : rows - 1;
-  const int lane = threadIdx.x & 15;
-  const long long si = at / a.heads, s = si / a.n;
+  const int lane = threadIdx.x % LANES, c = lane * 8;
+  const long long si = div_index(at, a.heads), s = div_index(si, a.n);
   const int h = (int)(at - si * a.heads), i = (int)(si - s * a.n);
-  const T *x = reinterpret_cast<const T *>(a.out.p) + s * a.out.s + (long long)i * a.out.r + h * a.out.h;
-  const T *y = reinterpret_cast<const T *>(a.dout.p) + s * a.dout.s + (long long)i * a.dout.r + h * a.dout.h;
+  const T *x = reinterpret_cast<const T *>(a.out.p) + s * a.out.s + (long long)i * a.out.r + h * a.out.h + c * a.out.c;
+  const T *y = reinterpret_cast<const T *>(a.dout.p) + s * a.dout.s + (long long)i * a.dout.r + h * a.dout.h + c * a.dout.c;
   float t = 0.f;
-  for (int c = lane * 8; c < a.dim; c += 128) {
 #pragma unroll
-    for (int e = 0; e < 8; e += 4) {
-      const float4 u = load4<T>(x + (c + e) * a.out.c, a.out.c, a.dim - c - e, g.vec & VO);
-      const float4 v = load4<T>(y + (c + e) * a.dout.c, a.dout.c, a.dim - c - e, g.vec & VDO);
-      t = fmaf(u.x, v.x, fmaf(u.y, v.y, fmaf(u.z, v.z, fmaf(u.w, v.w, t))));
-    }
+  for (int e = 0; e < 8; e += 4) {
+    const float4 u = load4<T>(x + e * a.out.c, a.out.c, a.dim - c - e, g.vec & VO);
+    const float4 v = load4<T>(y + e * a.dout.c, a.dout.c, a.dim - c - e, g.vec & VDO);
+    t = fmaf(u.x, v.x, fmaf(u.y, v.y, fmaf(u.z, v.z, fmaf(u.w, v.w, t))));
   }
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+  for (int o = LANES / 2; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
   if (lane == 0 && mine < rows) g.delta[(s * a.heads + h) * a.n + i] = t;
 }
 
@@ -454,18 +452,20 @@ void launch_train_attention_forward(const TrainAttention &a, void *work, cudaStr
   }
 }
 
-static void launch_train_delta(const TrainAttention &a, float *delta, cudaStream_t st) {
+template <int LANES>
+static void launch_delta(const TrainAttention &a, float *delta, cudaStream_t st) {
   const TaArgs g = ta_args(a, delta, a.n);
-  const long long rows = (long long)a.streams * a.heads * a.n;
-  if ((rows + 15) / 16 > 0x7fffffffLL) throw std::invalid_argument("attention: too many rows, heads and streams for one call");
-  if (a.bf16) train_delta_kernel<bf16><<<(unsigned)((rows + 15) / 16), 256, 0, st>>>(g);
-  else train_delta_kernel<float><<<(unsigned)((rows + 15) / 16), 256, 0, st>>>(g);
+  const long long blocks = ((long long)a.streams * a.heads * a.n + 256 / LANES - 1) / (256 / LANES);
+  if (blocks > 0x7fffffffLL) throw std::invalid_argument("attention: too many rows, heads and streams for one call");
+  if (a.bf16) train_delta_kernel<LANES, bf16><<<(unsigned)blocks, 256, 0, st>>>(g);
+  else train_delta_kernel<LANES, float><<<(unsigned)blocks, 256, 0, st>>>(g);
   LB_LAUNCH_CHECK();
 }
 
 void launch_train_attention_backward(const TrainAttention &a, float *delta, void *work, cudaStream_t st) {
   if (train_attention_f32_supports(a.bf16, a.dim)) return launch_train_attention_backward_f32(a, delta, work, st);
-  launch_train_delta(a, delta, st);
+  if (a.dim <= 64) launch_delta<8>(a, delta, st);
+  else launch_delta<16>(a, delta, st);
   if (train_attention_tc_supports(a, true)) return launch_train_attention_backward_tc(a, delta, st);
   if (a.bf16) {
     if (a.dim <= 32) backward<32, bf16>(a, delta, st);

@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(TT_FWD_THREADS, 2)
 train_forward_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                         const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TtArgs a) {
   constexpr int SLABS = D / 64, TILE = SLABS * TT_SLAB;
-  extern __shared__ unsigned char smem_raw[];
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
   const unsigned base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char *base_ptr = smem_raw + (base - smem_u32(smem_raw));
   const unsigned q_off = base, k_off = base + TILE, v_off = base + 2 * TILE, bars = base + 3 * TILE;
@@ -200,6 +200,8 @@ train_forward_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     const int row = r0 + q * 32 + lane;
     const int row_lo = a.span.lo(row), row_end = a.span.end(row, at.keys);
     const int warp_lo = a.span.lo(r0 + q * 32 + 31), warp_end = a.span.end(r0 + q * 32, at.keys);
+    // a negative factor's sign goes to the scores; zero is small, so that hidden scores of -infinity stay that
+    const float factor = fmaxf(fabsf(a.factor), 1e-30f);
     float m = TT_NEG, l = 0.f;
     bool ok = true;
     for (int i = 0; i < tiles && ok; ++i) {
@@ -216,17 +218,22 @@ train_forward_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         for (int c = 0; c < 4; ++c) tc_ld32(tmem_s + lanes + (unsigned)(c * 32), u[c]);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
       }
+      if (a.factor < 0.f) {
 #pragma unroll
-      for (int j = 0; j < TT_B; ++j) s[j] *= a.factor;
+        for (int j = 0; j < TT_B; ++j) s[j] = -s[j];
+      }
       if (!inside) {
 #pragma unroll
         for (int j = 0; j < TT_B; ++j)
-          if (j >= c_end || j < c_lo) s[j] = 2.f * TT_NEG;  // weight zero against any reference
+          if (j >= c_end || j < c_lo) s[j] = -INFINITY;
       }
       float mq[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-      for (int j = 4; j < TT_B; ++j) mq[j & 3] = fmaxf(mq[j & 3], s[j]);
-      const float mx = fmaxf(TT_NEG, fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3])));
+      for (int j = 4; j < TT_B; j += 8) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mq[e] = j + 4 + e < TT_B ? tt_max3(mq[e], s[j + e], s[j + 4 + e]) : fmaxf(mq[e], s[j + e]);
+      }
+      const float mx = fmaxf(TT_NEG, fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3])) * factor);
       const bool grow = mx > m + TT_SLACK;
       const float keep = grow ? tt_exp2(m - mx) : 1.f;
       if (grow) m = mx;
@@ -247,20 +254,22 @@ train_forward_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
           }
         }
       }
-      float lq[4] = {0.f, 0.f, 0.f, 0.f};
+      unsigned long long lq[4] = {0ull, 0ull, 0ull, 0ull};
+      const unsigned long long f2 = tt_two(factor, factor), m2 = tt_two(-m, -m);
 #pragma unroll
       for (int c0 = 0; c0 < TT_B; c0 += 32) {
         unsigned pk[16];
 #pragma unroll
         for (int j = 0; j < 32; j += 2) {
-          const float e0 = tt_exp2(s[c0 + j] - m), e1 = tt_exp2(s[c0 + j + 1] - m);
-          lq[j & 2] += e0;
-          lq[(j & 2) + 1] += e1;
+          const unsigned long long t = tt_fma2(tt_two(s[c0 + j], s[c0 + j + 1]), f2, m2);
+          const float e0 = tt_exp2(tt_lo(t)), e1 = tt_exp2(tt_hi(t));
+          lq[(j >> 1) & 3] = tt_add2(lq[(j >> 1) & 3], tt_two(e0, e1));
           pk[j >> 1] = tt_pack(e0, e1);
         }
         tc_st16(tmem_s + lanes + (unsigned)(c0 >> 1), pk);  // over the scores, which this warp has read
       }
-      l += (lq[0] + lq[1]) + (lq[2] + lq[3]);
+      lq[0] = tt_add2(tt_add2(lq[0], lq[1]), tt_add2(lq[2], lq[3]));
+      l += tt_lo(lq[0]) + tt_hi(lq[0]);
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
@@ -286,14 +295,17 @@ train_forward_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
   }
 }
 
-// Shared memory of the backward kernels: two resident tiles, two stages of two streamed tiles, statistics of the stages' rows.
+// Shared memory of the backward kernels: two resident tiles, NA stages of the streamed tiles that two products a turn apart read (rows
+// of q for dk, of k for dq) and NB of those that are done with sooner, statistics of the stages' rows. A load takes 1300 to 2000
+// clocks: with two stages of both the products waited 700 to 1200 of a turn's 2600 (D = 64).
 template <int D>
 struct TtBwd {
   static constexpr int SLABS = D / 64, TILE = SLABS * TT_SLAB;
-  static constexpr int STAGE_OFF = 2 * TILE;
-  static constexpr int STAT_OFF = STAGE_OFF + 4 * TILE;  // [2][2][128] floats
-  static constexpr int BAR_OFF = STAT_OFF + 2 * 2 * 128 * 4;
-  static constexpr int TOTAL = BAR_OFF + 128 + 1024;
+  static constexpr int NA = D == 64 ? 4 : 3, NB = D == 64 ? 4 : 2;
+  static constexpr int A_OFF = 2 * TILE, B_OFF = A_OFF + NA * TILE;
+  static constexpr int STAT_OFF = B_OFF + NB * TILE;  // [NB][2][128] floats
+  static constexpr int BAR_OFF = STAT_OFF + NB * 2 * 128 * 4;
+  static constexpr int TOTAL = BAR_OFF + 256 + 768;
   static_assert(TOTAL <= 227 * 1024, "");
 };
 
@@ -304,19 +316,22 @@ train_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     const __grid_constant__ TtArgs a) {
   using L = TtBwd<D>;
   constexpr int SLABS = L::SLABS, TILE = L::TILE;
-  extern __shared__ unsigned char smem_raw[];
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
   const unsigned base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char *base_ptr = smem_raw + (base - smem_u32(smem_raw));
   const unsigned k_off = base, v_off = base + TILE, bars = base + L::BAR_OFF;
-  auto q_tile = [&](int s) { return base + (unsigned)(L::STAGE_OFF + s * 2 * TILE); };
-  auto do_tile = [&](int s) { return base + (unsigned)(L::STAGE_OFF + (s * 2 + 1) * TILE); };
+  auto q_tile = [&](int s) { return base + (unsigned)(L::A_OFF + s * TILE); };
+  auto do_tile = [&](int s) { return base + (unsigned)(L::B_OFF + s * TILE); };
   float *stat = reinterpret_cast<float *>(base_ptr + L::STAT_OFF);
-  const unsigned kv_full = bars, s_full = bars + 8, p_ready = bars + 16, dp_full = bars + 24, ds_ready = bars + 32, done = bars + 40;
-  auto q_full = [&](int s) { return bars + 48u + 8u * s; };
-  auto q_empty = [&](int s) { return bars + 64u + 8u * s; };
-  auto stat_full = [&](int s) { return bars + 80u + 8u * s; };
-  volatile unsigned *tmem_holder = reinterpret_cast<volatile unsigned *>(base_ptr + L::BAR_OFF + 96);
-  volatile int *abort_flag = reinterpret_cast<volatile int *>(base_ptr + L::BAR_OFF + 100);
+  auto a_full = [&](int s) { return bars + 8u * s; };
+  auto a_empty = [&](int s) { return bars + 32u + 8u * s; };
+  auto b_full = [&](int s) { return bars + 64u + 8u * s; };
+  auto b_empty = [&](int s) { return bars + 96u + 8u * s; };
+  const unsigned kv_full = bars + 128, s_full = bars + 136, p_ready = bars + 144, dp_full = bars + 152, ds_ready = bars + 160,
+                 done = bars + 168;
+  auto stat_full = [&](int s) { return bars + 208u + 8u * s; };
+  volatile unsigned *tmem_holder = reinterpret_cast<volatile unsigned *>(base_ptr + L::BAR_OFF + 240);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(base_ptr + L::BAR_OFF + 244);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const TtPlace at = tt_place(a, a.groups, false);
   const int j0 = at.tile * TT_B, j1 = min(j0 + TT_B, at.keys);
@@ -331,9 +346,13 @@ train_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     for (unsigned bar : {kv_full, s_full, dp_full, done}) mbar_init(bar, 1);
     mbar_init(p_ready, 8);
     mbar_init(ds_ready, 8);
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(q_full(s), 1);
-      mbar_init(q_empty(s), 1);
+    for (int s = 0; s < L::NA; ++s) {
+      mbar_init(a_full(s), 1);
+      mbar_init(a_empty(s), 1);
+    }
+    for (int s = 0; s < L::NB; ++s) {
+      mbar_init(b_full(s), 1);
+      mbar_init(b_empty(s), 1);
       mbar_init(stat_full(s), 1);
     }
     *abort_flag = 0;
@@ -359,23 +378,30 @@ train_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     for (int h = at.head * a.share; h < (at.head + 1) * a.share && ok; ++h) {
       const long long stats = ((long long)at.stream * a.heads + h) * a.n;
       for (int t = 0; t < each; ++t, ++it) {
-        const int st = it & 1, r0 = lo + t * TT_B;
-        ok = mbar_wait_warp(q_empty(st), ((unsigned)(it >> 1) & 1u) ^ 1u, abort_flag, nullptr, 81);
+        const int sa = it % L::NA, st = it % L::NB, r0 = lo + t * TT_B;
+        ok = mbar_wait_warp(a_empty(sa), ((unsigned)(it / L::NA) & 1u) ^ 1u, abort_flag, nullptr, 80);
         if (!ok) break;
         if (lane == 0) {
-          mbar_expect_tx(q_full(st), 2u * TILE);
-          for (int s = 0; s < SLABS; ++s) {
-            tma_load_4d(q_tile(st) + s * TT_SLAB, &map_q, s * 64, h, r0, at.stream, q_full(st));
-            tma_load_4d(do_tile(st) + s * TT_SLAB, &map_do, s * 64, h, r0, at.stream, q_full(st));
-          }
+          mbar_expect_tx(a_full(sa), (unsigned)TILE);
+          for (int s = 0; s < SLABS; ++s) tma_load_4d(q_tile(sa) + s * TT_SLAB, &map_q, s * 64, h, r0, at.stream, a_full(sa));
+        }
+        __syncwarp();
+        ok = mbar_wait_warp(b_empty(st), ((unsigned)(it / L::NB) & 1u) ^ 1u, abort_flag, nullptr, 81);
+        if (!ok) {
+          ++it;  // (its rows of q are on their way)
+          break;
+        }
+        if (lane == 0) {
+          mbar_expect_tx(b_full(st), (unsigned)TILE);
+          for (int s = 0; s < SLABS; ++s) tma_load_4d(do_tile(st) + s * TT_SLAB, &map_do, s * 64, h, r0, at.stream, b_full(st));
         }
         // a row that does not exist or sees no key has no weights: 2^(s - infinity)
 #pragma unroll
         for (int e = lane; e < TT_B; e += 32) {
           const int row = r0 + e;
           const float z = row < a.n ? a.lse[stats + row] : -INFINITY;
-          stat[st * 256 + e] = z == -INFINITY ? INFINITY : z * TT_LOG2E;
-          stat[st * 256 + 128 + e] = row < a.n ? a.delta[stats + row] : 0.f;
+          stat[st * 256 + e] = z == -INFINITY ? -INFINITY : -(z * TT_LOG2E);  // both with the sign that they are added with
+          stat[st * 256 + 128 + e] = row < a.n ? -a.delta[stats + row] : 0.f;
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(stat_full(st));
@@ -385,60 +411,68 @@ train_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     if (*abort_flag && tiles > 0) {  // copies in flight must land before the shared memory goes away
       const unsigned long long limit = global_timer() + WAIT_LIMIT_NS;
       while (!mbar_try_wait(kv_full, 0) && global_timer() < limit) {}
-      for (int j = it > 2 ? it - 2 : 0; j < it; ++j)
-        while (!mbar_try_wait(q_full(j & 1), (unsigned)(j >> 1) & 1u) && global_timer() < limit) {}
+      for (int j = it > L::NA ? it - L::NA : 0; j < it; ++j)
+        while (!mbar_try_wait(a_full(j % L::NA), (unsigned)(j / L::NA) & 1u) && global_timer() < limit) {}
+      const int b_loads = ok ? it : it - 1;
+      for (int j = b_loads > L::NB ? b_loads - L::NB : 0; j < b_loads; ++j)
+        while (!mbar_try_wait(b_full(j % L::NB), (unsigned)(j / L::NB) & 1u) && global_timer() < limit) {}
     }
   } else if (warp == 1) {
     const int cols = (a.dim + 15) & ~15;
-    const unsigned long long k_rows = tt_rows(k_off), v_rows = tt_rows(v_off);
-    unsigned long long q_rows[2], do_rows[2], q_cols[2], do_cols[2];
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      q_rows[s] = tt_rows(q_tile(s));
-      do_rows[s] = tt_rows(do_tile(s));
-      q_cols[s] = tt_cols(q_tile(s));
-      do_cols[s] = tt_cols(do_tile(s));
-    }
+    const unsigned long long k_rows = tt_rows(k_off), v_rows = tt_rows(v_off), q_rows = tt_rows(q_tile(0)), do_rows = tt_rows(do_tile(0)),
+                             q_cols = tt_cols(q_tile(0)), do_cols = tt_cols(do_tile(0));
+    auto stage = [](int s) { return (unsigned long long)(s * (TILE >> 4)); };
     const unsigned idesc_s = umma_idesc_bf16(TT_B), idesc_d = umma_idesc_bf16(cols) | UMMA_B_MN_MAJOR;
     bool ok = true;
     if (tiles > 0) {
-      ok = mbar_wait_warp(kv_full, 0, abort_flag, nullptr, 82) && mbar_wait_warp(q_full(0), 0, abort_flag, nullptr, 83);
+      ok = mbar_wait_warp(kv_full, 0, abort_flag, nullptr, 82) && mbar_wait_warp(a_full(0), 0, abort_flag, nullptr, 83);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       if (ok && lane == 0) {
-        tt_mma_rows<D>(tmem_s, k_rows, q_rows[0], idesc_s);
+        tt_mma_rows<D>(tmem_s, k_rows, q_rows, idesc_s);
         tc_commit(s_full);
-        tt_mma_rows<D>(tmem_dp, v_rows, do_rows[0], idesc_s);
+      }
+      __syncwarp();
+      ok = ok && mbar_wait_warp(b_full(0), 0, abort_flag, nullptr, 83);
+      if (ok && lane == 0) {
+        tt_mma_rows<D>(tmem_dp, v_rows, do_rows, idesc_s);
         tc_commit(dp_full);
       }
       __syncwarp();
     }
     for (int i = 0; i < tiles && ok; ++i) {
-      const int st = i & 1, next = st ^ 1;
+      const int sa = i % L::NA, sb = i % L::NB, na = (i + 1) % L::NA, nb = (i + 1) % L::NB;
       ok = mbar_wait_warp(p_ready, (unsigned)i & 1u, abort_flag, nullptr, 84);
       if (!ok) break;
-      if (i + 1 < tiles) ok = mbar_wait_warp(q_full(next), (unsigned)((i + 1) >> 1) & 1u, abort_flag, nullptr, 85);
-      if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      if (lane == 0) {
-        tt_mma_weights<true>(tmem_dv, tmem_s, st ? do_cols[1] : do_cols[0], idesc_d, i > 0);
-        if (i + 1 < tiles) {
-          tt_mma_rows<D>(tmem_s, k_rows, next ? q_rows[1] : q_rows[0], idesc_s);
+      if (lane == 0) tt_mma_weights<true>(tmem_dv, tmem_s, do_cols + stage(sb), idesc_d, i > 0);
+      __syncwarp();
+      if (i + 1 < tiles) {
+        ok = mbar_wait_warp(a_full(na), (unsigned)((i + 1) / L::NA) & 1u, abort_flag, nullptr, 85);
+        if (!ok) break;
+        if (lane == 0) {
+          tt_mma_rows<D>(tmem_s, k_rows, q_rows + stage(na), idesc_s);
           tc_commit(s_full);
         }
+        __syncwarp();
       }
-      __syncwarp();
       ok = mbar_wait_warp(ds_ready, (unsigned)i & 1u, abort_flag, nullptr, 86);
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       if (lane == 0) {
-        tt_mma_weights<true>(tmem_dk, tmem_dp, st ? q_cols[1] : q_cols[0], idesc_d, i > 0);
-        tc_commit(q_empty(st));
-        if (i + 1 < tiles) {
-          tt_mma_rows<D>(tmem_dp, v_rows, next ? do_rows[1] : do_rows[0], idesc_s);
-          tc_commit(dp_full);
-        }
+        tt_mma_weights<true>(tmem_dk, tmem_dp, q_cols + stage(sa), idesc_d, i > 0);
+        tc_commit(a_empty(sa));
+        tc_commit(b_empty(sb));  // (the statistics beside it have been read too)
       }
       __syncwarp();
+      if (i + 1 < tiles) {
+        ok = mbar_wait_warp(b_full(nb), (unsigned)((i + 1) / L::NB) & 1u, abort_flag, nullptr, 85);
+        if (!ok) break;
+        if (lane == 0) {
+          tt_mma_rows<D>(tmem_dp, v_rows, do_rows + stage(nb), idesc_s);
+          tc_commit(dp_full);
+        }
+        __syncwarp();
+      }
     }
     if (tiles > 0 && lane == 0) tc_commit(done);
     __syncwarp();
@@ -453,13 +487,13 @@ train_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     const bool key_live = key < at.keys;
     bool ok = true;
     for (int i = 0; i < tiles && ok; ++i) {
-      const int st = i & 1, r0 = lo + i % each * TT_B + half * 64;
+      const int st = i % L::NB, r0 = lo + i % each * TT_B + half * 64;
       // rows r0 + c that see this key: [c_lo, c_end)
       const int c_lo = a.span.causal ? key - a.span.first - r0 : 0;
       const long long pe = a.span.window > 0 ? (long long)key + a.span.window - a.span.first - r0 : 64;
       const int c_end = !key_live ? 0 : pe < 64 ? (int)max(pe, 0LL) : 64;
       const bool inside = __all_sync(0xffffffffu, c_lo <= 0 && c_end >= 64);
-      ok = mbar_wait_warp(stat_full(st), (unsigned)(i >> 1) & 1u, abort_flag, nullptr, 87) &&
+      ok = mbar_wait_warp(stat_full(st), (unsigned)(i / L::NB) & 1u, abort_flag, nullptr, 87) &&
            mbar_wait_warp(s_full, (unsigned)i & 1u, abort_flag, nullptr, 88);
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -470,14 +504,16 @@ train_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         tc_ld32(tmem_s + lanes + (unsigned)(half * 64 + 32), u[1]);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
       }
-      const float4 *z = reinterpret_cast<const float4 *>(stat + st * 256 + half * 64);
+      const ulonglong2 *z = reinterpret_cast<const ulonglong2 *>(stat + st * 256 + half * 64);
+      const unsigned long long f2 = tt_two(a.factor, a.factor);
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const float4 v = z[j];
-        p[4 * j] = tt_exp2(fmaf(p[4 * j], a.factor, -v.x));
-        p[4 * j + 1] = tt_exp2(fmaf(p[4 * j + 1], a.factor, -v.y));
-        p[4 * j + 2] = tt_exp2(fmaf(p[4 * j + 2], a.factor, -v.z));
-        p[4 * j + 3] = tt_exp2(fmaf(p[4 * j + 3], a.factor, -v.w));
+      for (int j = 0; j < 64; j += 4) {
+        const ulonglong2 v = z[j >> 2];
+        const unsigned long long t = tt_fma2(tt_two(p[j], p[j + 1]), f2, v.x), u = tt_fma2(tt_two(p[j + 2], p[j + 3]), f2, v.y);
+        p[j] = tt_exp2(tt_lo(t));
+        p[j + 1] = tt_exp2(tt_hi(t));
+        p[j + 2] = tt_exp2(tt_lo(u));
+        p[j + 3] = tt_exp2(tt_hi(u));
       }
       if (!inside) {
 #pragma unroll
@@ -498,7 +534,7 @@ train_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       ok = mbar_wait_warp(dp_full, (unsigned)i & 1u, abort_flag, nullptr, 89);
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const float4 *de = reinterpret_cast<const float4 *>(stat + st * 256 + 128 + half * 64);
+      const ulonglong2 *de = reinterpret_cast<const ulonglong2 *>(stat + st * 256 + 128 + half * 64);
 #pragma unroll
       for (int c = 0; c < 64; c += 32) {
         unsigned u[32], w[16];
@@ -506,12 +542,13 @@ train_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
         for (int j = 0; j < 32; j += 4) {
-          const float4 v = de[(c + j) >> 2];
-          // (a weight of zero has no part even where the other factor is not finite)
-          const float x0 = (__uint_as_float(u[j]) - v.x) * p[c + j], x1 = (__uint_as_float(u[j + 1]) - v.y) * p[c + j + 1];
-          const float x2 = (__uint_as_float(u[j + 2]) - v.z) * p[c + j + 2], x3 = (__uint_as_float(u[j + 3]) - v.w) * p[c + j + 3];
-          w[j >> 1] = tt_pack(x0, x1);
-          w[(j >> 1) + 1] = tt_pack(x2, x3);
+          const ulonglong2 v = de[(c + j) >> 2];
+          const unsigned long long x = tt_mul2(tt_add2(tt_two(__uint_as_float(u[j]), __uint_as_float(u[j + 1])), v.x),
+                                               tt_two(p[c + j], p[c + j + 1]));
+          const unsigned long long y = tt_mul2(tt_add2(tt_two(__uint_as_float(u[j + 2]), __uint_as_float(u[j + 3])), v.y),
+                                               tt_two(p[c + j + 2], p[c + j + 3]));
+          w[j >> 1] = tt_pack(tt_lo(x), tt_hi(x));
+          w[(j >> 1) + 1] = tt_pack(tt_lo(y), tt_hi(y));
         }
         if (!key_live) {
 #pragma unroll
@@ -547,19 +584,22 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
                    const __grid_constant__ TtArgs a) {
   using L = TtBwd<D>;
   constexpr int SLABS = L::SLABS, TILE = L::TILE;
-  extern __shared__ unsigned char smem_raw[];
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
   const unsigned base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char *base_ptr = smem_raw + (base - smem_u32(smem_raw));
   const unsigned q_off = base, do_off = base + TILE, bars = base + L::BAR_OFF;
-  auto k_tile = [&](int s) { return base + (unsigned)(L::STAGE_OFF + s * 2 * TILE); };
-  auto v_tile = [&](int s) { return base + (unsigned)(L::STAGE_OFF + (s * 2 + 1) * TILE); };
+  auto k_tile = [&](int s) { return base + (unsigned)(L::A_OFF + s * TILE); };
+  auto v_tile = [&](int s) { return base + (unsigned)(L::B_OFF + s * TILE); };
   float *stat = reinterpret_cast<float *>(base_ptr + L::STAT_OFF);
-  const unsigned q_full = bars, s_full = bars + 8, s_free = bars + 16, dp_full = bars + 24, ds_ready = bars + 32, done = bars + 40;
-  auto k_full = [&](int s) { return bars + 48u + 8u * s; };
-  auto k_empty = [&](int s) { return bars + 64u + 8u * s; };
-  auto halves = [&](int q) { return bars + 80u + 8u * q; };  // of the two warps that share 32 rows
-  volatile unsigned *tmem_holder = reinterpret_cast<volatile unsigned *>(base_ptr + L::BAR_OFF + 112);
-  volatile int *abort_flag = reinterpret_cast<volatile int *>(base_ptr + L::BAR_OFF + 116);
+  auto a_full = [&](int s) { return bars + 8u * s; };
+  auto a_empty = [&](int s) { return bars + 32u + 8u * s; };
+  auto b_full = [&](int s) { return bars + 64u + 8u * s; };
+  auto b_empty = [&](int s) { return bars + 96u + 8u * s; };
+  const unsigned q_full = bars + 128, s_full = bars + 136, s_free = bars + 144, dp_full = bars + 152, ds_ready = bars + 160,
+                 done = bars + 168;
+  auto halves = [&](int q) { return bars + 176u + 8u * q; };  // of the two warps that share 32 rows
+  volatile unsigned *tmem_holder = reinterpret_cast<volatile unsigned *>(base_ptr + L::BAR_OFF + 240);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(base_ptr + L::BAR_OFF + 244);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const TtPlace at = tt_place(a, a.heads, a.span.causal != 0);
   const int r0 = at.tile * TT_B, r1 = min(r0 + TT_B, a.n), kh = at.head / a.share;
@@ -571,9 +611,13 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     mbar_init(s_free, 8);
     mbar_init(ds_ready, 8);
     for (int q = 0; q < 4; ++q) mbar_init(halves(q), 2);
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(k_full(s), 1);
-      mbar_init(k_empty(s), 1);
+    for (int s = 0; s < L::NA; ++s) {
+      mbar_init(a_full(s), 1);
+      mbar_init(a_empty(s), 1);
+    }
+    for (int s = 0; s < L::NB; ++s) {
+      mbar_init(b_full(s), 1);
+      mbar_init(b_empty(s), 1);
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -596,40 +640,56 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       }
     }
     for (; it < tiles; ++it) {
-      const int st = it & 1, j0 = lo + it * TT_B;
-      ok = mbar_wait_warp(k_empty(st), ((unsigned)(it >> 1) & 1u) ^ 1u, abort_flag, nullptr, 91);
+      const int sa = it % L::NA, sb = it % L::NB, j0 = lo + it * TT_B;
+      ok = mbar_wait_warp(a_empty(sa), ((unsigned)(it / L::NA) & 1u) ^ 1u, abort_flag, nullptr, 91);
       if (!ok) break;
       if (lane == 0) {
-        mbar_expect_tx(k_full(st), 2u * TILE);
-        for (int s = 0; s < SLABS; ++s) {
-          tma_load_4d(k_tile(st) + s * TT_SLAB, &map_k, s * 64, kh, j0, at.stream, k_full(st));
-          tma_load_4d(v_tile(st) + s * TT_SLAB, &map_v, s * 64, kh, j0, at.stream, k_full(st));
-        }
+        mbar_expect_tx(a_full(sa), (unsigned)TILE);
+        for (int s = 0; s < SLABS; ++s) tma_load_4d(k_tile(sa) + s * TT_SLAB, &map_k, s * 64, kh, j0, at.stream, a_full(sa));
+      }
+      __syncwarp();
+      ok = mbar_wait_warp(b_empty(sb), ((unsigned)(it / L::NB) & 1u) ^ 1u, abort_flag, nullptr, 91);
+      if (!ok) {
+        ++it;  // (its keys are on their way)
+        break;
+      }
+      if (lane == 0) {
+        mbar_expect_tx(b_full(sb), (unsigned)TILE);
+        for (int s = 0; s < SLABS; ++s) tma_load_4d(v_tile(sb) + s * TT_SLAB, &map_v, s * 64, kh, j0, at.stream, b_full(sb));
       }
       __syncwarp();
     }
     if (*abort_flag && tiles > 0) {  // copies in flight must land before the shared memory goes away
       const unsigned long long limit = global_timer() + WAIT_LIMIT_NS;
       while (!mbar_try_wait(q_full, 0) && global_timer() < limit) {}
-      for (int j = it > 2 ? it - 2 : 0; j < it; ++j)
-        while (!mbar_try_wait(k_full(j & 1), (unsigned)(j >> 1) & 1u) && global_timer() < limit) {}
+      for (int j = it > L::NA ? it - L::NA : 0; j < it; ++j)
+        while (!mbar_try_wait(a_full(j % L::NA), (unsigned)(j / L::NA) & 1u) && global_timer() < limit) {}
+      const int b_loads = ok ? it : it - 1;
+      for (int j = b_loads > L::NB ? b_loads - L::NB : 0; j < b_loads; ++j)
+        while (!mbar_try_wait(b_full(j % L::NB), (unsigned)(j / L::NB) & 1u) && global_timer() < limit) {}
     }
   } else if (warp == 1) {
     const int cols = (a.dim + 15) & ~15;
-    const unsigned long long q_rows = tt_rows(q_off), do_rows = tt_rows(do_off);
-    unsigned long long k_rows[2], v_rows[2], k_cols[2];
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      k_rows[s] = tt_rows(k_tile(s));
-      v_rows[s] = tt_rows(v_tile(s));
-      k_cols[s] = tt_cols(k_tile(s));
-    }
+    const unsigned long long q_rows = tt_rows(q_off), do_rows = tt_rows(do_off), k_rows = tt_rows(k_tile(0)), v_rows = tt_rows(v_tile(0)),
+                             k_cols = tt_cols(k_tile(0));
+    auto stage = [](int s) { return (unsigned long long)(s * (TILE >> 4)); };
     const unsigned idesc_s = umma_idesc_bf16(TT_B), idesc_d = umma_idesc_bf16(cols) | UMMA_B_MN_MAJOR;
     // keys behind the stream's length must not meet the zeros of dS as anything but zeros
     auto arrived = [&](int i) {
-      if (!mbar_wait_warp(k_full(i & 1), (unsigned)(i >> 1) & 1u, abort_flag, nullptr, 92)) return false;
+      if (!mbar_wait_warp(a_full(i % L::NA), (unsigned)(i / L::NA) & 1u, abort_flag, nullptr, 92)) return false;
       const int have = at.keys - (lo + i * TT_B);
-      if (have < TT_B && at.keys < a.m) tt_clear_rows(base_ptr + (k_tile(i & 1) - base), SLABS, have, lane);
+      if (have < TT_B && at.keys < a.m) tt_clear_rows(base_ptr + (k_tile(i % L::NA) - base), SLABS, have, lane);
+      return true;
+    };
+    auto upstream = [&](int i) {  // dP of tile i
+      const int sb = i % L::NB;
+      if (!mbar_wait_warp(b_full(sb), (unsigned)(i / L::NB) & 1u, abort_flag, nullptr, 92)) return false;
+      if (lane == 0) {
+        tt_mma_rows<D>(tmem_dp, do_rows, v_rows + stage(sb), idesc_s);
+        tc_commit(dp_full);
+        tc_commit(b_empty(sb));
+      }
+      __syncwarp();
       return true;
     };
     bool ok = true;
@@ -637,21 +697,20 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       ok = mbar_wait_warp(q_full, 0, abort_flag, nullptr, 93) && arrived(0);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       if (ok && lane == 0) {
-        tt_mma_rows<D>(tmem_s, q_rows, k_rows[0], idesc_s);
+        tt_mma_rows<D>(tmem_s, q_rows, k_rows, idesc_s);
         tc_commit(s_full);
-        tt_mma_rows<D>(tmem_dp, do_rows, v_rows[0], idesc_s);
-        tc_commit(dp_full);
       }
       __syncwarp();
+      ok = ok && upstream(0);
     }
     for (int i = 0; i < tiles && ok; ++i) {
-      const int st = i & 1, next = st ^ 1;
+      const int sa = i % L::NA, na = (i + 1) % L::NA;
       if (i + 1 < tiles) {
-        ok = mbar_wait_warp(s_free, (unsigned)i & 1u, abort_flag, nullptr, 94) && arrived(i + 1);
+        ok = arrived(i + 1) && mbar_wait_warp(s_free, (unsigned)i & 1u, abort_flag, nullptr, 94);
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         if (lane == 0) {
-          tt_mma_rows<D>(tmem_s, q_rows, next ? k_rows[1] : k_rows[0], idesc_s);
+          tt_mma_rows<D>(tmem_s, q_rows, k_rows + stage(na), idesc_s);
           tc_commit(s_full);
         }
         __syncwarp();
@@ -660,14 +719,11 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       if (lane == 0) {
-        tt_mma_weights<true>(tmem_dq, tmem_dp, st ? k_cols[1] : k_cols[0], idesc_d, i > 0);
-        tc_commit(k_empty(st));
-        if (i + 1 < tiles) {
-          tt_mma_rows<D>(tmem_dp, do_rows, next ? v_rows[1] : v_rows[0], idesc_s);
-          tc_commit(dp_full);
-        }
+        tt_mma_weights<true>(tmem_dq, tmem_dp, k_cols + stage(sa), idesc_d, i > 0);
+        tc_commit(a_empty(sa));
       }
       __syncwarp();
+      if (i + 1 < tiles) ok = upstream(i + 1);
     }
     if (tiles > 0 && lane == 0) tc_commit(done);
     __syncwarp();
@@ -684,7 +740,7 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     const long long x = ((long long)at.stream * a.heads + at.head) * a.n + row;
     const float z = row < a.n ? a.lse[x] : -INFINITY;
     float delta = row < a.n ? a.delta[x] : 0.f;
-    const float lse = z == -INFINITY ? INFINITY : z * TT_LOG2E;  // a row that sees no key has no weights: 2^(s - infinity)
+    const float lse = z == -INFINITY ? -INFINITY : -(z * TT_LOG2E);  // to add; a row that sees no key has no weights: 2^(s - infinity)
     // dout . out is off by what out was rounded by, which counts in rows of few keys. Where all of a row's keys lie in this one
     // tile, the same sum over keys, p dP, is at hand in 32 bits (the kernel of dk and dv then finds it in place of the other).
     auto exact_delta = [&](const float (&p)[64], int half, int c_lo, int c_end) {
@@ -725,8 +781,13 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(s_free);
+      const unsigned long long f2 = tt_two(a.factor, a.factor), z2 = tt_two(lse, lse);
 #pragma unroll
-      for (int j = 0; j < 64; ++j) p[j] = tt_exp2(fmaf(p[j], a.factor, -lse));
+      for (int j = 0; j < 64; j += 2) {
+        const unsigned long long t = tt_fma2(tt_two(p[j], p[j + 1]), f2, z2);
+        p[j] = tt_exp2(tt_lo(t));
+        p[j + 1] = tt_exp2(tt_hi(t));
+      }
       ok = mbar_wait_warp(dp_full, (unsigned)i & 1u, abort_flag, nullptr, 97);
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -741,8 +802,14 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         unsigned u[32], w[16];
         tc_ld32(tmem_dp + lanes + (unsigned)(half * 64 + c), u);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        const unsigned long long d2 = tt_two(-delta, -delta);
 #pragma unroll
-        for (int j = 0; j < 32; ++j) p[c + j] *= __uint_as_float(u[j]) - delta;
+        for (int j = 0; j < 32; j += 2) {
+          const unsigned long long x = tt_mul2(tt_add2(tt_two(__uint_as_float(u[j]), __uint_as_float(u[j + 1])), d2),
+                                               tt_two(p[c + j], p[c + j + 1]));
+          p[c + j] = tt_lo(x);
+          p[c + j + 1] = tt_hi(x);
+        }
         if (!inside) {  // (a weight of zero has no part even where the other factor is not finite)
 #pragma unroll
           for (int j = 0; j < 32; ++j)

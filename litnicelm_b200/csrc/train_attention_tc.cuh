@@ -28,6 +28,33 @@ __device__ __forceinline__ unsigned tt_pack(float a, float b) {
   return *reinterpret_cast<const unsigned *>(&v);
 }
 
+// Two 32-bit operations in one instruction.
+__device__ __forceinline__ unsigned long long tt_two(float a, float b) {
+  return (unsigned long long)__float_as_uint(a) | (unsigned long long)__float_as_uint(b) << 32;
+}
+__device__ __forceinline__ float tt_lo(unsigned long long x) { return __uint_as_float((unsigned)x); }
+__device__ __forceinline__ float tt_hi(unsigned long long x) { return __uint_as_float((unsigned)(x >> 32)); }
+__device__ __forceinline__ unsigned long long tt_fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+  unsigned long long d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ unsigned long long tt_add2(unsigned long long a, unsigned long long b) {
+  unsigned long long d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ unsigned long long tt_mul2(unsigned long long a, unsigned long long b) {
+  unsigned long long d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float tt_max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 struct TtArgs {
   int n, m, heads, groups, share, streams, dim, tiles;
   TrainSpan span;
