@@ -407,7 +407,7 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_ah, const __grid_const
              mbar_wait_warp(chain_empty(buf), ((unsigned)(it / CHAINS) & 1u) ^ 1u, abort_flag, nullptr, 62);
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        if (lane == 0) {
+        if (tc_elect()) {
           const unsigned st = base + (unsigned)(s * L::STAGE), d = tmem + (unsigned)(buf * T);
           const unsigned long long a0 = A_MN ? umma_desc_mn128(st, 8192u) : umma_desc_k128(st);
           const unsigned long long b0 = B_MN ? umma_desc_mn128(st + 2 * L::TILE, 8192u) : umma_desc_k128(st + 2 * L::TILE);
@@ -427,7 +427,7 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_ah, const __grid_const
       }
     }
     if (!ok) {  // what was issued ends, within the limit, before the shared memory goes away
-      if (lane == 0) ns_commit<PAIR>(done);
+      if (tc_elect()) ns_commit<PAIR>(done);
       __syncwarp();
       const unsigned long long limit = global_timer() + WAIT_LIMIT_NS;
       while (!mbar_try_wait(done, 0u) && global_timer() < limit) {}

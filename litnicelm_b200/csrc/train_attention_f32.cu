@@ -257,7 +257,7 @@ train_forward_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       ok = TF_WAIT(k_full, i, 104);
       if (!ok) break;
       TF_AFTER();
-      if (lane == 0) {
+      if (tc_elect()) {
         tf_mma_rows(tmem_s, q_off, k_off, idesc_s);
         tc_commit(s_full);
       }
@@ -265,14 +265,14 @@ train_forward_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       ok = TF_WAIT(v_full, i, 105) && TF_WAIT(p_ready, i, 106);
       if (!ok) break;
       TF_AFTER();
-      if (lane == 0) {
+      if (tc_elect()) {
         tf_mma_weights(tmem_o, tmem_s, v_off, idesc_o);
         tc_commit(o_full);
       }
       __syncwarp();
     }
     if (!ok) {  // a bounded chance for the tensor pipe to finish before tensor memory is freed
-      if (lane == 0) tc_commit(o_full);
+      if (tc_elect()) tc_commit(o_full);
       __syncwarp();
       const unsigned long long limit = global_timer() + WAIT_LIMIT_NS;
       while (!mbar_try_wait(o_full, (unsigned)i & 1u) && global_timer() < limit) {}
@@ -456,14 +456,14 @@ train_dkv_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       ok = TF_WAIT(q_full, i, 113);
       if (!ok) break;
       TF_AFTER();
-      if (lane == 0) {
+      if (tc_elect()) {
         tf_mma_rows(tmem_s, k_off, q_off, idesc_s);
         tc_commit(s_full);
       }
       __syncwarp();
       ok = TF_WAIT(do_full, i, 114);
       if (!ok) break;
-      if (lane == 0) {
+      if (tc_elect()) {
         tf_mma_rows(tmem_dp, v_off, do_off, idesc_s);
         tc_commit(dp_full);
       }
@@ -471,7 +471,7 @@ train_dkv_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       ok = TF_WAIT(p_ready, i, 115);
       if (!ok) break;
       TF_AFTER();
-      if (lane == 0) {
+      if (tc_elect()) {
         tf_mma_weights(tmem_dv, tmem_s, do_off, idesc_d);
         tc_commit(dv_full);
       }
@@ -479,14 +479,14 @@ train_dkv_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       ok = TF_WAIT(ds_ready, i, 116);
       if (!ok) break;
       TF_AFTER();
-      if (lane == 0) {
+      if (tc_elect()) {
         tf_mma_weights(tmem_dk, tmem_dp, q_off, idesc_d);
         tc_commit(dk_full);
       }
       __syncwarp();
     }
     if (!ok) {  // a bounded chance for the tensor pipe to finish before tensor memory is freed
-      if (lane == 0) tc_commit(dk_full);
+      if (tc_elect()) tc_commit(dk_full);
       __syncwarp();
       const unsigned long long limit = global_timer() + WAIT_LIMIT_NS;
       while (!mbar_try_wait(dk_full, (unsigned)i & 1u) && global_timer() < limit) {}
@@ -663,14 +663,14 @@ train_dq_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       if (!ok) break;
       TF_AFTER();
       // (over dP and its parts: dS k of the tile before has read them, in the order of issue; over S: read before ds_ready)
-      if (lane == 0) {
+      if (tc_elect()) {
         tf_mma_rows(tmem_dp, do_off, v_off, idesc_s);
         tc_commit(dp_full);
       }
       __syncwarp();
       ok = TF_WAIT(k_full, i, 135);
       if (!ok) break;
-      if (lane == 0) {
+      if (tc_elect()) {
         tf_mma_rows(tmem_s, q_off, k_off, idesc_s);
         tc_commit(s_full);
       }
@@ -678,14 +678,14 @@ train_dq_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       ok = TF_WAIT(ds_ready, i, 136);
       if (!ok) break;
       TF_AFTER();
-      if (lane == 0) {
+      if (tc_elect()) {
         tf_mma_weights(tmem_dq, tmem_dp, k_off, idesc_d);
         tc_commit(dq_full);
       }
       __syncwarp();
     }
     if (!ok) {  // a bounded chance for the tensor pipe to finish before tensor memory is freed
-      if (lane == 0) tc_commit(dq_full);
+      if (tc_elect()) tc_commit(dq_full);
       __syncwarp();
       const unsigned long long limit = global_timer() + WAIT_LIMIT_NS;
       while (!mbar_try_wait(dq_full, (unsigned)i & 1u) && global_timer() < limit) {}

@@ -71,6 +71,10 @@ __device__ __forceinline__ void tt_clear_rows(unsigned char *tile, int slabs, in
   __syncwarp();
 }
 
+// 2^x of both halves. (Of a quarter of them by a polynomial on the FMA pipe, as the unit that this instruction runs on takes 1024 clocks
+// a tile: forward 75 -> 80 us, dq and dkv 2 % less, at D = 128 10 % more. So not.)
+__device__ __forceinline__ unsigned long long tt_exp2_two(unsigned long long x) { return tt_two(tt_exp2(tt_lo(x)), tt_exp2(tt_hi(x))); }
+
 // S (128 x 128) = rows of a . rows of b over dim, both with contiguous dim. The loops that issue products are unrolled, with
 // descriptors that differ by constants: with a loop over the steps that dim needs, each instruction's descriptors took the one
 // issuing thread about 130 clocks, twice what the tensor pipe takes for the product.
@@ -169,7 +173,7 @@ train_forward_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       ok = mbar_wait_warp(k_full, (unsigned)i & 1u, abort_flag, nullptr, 74);
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      if (lane == 0) {
+      if (tc_elect()) {
         tt_mma_rows<D>(tmem_s, q_rows, k_rows, idesc_s);
         tc_commit(k_free);
         tc_commit(s_full);
@@ -182,14 +186,14 @@ train_forward_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       ok = mbar_wait_warp(p_ready, (unsigned)i & 1u, abort_flag, nullptr, 76);
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      if (lane == 0) {
+      if (tc_elect()) {
         tt_mma_weights<false>(tmem_o, tmem_s, v_cols, idesc_o, i > 0);
         tc_commit(o_full);
       }
       __syncwarp();
     }
     if (!ok) {  // a bounded chance for the tensor pipe to finish before tensor memory is freed
-      if (lane == 0) tc_commit(o_full);
+      if (tc_elect()) tc_commit(o_full);
       __syncwarp();
       const unsigned long long limit = global_timer() + WAIT_LIMIT_NS;
       while (!mbar_try_wait(o_full, (unsigned)i & 1u) && global_timer() < limit) {}
@@ -229,19 +233,19 @@ train_forward_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       }
       float mq[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-      for (int j = 4; j < TT_B; j += 8) {
+      for (int j = 4; j < TT_B; j += 4) {
+        if ((j >> 2) & 1) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) mq[e] = j + 4 + e < TT_B ? tt_max3(mq[e], s[j + e], s[j + 4 + e]) : fmaxf(mq[e], s[j + e]);
+          for (int e = 0; e < 4; ++e) mq[e] = tt_max3(mq[e], s[j + e], j + 4 < TT_B ? s[(j + 4 + e) % TT_B] : s[j + e]);
+        }
       }
-      const float mx = fmaxf(TT_NEG, fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3])) * factor);
+      const float top = tt_max3(tt_max3(mq[0], mq[1], mq[2]), mq[3], mq[3]) * factor;
+      const float mx = fmaxf(TT_NEG, top);
       const bool grow = mx > m + TT_SLACK;
       const float keep = grow ? tt_exp2(m - mx) : 1.f;
       if (grow) m = mx;
-      l *= keep;
-      if (i > 0) {
-        ok = mbar_wait_warp(o_full, (unsigned)(i - 1) & 1u, abort_flag, nullptr, 78);
-        if (!ok) break;
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      l = l * keep + (mx - mx) + (top != top ? top : 0.f);  // a score that is no number, or infinite, shows in the sum
+      if (i > 0) {  // (the scores are there, so the product before them is done)
         if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll 1
           for (int c0 = 0; c0 < a.dim; c0 += 16) {
@@ -261,10 +265,9 @@ train_forward_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         unsigned pk[16];
 #pragma unroll
         for (int j = 0; j < 32; j += 2) {
-          const unsigned long long t = tt_fma2(tt_two(s[c0 + j], s[c0 + j + 1]), f2, m2);
-          const float e0 = tt_exp2(tt_lo(t)), e1 = tt_exp2(tt_hi(t));
-          lq[(j >> 1) & 3] = tt_add2(lq[(j >> 1) & 3], tt_two(e0, e1));
-          pk[j >> 1] = tt_pack(e0, e1);
+          const unsigned long long e = tt_exp2_two(tt_fma2(tt_two(s[c0 + j], s[c0 + j + 1]), f2, m2));
+          lq[(j >> 1) & 3] = tt_add2(lq[(j >> 1) & 3], e);
+          pk[j >> 1] = tt_pack(tt_lo(e), tt_hi(e));
         }
         tc_st16(tmem_s + lanes + (unsigned)(c0 >> 1), pk);  // over the scores, which this warp has read
       }
@@ -427,13 +430,13 @@ train_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     if (tiles > 0) {
       ok = mbar_wait_warp(kv_full, 0, abort_flag, nullptr, 82) && mbar_wait_warp(a_full(0), 0, abort_flag, nullptr, 83);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      if (ok && lane == 0) {
+      if (ok && tc_elect()) {
         tt_mma_rows<D>(tmem_s, k_rows, q_rows, idesc_s);
         tc_commit(s_full);
       }
       __syncwarp();
       ok = ok && mbar_wait_warp(b_full(0), 0, abort_flag, nullptr, 83);
-      if (ok && lane == 0) {
+      if (ok && tc_elect()) {
         tt_mma_rows<D>(tmem_dp, v_rows, do_rows, idesc_s);
         tc_commit(dp_full);
       }
@@ -444,12 +447,12 @@ train_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       ok = mbar_wait_warp(p_ready, (unsigned)i & 1u, abort_flag, nullptr, 84);
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      if (lane == 0) tt_mma_weights<true>(tmem_dv, tmem_s, do_cols + stage(sb), idesc_d, i > 0);
+      if (tc_elect()) tt_mma_weights<true>(tmem_dv, tmem_s, do_cols + stage(sb), idesc_d, i > 0);
       __syncwarp();
       if (i + 1 < tiles) {
         ok = mbar_wait_warp(a_full(na), (unsigned)((i + 1) / L::NA) & 1u, abort_flag, nullptr, 85);
         if (!ok) break;
-        if (lane == 0) {
+        if (tc_elect()) {
           tt_mma_rows<D>(tmem_s, k_rows, q_rows + stage(na), idesc_s);
           tc_commit(s_full);
         }
@@ -458,7 +461,7 @@ train_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       ok = mbar_wait_warp(ds_ready, (unsigned)i & 1u, abort_flag, nullptr, 86);
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      if (lane == 0) {
+      if (tc_elect()) {
         tt_mma_weights<true>(tmem_dk, tmem_dp, q_cols + stage(sa), idesc_d, i > 0);
         tc_commit(a_empty(sa));
         tc_commit(b_empty(sb));  // (the statistics beside it have been read too)
@@ -467,14 +470,14 @@ train_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       if (i + 1 < tiles) {
         ok = mbar_wait_warp(b_full(nb), (unsigned)((i + 1) / L::NB) & 1u, abort_flag, nullptr, 85);
         if (!ok) break;
-        if (lane == 0) {
+        if (tc_elect()) {
           tt_mma_rows<D>(tmem_dp, v_rows, do_rows + stage(nb), idesc_s);
           tc_commit(dp_full);
         }
         __syncwarp();
       }
     }
-    if (tiles > 0 && lane == 0) tc_commit(done);
+    if (tiles > 0 && tc_elect()) tc_commit(done);
     __syncwarp();
     if (!ok) {  // a bounded chance for the tensor pipe to finish before tensor memory is freed
       const unsigned long long limit = global_timer() + WAIT_LIMIT_NS;
@@ -509,11 +512,12 @@ train_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 #pragma unroll
       for (int j = 0; j < 64; j += 4) {
         const ulonglong2 v = z[j >> 2];
-        const unsigned long long t = tt_fma2(tt_two(p[j], p[j + 1]), f2, v.x), u = tt_fma2(tt_two(p[j + 2], p[j + 3]), f2, v.y);
-        p[j] = tt_exp2(tt_lo(t));
-        p[j + 1] = tt_exp2(tt_hi(t));
-        p[j + 2] = tt_exp2(tt_lo(u));
-        p[j + 3] = tt_exp2(tt_hi(u));
+        const unsigned long long t = tt_exp2_two(tt_fma2(tt_two(p[j], p[j + 1]), f2, v.x));
+        const unsigned long long u = tt_exp2_two(tt_fma2(tt_two(p[j + 2], p[j + 3]), f2, v.y));
+        p[j] = tt_lo(t);
+        p[j + 1] = tt_hi(t);
+        p[j + 2] = tt_lo(u);
+        p[j + 3] = tt_hi(u);
       }
       if (!inside) {
 #pragma unroll
@@ -684,7 +688,7 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     auto upstream = [&](int i) {  // dP of tile i
       const int sb = i % L::NB;
       if (!mbar_wait_warp(b_full(sb), (unsigned)(i / L::NB) & 1u, abort_flag, nullptr, 92)) return false;
-      if (lane == 0) {
+      if (tc_elect()) {
         tt_mma_rows<D>(tmem_dp, do_rows, v_rows + stage(sb), idesc_s);
         tc_commit(dp_full);
         tc_commit(b_empty(sb));
@@ -696,7 +700,7 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     if (tiles > 0) {
       ok = mbar_wait_warp(q_full, 0, abort_flag, nullptr, 93) && arrived(0);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      if (ok && lane == 0) {
+      if (ok && tc_elect()) {
         tt_mma_rows<D>(tmem_s, q_rows, k_rows, idesc_s);
         tc_commit(s_full);
       }
@@ -709,7 +713,7 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         ok = arrived(i + 1) && mbar_wait_warp(s_free, (unsigned)i & 1u, abort_flag, nullptr, 94);
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        if (lane == 0) {
+        if (tc_elect()) {
           tt_mma_rows<D>(tmem_s, q_rows, k_rows + stage(na), idesc_s);
           tc_commit(s_full);
         }
@@ -718,14 +722,14 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       ok = mbar_wait_warp(ds_ready, (unsigned)i & 1u, abort_flag, nullptr, 95);
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      if (lane == 0) {
+      if (tc_elect()) {
         tt_mma_weights<true>(tmem_dq, tmem_dp, k_cols + stage(sa), idesc_d, i > 0);
         tc_commit(a_empty(sa));
       }
       __syncwarp();
       if (i + 1 < tiles) ok = upstream(i + 1);
     }
-    if (tiles > 0 && lane == 0) tc_commit(done);
+    if (tiles > 0 && tc_elect()) tc_commit(done);
     __syncwarp();
     if (!ok) {  // a bounded chance for the tensor pipe to finish before tensor memory is freed
       const unsigned long long limit = global_timer() + WAIT_LIMIT_NS;
@@ -784,9 +788,9 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       const unsigned long long f2 = tt_two(a.factor, a.factor), z2 = tt_two(lse, lse);
 #pragma unroll
       for (int j = 0; j < 64; j += 2) {
-        const unsigned long long t = tt_fma2(tt_two(p[j], p[j + 1]), f2, z2);
-        p[j] = tt_exp2(tt_lo(t));
-        p[j + 1] = tt_exp2(tt_hi(t));
+        const unsigned long long t = tt_exp2_two(tt_fma2(tt_two(p[j], p[j + 1]), f2, z2));
+        p[j] = tt_lo(t);
+        p[j + 1] = tt_hi(t);
       }
       ok = mbar_wait_warp(dp_full, (unsigned)i & 1u, abort_flag, nullptr, 97);
       if (!ok) break;

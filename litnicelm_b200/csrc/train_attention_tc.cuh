@@ -49,9 +49,10 @@ __device__ __forceinline__ unsigned long long tt_mul2(unsigned long long a, unsi
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
+// The largest of three, NaN if one of them is.
 __device__ __forceinline__ float tt_max3(float a, float b, float c) {
   float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
 
