@@ -6,10 +6,15 @@
 // Rows of weight 0 are not read: their logp and gradient are 0. A target outside the vocabulary makes its row's logp and
 // gradient, and the loss, NaN.
 //
-// One block per row: maximum and sum in one pass (a running pair per thread), the gradient in a second one. Row losses are
-// summed in row order in 64 bits, so the loss does not depend on the order in which blocks finish.
-// Bound: HBM, one read of the logits and one write of the gradient.
+// Up to 32768 columns a row stays in registers between its statistics and its gradient: read once, one exponential an element,
+// written once. A warp takes a row of up to 1024 columns, 128, 256 or 512 threads with 64 elements each take longer ones. Beyond,
+// 512 threads read the row twice, the second time from L2 (two blocks an SM, so that their rows fit there). Row losses are summed in
+// row order in 64 bits, so the loss does not depend on the order in which blocks finish.
+// Bound: HBM, one read of the logits and one write of the gradient. 4096 x 32000 in 32 bits, three in ten rows masked: see the
+// launcher.
 #include "train_ops.cuh"
+#include "gemm_tc.cuh"
+#include "tc_ptx.cuh"
 
 #include <cuda_bf16.h>
 
@@ -19,7 +24,6 @@ namespace {
 
 typedef __nv_bfloat16 bf16;
 
-constexpr int PL_THREADS = 256;
 constexpr float PL_LOG2E = 1.4426950408889634f;
 
 struct PlWork {
@@ -48,24 +52,41 @@ __device__ __forceinline__ double ordered_block_sum(const T *x, int n) {
 }
 
 __global__ void __launch_bounds__(1024) policy_weight_kernel(const float *weight, int rows, PlWork w) {
+  pdl_launch_dependents();
   const double s = ordered_block_sum(weight, rows);
   if (threadIdx.x == 0) *w.total = s;
 }
 __global__ void __launch_bounds__(1024) policy_join_kernel(int rows, PlWork w, float *loss) {
+  pdl_wait();
   const double s = ordered_block_sum(w.row_loss, rows);
   if (threadIdx.x == 0) *loss = (float)s;
 }
 
+// 2^x; below 2^-126 0
+__device__ __forceinline__ float pl_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// What the loss of a row needs beside its logits; read before them, by the thread that finishes the row.
+struct PlTerms {
+  float adv, old, ref;
+};
+__device__ __forceinline__ PlTerms terms_of(const PolicyLoss &a, int row) {
+  return PlTerms{a.advantage[row], a.old_logp[row], a.kl_weight != 0.f ? a.ref_logp[row] : 0.f};
+}
+
 // The row's share of the loss and its derivative in logp.
-__device__ __forceinline__ void row_terms(const PolicyLoss &a, float logp, int row, float share, double &loss, float &g) {
-  const float adv = a.advantage[row], r = expf(logp - a.old_logp[row]);
+__device__ __forceinline__ void row_terms(const PolicyLoss &a, const PlTerms &t, float logp, float share, double &loss, float &g) {
+  const float r = expf(logp - t.old);
   const float low = 1.f - a.clip_low, high = 1.f + a.clip_high;
-  const float taken = r * adv, clipped = fminf(fmaxf(r, low), high) * adv;
+  const float taken = r * t.adv, clipped = fminf(fmaxf(r, low), high) * t.adv;
   float value = taken != taken ? taken : -fminf(taken, clipped);
-  float d = (adv >= 0.f ? r <= high : r >= low) ? -taken : 0.f;
+  float d = (t.adv >= 0.f ? r <= high : r >= low) ? -taken : 0.f;
   if (r != r) d = r;
   if (a.kl_weight != 0.f) {
-    const float diff = a.ref_logp[row] - logp, e = expf(diff);
+    const float diff = t.ref - logp, e = expf(diff);
     value += a.kl_weight * (fabsf(diff) < 0.25f ? expm1f(diff) - diff : e - diff - 1.f);
     d += a.kl_weight * -expm1f(diff);
   }
@@ -73,147 +94,430 @@ __device__ __forceinline__ void row_terms(const PolicyLoss &a, float logp, int r
   g = d * share;
 }
 
-template <typename T, int V>
-struct Vec;
+template <typename T>
+struct PlVec;
 template <>
-struct Vec<float, 4> { typedef float4 type; };
+struct PlVec<float> { static constexpr int V = 4; };
 template <>
-struct Vec<bf16, 8> { typedef uint4 type; };
+struct PlVec<bf16> { static constexpr int V = 8; };
 
-template <typename T, int V>
-__device__ __forceinline__ void unpack(const typename Vec<T, V>::type &u, float (&x)[V]) {
+// V consecutive elements; of those before `count`.
+template <typename T>
+__device__ __forceinline__ void load_vec(const T *p, float *x) {
+  const uint4 u = __ldcs(reinterpret_cast<const uint4 *>(p));
   const T *t = reinterpret_cast<const T *>(&u);
 #pragma unroll
-  for (int i = 0; i < V; ++i) x[i] = to_float(t[i]);
+  for (int i = 0; i < PlVec<T>::V; ++i) x[i] = to_float(t[i]);
+}
+template <typename T>
+__device__ __forceinline__ void store_vec(T *p, const float *x) {
+  uint4 u;
+  T *t = reinterpret_cast<T *>(&u);
+#pragma unroll
+  for (int i = 0; i < PlVec<T>::V; ++i) from_float(t + i, x[i]);
+  __stcs(reinterpret_cast<uint4 *>(p), u);
 }
 
-template <typename T, int V>  // V elements of 16 bytes at a time where rows allow it, else one at a time
-__global__ void __launch_bounds__(PL_THREADS)
-policy_rows_kernel(const __grid_constant__ PolicyLoss a, PlWork w, int vec, int dvec) {
-  const int row = blockIdx.x, tid = threadIdx.x;
-  const float weight = a.weight ? a.weight[row] : 1.f;
+struct PlForms {
+  int vec, dvec;  // rows of logits and of the gradient on 16-byte boundaries
+};
+
+// What a row is: its share of the loss, or why it has none (fill: 0 for weight 0, NaN for a bad target).
+struct PlRow {
+  float weight;
+  int target;
+  bool fills;
+  float fill;
+};
+__device__ __forceinline__ PlRow row_of(const PolicyLoss &a, int row) {
+  PlRow r;
+  r.weight = a.weight ? a.weight[row] : 1.f;
+  r.target = r.weight != 0.f ? a.targets[row] : 0;
+  r.fills = r.weight == 0.f || r.target < 0 || r.target >= a.vocab;
+  r.fill = r.weight == 0.f ? 0.f : NAN;
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void fill_row(const PolicyLoss &a, const PlWork &w, const PlForms &f, int row, float fill, int at, int threads) {
+  if (at == 0) {
+    a.logp[row] = fill;
+    w.row_loss[row] = fill;
+  }
+  if (!a.dlogits) return;
+  constexpr int V = PlVec<T>::V;
+  T *dx = reinterpret_cast<T *>(a.dlogits) + row * a.dld;
+  int c = 0;
+  if (f.dvec) {
+    float x[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = fill;
+    for (c = at * V; c + V <= a.vocab; c += threads * V) store_vec(dx + c, x);
+    c = a.vocab / V * V;
+  }
+  for (c += at; c < a.vocab; c += threads) from_float(dx + c, fill);
+}
+// 1 / the weights' sum, once it is there.
+__device__ __forceinline__ double inverse_total(const PolicyLoss &a, const PlWork &w) {
+  return 1.0 / (a.weight ? *static_cast<volatile double *>(w.total) : (double)a.rows);
+}
+// Loss and slope of a row from its statistics, by one thread: the slope in the logits comes back.
+__device__ __forceinline__ float finish_row(const PolicyLoss &a, const PlWork &w, int row, const PlTerms &t, float share, float z, float top,
+                                            float sum) {
+  const float logp = (z - top) * a.inv_temp - logf(sum);
+  double loss;
+  float slope;
+  row_terms(a, t, logp, share, loss, slope);
+  a.logp[row] = logp;
+  w.row_loss[row] = loss;
+  return slope * a.inv_temp;
+}
+
+// THREADS to a row, ROWS rows to a block (THREADS = 32: a warp each), up to 64 (32) elements to a thread, all in registers.
+template <typename T, int THREADS, int ROWS>
+__global__ void __launch_bounds__(THREADS *ROWS)
+policy_row_kernel(const __grid_constant__ PolicyLoss a, PlWork w, PlForms f) {
+  constexpr int V = PlVec<T>::V, N = (THREADS == 32 ? 32 : 64) / V, WARPS = THREADS / 32;
+  const int at = threadIdx.x % THREADS, row = blockIdx.x * ROWS + threadIdx.x / THREADS;
+  __shared__ float red[2][WARPS];
+  __shared__ float out[1];
+  if (ROWS > 1 && row >= a.rows) return;  // (a whole warp)
+  const PlRow r = row_of(a, row);
+  if (r.fills) {
+    if (a.weight) pdl_wait();  // (an earlier call's sums have been read)
+    return fill_row<T>(a, w, f, row, r.fill, at, THREADS);
+  }
   const T *x = reinterpret_cast<const T *>(a.logits) + row * a.ld;
   T *dx = reinterpret_cast<T *>(a.dlogits) + row * a.dld;
-  float share, slope, logp;
-  const double total = a.weight ? *w.total : (double)a.rows;
-  const int target = weight != 0.f ? a.targets[row] : 0;
-  if (weight == 0.f || target < 0 || target >= a.vocab) {
-    const float fill = weight == 0.f ? 0.f : NAN;
-    if (tid == 0) {
-      a.logp[row] = fill;
-      w.row_loss[row] = fill;
-    }
-    if (a.dlogits)
-      for (int c = tid; c < a.vocab; c += PL_THREADS) from_float(dx + c, fill);
-    return;
-  }
-  share = (float)((double)weight / total);
-  // exp2(z * f - top), top = max * f
-  const float f = a.inv_temp * PL_LOG2E;
-  float m = -INFINITY, s = 0.f;
-  auto add = [&](float z) {
-    if (z > m) {
-      s = s * exp2f((m - z) * f);
-      m = z;
-    }
-    s += z == -INFINITY ? 0.f : exp2f((z - m) * f);
-  };
-  if (vec) {
-    const int n = a.vocab / V * V;
-    for (int c = tid * V; c < n; c += PL_THREADS * V) {
-      float z[V];
-      unpack<T, V>(*reinterpret_cast<const typename Vec<T, V>::type *>(x + c), z);
-      float top = z[0];
+  const PlTerms t = at == 0 ? terms_of(a, row) : PlTerms{};
+  const float zt = at == 0 ? to_float(x[r.target]) : 0.f;
+  float z[N * V];
+  // vectors: element (i THREADS + at) V + j; one at a time: (i V + j) THREADS + at
+  auto place = [&](int i, int j) { return f.vec ? (i * THREADS + at) * V + j : (i * V + j) * THREADS + at; };
+  if (f.vec) {
 #pragma unroll
-      for (int i = 1; i < V; ++i) top = fmaxf(top, z[i]);
-      if (top > m) {
-        s = s * exp2f((m - top) * f);
-        m = top;
-      }
-      if (m != -INFINITY) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) s += exp2f((z[i] - m) * f);
+    for (int i = 0; i < N; ++i) {
+      const int c = (i * THREADS + at) * V;
+      if (c + V <= a.vocab) {
+        load_vec(x + c, z + i * V);
       } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) s += z[i] == z[i] ? 0.f : z[i];
+        for (int j = 0; j < V; ++j) z[i * V + j] = c + j < a.vocab ? to_float(x[c + j]) : -INFINITY;
       }
     }
-    for (int c = n + tid; c < a.vocab; c += PL_THREADS) add(to_float(x[c]));
   } else {
-    for (int c = tid; c < a.vocab; c += PL_THREADS) add(to_float(x[c]));
+#pragma unroll
+    for (int i = 0; i < N * V; ++i) z[i] = i * THREADS + at < a.vocab ? to_float(x[i * THREADS + at]) : -INFINITY;
   }
-  __shared__ float sm_m[PL_THREADS / 32], sm_s[PL_THREADS / 32];
+  auto all = [&](float v, bool sum, int which) {  // over the row's threads
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const float u = __shfl_xor_sync(0xffffffffu, v, o);
+      v = sum ? v + u : fmaxf(v, u);
+    }
+    if (WARPS == 1) return v;
+    if ((at & 31) == 0) red[which][at >> 5] = v;
+    __syncthreads();
+    v = red[which][0];
+#pragma unroll
+    for (int i = 1; i < WARPS; ++i) v = sum ? v + red[which][i] : fmaxf(v, red[which][i]);
+    return v;
+  };
+  float top = z[0];
+#pragma unroll
+  for (int i = 1; i < N * V; ++i) top = fmaxf(top, z[i]);
+  top = all(top, false, 0);
+  const float factor = a.inv_temp * PL_LOG2E;
+  float s4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < N * V; ++i) {
+    z[i] = pl_exp2((z[i] - top) * factor);
+    s4[i & 3] += z[i];
+  }
+  const float sum = all((s4[0] + s4[1]) + (s4[2] + s4[3]), true, 1);
+  if (a.weight) pdl_wait();  // the weights' sum is there
+  float slope;
+  const float share = at == 0 ? (float)((double)r.weight * inverse_total(a, w)) : 0.f;
+  if (WARPS == 1) {
+    slope = at == 0 ? finish_row(a, w, row, t, share, zt, top, sum) : 0.f;
+    slope = __shfl_sync(0xffffffffu, slope, 0);
+  } else {
+    if (at == 0) out[0] = finish_row(a, w, row, t, share, zt, top, sum);
+    __syncthreads();
+    slope = out[0];
+  }
+  if (!a.dlogits) return;
+  const float per = -slope / sum;
+#pragma unroll
+  for (int i = 0; i < N * V; ++i) z[i] *= per;
+  if (f.vec && f.dvec) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = (i * THREADS + at) * V;
+      if (c <= r.target && r.target < c + V) {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (c + j == r.target) z[i * V + j] += slope;
+      }
+      if (c + V <= a.vocab) {
+        store_vec(dx + c, z + i * V);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (c + j < a.vocab) from_float(dx + c + j, z[i * V + j]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const int c = place(i, j);
+        if (c < a.vocab) from_float(dx + c, c == r.target ? z[i * V + j] + slope : z[i * V + j]);
+      }
+  }
+}
+
+// The same for rows of 8193 to 32768 columns on 16-byte boundaries: a block of 1024 threads per SM walks rows, 32 elements to a thread, and
+// brings the next row into shared memory while it works on one.
+constexpr int PL_STREAM = 1024;
+template <typename T>
+__global__ void __launch_bounds__(PL_STREAM, 1)
+policy_stream_kernel(const __grid_constant__ PolicyLoss a, PlWork w, PlForms f) {
+  constexpr int V = PlVec<T>::V, N = 32 / V, WARPS = PL_STREAM / 32;
+  extern __shared__ __align__(16) unsigned char sm_row[];
+  __shared__ __align__(8) unsigned long long bar_word;
+  __shared__ float red[2][WARPS], out[1];
+  __shared__ int abort_word;
+  const int tid = threadIdx.x, whole = a.vocab / V * V;
+  const unsigned bar = smem_u32(&bar_word);
+  auto fetch = [&](int row) {  // by one thread: the row's whole vectors, if it is read at all
+    if (row >= a.rows || row_of(a, row).fills) return;
+    const unsigned bytes = (unsigned)whole * (unsigned)sizeof(T);
+    mbar_expect_tx(bar, bytes);
+    bulk_load(smem_u32(sm_row), reinterpret_cast<const T *>(a.logits) + row * a.ld, bytes, bar);
+  };
+  if (tid == 0) {
+    mbar_init(bar, 1);
+    abort_word = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    fetch(blockIdx.x);
+  }
+  __syncthreads();
+  if (a.weight) pdl_wait();
+  unsigned phase = 0;
+  const float factor = a.inv_temp * PL_LOG2E;
+  const double inverse = tid == 0 ? inverse_total(a, w) : 0.0;
+  for (int row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const PlRow r = row_of(a, row);
+    if (r.fills) {
+      if (tid == 0) fetch(row + gridDim.x);
+      fill_row<T>(a, w, f, row, r.fill, tid, PL_STREAM);
+      continue;
+    }
+    const T *x = reinterpret_cast<const T *>(a.logits) + row * a.ld;
+    T *dx = reinterpret_cast<T *>(a.dlogits) + row * a.dld;
+    const PlTerms t = tid == 0 ? terms_of(a, row) : PlTerms{};
+    const float zt = tid == 0 ? to_float(x[r.target]) : 0.f, share = (float)((double)r.weight * inverse);
+    const bool there = mbar_wait(bar, phase & 1u, reinterpret_cast<volatile int *>(&abort_word), nullptr, 141);
+    ++phase;
+    float z[32];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = (i * PL_STREAM + tid) * V;
+      if (c < whole) {
+        const uint4 u = *reinterpret_cast<const uint4 *>(sm_row + (size_t)c * sizeof(T));
+        const T *e = reinterpret_cast<const T *>(&u);
+#pragma unroll
+        for (int j = 0; j < V; ++j) z[i * V + j] = to_float(e[j]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) z[i * V + j] = c + j < a.vocab ? to_float(x[c + j]) : -INFINITY;
+      }
+    }
+    if (!__syncthreads_and(there)) {  // the row did not come
+      fill_row<T>(a, w, f, row, NAN, tid, PL_STREAM);
+      continue;
+    }
+    if (tid == 0) fetch(row + gridDim.x);
+    auto all = [&](float v, bool sum, int which) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        const float u = __shfl_xor_sync(0xffffffffu, v, o);
+        v = sum ? v + u : fmaxf(v, u);
+      }
+      if ((tid & 31) == 0) red[which][tid >> 5] = v;
+      __syncthreads();
+      v = red[which][tid & 31];
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        const float u = __shfl_xor_sync(0xffffffffu, v, o);
+        v = sum ? v + u : fmaxf(v, u);
+      }
+      return v;
+    };
+    float top = z[0];
+#pragma unroll
+    for (int i = 1; i < 32; ++i) top = fmaxf(top, z[i]);
+    top = all(top, false, 0);
+    float s4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      z[i] = pl_exp2((z[i] - top) * factor);
+      s4[i & 3] += z[i];
+    }
+    const float sum = all((s4[0] + s4[1]) + (s4[2] + s4[3]), true, 1);
+    if (tid == 0) out[0] = finish_row(a, w, row, t, share, zt, top, sum);
+    __syncthreads();
+    if (!a.dlogits) continue;
+    const float slope = out[0], per = -slope / sum;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = (i * PL_STREAM + tid) * V;
+      float d[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        d[j] = z[i * V + j] * per;
+        if (c + j == r.target) d[j] += slope;
+      }
+      if (f.dvec && c < whole) {
+        store_vec(dx + c, d);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (c + j < a.vocab) from_float(dx + c + j, d[j]);
+      }
+    }
+  }
+}
+
+// Any number of columns: a running maximum and sum per thread, then the row again.
+constexpr int PL_LONG = 512;
+template <typename T>
+__global__ void __launch_bounds__(PL_LONG, 2)
+policy_long_kernel(const __grid_constant__ PolicyLoss a, PlWork w, PlForms f) {
+  constexpr int V = PlVec<T>::V, AHEAD = 4, WARPS = PL_LONG / 32;
+  const int row = blockIdx.x, tid = threadIdx.x;
+  const PlRow r = row_of(a, row);
+  if (r.fills) {
+    if (a.weight) pdl_wait();
+    return fill_row<T>(a, w, f, row, r.fill, tid, PL_LONG);
+  }
+  const T *x = reinterpret_cast<const T *>(a.logits) + row * a.ld;
+  T *dx = reinterpret_cast<T *>(a.dlogits) + row * a.dld;
+  const float factor = a.inv_temp * PL_LOG2E;
+  float m = -INFINITY, s = 0.f;
+  auto add = [&](const float *z, int n) {
+    float top = z[0];
+    for (int i = 1; i < n; ++i) top = fmaxf(top, z[i]);
+    if (top > m) {
+      s *= pl_exp2((m - top) * factor);
+      m = top;
+    }
+    const float base = m == -INFINITY ? 0.f : m;
+    for (int i = 0; i < n; ++i) s += pl_exp2((z[i] - base) * factor);
+  };
+  const int whole = f.vec ? a.vocab / V * V : 0;  // columns that vectors cover
+  for (int c = tid * V; c < whole; c += PL_LONG * V * AHEAD) {
+    float z[AHEAD * V];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const int at = c + u * PL_LONG * V;
+      if (at < whole) {
+        const uint4 q = *reinterpret_cast<const uint4 *>(x + at);
+        const T *t = reinterpret_cast<const T *>(&q);
+#pragma unroll
+        for (int i = 0; i < V; ++i) z[u * V + i] = to_float(t[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) z[u * V + i] = -INFINITY;
+      }
+    }
+    add(z, AHEAD * V);
+  }
+  for (int c = whole + tid; c < a.vocab; c += PL_LONG) {
+    const float z = to_float(x[c]);
+    add(&z, 1);
+  }
+  __shared__ float sm_m[WARPS], sm_s[WARPS], out[3];
   auto join = [&](float m2, float s2) {
-    const float top = fmaxf(m, m2);
-    const float base = top == -INFINITY ? 0.f : top;
-    s = s * exp2f((m - base) * f) + s2 * exp2f((m2 - base) * f);
+    const float top = fmaxf(m, m2), base = top == -INFINITY ? 0.f : top;
+    s = s * pl_exp2((m - base) * factor) + s2 * pl_exp2((m2 - base) * factor);
     m = top;
   };
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) join(__shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, s, o));
+  for (int o = 16; o > 0; o >>= 1) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+    join(m2, s2);
+  }
   if ((tid & 31) == 0) {
     sm_m[tid >> 5] = m;
     sm_s[tid >> 5] = s;
   }
-  __shared__ float out[2];
   __syncthreads();
   if (tid < 32) {
-    m = tid < PL_THREADS / 32 ? sm_m[tid] : -INFINITY;
-    s = tid < PL_THREADS / 32 ? sm_s[tid] : 0.f;
+    m = tid < WARPS ? sm_m[tid] : -INFINITY;
+    s = tid < WARPS ? sm_s[tid] : 0.f;
 #pragma unroll
-    for (int o = PL_THREADS / 64; o > 0; o >>= 1) join(__shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, s, o));
+    for (int o = WARPS / 2; o > 0; o >>= 1) {
+      const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+      join(m2, s2);
+    }
     if (tid == 0) {
-      logp = (to_float(x[target]) - m) * a.inv_temp - logf(s);
-      double loss;
-      row_terms(a, logp, row, share, loss, slope);
-      a.logp[row] = logp;
-      w.row_loss[row] = loss;
-      out[0] = slope;
+      if (a.weight) pdl_wait();  // the weights' sum is there
+      if (m == -INFINITY) s = NAN;  // a row that is masked altogether is not a distribution
+      out[0] = finish_row(a, w, row, terms_of(a, row), (float)((double)r.weight * inverse_total(a, w)), to_float(x[r.target]), m, s);
       out[1] = m;
-      sm_s[0] = s;
+      out[2] = s;
     }
   }
   __syncthreads();
   if (!a.dlogits) return;
-  slope = out[0] * a.inv_temp;
+  const float slope = out[0], per = -slope / out[2];
   m = out[1];
-  const float per = -slope / sm_s[0];
-  // the block's maximum subtracted before the factor: exact where the logits are near it
-  if (vec && dvec) {
-    const int n = a.vocab / V * V;
-    for (int c = tid * V; c < n; c += PL_THREADS * V) {
-      typename Vec<T, V>::type u = *reinterpret_cast<const typename Vec<T, V>::type *>(x + c);
-      float z[V];
-      unpack<T, V>(u, z);
-      T *t = reinterpret_cast<T *>(&u);
+  const int both = f.dvec ? whole : 0;
+  for (int c = tid * V; c < both; c += PL_LONG * V * AHEAD) {
+    uint4 q[AHEAD];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+      if (c + u * PL_LONG * V < both) q[u] = __ldcs(reinterpret_cast<const uint4 *>(x + c + u * PL_LONG * V));
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const int at = c + u * PL_LONG * V;
+      if (at >= both) break;
+      const T *t = reinterpret_cast<const T *>(&q[u]);
+      float d[V];
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        float d = exp2f((z[i] - m) * f) * per;
-        if (c + i == target) d += slope;
-        from_float(t + i, d);
+        d[i] = pl_exp2((to_float(t[i]) - m) * factor) * per;
+        if (at + i == r.target) d[i] += slope;
       }
-      *reinterpret_cast<typename Vec<T, V>::type *>(dx + c) = u;
+      store_vec(dx + at, d);
     }
-    for (int c = n + tid; c < a.vocab; c += PL_THREADS) {
-      float d = exp2f((to_float(x[c]) - m) * f) * per;
-      if (c == target) d += slope;
-      from_float(dx + c, d);
-    }
-  } else {
-    for (int c = tid; c < a.vocab; c += PL_THREADS) {
-      float d = exp2f((to_float(x[c]) - m) * f) * per;
-      if (c == target) d += slope;
-      from_float(dx + c, d);
-    }
+  }
+  for (int c = both + tid; c < a.vocab; c += PL_LONG) {
+    const float d = pl_exp2((to_float(x[c]) - m) * factor) * per;
+    from_float(dx + c, c == r.target ? d + slope : d);
   }
 }
 
-template <typename T, int V>
+template <typename T>
 void launch_rows(const PolicyLoss &a, const PlWork &w, cudaStream_t st) {
-  const bool vec = a.ld % V == 0 && (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0;
-  const bool dvec = a.dld % V == 0 && (reinterpret_cast<uintptr_t>(a.dlogits) & 15) == 0;
-  policy_rows_kernel<T, V><<<(unsigned)a.rows, PL_THREADS, 0, st>>>(a, w, vec, dvec);
-  LB_LAUNCH_CHECK();
+  constexpr int V = PlVec<T>::V;
+  PlForms f;
+  f.vec = (a.rows == 1 || a.ld % V == 0) && (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0;
+  f.dvec = (a.rows == 1 || a.dld % V == 0) && (reinterpret_cast<uintptr_t>(a.dlogits) & 15) == 0;
+  const bool pdl = a.weight != nullptr;  // behind the sum of the weights, which was launched the ordinary way: what came before it is done
+  const unsigned rows = (unsigned)a.rows;
+  if (a.vocab <= 1024) launch_pdl(policy_row_kernel<T, 32, 4>, dim3((rows + 3) / 4), dim3(128), 0, st, pdl, a, w, f);
+  else if (a.vocab <= 8192) launch_pdl(policy_row_kernel<T, 128, 1>, dim3(rows), dim3(128), 0, st, pdl, a, w, f);
+  else if (f.vec && a.vocab <= 32768) {
+    static SharedMemoryOnce once;
+    once.set(policy_stream_kernel<T>, 32768 * (int)sizeof(T));
+    launch_pdl(policy_stream_kernel<T>, dim3(rows < 148 ? rows : 148), dim3(PL_STREAM), (size_t)a.vocab * sizeof(T), st, pdl, a, w, f);
+  } else if (a.vocab <= 16384) launch_pdl(policy_row_kernel<T, 256, 1>, dim3(rows), dim3(256), 0, st, pdl, a, w, f);
+  else if (a.vocab <= 32768) launch_pdl(policy_row_kernel<T, 512, 1>, dim3(rows), dim3(512), 0, st, pdl, a, w, f);
+  else launch_pdl(policy_long_kernel<T>, dim3(rows), dim3(PL_LONG), 0, st, pdl, a, w, f);
 }
 
 }  // namespace
@@ -226,10 +530,9 @@ void launch_policy_loss(const PolicyLoss &a, void *workspace, cudaStream_t st) {
     policy_weight_kernel<<<1, 1024, 0, st>>>(a.weight, a.rows, w);
     LB_LAUNCH_CHECK();
   }
-  if (a.bf16) launch_rows<bf16, 8>(a, w, st);
-  else launch_rows<float, 4>(a, w, st);
-  policy_join_kernel<<<1, 1024, 0, st>>>(a.rows, w, a.loss);
-  LB_LAUNCH_CHECK();
+  if (a.bf16) launch_rows<bf16>(a, w, st);
+  else launch_rows<float>(a, w, st);
+  launch_pdl(policy_join_kernel, dim3(1), dim3(1024), 0, st, true, a.rows, w, a.loss);
 }
 
 }  // namespace lb
