@@ -69,11 +69,7 @@ __device__ __forceinline__ int ns_exp_b(float rho, int k) {
   return ns_exponent(fminf(2.85f, 4.8f * s * s));
 }
 
-__device__ __forceinline__ void ns_split(float z, __half &hi, __half &lo) {  // z already scaled
-  hi = __float2half_rn(z);
-  lo = __float2half_rn((z - __half2float(hi)) * 2048.f);
-}
-// Two at once: a conversion of two values costs what one does.
+// Two values, already scaled, as pairs: a conversion of two costs what one does.
 __device__ __forceinline__ void ns_split2(float a, float b, unsigned &hi, unsigned &lo) {
   const __half2 h = __floats2half2_rn(a, b);
   const float2 f = __half22float2(h);
@@ -127,29 +123,54 @@ __device__ __forceinline__ double ns_block_sum(double s) {
 
 enum { VEC_G = 1, VEC_M = 2, VEC_P = 4 };
 
+// Four groups of four elements at a time and thread, so that their loads are in flight together (with one the three kernels around
+// the products took 125 us on four matrices of 4096 x 1024, see launch_muon).
+constexpr int NS_AHEAD = 4;
+template <typename F>
+__device__ __forceinline__ void for_quads(long long rows, long long quads, F f) {
+  const long long all = rows * quads, step = 256LL * gridDim.x;
+  for (long long e0 = blockIdx.x * 256LL + threadIdx.x; e0 < all; e0 += NS_AHEAD * step) {
+    long long r[NS_AHEAD], c[NS_AHEAD];
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < NS_AHEAD; ++i) {
+      const long long e = e0 + i * step < all ? e0 + i * step : e0;  // (a group past the end is the first one's again, and not used)
+      r[i] = div_index(e, quads);
+      c[i] = (e - r[i] * quads) * 4;
+      n += e0 + i * step < all;
+    }
+    f(r, c, n);
+  }
+}
+
 __global__ void __launch_bounds__(256) muon_begin_kernel(const __grid_constant__ MuonStep g, NsWork w, unsigned vec) {
   pdl_launch_dependents();
   pdl_wait();
-  const long long batch = blockIdx.y, quads = (g.grads.cols + 3) / 4, each = g.grads.rows * quads;
+  const long long batch = blockIdx.y;
   const long long go = batch_offset(g.grads, batch), mo = g.step ? batch_offset(g.momentum, batch) : 0;
   double sum = 0.0;
-  for (long long e = blockIdx.x * 256LL + threadIdx.x; e < each; e += 256LL * gridDim.x) {
-    const long long r = div_index(e, quads), c = (e - r * quads) * 4;
-    float u[4];
-    load4(g.grads, go, r, c, vec & VEC_G, u);
-    if (g.step) {
-      float m[4];
-      load4(g.momentum, mo, r, c, vec & VEC_M, m);
+  for_quads(g.grads.rows, (g.grads.cols + 3) / 4, [&](const long long(&r)[NS_AHEAD], const long long(&c)[NS_AHEAD], int n) {
+    float u[NS_AHEAD][4], m[NS_AHEAD][4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        m[j] = fmaf(g.mu, m[j], u[j]);
-        u[j] = g.nesterov ? fmaf(g.mu, m[j], u[j]) : m[j];
-      }
-      store4(g.momentum, mo, r, c, vec & VEC_M, m);
+    for (int i = 0; i < NS_AHEAD; ++i) {
+      load4(g.grads, go, r[i], c[i], vec & VEC_G, u[i]);
+      if (g.step) load4(g.momentum, mo, r[i], c[i], vec & VEC_M, m[i]);
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) sum += (double)u[j] * (double)u[j];
-  }
+    for (int i = 0; i < NS_AHEAD; ++i) {
+      if (i >= n) break;
+      if (g.step) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          m[i][j] = fmaf(g.mu, m[i][j], u[i][j]);
+          u[i][j] = g.nesterov ? fmaf(g.mu, m[i][j], u[i][j]) : m[i][j];
+        }
+        store4(g.momentum, mo, r[i], c[i], vec & VEC_M, m[i]);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum += (double)u[i][j] * (double)u[i][j];
+    }
+  });
   sum = ns_block_sum(sum);
   if (threadIdx.x == 0) w.parts[batch * NS_PARTS + blockIdx.x] = sum;
 }
@@ -157,7 +178,7 @@ __global__ void __launch_bounds__(256) muon_begin_kernel(const __grid_constant__
 __global__ void __launch_bounds__(256) muon_pair_kernel(const __grid_constant__ MuonStep g, NsWork w, unsigned vec, int parts) {
   pdl_launch_dependents();
   pdl_wait();
-  const long long batch = blockIdx.y, quads = w.ldx / 4, each = g.grads.rows * quads;
+  const long long batch = blockIdx.y;
   const long long go = batch_offset(g.grads, batch), mo = g.step ? batch_offset(g.momentum, batch) : 0;
   const double norm = sqrt(ns_block_sum((int)threadIdx.x < parts ? w.parts[batch * NS_PARTS + threadIdx.x] : 0.0));
   const double inv = 1.0 / (norm + (double)NS_EPS);
@@ -165,49 +186,65 @@ __global__ void __launch_bounds__(256) muon_pair_kernel(const __grid_constant__ 
   if (blockIdx.x == 0 && threadIdx.x == 0) w.rho[batch] = rho;
   const double scale = inv * (double)ns_pow2(ns_exp_x(rho, 0));
   __half *hi = w.x[0].hi + batch * g.grads.rows * w.ldx, *lo = w.x[0].lo + batch * g.grads.rows * w.ldx;
-  for (long long e = blockIdx.x * 256LL + threadIdx.x; e < each; e += 256LL * gridDim.x) {
-    const long long r = div_index(e, quads), c = (e - r * quads) * 4;
-    float u[4] = {0.f, 0.f, 0.f, 0.f};
-    if (c < g.grads.cols) load4(g.grads, go, r, c, vec & VEC_G, u);
-    if (g.step && c < g.grads.cols) {
-      float m[4];
-      load4(g.momentum, mo, r, c, vec & VEC_M, m);
+  for_quads(g.grads.rows, w.ldx / 4, [&](const long long(&r)[NS_AHEAD], const long long(&c)[NS_AHEAD], int n) {
+    float u[NS_AHEAD][4], m[NS_AHEAD][4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) u[j] = g.nesterov ? fmaf(g.mu, m[j], u[j]) : m[j];
+    for (int i = 0; i < NS_AHEAD; ++i) {
+      const bool in = c[i] < g.grads.cols;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) u[i][j] = m[i][j] = 0.f;
+      if (in) load4(g.grads, go, r[i], c[i], vec & VEC_G, u[i]);
+      if (in && g.step) load4(g.momentum, mo, r[i], c[i], vec & VEC_M, m[i]);
     }
-    __half h[4], l[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) ns_split((float)((double)u[j] * scale), h[j], l[j]);
-    *reinterpret_cast<uint2 *>(hi + r * w.ldx + c) = *reinterpret_cast<const uint2 *>(h);
-    *reinterpret_cast<uint2 *>(lo + r * w.ldx + c) = *reinterpret_cast<const uint2 *>(l);
-  }
+    for (int i = 0; i < NS_AHEAD; ++i) {
+      if (i >= n) break;
+      unsigned h[2], l[2];
+      float x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float v = !g.step ? u[i][j] : g.nesterov ? fmaf(g.mu, m[i][j], u[i][j]) : m[i][j];
+        x[j] = (float)((double)v * scale);
+      }
+      ns_split2(x[0], x[1], h[0], l[0]);
+      ns_split2(x[2], x[3], h[1], l[1]);
+      *reinterpret_cast<uint2 *>(hi + r[i] * w.ldx + c[i]) = make_uint2(h[0], h[1]);
+      *reinterpret_cast<uint2 *>(lo + r[i] * w.ldx + c[i]) = make_uint2(l[0], l[1]);
+    }
+  });
 }
 
 __global__ void __launch_bounds__(256) muon_end_kernel(const __grid_constant__ MuonStep g, NsWork w, unsigned vec, float keep,
                                                        float rate) {
   pdl_launch_dependents();
   pdl_wait();
-  const long long batch = blockIdx.y, quads = (g.grads.cols + 3) / 4, each = g.grads.rows * quads;
+  const long long batch = blockIdx.y;
   const long long po = batch_offset(g.params, batch);
   const Pair x = w.x[g.steps & 1];
   const __half *hi = x.hi + batch * g.grads.rows * w.ldx, *lo = x.lo + batch * g.grads.rows * w.ldx;
   const float scale = ns_pow2(-ns_exp_x(w.rho[batch], g.steps));
-  for (long long e = blockIdx.x * 256LL + threadIdx.x; e < each; e += 256LL * gridDim.x) {
-    const long long r = div_index(e, quads), c = (e - r * quads) * 4;
-    __half h[4], l[4];
-    *reinterpret_cast<uint2 *>(h) = *reinterpret_cast<const uint2 *>(hi + r * w.ldx + c);
-    *reinterpret_cast<uint2 *>(l) = *reinterpret_cast<const uint2 *>(lo + r * w.ldx + c);
-    float v[4];
+  for_quads(g.grads.rows, (g.grads.cols + 3) / 4, [&](const long long(&r)[NS_AHEAD], const long long(&c)[NS_AHEAD], int n) {
+    uint2 h[NS_AHEAD], l[NS_AHEAD];
+    float p[NS_AHEAD][4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = ns_value(h[j], l[j]) * scale;
-    if (g.step) {
-      float p[4];
-      load4(g.params, po, r, c, vec & VEC_P, p);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = fmaf(-rate, v[j], p[j] * keep);
+    for (int i = 0; i < NS_AHEAD; ++i) {
+      h[i] = *reinterpret_cast<const uint2 *>(hi + r[i] * w.ldx + c[i]);
+      l[i] = *reinterpret_cast<const uint2 *>(lo + r[i] * w.ldx + c[i]);
+      if (g.step) load4(g.params, po, r[i], c[i], vec & VEC_P, p[i]);
     }
-    store4(g.params, po, r, c, vec & VEC_P, v);
-  }
+#pragma unroll
+    for (int i = 0; i < NS_AHEAD; ++i) {
+      if (i >= n) break;
+      const __half *hh = reinterpret_cast<const __half *>(&h[i]), *ll = reinterpret_cast<const __half *>(&l[i]);
+      float v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[j] = ns_value(hh[j], ll[j]) * scale;
+        if (g.step) v[j] = fmaf(-rate, v[j], p[i][j] * keep);
+      }
+      store4(g.params, po, r[i], c[i], vec & VEC_P, v);
+    }
+  });
 }
 
 // ---- the products of a step -------------------------------------------------------------------------------------------------------
@@ -755,8 +792,10 @@ void launch_muon(const MuonStep &g, void *workspace, cudaStream_t st) {
   ns_layout(count, m, n, static_cast<char *>(workspace), &w);
   const unsigned vec = (rows16(g.grads) ? VEC_G : 0) | (g.step && rows16(g.momentum) ? VEC_M : 0) | (rows16(g.params) ? VEC_P : 0);
   const long long quads = m * ((n + 3) / 4), blocks = (quads + 255) / 256;
-  const unsigned parts = (unsigned)(blocks < NS_PARTS ? blocks : NS_PARTS);
-  const dim3 grid(parts, (unsigned)count), wide((unsigned)(blocks < 1184 ? blocks : 1184), (unsigned)count);
+  // as many blocks of a matrix as fill the chip together with the others', four groups to a thread where there are more
+  const long long fill = (148 * 8 + count - 1) / count, each = blocks < fill ? blocks : fill;
+  const unsigned parts = (unsigned)(each < NS_PARTS ? each : NS_PARTS);
+  const dim3 grid(parts, (unsigned)count), wide((unsigned)each, (unsigned)count);
   launch_pdl(muon_begin_kernel, grid, dim3(256), 0, st, true, g, w, vec);
   launch_pdl(muon_pair_kernel, wide, dim3(256), 0, st, true, g, w, vec, (int)parts);
   for (int i = 0; i < g.steps; ++i) {
