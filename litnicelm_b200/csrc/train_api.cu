@@ -140,8 +140,8 @@ uint64_t delta_bytes(LitniceView q) { return ((uint64_t)q->dims[0] * (uint64_t)q
 uint64_t attention_workspace(LitniceView q, LitniceView k, bool backward) {
   if (k->dims[0] != q->dims[0]) bad("k has another number of streams than q");
   uint64_t need = 256 + (backward ? delta_bytes(q) : 0);
-  if (train_attention_f32_supports(q->dtype == LITNICE_B200_VIEW_BF16, q->dims[3]))
-    need += train_attention_f32_workspace(q->dims[0], q->dims[1], k->dims[1], q->dims[2], k->dims[2], backward);
+  if (q->dtype != LITNICE_B200_VIEW_BF16)
+    need += train_attention_f32_workspace(q->dims[0], q->dims[1], k->dims[1], q->dims[2], k->dims[2], q->dims[3], backward);
   return need;
 }
 

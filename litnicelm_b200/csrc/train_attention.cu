@@ -1,4 +1,5 @@
-// Attention with its backward pass for training, 32-bit arithmetic throughout, any sizes and strides:
+// Attention with its backward pass for training: bfloat16 operands that the tensor-core kernels cannot address (any sizes and
+// strides), 32-bit arithmetic throughout:
 //   forward   s_ij = scale q_i . k_j,  lse_i = log sum_j exp s_ij,  out_i = sum_j exp(s_ij - lse_i) v_j
 //   backward  p_ij = exp(s_ij - lse_i) again from q, k and lse, delta_i = dout_i . out_i,
 //             ds_ij = scale p_ij (dout_i . v_j - delta_i),
@@ -23,30 +24,19 @@ typedef __nv_bfloat16 bf16;
 constexpr int TA_B = 64, TA_THREADS = 128;
 constexpr float TA_LOG2E = 1.4426950408889634f;
 
-__device__ __forceinline__ float to_float(float x) { return x; }
-__device__ __forceinline__ float to_float(bf16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ void from_float(float *p, float x) { *p = x; }
-__device__ __forceinline__ void from_float(bf16 *p, float x) { *p = __float2bfloat16_rn(x); }
-
 // Four consecutive elements of a row, of which `count` exist.
-template <typename T>
-__device__ __forceinline__ float4 load4(const T *p, long long c, int count, bool vec) {
+__device__ __forceinline__ float4 load4(const bf16 *p, long long c, int count, bool vec) {
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
   if (vec && count >= 4) {
-    if constexpr (sizeof(T) == 4) {
-      v = *reinterpret_cast<const float4 *>(p);
-    } else {
-      const uint2 u = *reinterpret_cast<const uint2 *>(p);
-      const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&u.x));
-      const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&u.y));
-      v = make_float4(a.x, a.y, b.x, b.y);
-    }
-    return v;
+    const uint2 u = *reinterpret_cast<const uint2 *>(p);
+    const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&u.x));
+    const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&u.y));
+    return make_float4(a.x, a.y, b.x, b.y);
   }
-  if (count > 0) v.x = to_float(p[0]);
-  if (count > 1) v.y = to_float(p[c]);
-  if (count > 2) v.z = to_float(p[2 * c]);
-  if (count > 3) v.w = to_float(p[3 * c]);
+  if (count > 0) v.x = __bfloat162float(p[0]);
+  if (count > 1) v.y = __bfloat162float(p[c]);
+  if (count > 2) v.z = __bfloat162float(p[2 * c]);
+  if (count > 3) v.w = __bfloat162float(p[3 * c]);
   return v;
 }
 
@@ -59,15 +49,15 @@ struct TaArgs {
 enum { VQ = 1, VK = 2, VV = 4, VDO = 8, VO = 16 };
 
 // Rows r0 .. r0 + 63 of a head into shared memory, those from `end` on and the columns behind dim as zeros.
-template <int D, typename T>
+template <int D>
 __device__ __forceinline__ void load_tile(float *to, const HeadView &x, long long base, int r0, int end, int dim, bool vec) {
   constexpr int LD = D + 4, Q = D / 4;
-  const T *p = reinterpret_cast<const T *>(x.p) + base;
+  const bf16 *p = reinterpret_cast<const bf16 *>(x.p) + base;
 #pragma unroll 4
   for (int e = threadIdx.x; e < TA_B * Q; e += TA_THREADS) {
     const int r = e / Q, c = e % Q * 4;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (r0 + r < end) v = load4<T>(p + (long long)(r0 + r) * x.r + c * x.c, x.c, dim - c, vec);
+    if (r0 + r < end) v = load4(p + (long long)(r0 + r) * x.r + c * x.c, x.c, dim - c, vec);
     *reinterpret_cast<float4 *>(to + r * LD + c) = v;
   }
 }
@@ -132,12 +122,12 @@ __device__ __forceinline__ void tile_mul(const float *w, const float *b, float (
   }
 }
 
-template <int D, typename T>
+template <int D>
 __device__ __forceinline__ void store_tile(const HeadView &x, long long base, int r0, int end, int dim, float (&acc)[8][D / 16],
                                            const float (&factor)[8]) {
   constexpr int W = D >= 64 ? 4 : 2;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  T *p = reinterpret_cast<T *>(x.p) + base;
+  bf16 *p = reinterpret_cast<bf16 *>(x.p) + base;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int r = r0 + i * 8 + ty;
@@ -145,7 +135,7 @@ __device__ __forceinline__ void store_tile(const HeadView &x, long long base, in
 #pragma unroll
     for (int c = 0; c < D / 16; ++c) {
       const int col = (c / W) * 64 + tx * W + c % W;
-      if (col < dim) from_float(p + (long long)r * x.r + col * x.c, acc[i][c] * factor[i]);
+      if (col < dim) p[(long long)r * x.r + col * x.c] = __float2bfloat16_rn(acc[i][c] * factor[i]);
     }
   }
 }
@@ -178,7 +168,7 @@ __device__ __forceinline__ TaPlace ta_place(const TaArgs &g, int heads, bool las
   return p;
 }
 
-template <int D, typename T>
+template <int D>
 __global__ void __launch_bounds__(TA_THREADS)
 train_attention_forward_kernel(const __grid_constant__ TaArgs g) {
   constexpr int LD = D + 4;
@@ -191,7 +181,7 @@ train_attention_forward_kernel(const __grid_constant__ TaArgs g) {
   const int r0 = at.tile * TA_B, r1 = min(r0 + TA_B, a.n), kh = at.head / (a.heads / a.groups);
   const long long qb = at.stream * a.q.s + at.head * a.q.h, kb = at.stream * a.k.s + kh * a.k.h,
                   vb = at.stream * a.v.s + kh * a.v.h;
-  load_tile<D, T>(sq, a.q, qb, r0, a.n, a.dim, g.vec & VQ);
+  load_tile<D>(sq, a.q, qb, r0, a.n, a.dim, g.vec & VQ);
   const int lo = span.lo(r0) / TA_B * TA_B, end = span.end(r1 - 1, at.keys);
   float o[8][D / 16], m[8], l[8];
 #pragma unroll
@@ -204,8 +194,8 @@ train_attention_forward_kernel(const __grid_constant__ TaArgs g) {
   const float f = a.scale * TA_LOG2E;
   for (int j0 = lo; j0 < end; j0 += TA_B) {
     __syncthreads();
-    load_tile<D, T>(sk, a.k, kb, j0, at.keys, a.dim, g.vec & VK);
-    load_tile<D, T>(sv, a.v, vb, j0, at.keys, a.dim, g.vec & VV);
+    load_tile<D>(sk, a.k, kb, j0, at.keys, a.dim, g.vec & VK);
+    load_tile<D>(sv, a.v, vb, j0, at.keys, a.dim, g.vec & VV);
     __syncthreads();
     float s[8][4];
     tile_dot<D>(sq, sk, s);
@@ -245,11 +235,11 @@ train_attention_forward_kernel(const __grid_constant__ TaArgs g) {
     if (tx == 0 && row < a.n)
       a.lse[((long long)at.stream * a.heads + at.head) * a.n + row] = total == 0.f ? -INFINITY : m[i] / TA_LOG2E + logf(total);
   }
-  store_tile<D, T>(a.out, at.stream * a.out.s + at.head * a.out.h, r0, a.n, a.dim, o, inv);
+  store_tile<D>(a.out, at.stream * a.out.s + at.head * a.out.h, r0, a.n, a.dim, o, inv);
 }
 
 // A row by LANES lanes, eight elements each.
-template <int LANES, typename T>
+template <int LANES>
 __global__ void __launch_bounds__(256) train_delta_kernel(const __grid_constant__ TaArgs g) {
   const TrainAttention &a = g.a;
   // rows in the order of memory as layers leave it, [streams, n, heads]: neighbours of a warp read on
@@ -258,13 +248,13 @@ __global__ void __launch_bounds__(256) train_delta_kernel(const __grid_constant_
   const int lane = threadIdx.x % LANES, c = lane * 8;
   const long long si = div_index(at, a.heads), s = div_index(si, a.n);
   const int h = (int)(at - si * a.heads), i = (int)(si - s * a.n);
-  const T *x = reinterpret_cast<const T *>(a.out.p) + s * a.out.s + (long long)i * a.out.r + h * a.out.h + c * a.out.c;
-  const T *y = reinterpret_cast<const T *>(a.dout.p) + s * a.dout.s + (long long)i * a.dout.r + h * a.dout.h + c * a.dout.c;
+  const bf16 *x = reinterpret_cast<const bf16 *>(a.out.p) + s * a.out.s + (long long)i * a.out.r + h * a.out.h + c * a.out.c;
+  const bf16 *y = reinterpret_cast<const bf16 *>(a.dout.p) + s * a.dout.s + (long long)i * a.dout.r + h * a.dout.h + c * a.dout.c;
   float t = 0.f;
 #pragma unroll
   for (int e = 0; e < 8; e += 4) {
-    const float4 u = load4<T>(x + e * a.out.c, a.out.c, a.dim - c - e, g.vec & VO);
-    const float4 v = load4<T>(y + e * a.dout.c, a.dout.c, a.dim - c - e, g.vec & VDO);
+    const float4 u = load4(x + e * a.out.c, a.out.c, a.dim - c - e, g.vec & VO);
+    const float4 v = load4(y + e * a.dout.c, a.dout.c, a.dim - c - e, g.vec & VDO);
     t = fmaf(u.x, v.x, fmaf(u.y, v.y, fmaf(u.z, v.z, fmaf(u.w, v.w, t))));
   }
 #pragma unroll
@@ -272,7 +262,7 @@ __global__ void __launch_bounds__(256) train_delta_kernel(const __grid_constant_
   if (lane == 0 && mine < rows) g.delta[(s * a.heads + h) * a.n + i] = t;
 }
 
-template <int D, typename T>
+template <int D>
 __global__ void __launch_bounds__(TA_THREADS)
 train_attention_dq_kernel(const __grid_constant__ TaArgs g) {
   constexpr int LD = D + 4;
@@ -285,8 +275,8 @@ train_attention_dq_kernel(const __grid_constant__ TaArgs g) {
   const int r0 = at.tile * TA_B, r1 = min(r0 + TA_B, a.n), kh = at.head / (a.heads / a.groups);
   const long long qb = at.stream * a.q.s + at.head * a.q.h, kb = at.stream * a.k.s + kh * a.k.h,
                   vb = at.stream * a.v.s + kh * a.v.h, db = at.stream * a.dout.s + at.head * a.dout.h;
-  load_tile<D, T>(sq, a.q, qb, r0, a.n, a.dim, g.vec & VQ);
-  load_tile<D, T>(sdo, a.dout, db, r0, a.n, a.dim, g.vec & VDO);
+  load_tile<D>(sq, a.q, qb, r0, a.n, a.dim, g.vec & VQ);
+  load_tile<D>(sdo, a.dout, db, r0, a.n, a.dim, g.vec & VDO);
   float lse[8], delta[8], acc[8][D / 16], one[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -302,8 +292,8 @@ train_attention_dq_kernel(const __grid_constant__ TaArgs g) {
   const float f = a.scale * TA_LOG2E;
   for (int j0 = lo; j0 < end; j0 += TA_B) {
     __syncthreads();
-    load_tile<D, T>(sk, a.k, kb, j0, at.keys, a.dim, g.vec & VK);
-    load_tile<D, T>(sv, a.v, vb, j0, at.keys, a.dim, g.vec & VV);
+    load_tile<D>(sk, a.k, kb, j0, at.keys, a.dim, g.vec & VK);
+    load_tile<D>(sv, a.v, vb, j0, at.keys, a.dim, g.vec & VV);
     __syncthreads();
     float s[8][4], dp[8][4];
     tile_dot<D>(sq, sk, s);
@@ -321,10 +311,10 @@ train_attention_dq_kernel(const __grid_constant__ TaArgs g) {
     __syncthreads();
     tile_mul<D>(sp, sk, acc);
   }
-  store_tile<D, T>(a.dq, at.stream * a.dq.s + at.head * a.dq.h, r0, a.n, a.dim, acc, one);
+  store_tile<D>(a.dq, at.stream * a.dq.s + at.head * a.dq.h, r0, a.n, a.dim, acc, one);
 }
 
-template <int D, typename T>
+template <int D>
 __global__ void __launch_bounds__(TA_THREADS)
 train_attention_dkv_kernel(const __grid_constant__ TaArgs g) {
   constexpr int LD = D + 4;
@@ -345,8 +335,8 @@ train_attention_dkv_kernel(const __grid_constant__ TaArgs g) {
     for (int c = 0; c < D / 16; ++c) dk[i][c] = dv[i][c] = 0.f;
   }
   if (j0 < at.keys) {
-    load_tile<D, T>(sk, a.k, kb, j0, at.keys, a.dim, g.vec & VK);
-    load_tile<D, T>(sv, a.v, vb, j0, at.keys, a.dim, g.vec & VV);
+    load_tile<D>(sk, a.k, kb, j0, at.keys, a.dim, g.vec & VK);
+    load_tile<D>(sv, a.v, vb, j0, at.keys, a.dim, g.vec & VV);
     // rows that see a key of this tile
     const int j1 = min(j0 + TA_B, at.keys);
     const int lo = a.causal ? max(0, j0 - a.first) / TA_B * TA_B : 0;
@@ -358,8 +348,8 @@ train_attention_dkv_kernel(const __grid_constant__ TaArgs g) {
       const long long stat = ((long long)at.stream * a.heads + h) * a.n;
       for (int r0 = lo; r0 < end; r0 += TA_B) {
         __syncthreads();
-        load_tile<D, T>(sq, a.q, qb, r0, a.n, a.dim, g.vec & VQ);
-        load_tile<D, T>(sdo, a.dout, db, r0, a.n, a.dim, g.vec & VDO);
+        load_tile<D>(sq, a.q, qb, r0, a.n, a.dim, g.vec & VQ);
+        load_tile<D>(sdo, a.dout, db, r0, a.n, a.dim, g.vec & VDO);
         __syncthreads();
         float s[8][4];
         tile_dot<D>(sk, sq, s);
@@ -392,14 +382,12 @@ train_attention_dkv_kernel(const __grid_constant__ TaArgs g) {
       }
     }
   }
-  store_tile<D, T>(a.dk, at.stream * a.dk.s + at.head * a.dk.h, j0, a.m, a.dim, dk, scales);
-  store_tile<D, T>(a.dv, at.stream * a.dv.s + at.head * a.dv.h, j0, a.m, a.dim, dv, one);
+  store_tile<D>(a.dk, at.stream * a.dk.s + at.head * a.dk.h, j0, a.m, a.dim, dk, scales);
+  store_tile<D>(a.dv, at.stream * a.dv.s + at.head * a.dv.h, j0, a.m, a.dim, dv, one);
 }
 
-bool rows_vec(const HeadView &x, int bf) {
-  const long long quad = 4;
-  return x.c == 1 && x.r % quad == 0 && x.h % quad == 0 && x.s % quad == 0 &&
-         reinterpret_cast<uintptr_t>(x.p) % (bf ? 8 : 16) == 0;
+bool rows_vec(const HeadView &x) {
+  return x.c == 1 && x.r % 4 == 0 && x.h % 4 == 0 && x.s % 4 == 0 && reinterpret_cast<uintptr_t>(x.p) % 8 == 0;
 }
 
 TaArgs ta_args(const TrainAttention &a, float *delta, int rows) {
@@ -407,8 +395,8 @@ TaArgs ta_args(const TrainAttention &a, float *delta, int rows) {
   g.a = a;
   g.delta = delta;
   g.tiles = (rows + TA_B - 1) / TA_B;
-  g.vec = (rows_vec(a.q, a.bf16) ? VQ : 0) | (rows_vec(a.k, a.bf16) ? VK : 0) | (rows_vec(a.v, a.bf16) ? VV : 0) |
-          (a.dout.p && rows_vec(a.dout, a.bf16) ? VDO : 0) | (a.out.p && rows_vec(a.out, a.bf16) ? VO : 0);
+  g.vec = (rows_vec(a.q) ? VQ : 0) | (rows_vec(a.k) ? VK : 0) | (rows_vec(a.v) ? VV : 0) |
+          (a.dout.p && rows_vec(a.dout) ? VDO : 0) | (a.out.p && rows_vec(a.out) ? VO : 0);
   return g;
 }
 
@@ -426,54 +414,45 @@ void launch(F kernel, const TaArgs &g, unsigned grid, int d, int tiles, cudaStre
   LB_LAUNCH_CHECK();
 }
 
-template <int D, typename T>
+template <int D>
 void forward(const TaArgs &g, cudaStream_t st) {
-  launch(train_attention_forward_kernel<D, T>, g, ta_grid(g, g.a.heads), D, 3, st);
+  launch(train_attention_forward_kernel<D>, g, ta_grid(g, g.a.heads), D, 3, st);
 }
-template <int D, typename T>
+template <int D>
 void backward(const TrainAttention &a, float *delta, cudaStream_t st) {
   const TaArgs gk = ta_args(a, delta, a.m), gq = ta_args(a, delta, a.n);
-  launch(train_attention_dkv_kernel<D, T>, gk, ta_grid(gk, a.groups), D, 4, st);
-  launch(train_attention_dq_kernel<D, T>, gq, ta_grid(gq, a.heads), D, 4, st);
+  launch(train_attention_dkv_kernel<D>, gk, ta_grid(gk, a.groups), D, 4, st);
+  launch(train_attention_dq_kernel<D>, gq, ta_grid(gq, a.heads), D, 4, st);
+}
+
+template <int LANES>
+void launch_delta(const TrainAttention &a, float *delta, cudaStream_t st) {
+  const TaArgs g = ta_args(a, delta, a.n);
+  const long long blocks = ((long long)a.streams * a.heads * a.n + 256 / LANES - 1) / (256 / LANES);
+  if (blocks > 0x7fffffffLL) throw std::invalid_argument("attention: too many rows, heads and streams for one call");
+  train_delta_kernel<LANES><<<(unsigned)blocks, 256, 0, st>>>(g);
+  LB_LAUNCH_CHECK();
 }
 
 }  // namespace
 
 void launch_train_attention_forward(const TrainAttention &a, void *work, cudaStream_t st) {
-  if (train_attention_f32_supports(a.bf16, a.dim)) return launch_train_attention_forward_f32(a, work, st);
+  if (!a.bf16) return launch_train_attention_forward_f32(a, work, st);
   if (train_attention_tc_supports(a, false)) return launch_train_attention_forward_tc(a, st);
   const TaArgs g = ta_args(a, nullptr, a.n);
-  if (a.bf16) {
-    if (a.dim <= 32) forward<32, bf16>(g, st);
-    else if (a.dim <= 64) forward<64, bf16>(g, st);
-    else forward<128, bf16>(g, st);
-  } else {
-    forward<128, float>(g, st);
-  }
-}
-
-template <int LANES>
-static void launch_delta(const TrainAttention &a, float *delta, cudaStream_t st) {
-  const TaArgs g = ta_args(a, delta, a.n);
-  const long long blocks = ((long long)a.streams * a.heads * a.n + 256 / LANES - 1) / (256 / LANES);
-  if (blocks > 0x7fffffffLL) throw std::invalid_argument("attention: too many rows, heads and streams for one call");
-  if (a.bf16) train_delta_kernel<LANES, bf16><<<(unsigned)blocks, 256, 0, st>>>(g);
-  else train_delta_kernel<LANES, float><<<(unsigned)blocks, 256, 0, st>>>(g);
-  LB_LAUNCH_CHECK();
+  if (a.dim <= 32) forward<32>(g, st);
+  else if (a.dim <= 64) forward<64>(g, st);
+  else forward<128>(g, st);
 }
 
 void launch_train_attention_backward(const TrainAttention &a, float *delta, void *work, cudaStream_t st) {
-  if (train_attention_f32_supports(a.bf16, a.dim)) return launch_train_attention_backward_f32(a, delta, work, st);
+  if (!a.bf16) return launch_train_attention_backward_f32(a, delta, work, st);
   if (a.dim <= 64) launch_delta<8>(a, delta, st);
   else launch_delta<16>(a, delta, st);
   if (train_attention_tc_supports(a, true)) return launch_train_attention_backward_tc(a, delta, st);
-  if (a.bf16) {
-    if (a.dim <= 32) backward<32, bf16>(a, delta, st);
-    else if (a.dim <= 64) backward<64, bf16>(a, delta, st);
-    else backward<128, bf16>(a, delta, st);
-  } else {
-    backward<128, float>(a, delta, st);
-  }
+  if (a.dim <= 32) backward<32>(a, delta, st);
+  else if (a.dim <= 64) backward<64>(a, delta, st);
+  else backward<128>(a, delta, st);
 }
 
 }  // namespace lb

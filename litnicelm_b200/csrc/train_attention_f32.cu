@@ -1,5 +1,4 @@
-// Attention with its backward pass for training in 32 bits on the sm_100a tensor cores, heads of up to 64 dimensions. The
-// mathematics is that of train_attention.cu, the division of work that of train_attention_tc.cu.
+// Attention with its backward pass for training in 32 bits on the sm_100a tensor cores. The mathematics is that of train_attention.cu, the division of work that of train_attention_tc.cu.
 //
 // Operands are in three bfloat16 parts, x = x0 + x1 + x2, each the part before it left over: all 24 bits of a finite x. A product
 // is the six of parts whose terms count, smallest first: (0,2) (2,0) (1,1) (0,1) (1,0) (0,0); what is left out is below 2^-23 of a
@@ -8,6 +7,10 @@
 // (which also clears keys behind a stream's length and sums dout . out), weights and their gradients in registers on their way
 // to tensor memory: of the 128 columns that a tile's scores took, each half of the warps writes the first two parts over its own
 // 64, and the third behind them.
+//
+// Heads of more than 64 dimensions (H = 2): a tile's parts are 96 KB, and two tiles of products do not fit beside two resident ones. A
+// CTA then makes 64 of the result's dimensions, and its products' operands come in units of 64 dimensions through four places of shared
+// memory, all four together where a sum runs over all dimensions (small parts first there too).
 //
 // A CTA: warp 0 issues TMA, warp 1 owns tensor memory and issues the MMAs, eight warps (a thread: a row or key, half of the
 // tile's columns, half of the dimensions of a sum). Every wait is bounded; one that runs out ends the CTA, whose results are then NaN.
@@ -24,12 +27,12 @@ constexpr int TF_THREADS = 320, TF_PART = TT_SLAB, TF_TILE = 3 * TF_PART;
 struct TfTensor {
   HeadView x;
   int rows, heads, keys;  // keys: rows behind a stream's length are cleared
-  bf16 *part;             // [3][streams][heads][rows][64]
+  bf16 *part;             // [3][streams][heads][rows][64 H]
   int blocks, vec;
 };
 struct TfSplit {
   TfTensor t[4];
-  int count, streams, dim, m;
+  int count, streams, dim, chunks;  // chunks: of eight elements, 8 H to a row
   const int *lengths;
   HeadView out;           // with delta: of the last tensor, dout
   float *delta;
@@ -39,8 +42,9 @@ __global__ void __launch_bounds__(256) train_split_kernel(const __grid_constant_
   int b = (int)blockIdx.x, which = 0;
   while (which + 1 < g.count && b >= g.t[which].blocks) b -= g.t[which++].blocks;
   const TfTensor &t = g.t[which];
-  const int per = (t.rows + 31) / 32, head_at = b / per, s = head_at / t.heads, h = head_at - s * t.heads;
-  const int row = (b - head_at * per) * 32 + (int)threadIdx.x / 8, c = (int)threadIdx.x % 8 * 8;
+  const int each_block = 256 / g.chunks, per = (t.rows + each_block - 1) / each_block;
+  const int head_at = b / per, s = head_at / t.heads, h = head_at - s * t.heads;
+  const int row = (b - head_at * per) * each_block + (int)threadIdx.x / g.chunks, c = (int)threadIdx.x % g.chunks * 8;
   const bool in = row < t.rows;
   const int live = t.keys && g.lengths ? max(0, min(t.rows, g.lengths[s])) : t.rows;
   float x[8] = {};
@@ -71,7 +75,7 @@ __global__ void __launch_bounds__(256) train_split_kernel(const __grid_constant_
         e -= f.y;
       }
     }
-    const long long each = (long long)g.streams * t.heads * t.rows * 64, to = ((long long)head_at * t.rows + row) * 64 + c;
+    const long long ld = g.chunks * 8, each = (long long)g.streams * t.heads * t.rows * ld, to = ((long long)head_at * t.rows + row) * ld + c;
 #pragma unroll
     for (int q = 0; q < 3; ++q) *reinterpret_cast<uint4 *>(t.part + q * each + to) = make_uint4(w[q][0], w[q][1], w[q][2], w[q][3]);
   }
@@ -84,8 +88,7 @@ __global__ void __launch_bounds__(256) train_split_kernel(const __grid_constant_
       for (int j = 0; j < 8; ++j)
         if (c + j < g.dim) d = fmaf(x[j], o[j * g.out.c], d);
     }
-#pragma unroll
-    for (int o = 4; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+    for (int o = g.chunks / 2; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
     if (in && c == 0) g.delta[(long long)head_at * t.rows + row] = d;
   }
 }
@@ -94,8 +97,8 @@ __global__ void __launch_bounds__(256) train_split_kernel(const __grid_constant_
 
 // Parts of the two operands of a product, in the order of their size.
 
-// The product of rows of a and rows of b over the (up to 64) dimensions, smallest parts first. (Descriptors differ by constants:
-// see tt_mma_rows in train_attention_tc.cu.)
+// The product of rows of a and rows of b over 64 dimensions, smallest parts first. (Descriptors differ by constants: see tt_mma_rows in
+// train_attention_tc.cu.)
 __device__ __forceinline__ void tf_mma_rows(unsigned d, unsigned a, unsigned b, unsigned idesc) {
   const unsigned long long da = umma_desc_k128(a), db = umma_desc_k128(b);
 #pragma unroll
@@ -163,9 +166,78 @@ __device__ __forceinline__ void tf_store_sums(const HeadView &o, long long off, 
   }
 }
 // Three parts of 128 rows of head `at` (of `each` heads in all).
-__device__ __forceinline__ void tf_load(unsigned to, const CUtensorMap *map, int row, int at, int each, unsigned bar) {
+__device__ __forceinline__ void tf_load(unsigned to, const CUtensorMap *map, int row, int at, int each, unsigned bar, int x = 0) {
 #pragma unroll
-  for (int p = 0; p < 3; ++p) tma_load_4d(to + p * TF_PART, map, 0, 0, row, p * each + at, bar);
+  for (int p = 0; p < 3; ++p) tma_load_4d(to + p * TF_PART, map, x, 0, row, p * each + at, bar);
+}
+
+// Units of 64 dimensions through four places of shared memory (H = 2): the producer's and the consumer's count of units. Barriers:
+// full of place s at bars + 8 s, empty at bars + 32 + 8 s.
+struct TfRing {
+  unsigned base, bars;
+  int at = 0;
+  __device__ unsigned place(int u) const { return base + (unsigned)((u & 3) * TF_TILE); }
+  __device__ unsigned full(int u) const { return bars + 8u * (u & 3); }
+  __device__ unsigned empty(int u) const { return bars + 32u + 8u * (u & 3); }
+};
+__device__ __forceinline__ bool tf_put(TfRing &r, const CUtensorMap *map, int x, int row, int head, int each, int lane,
+                                       volatile int *abort_flag) {
+  if (!mbar_wait_warp(r.empty(r.at), ((unsigned)(r.at >> 2) & 1u) ^ 1u, abort_flag, nullptr, 142)) return false;
+  if (lane == 0) {
+    mbar_expect_tx(r.full(r.at), TF_TILE);
+    tf_load(r.place(r.at), map, row, head, each, r.full(r.at), x);
+  }
+  __syncwarp();
+  ++r.at;
+  return true;
+}
+__device__ __forceinline__ bool tf_take(const TfRing &r, int u, volatile int *abort_flag) {
+  return mbar_wait_warp(r.full(u), (unsigned)(u >> 2) & 1u, abort_flag, nullptr, 143);
+}
+__device__ __forceinline__ void tf_drain(const TfRing &r) {  // copies in flight land before the shared memory goes away
+  const unsigned long long limit = global_timer() + WAIT_LIMIT_NS;
+  for (int u = r.at > 4 ? r.at - 4 : 0; u < r.at; ++u)
+    while (!mbar_try_wait(r.full(u), (unsigned)(u >> 2) & 1u) && global_timer() < limit) {}
+}
+// Four units a0 b0 a1 b1 from the ring's next places: d = a . b over 128 dimensions. Issued and given back.
+__device__ __forceinline__ bool tf_mma_ring(TfRing &r, unsigned d, unsigned idesc, unsigned done, volatile int *abort_flag) {
+  for (int u = 0; u < 4; ++u)
+    if (!tf_take(r, r.at + u, abort_flag)) return false;
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  if (tc_elect()) {
+    // units in order of place: a0, b0, a1, b1 start at any of the four
+    const unsigned a0 = r.place(r.at), b0 = r.place(r.at + 1), a1 = r.place(r.at + 2), b1 = r.place(r.at + 3);
+    const unsigned long long da[2] = {umma_desc_k128(a0), umma_desc_k128(a1)}, db[2] = {umma_desc_k128(b0), umma_desc_k128(b1)};
+#pragma unroll
+    for (int p = 0; p < 6; ++p) {
+      const int pa = p == 0 ? 0 : p == 1 ? 2 : p == 2 ? 1 : p == 3 ? 0 : p == 4 ? 1 : 0;
+      const int pb = p == 0 ? 2 : p == 1 ? 0 : p == 2 ? 1 : p == 3 ? 1 : p == 4 ? 0 : 0;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks)
+          tc_mma_f16(d, da[h] + (unsigned long long)(pa * (TF_PART >> 4) + ks * 2), db[h] + (unsigned long long)(pb * (TF_PART >> 4) + ks * 2),
+                     idesc, (p | h | ks) ? 1u : 0u);
+    }
+    for (int u = 0; u < 4; ++u) tc_commit(r.empty(r.at + u));
+    tc_commit(done);
+  }
+  __syncwarp();
+  r.at += 4;
+  return true;
+}
+// One unit: d = weights . its rows.
+__device__ __forceinline__ bool tf_mma_ring_weights(TfRing &r, unsigned d, unsigned w, unsigned idesc, unsigned done, volatile int *abort_flag) {
+  if (!tf_take(r, r.at, abort_flag)) return false;
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  if (tc_elect()) {
+    tf_mma_weights(d, w, r.place(r.at), idesc);
+    tc_commit(r.empty(r.at));
+    tc_commit(done);
+  }
+  __syncwarp();
+  ++r.at;
+  return true;
 }
 
 #define TF_WAIT(bar, parity, where) mbar_wait_warp(bar, (unsigned)(parity) & 1u, abort_flag, nullptr, where)
@@ -178,26 +250,27 @@ __device__ __forceinline__ void tf_load(unsigned to, const CUtensorMap *map, int
     if (lane == 0) mbar_arrive(bar);                                        \
   } while (0)
 
-constexpr int TF_STAT_OFF = 4 * TF_TILE, TF_BAR_OFF = TF_STAT_OFF + 4 * 128 * 4, TF_SMEM = TF_BAR_OFF + 128 + 1024;
-constexpr int TF_FWD_STAT_OFF = 3 * TF_TILE, TF_FWD_BAR_OFF = TF_FWD_STAT_OFF + 4 * 128 * 4, TF_FWD_SMEM = TF_FWD_BAR_OFF + 128 + 1024;
+constexpr int TF_STAT_OFF = 4 * TF_TILE, TF_BAR_OFF = TF_STAT_OFF + 4 * 128 * 4, TF_SMEM = TF_BAR_OFF + 256 + 1024;
 static_assert(TF_SMEM <= 227 * 1024, "");
 
 // ---- forward --------------------------------------------------------------------------------------------------------------------
 
+template <int H>
 __global__ void __launch_bounds__(TF_THREADS, 1)
 train_forward_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                          const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TtArgs a) {
   extern __shared__ unsigned char smem_raw[];
   const unsigned base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char *base_ptr = smem_raw + (base - smem_u32(smem_raw));
-  const unsigned q_off = base, k_off = base + TF_TILE, v_off = base + 2 * TF_TILE, bars = base + TF_FWD_BAR_OFF;
-  float *stat = reinterpret_cast<float *>(base_ptr + TF_FWD_STAT_OFF);
-  const unsigned q_full = bars, k_full = bars + 8, v_full = bars + 16, s_full = bars + 24, p_ready = bars + 32, o_full = bars + 40;
-  auto halves = [&](int q) { return bars + 48u + 8u * q; };  // of the two warps that share 32 rows
-  volatile unsigned *tmem_holder = reinterpret_cast<volatile unsigned *>(base_ptr + TF_FWD_BAR_OFF + 96);
-  volatile int *abort_flag = reinterpret_cast<volatile int *>(base_ptr + TF_FWD_BAR_OFF + 100);
+  const unsigned q_off = base, k_off = base + TF_TILE, v_off = base + 2 * TF_TILE, bars = base + TF_BAR_OFF;
+  float *stat = reinterpret_cast<float *>(base_ptr + TF_STAT_OFF);
+  const unsigned q_full = bars + 64, k_full = bars + 72, v_full = bars + 80, s_full = bars + 88, p_ready = bars + 96, o_full = bars + 104;
+  auto halves = [&](int q) { return bars + 112u + 8u * q; };  // of the two warps that share 32 rows
+  volatile unsigned *tmem_holder = reinterpret_cast<volatile unsigned *>(base_ptr + TF_BAR_OFF + 240);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(base_ptr + TF_BAR_OFF + 244);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const TtPlace at = tt_place(a, a.heads, a.span.causal != 0);
+  const int oh = H == 2 ? (int)blockIdx.x & 1 : 0;  // which 64 dimensions of the result
+  const TtPlace at = tt_place(a, a.heads, a.span.causal != 0, H);
   const int r0 = at.tile * TT_B, r1 = min(r0 + TT_B, a.n), kh = at.head / a.share;
   const int lo = a.span.lo(r0), end = a.span.end(r1 - 1, at.keys);
   const int tiles = end > lo ? (end - lo + TT_B - 1) / TT_B : 0;
@@ -206,6 +279,8 @@ train_forward_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     for (unsigned bar : {q_full, k_full, v_full, s_full, o_full}) mbar_init(bar, 1);
     mbar_init(p_ready, 8);
     for (int q = 0; q < 4; ++q) mbar_init(halves(q), 2);
+    if (H == 2)
+      for (int i = 0; i < 8; ++i) mbar_init(bars + 8u * i, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -218,6 +293,20 @@ train_forward_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   pdl_wait();
 
   if (warp == 0) {
+    if constexpr (H == 2) {
+      TfRing ring{base, bars};
+      const int query_head = at.stream * a.heads + at.head, key_head = at.stream * a.groups + kh;
+      const int queries = a.streams * a.heads, keys = a.streams * a.groups;
+      bool ok = true;
+      for (int i = 0; i < tiles && ok; ++i) {
+        const int j0 = lo + i * TT_B;
+        for (int d = 0; d < 2 && ok; ++d)
+          ok = tf_put(ring, &map_q, d * 64, r0, query_head, queries, lane, abort_flag) &&
+               tf_put(ring, &map_k, d * 64, j0, key_head, keys, lane, abort_flag);
+        ok = ok && tf_put(ring, &map_v, oh * 64, j0, key_head, keys, lane, abort_flag);
+      }
+      if (*abort_flag) tf_drain(ring);
+    } else {
     int k_loads = 0, v_loads = 0;
     bool ok = true;
     if (lane == 0 && tiles > 0) {
@@ -248,12 +337,19 @@ train_forward_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       while (k_loads > 0 && !mbar_try_wait(k_full, (unsigned)(k_loads - 1) & 1u) && global_timer() < limit) {}
       while (v_loads > 0 && !mbar_try_wait(v_full, (unsigned)(v_loads - 1) & 1u) && global_timer() < limit) {}
     }
+    }
   } else if (warp == 1) {
-    const int cols = (a.dim + 15) & ~15;
+    const int cols = H == 2 ? 64 : (a.dim + 15) & ~15;
     const unsigned idesc_s = umma_idesc_bf16(TT_B), idesc_o = umma_idesc_bf16(cols) | UMMA_B_MN_MAJOR;
-    bool ok = tiles > 0 ? TF_WAIT(q_full, 0, 103) : true;
+    bool ok = H == 2 || tiles == 0 ? true : TF_WAIT(q_full, 0, 103);
     int i = 0;
+    TfRing ring{base, bars};
     for (; i < tiles && ok; ++i) {
+      if constexpr (H == 2) {
+        ok = tf_mma_ring(ring, tmem_s, idesc_s, s_full, abort_flag) && TF_WAIT(p_ready, i, 106) &&
+             tf_mma_ring_weights(ring, tmem_o, tmem_s, idesc_o, o_full, abort_flag);
+        continue;
+      }
       ok = TF_WAIT(k_full, i, 104);
       if (!ok) break;
       TF_AFTER();
@@ -349,9 +445,9 @@ train_forward_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     ok = __all_sync(0xffffffffu, ok && !*abort_flag);
     const bool empty = row_end <= row_lo;
     if (row < a.n) {
-      tf_store_sums(a.o1, at.stream * a.o1.s + (long long)row * a.o1.r + at.head * a.o1.h, a, half * 32, sum,
+      tf_store_sums(a.o1, at.stream * a.o1.s + (long long)row * a.o1.r + at.head * a.o1.h, a, oh * 64 + half * 32, sum,
                     !ok ? NAN : empty ? 0.f : 1.0f / l);
-      if (half == 0)
+      if (half == 0 && oh == 0)
         a.lse[((long long)at.stream * a.heads + at.head) * a.n + row] =
             !ok ? NAN : empty ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
     }
@@ -368,6 +464,7 @@ train_forward_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
 
 // ---- dk and dv ------------------------------------------------------------------------------------------------------------------
 
+template <int H>
 __global__ void __launch_bounds__(TF_THREADS, 1)
 train_dkv_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                      const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do,
@@ -377,12 +474,13 @@ train_dkv_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
   unsigned char *base_ptr = smem_raw + (base - smem_u32(smem_raw));
   const unsigned k_off = base, v_off = base + TF_TILE, q_off = base + 2 * TF_TILE, do_off = base + 3 * TF_TILE, bars = base + TF_BAR_OFF;
   float *stat = reinterpret_cast<float *>(base_ptr + TF_STAT_OFF);  // [2][lse, delta][128]
-  const unsigned kv_full = bars, q_full = bars + 8, do_full = bars + 16, stat_full = bars + 24, s_full = bars + 32, p_ready = bars + 40,
-                 dp_full = bars + 48, ds_ready = bars + 56, dv_full = bars + 64, dk_full = bars + 72;
-  volatile unsigned *tmem_holder = reinterpret_cast<volatile unsigned *>(base_ptr + TF_BAR_OFF + 96);
-  volatile int *abort_flag = reinterpret_cast<volatile int *>(base_ptr + TF_BAR_OFF + 100);
+  const unsigned kv_full = bars + 64, q_full = bars + 72, do_full = bars + 80, stat_full = bars + 88, s_full = bars + 96, p_ready = bars + 104,
+                 dp_full = bars + 112, ds_ready = bars + 120, dv_full = bars + 128, dk_full = bars + 136;
+  volatile unsigned *tmem_holder = reinterpret_cast<volatile unsigned *>(base_ptr + TF_BAR_OFF + 240);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(base_ptr + TF_BAR_OFF + 244);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const TtPlace at = tt_place(a, a.groups, false);
+  const int oh = H == 2 ? (int)blockIdx.x & 1 : 0;  // which 64 dimensions of the result
+  const TtPlace at = tt_place(a, a.groups, false, H);
   const int j0 = at.tile * TT_B, j1 = min(j0 + TT_B, at.keys);
   // rows that see a key of this tile: from lo on, to row_end
   const int lo = a.span.causal ? max(0, j0 - a.span.first) / TT_B * TT_B : 0;
@@ -395,6 +493,8 @@ train_dkv_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
     for (unsigned bar : {kv_full, q_full, do_full, stat_full, s_full, dp_full, dv_full, dk_full}) mbar_init(bar, 1);
     mbar_init(p_ready, 8);
     mbar_init(ds_ready, 8);
+    if (H == 2)
+      for (int i = 0; i < 8; ++i) mbar_init(bars + 8u * i, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -407,9 +507,10 @@ train_dkv_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
   pdl_wait();
 
   if (warp == 0) {
+    TfRing ring{base, bars};
     int it = 0;
     bool ok = true;
-    if (lane == 0 && tiles > 0) {
+    if (H == 1 && lane == 0 && tiles > 0) {
       mbar_expect_tx(kv_full, 2u * TF_TILE);
       tf_load(k_off, &map_k, j0, at.stream * a.groups + at.head, a.streams * a.groups, kv_full);
       tf_load(v_off, &map_v, j0, at.stream * a.groups + at.head, a.streams * a.groups, kv_full);
@@ -422,7 +523,7 @@ train_dkv_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         // (the statistics' other buffer may be read while this one is filled: the tile before last is done)
         if (it > 0) ok = TF_WAIT(dk_full, it - 1, 111);
         if (!ok) break;
-        if (lane == 0) {
+        if (H == 1 && lane == 0) {
           mbar_expect_tx(q_full, TF_TILE);
           tf_load(q_off, &map_q, r0, query_head, a.streams * a.heads, q_full);
           mbar_expect_tx(do_full, TF_TILE);
@@ -439,20 +540,41 @@ train_dkv_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         __syncwarp();
         if (lane == 0) mbar_arrive(stat_full);
         __syncwarp();
+        if constexpr (H == 2) {
+          const int key_head = at.stream * a.groups + at.head, queries = a.streams * a.heads, keys = a.streams * a.groups;
+          for (int d = 0; d < 2 && ok; ++d)
+            ok = tf_put(ring, &map_k, d * 64, j0, key_head, keys, lane, abort_flag) &&
+                 tf_put(ring, &map_q, d * 64, r0, query_head, queries, lane, abort_flag);
+          for (int d = 0; d < 2 && ok; ++d)
+            ok = tf_put(ring, &map_v, d * 64, j0, key_head, keys, lane, abort_flag) &&
+                 tf_put(ring, &map_do, d * 64, r0, query_head, queries, lane, abort_flag);
+          ok = ok && tf_put(ring, &map_do, oh * 64, r0, query_head, queries, lane, abort_flag) &&
+               tf_put(ring, &map_q, oh * 64, r0, query_head, queries, lane, abort_flag);
+          if (!ok) break;
+        }
       }
     }
-    if (*abort_flag && tiles > 0) {  // copies in flight must land before the shared memory goes away
+    if (H == 2) {
+      if (*abort_flag) tf_drain(ring);
+    } else if (*abort_flag && tiles > 0) {  // copies in flight must land before the shared memory goes away
       const unsigned long long limit = global_timer() + WAIT_LIMIT_NS;
       while (!mbar_try_wait(kv_full, 0) && global_timer() < limit) {}
       while (it > 0 && !mbar_try_wait(q_full, (unsigned)(it - 1) & 1u) && global_timer() < limit) {}
       while (it > 0 && !mbar_try_wait(do_full, (unsigned)(it - 1) & 1u) && global_timer() < limit) {}
     }
   } else if (warp == 1) {
-    const int cols = (a.dim + 15) & ~15;
+    const int cols = H == 2 ? 64 : (a.dim + 15) & ~15;
     const unsigned idesc_s = umma_idesc_bf16(TT_B), idesc_d = umma_idesc_bf16(cols) | UMMA_B_MN_MAJOR;
-    bool ok = tiles > 0 ? TF_WAIT(kv_full, 0, 112) : true;
+    bool ok = H == 2 || tiles == 0 ? true : TF_WAIT(kv_full, 0, 112);
     int i = 0;
+    TfRing ring{base, bars};
     for (; i < tiles && ok; ++i) {
+      if constexpr (H == 2) {
+        ok = tf_mma_ring(ring, tmem_s, idesc_s, s_full, abort_flag) && tf_mma_ring(ring, tmem_dp, idesc_s, dp_full, abort_flag) &&
+             TF_WAIT(p_ready, i, 115) && tf_mma_ring_weights(ring, tmem_dv, tmem_s, idesc_d, dv_full, abort_flag) &&
+             TF_WAIT(ds_ready, i, 116) && tf_mma_ring_weights(ring, tmem_dk, tmem_dp, idesc_d, dk_full, abort_flag);
+        continue;
+      }
       ok = TF_WAIT(q_full, i, 113);
       if (!ok) break;
       TF_AFTER();
@@ -569,8 +691,8 @@ train_dkv_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
     }
     ok = __all_sync(0xffffffffu, ok && !*abort_flag);
     if (key < a.m) {
-      tf_store_sums(a.o1, at.stream * a.o1.s + (long long)key * a.o1.r + at.head * a.o1.h, a, half * 32, dk, ok ? a.scale : NAN);
-      tf_store_sums(a.o2, at.stream * a.o2.s + (long long)key * a.o2.r + at.head * a.o2.h, a, half * 32, dv, ok ? 1.f : NAN);
+      tf_store_sums(a.o1, at.stream * a.o1.s + (long long)key * a.o1.r + at.head * a.o1.h, a, oh * 64 + half * 32, dk, ok ? a.scale : NAN);
+      tf_store_sums(a.o2, at.stream * a.o2.s + (long long)key * a.o2.r + at.head * a.o2.h, a, oh * 64 + half * 32, dv, ok ? 1.f : NAN);
     }
   }
   __syncwarp();
@@ -585,6 +707,7 @@ train_dkv_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
 
 // ---- dq -------------------------------------------------------------------------------------------------------------------------
 
+template <int H>
 __global__ void __launch_bounds__(TF_THREADS, 1)
 train_dq_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                     const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do,
@@ -593,12 +716,13 @@ train_dq_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
   const unsigned base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char *base_ptr = smem_raw + (base - smem_u32(smem_raw));
   const unsigned q_off = base, do_off = base + TF_TILE, k_off = base + 2 * TF_TILE, v_off = base + 3 * TF_TILE, bars = base + TF_BAR_OFF;
-  const unsigned q_full = bars, k_full = bars + 8, v_full = bars + 16, s_full = bars + 24, dp_full = bars + 32, ds_ready = bars + 40,
-                 dq_full = bars + 48;
-  volatile unsigned *tmem_holder = reinterpret_cast<volatile unsigned *>(base_ptr + TF_BAR_OFF + 96);
-  volatile int *abort_flag = reinterpret_cast<volatile int *>(base_ptr + TF_BAR_OFF + 100);
+  const unsigned q_full = bars + 64, k_full = bars + 72, v_full = bars + 80, s_full = bars + 88, dp_full = bars + 96, ds_ready = bars + 104,
+                 dq_full = bars + 112;
+  volatile unsigned *tmem_holder = reinterpret_cast<volatile unsigned *>(base_ptr + TF_BAR_OFF + 240);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(base_ptr + TF_BAR_OFF + 244);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const TtPlace at = tt_place(a, a.heads, a.span.causal != 0);
+  const int oh = H == 2 ? (int)blockIdx.x & 1 : 0;  // which 64 dimensions of the result
+  const TtPlace at = tt_place(a, a.heads, a.span.causal != 0, H);
   const int r0 = at.tile * TT_B, r1 = min(r0 + TT_B, a.n), kh = at.head / a.share;
   const int lo = a.span.lo(r0), end = a.span.end(r1 - 1, at.keys);
   const int tiles = end > lo ? (end - lo + TT_B - 1) / TT_B : 0;
@@ -606,6 +730,8 @@ train_dq_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
   if (threadIdx.x == 0) {
     for (unsigned bar : {q_full, k_full, v_full, s_full, dp_full, dq_full}) mbar_init(bar, 1);
     mbar_init(ds_ready, 8);
+    if (H == 2)
+      for (int i = 0; i < 8; ++i) mbar_init(bars + 8u * i, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -618,6 +744,23 @@ train_dq_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
   pdl_wait();
 
   if (warp == 0) {
+    if constexpr (H == 2) {
+      TfRing ring{base, bars};
+      const int query_head = at.stream * a.heads + at.head, key_head = at.stream * a.groups + kh;
+      const int queries = a.streams * a.heads, keys = a.streams * a.groups;
+      bool ok = true;
+      for (int i = 0; i < tiles && ok; ++i) {
+        const int j0 = lo + i * TT_B;
+        for (int d = 0; d < 2 && ok; ++d)
+          ok = tf_put(ring, &map_do, d * 64, r0, query_head, queries, lane, abort_flag) &&
+               tf_put(ring, &map_v, d * 64, j0, key_head, keys, lane, abort_flag);
+        for (int d = 0; d < 2 && ok; ++d)
+          ok = tf_put(ring, &map_q, d * 64, r0, query_head, queries, lane, abort_flag) &&
+               tf_put(ring, &map_k, d * 64, j0, key_head, keys, lane, abort_flag);
+        ok = ok && tf_put(ring, &map_k, oh * 64, j0, key_head, keys, lane, abort_flag);
+      }
+      if (*abort_flag) tf_drain(ring);
+    } else {
     int it = 0;
     bool ok = true;
     const int query_head = at.stream * a.heads + at.head, key_head = at.stream * a.groups + kh;
@@ -653,12 +796,19 @@ train_dq_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       const int k_loads = ok ? it : it - 1;
       while (k_loads > 0 && !mbar_try_wait(k_full, (unsigned)(k_loads - 1) & 1u) && global_timer() < limit) {}
     }
+    }
   } else if (warp == 1) {
-    const int cols = (a.dim + 15) & ~15;
+    const int cols = H == 2 ? 64 : (a.dim + 15) & ~15;
     const unsigned idesc_s = umma_idesc_bf16(TT_B), idesc_d = umma_idesc_bf16(cols) | UMMA_B_MN_MAJOR;
-    bool ok = tiles > 0 ? TF_WAIT(q_full, 0, 133) : true;
+    bool ok = H == 2 || tiles == 0 ? true : TF_WAIT(q_full, 0, 133);
     int i = 0;
+    TfRing ring{base, bars};
     for (; i < tiles && ok; ++i) {
+      if constexpr (H == 2) {
+        ok = tf_mma_ring(ring, tmem_dp, idesc_s, dp_full, abort_flag) && tf_mma_ring(ring, tmem_s, idesc_s, s_full, abort_flag) &&
+             TF_WAIT(ds_ready, i, 136) && tf_mma_ring_weights(ring, tmem_dq, tmem_dp, idesc_d, dq_full, abort_flag);
+        continue;
+      }
       ok = TF_WAIT(v_full, i, 134);
       if (!ok) break;
       TF_AFTER();
@@ -741,7 +891,7 @@ train_dq_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     }
     ok = __all_sync(0xffffffffu, ok && !*abort_flag);
     if (row < a.n)
-      tf_store_sums(a.o1, at.stream * a.o1.s + (long long)row * a.o1.r + at.head * a.o1.h, a, half * 32, sum, ok ? a.scale : NAN);
+      tf_store_sums(a.o1, at.stream * a.o1.s + (long long)row * a.o1.r + at.head * a.o1.h, a, oh * 64 + half * 32, sum, ok ? a.scale : NAN);
   }
   __syncwarp();
   pdl_launch_dependents();
@@ -755,7 +905,9 @@ train_dq_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 
 // ---- host -----------------------------------------------------------------------------------------------------------------------
 
-size_t part_bytes(long long streams, long long heads, long long rows) { return (size_t)(streams * heads * rows) * 64 * 3 * 2; }
+size_t part_bytes(long long streams, long long heads, long long rows, long long dim) {
+  return (size_t)(streams * heads * rows) * (dim > 64 ? 128 : 64) * 3 * 2;
+}
 
 bool rows16(const HeadView &x) {
   return x.c == 1 && reinterpret_cast<uintptr_t>(x.p) % 16 == 0 && x.s % 4 == 0 && x.r % 4 == 0 && x.h % 4 == 0;
@@ -763,13 +915,14 @@ bool rows16(const HeadView &x) {
 
 struct Parts {
   bf16 *p;
-  int streams, rows, heads;
+  int streams, rows, heads, dim;
 };
 
 CUtensorMap part_map(const Parts &x) {
   CUtensorMap map;
-  const unsigned long long extent[4] = {64, 1, (unsigned long long)x.rows, 3ull * x.streams * x.heads};
-  const unsigned long long strides[3] = {128, 128, (unsigned long long)x.rows * 128};
+  const unsigned long long cols = x.dim > 64 ? 128 : 64;
+  const unsigned long long extent[4] = {cols, 1, (unsigned long long)x.rows, 3ull * x.streams * x.heads};
+  const unsigned long long strides[3] = {cols * 2, cols * 2, (unsigned long long)x.rows * cols * 2};
   tc_make_map_heads(&map, x.p, extent, strides, TT_B);
   return map;
 }
@@ -780,6 +933,7 @@ void split(const TrainAttention &a, char *work, float *delta, Parts (&parts)[4],
   g.count = delta ? 4 : 3;
   g.streams = a.streams;
   g.dim = a.dim;
+  g.chunks = a.dim > 64 ? 16 : 8;
   g.lengths = a.lengths;
   g.out = a.out;
   g.delta = delta;
@@ -794,13 +948,14 @@ void split(const TrainAttention &a, char *work, float *delta, Parts (&parts)[4],
     t.keys = keys;
     t.vec = rows16(t.x);
     t.part = reinterpret_cast<bf16 *>(work);
-    const long long b = (long long)a.streams * t.heads * ((t.rows + 31) / 32);
+    const int each = 256 / g.chunks;
+    const long long b = (long long)a.streams * t.heads * ((t.rows + each - 1) / each);
     blocks += b;
     if (blocks > 0x7fffffffLL || 3LL * a.streams * t.heads > 0x7fffffffLL)
       throw std::invalid_argument("attention: too many rows, heads and streams for one call");
     t.blocks = (int)b;
-    parts[i] = Parts{t.part, a.streams, t.rows, t.heads};
-    work += part_bytes(a.streams, t.heads, t.rows);
+    parts[i] = Parts{t.part, a.streams, t.rows, t.heads, a.dim};
+    work += part_bytes(a.streams, t.heads, t.rows, a.dim);
   }
   train_split_kernel<<<(unsigned)blocks, 256, 0, st>>>(g);
   LB_LAUNCH_CHECK();
@@ -808,43 +963,57 @@ void split(const TrainAttention &a, char *work, float *delta, Parts (&parts)[4],
 
 }  // namespace
 
-bool train_attention_f32_supports(int bf16, long long dim) { return !bf16 && dim <= 64; }
-
-size_t train_attention_f32_workspace(long long streams, long long n, long long m, long long heads, long long groups, bool backward) {
-  return (backward ? 2 : 1) * part_bytes(streams, heads, n) + 2 * part_bytes(streams, groups, m);
+size_t train_attention_f32_workspace(long long streams, long long n, long long m, long long heads, long long groups, long long dim,
+                                     bool backward) {
+  return (backward ? 2 : 1) * part_bytes(streams, heads, n, dim) + 2 * part_bytes(streams, groups, m, dim);
 }
 
-void launch_train_attention_forward_f32(const TrainAttention &a, void *work, cudaStream_t st) {
-  Parts p[4];
-  split(a, static_cast<char *>(work), nullptr, p, st);
+namespace {
+
+template <int H>
+void forward(const TrainAttention &a, const Parts (&p)[4], cudaStream_t st) {
   TtArgs t = tt_args(a, a.n);
   t.o1 = a.out;
   t.vec = rows16(a.out);
   static SharedMemoryOnce once;
-  once.set(train_forward_f32_kernel, TF_FWD_SMEM);
-  launch_pdl(train_forward_f32_kernel, dim3(tt_grid(t, a.heads)), dim3(TF_THREADS), TF_FWD_SMEM, st, true, part_map(p[0]), part_map(p[1]),
-             part_map(p[2]), t);
+  once.set(train_forward_f32_kernel<H>, TF_SMEM);
+  launch_pdl(train_forward_f32_kernel<H>, dim3(tt_grid(t, a.heads, H)), dim3(TF_THREADS), TF_SMEM, st, true, part_map(p[0]),
+             part_map(p[1]), part_map(p[2]), t);
 }
 
-void launch_train_attention_backward_f32(const TrainAttention &a, float *delta, void *work, cudaStream_t st) {
-  Parts p[4];
-  split(a, static_cast<char *>(work), delta, p, st);
+template <int H>
+void backward(const TrainAttention &a, float *delta, const Parts (&p)[4], cudaStream_t st) {
   const CUtensorMap mq = part_map(p[0]), mk = part_map(p[1]), mv = part_map(p[2]), md = part_map(p[3]);
   TtArgs t = tt_args(a, a.m);
   t.delta = delta;
   t.o1 = a.dk;
   t.o2 = a.dv;
   t.vec = rows16(a.dk) && rows16(a.dv);
-  static SharedMemoryOnce once_dkv;
-  once_dkv.set(train_dkv_f32_kernel, TF_SMEM);
-  launch_pdl(train_dkv_f32_kernel, dim3(tt_grid(t, a.groups)), dim3(TF_THREADS), TF_SMEM, st, true, mq, mk, mv, md, t);
+  static SharedMemoryOnce once_dkv, once_dq;
+  once_dkv.set(train_dkv_f32_kernel<H>, TF_SMEM);
+  launch_pdl(train_dkv_f32_kernel<H>, dim3(tt_grid(t, a.groups, H)), dim3(TF_THREADS), TF_SMEM, st, true, mq, mk, mv, md, t);
   t = tt_args(a, a.n);
   t.delta = delta;
   t.o1 = a.dq;
   t.vec = rows16(a.dq);
-  static SharedMemoryOnce once_dq;
-  once_dq.set(train_dq_f32_kernel, TF_SMEM);
-  launch_pdl(train_dq_f32_kernel, dim3(tt_grid(t, a.heads)), dim3(TF_THREADS), TF_SMEM, st, true, mq, mk, mv, md, t);
+  once_dq.set(train_dq_f32_kernel<H>, TF_SMEM);
+  launch_pdl(train_dq_f32_kernel<H>, dim3(tt_grid(t, a.heads, H)), dim3(TF_THREADS), TF_SMEM, st, true, mq, mk, mv, md, t);
+}
+
+}  // namespace
+
+void launch_train_attention_forward_f32(const TrainAttention &a, void *work, cudaStream_t st) {
+  Parts p[4];
+  split(a, static_cast<char *>(work), nullptr, p, st);
+  if (a.dim <= 64) forward<1>(a, p, st);
+  else forward<2>(a, p, st);
+}
+
+void launch_train_attention_backward_f32(const TrainAttention &a, float *delta, void *work, cudaStream_t st) {
+  Parts p[4];
+  split(a, static_cast<char *>(work), delta, p, st);
+  if (a.dim <= 64) backward<1>(a, delta, p, st);
+  else backward<2>(a, delta, p, st);
 }
 
 }  // namespace lb

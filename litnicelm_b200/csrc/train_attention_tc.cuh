@@ -70,8 +70,8 @@ struct TtArgs {
 struct TtPlace {
   int tile, head, stream, keys;
 };
-__device__ __forceinline__ TtPlace tt_place(const TtArgs &a, int heads, bool last_first) {
-  const int each = heads * a.streams, b = (int)blockIdx.x;
+__device__ __forceinline__ TtPlace tt_place(const TtArgs &a, int heads, bool last_first, int ctas = 1) {  // ctas: to a tile
+  const int each = heads * a.streams, b = (int)blockIdx.x / ctas;
   const int t = b / each, rest = b - t * each;
   TtPlace p;
   p.tile = last_first ? a.tiles - 1 - t : t;
@@ -106,8 +106,8 @@ TtArgs tt_args(const TrainAttention &a, int rows) {
   return t;
 }
 
-unsigned tt_grid(const TtArgs &t, int heads) {
-  const long long blocks = (long long)t.tiles * heads * t.streams;
+unsigned tt_grid(const TtArgs &t, int heads, int ctas = 1) {
+  const long long blocks = (long long)t.tiles * heads * t.streams * ctas;
   if (blocks > 0x7fffffffLL) throw std::invalid_argument("attention: too many rows, heads and streams for one call");
   return (unsigned)blocks;
 }

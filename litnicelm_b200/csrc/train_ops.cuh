@@ -33,8 +33,8 @@ struct TrainSpan {
 
 constexpr int TRAIN_MAX_DIM = 128;
 
-// train_attention.cu: any sizes and strides, 32-bit arithmetic throughout; dispatches to the two below. `work`:
-// train_attention_f32_workspace bytes where train_attention_f32_supports.
+// train_attention.cu: bfloat16 of any sizes and strides, 32-bit arithmetic throughout; dispatches to the two below. `work`:
+// train_attention_f32_workspace bytes for 32-bit operands.
 void launch_train_attention_forward(const TrainAttention &a, void *work, cudaStream_t st);
 void launch_train_attention_backward(const TrainAttention &a, float *delta, void *work, cudaStream_t st);
 
@@ -44,8 +44,8 @@ void launch_train_attention_forward_tc(const TrainAttention &a, cudaStream_t st)
 void launch_train_attention_backward_tc(const TrainAttention &a, float *delta, cudaStream_t st);
 
 // train_attention_f32.cu: 32 bits on the tensor cores
-bool train_attention_f32_supports(int bf16, long long dim);
-size_t train_attention_f32_workspace(long long streams, long long n, long long m, long long heads, long long groups, bool backward);
+size_t train_attention_f32_workspace(long long streams, long long n, long long m, long long heads, long long groups, long long dim,
+                                     bool backward);
 void launch_train_attention_forward_f32(const TrainAttention &a, void *work, cudaStream_t st);
 void launch_train_attention_backward_f32(const TrainAttention &a, float *delta, void *work, cudaStream_t st);
 
