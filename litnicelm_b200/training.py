@@ -16,6 +16,7 @@ while it records. There is no fallback: without the library or without a GPU eve
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 import struct
 from typing import Optional, Tuple
@@ -24,7 +25,7 @@ import torch
 
 from .plugin import NativeError, load_library
 
-_VIEW = struct.Struct("<IIQI4x4q12q")  # BackendTensorView
+_VIEW, _ADDRESS = struct.Struct("<IIQI4x4q12q"), struct.Struct("<Q")  # BackendTensorView, its address 8 bytes in
 _KINDS = {torch.float32: 0, torch.int32: 1, torch.bfloat16: 2}
 
 
@@ -80,35 +81,46 @@ def _tensor(t, name: str):
         raise TypeError(f"{name} is not a tensor")
 
 
+@functools.lru_cache(maxsize=4096)
+def _view_head(dtype, shape, strides, name) -> bytes:
+    """A view without its address."""
+    kind, rank = _KINDS.get(dtype), len(shape)
+    if kind is None:
+        raise TypeError(f"{name} has type {dtype}")
+    if rank > 6:
+        raise ValueError(f"{name} has {rank} axes")
+    size = 2 if dtype is torch.bfloat16 else 4
+    # (rows, cols and their strides repeat the axes; these entries read the axes)
+    return _VIEW.pack(1, kind, 0, rank, 0, 0, 0, 0, *shape, *_PAD[rank], *[x * size for x in strides], *_PAD[rank])
+
+
 def _views(names, tensors):
     """(addresses of the tensors' views, the memory that holds them), checked to be CUDA tensors of one device that autograd does
     not record."""
-    recording = torch.is_grad_enabled()
-    device, at, raw = None, 0, bytearray(152 * len(tensors))
+    recording, device, heads, at = torch.is_grad_enabled(), None, [], 8
     for name, t in zip(names, tensors):
-        _tensor(t, name)
-        if device is None:
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} is not a tensor")
+        if t.device != device:
+            if device is not None:
+                raise ValueError(f"{name} is on {t.device}, not on {device}")
             device = t.device
             if device.type != "cuda":
                 raise ValueError(f"{name} is not a CUDA tensor")
-        elif t.device != device:
-            raise ValueError(f"{name} is on {t.device}, not on {device}")
         if recording and t.requires_grad:
             raise ValueError(name + _GRAD_REFUSED)
-        kind = _KINDS.get(t.dtype)
-        if kind is None:
-            raise TypeError(f"{name} has type {t.dtype}")
-        shape, size = t.shape, t.element_size()
-        rank = len(shape)
-        if rank > 6:
-            raise ValueError(f"{name} has {rank} axes")
-        more = _PAD[rank]
-        # (rows, cols and their strides repeat the axes; these entries read the axes)
-        _VIEW.pack_into(raw, at, 1, kind, t.data_ptr(), rank, 0, 0, 0, 0, *shape, *more, *[x * size for x in t.stride()], *more)
+        heads.append(_view_head(t.dtype, t.shape, t.stride(), name))
+    raw = bytearray().join(heads)
+    for t in tensors:
+        _ADDRESS.pack_into(raw, at, t.data_ptr())
         at += 152
-    held = (C.c_char * at).from_buffer(raw)
+    held = (C.c_char * len(raw)).from_buffer(raw)
     base = C.addressof(held)
-    return range(base, base + at, 152), held
+    return range(base, base + len(raw), 152), held
+
+
+def _like(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _run(device: torch.device, fn, *args):
@@ -126,7 +138,7 @@ def _run(device: torch.device, fn, *args):
 def _workspace(nbytes: int, device) -> torch.Tensor:
     if nbytes == 0:
         raise _error(-1)
-    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)  # (on a 512-byte boundary)
 
 
 def _vector(t: Optional[torch.Tensor], name: str, count: int, dtype, device) -> Optional[int]:
@@ -161,7 +173,7 @@ def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scal
     Row i stands at position first + i and sees key j if j < m, j < lengths[stream], with ``causal`` j <= first + i, with a
     ``window`` j > first + i - window. A row that sees no key has out 0 and lse -inf. scale: 1 / sqrt(dim) if None."""
     _tensor(q, "q")
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
+    out = _like(q) if out is None else out
     (vq, vk, vv, vo), held = _views(("q", "k", "v", "out"), (q, k, v, out))
     o = _options(q, scale, causal, first, window, lengths)
     streams, n, heads = q.shape[:3]
@@ -181,9 +193,9 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
     shared by query heads receive the sum over those. dq, dk and dv may be given, slices of one buffer for instance."""
     for t, name in ((q, "q"), (k, "k"), (v, "v"), (lse, "lse")):
         _tensor(t, name)
-    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device) if dq is None else dq
-    dk = torch.empty(k.shape, dtype=k.dtype, device=k.device) if dk is None else dk
-    dv = torch.empty(v.shape, dtype=v.dtype, device=v.device) if dv is None else dv
+    dq = _like(q) if dq is None else dq
+    dk = _like(k) if dk is None else dk
+    dv = _like(v) if dv is None else dv
     (vd, vq, vk, vv, vo, wq, wk, wv), held = _views(("dout", "q", "k", "v", "out", "dq", "dk", "dv"), (dout, q, k, v, out, dq, dk, dv))
     o = _options(q, scale, causal, first, window, lengths)
     streams, n, heads = q.shape[:3]
@@ -212,7 +224,7 @@ def policy_loss(logits: torch.Tensor, targets: torch.Tensor, old_logp: torch.Ten
         raise ValueError("logits must be [rows, vocab]")
     rows, dev = logits.shape[0], logits.device
     if gradient:
-        dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=dev) if dlogits is None else dlogits
+        dlogits = _like(logits) if dlogits is None else dlogits
         (vz, vd), held = _views(("logits", "dlogits"), (logits, dlogits))
     else:
         (vz,), held = _views(("logits",), (logits,))
@@ -232,7 +244,7 @@ def orthogonalise(x: torch.Tensor, *, steps: int = 5, out: Optional[torch.Tensor
     """Every matrix of x [..., m, n] float32 with its singular values driven towards 1: X = x / (|x| + 1e-7), then ``steps`` times
     X <- 3.4445 X + (-4.7750 A + 2.0315 A A) X with A = X X^T (in the smaller side's space). out may be x."""
     _tensor(x, "x")
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
+    out = _like(x) if out is None else out
     (vx, vo), held = _views(("x", "out"), (x, out))
     lib = _library()
     work = _workspace(lib.litnice_b200_orthogonalise_workspace(vx), x.device)
