@@ -241,6 +241,7 @@ train_attention_forward_kernel(const __grid_constant__ TaArgs g) {
 // A row by LANES lanes, eight elements each.
 template <int LANES>
 __global__ void __launch_bounds__(256) train_delta_kernel(const __grid_constant__ TaArgs g) {
+  pdl_launch_dependents();
   const TrainAttention &a = g.a;
   // rows in the order of memory as layers leave it, [streams, n, heads]: neighbours of a warp read on
   const long long rows = (long long)a.streams * a.heads * a.n, mine = blockIdx.x * (256LL / LANES) + threadIdx.x / LANES;

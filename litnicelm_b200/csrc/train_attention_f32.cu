@@ -39,6 +39,7 @@ struct TfSplit {
 };
 
 __global__ void __launch_bounds__(256) train_split_kernel(const __grid_constant__ TfSplit g) {
+  pdl_launch_dependents();
   int b = (int)blockIdx.x, which = 0;
   while (which + 1 < g.count && b >= g.t[which].blocks) b -= g.t[which++].blocks;
   const TfTensor &t = g.t[which];

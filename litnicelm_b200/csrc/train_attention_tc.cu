@@ -367,6 +367,7 @@ train_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const unsigned tmem_s = *tmem_holder, tmem_dp = tmem_s + 128, tmem_dv = tmem_s + 256, tmem_dk = tmem_dv + D;
+  pdl_wait();
 
   if (warp == 0) {
     int it = 0;
@@ -573,6 +574,7 @@ train_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                  __all_sync(0xffffffffu, ok && !*abort_flag));
   }
   __syncwarp();
+  pdl_launch_dependents();
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   if (warp == 1) {
@@ -632,6 +634,7 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const unsigned tmem_s = *tmem_holder, tmem_dp = tmem_s + 128, tmem_dq = tmem_s + 256;
+  pdl_wait();
 
   if (warp == 0) {
     int it = 0;
@@ -835,6 +838,7 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     tt_store_row(o, row < a.n, a, tmem_dq + lanes, half ? mid : 0, half ? cols : mid, a.scale, tiles == 0, __all_sync(0xffffffffu, ok && !*abort_flag));
   }
   __syncwarp();
+  pdl_launch_dependents();
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   if (warp == 1) {
@@ -888,8 +892,7 @@ void backward(const TrainAttention &a, float *delta, cudaStream_t st) {
   t.vec = tt_rows16(a.dq);
   static SharedMemoryOnce once_dq;
   once_dq.set(train_dq_tc_kernel<D>, smem);
-  train_dq_tc_kernel<D><<<tt_grid(t, a.heads), TT_BWD_THREADS, smem, st>>>(mq, mk, mv, md, t);
-  LB_LAUNCH_CHECK();
+  launch_pdl(train_dq_tc_kernel<D>, dim3(tt_grid(t, a.heads)), dim3(TT_BWD_THREADS), (size_t)smem, st, true, mq, mk, mv, md, t);
   t = tt_args(a, a.m);
   t.delta = delta;
   t.o1 = a.dk;
@@ -897,8 +900,7 @@ void backward(const TrainAttention &a, float *delta, cudaStream_t st) {
   t.vec = tt_rows16(a.dk) && tt_rows16(a.dv);
   static SharedMemoryOnce once_dkv;
   once_dkv.set(train_dkv_tc_kernel<D>, smem);
-  train_dkv_tc_kernel<D><<<tt_grid(t, a.groups), TT_BWD_THREADS, smem, st>>>(mq, mk, mv, md, t);
-  LB_LAUNCH_CHECK();
+  launch_pdl(train_dkv_tc_kernel<D>, dim3(tt_grid(t, a.groups)), dim3(TT_BWD_THREADS), (size_t)smem, st, true, mq, mk, mv, md, t);
 }
 
 }  // namespace
