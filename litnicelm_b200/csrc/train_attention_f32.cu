@@ -38,6 +38,11 @@ struct TfSplit {
   float *delta;
 };
 
+__device__ __forceinline__ float tf_in_range(float x) {
+  const float top = 3.3895313892515355e38f;  // (2 - 2^-7) 2^127, the largest bfloat16
+  return fabsf(x) > top && fabsf(x) < INFINITY ? copysignf(top, x) : x;
+}
+
 __global__ void __launch_bounds__(256) train_split_kernel(const __grid_constant__ TfSplit g) {
   pdl_launch_dependents();
   int b = (int)blockIdx.x, which = 0;
@@ -69,7 +74,8 @@ __global__ void __launch_bounds__(256) train_split_kernel(const __grid_constant_
       float a = x[j], e = x[j + 1];
 #pragma unroll
       for (int q = 0; q < 3; ++q) {
-        const __nv_bfloat162 v = __floats2bfloat162_rn(a, e);
+        // (the first part of a finite element is finite: the last 2^119 below the largest would round to infinity)
+        const __nv_bfloat162 v = q ? __floats2bfloat162_rn(a, e) : __floats2bfloat162_rn(tf_in_range(a), tf_in_range(e));
         w[q][j >> 1] = *reinterpret_cast<const unsigned *>(&v);
         const float2 f = __bfloat1622float2(v);
         a -= f.x;
@@ -676,6 +682,11 @@ train_dkv_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
             p[c * 32 + j + 2] *= __uint_as_float(u[c][j + 2]) - v.z;
             p[c * 32 + j + 3] *= __uint_as_float(u[c][j + 3]) - v.w;
           }
+        if (!inside) {  // (a weight of zero has no part even where the other factor is not finite)
+#pragma unroll
+          for (int j = 0; j < 64; ++j)
+            if (j < c_lo || j >= c_end) p[j] = 0.f;
+        }
       }
       tf_store_parts(tmem_dp + lanes, half, 0, p);
       tf_store_parts(tmem_dp + lanes, half, 32, p + 32);

@@ -98,6 +98,65 @@ __device__ __forceinline__ void tt_mma_weights(unsigned d, unsigned w, unsigned 
 __device__ __forceinline__ unsigned long long tt_rows(unsigned tile) { return umma_desc_k128(tile); }
 __device__ __forceinline__ unsigned long long tt_cols(unsigned tile) { return umma_desc_mn128(tile, TT_SLAB); }
 
+// A row's scores of a tile (128 registers) to its new reference m; keep: what its sums are worth under it.
+__device__ __forceinline__ bool tt_reference(float (&s)[TT_B], const TtArgs &a, float factor, bool inside, int c_lo, int c_end, float &m,
+                                             float &l, float &keep) {
+  if (a.factor < 0.f) {
+#pragma unroll
+    for (int j = 0; j < TT_B; ++j) s[j] = -s[j];
+  }
+  if (!inside) {
+#pragma unroll
+    for (int j = 0; j < TT_B; ++j)
+      if (j >= c_end || j < c_lo) s[j] = -INFINITY;
+  }
+  float mq[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+  for (int j = 4; j < TT_B; j += 4) {
+    if ((j >> 2) & 1) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mq[e] = tt_max3(mq[e], s[j + e], j + 4 < TT_B ? s[(j + 4 + e) % TT_B] : s[j + e]);
+    }
+  }
+  const float top = tt_max3(tt_max3(mq[0], mq[1], mq[2]), mq[3], mq[3]) * factor;
+  const float mx = fmaxf(TT_NEG, top);
+  const bool grow = mx > m + TT_SLACK;
+  keep = grow ? tt_exp2(m - mx) : 1.f;
+  if (grow) m = mx;
+  l = l * keep + (mx - mx) + (top != top ? top : 0.f);  // a score that is no number, or infinite, shows in the sum
+  return grow;
+}
+// The weights 2^(factor s - m), summed into l, as bfloat16 over the scores' own columns, which this warp has read.
+__device__ __forceinline__ void tt_weights(const float (&s)[TT_B], float factor, float m, float &l, unsigned tmem) {
+  unsigned long long lq[4] = {0ull, 0ull, 0ull, 0ull};
+  const unsigned long long f2 = tt_two(factor, factor), m2 = tt_two(-m, -m);
+#pragma unroll
+  for (int c0 = 0; c0 < TT_B; c0 += 32) {
+    unsigned pk[16];
+#pragma unroll
+    for (int j = 0; j < 32; j += 2) {
+      const unsigned long long e = tt_exp2_two(tt_fma2(tt_two(s[c0 + j], s[c0 + j + 1]), f2, m2));
+      lq[(j >> 1) & 3] = tt_add2(lq[(j >> 1) & 3], e);
+      pk[j >> 1] = tt_pack(tt_lo(e), tt_hi(e));
+    }
+    tc_st16(tmem + (unsigned)(c0 >> 1), pk);
+  }
+  lq[0] = tt_add2(tt_add2(lq[0], lq[1]), tt_add2(lq[2], lq[3]));
+  l += tt_lo(lq[0]) + tt_hi(lq[0]);
+}
+// This lane's accumulator row times keep.
+__device__ __forceinline__ void tt_rescale(unsigned tmem, int dim, float keep) {
+#pragma unroll 1
+  for (int c0 = 0; c0 < dim; c0 += 16) {
+    unsigned r[16];
+    tc_ld16(tmem + (unsigned)c0, r);
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * keep);
+    tc_st16(tmem + (unsigned)c0, r);
+  }
+}
+
 template <int D>
 __global__ void __launch_bounds__(TT_FWD_THREADS, 2)
 train_forward_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -222,57 +281,11 @@ train_forward_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         for (int c = 0; c < 4; ++c) tc_ld32(tmem_s + lanes + (unsigned)(c * 32), u[c]);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
       }
-      if (a.factor < 0.f) {
-#pragma unroll
-        for (int j = 0; j < TT_B; ++j) s[j] = -s[j];
-      }
-      if (!inside) {
-#pragma unroll
-        for (int j = 0; j < TT_B; ++j)
-          if (j >= c_end || j < c_lo) s[j] = -INFINITY;
-      }
-      float mq[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-      for (int j = 4; j < TT_B; j += 4) {
-        if ((j >> 2) & 1) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) mq[e] = tt_max3(mq[e], s[j + e], j + 4 < TT_B ? s[(j + 4 + e) % TT_B] : s[j + e]);
-        }
-      }
-      const float top = tt_max3(tt_max3(mq[0], mq[1], mq[2]), mq[3], mq[3]) * factor;
-      const float mx = fmaxf(TT_NEG, top);
-      const bool grow = mx > m + TT_SLACK;
-      const float keep = grow ? tt_exp2(m - mx) : 1.f;
-      if (grow) m = mx;
-      l = l * keep + (mx - mx) + (top != top ? top : 0.f);  // a score that is no number, or infinite, shows in the sum
-      if (i > 0) {  // (the scores are there, so the product before them is done)
-        if (__any_sync(0xffffffffu, grow)) {
-#pragma unroll 1
-          for (int c0 = 0; c0 < a.dim; c0 += 16) {
-            unsigned r[16];
-            tc_ld16(tmem_o + lanes + (unsigned)c0, r);
-            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-            for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * keep);
-            tc_st16(tmem_o + lanes + (unsigned)c0, r);
-          }
-        }
-      }
-      unsigned long long lq[4] = {0ull, 0ull, 0ull, 0ull};
-      const unsigned long long f2 = tt_two(factor, factor), m2 = tt_two(-m, -m);
-#pragma unroll
-      for (int c0 = 0; c0 < TT_B; c0 += 32) {
-        unsigned pk[16];
-#pragma unroll
-        for (int j = 0; j < 32; j += 2) {
-          const unsigned long long e = tt_exp2_two(tt_fma2(tt_two(s[c0 + j], s[c0 + j + 1]), f2, m2));
-          lq[(j >> 1) & 3] = tt_add2(lq[(j >> 1) & 3], e);
-          pk[j >> 1] = tt_pack(tt_lo(e), tt_hi(e));
-        }
-        tc_st16(tmem_s + lanes + (unsigned)(c0 >> 1), pk);  // over the scores, which this warp has read
-      }
-      lq[0] = tt_add2(tt_add2(lq[0], lq[1]), tt_add2(lq[2], lq[3]));
-      l += tt_lo(lq[0]) + tt_hi(lq[0]);
+      float keep;
+      const bool grow = tt_reference(s, a, factor, inside, c_lo, c_end, m, l, keep);
+      // (the scores are there, so the product before them is done)
+      if (i > 0 && __any_sync(0xffffffffu, grow)) tt_rescale(tmem_o + lanes, a.dim, keep);
+      tt_weights(s, factor, m, l, tmem_s + lanes);
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
@@ -295,6 +308,219 @@ train_forward_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
   if (warp == 1) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_s), "r"(256u));
+  }
+}
+
+// The same for heads of up to 64 dimensions and more than 128 rows: one CTA per SM takes two tiles of 128 rows, A and B, with four warps
+// each, and walks the tiles of keys once for both. Tensor memory holds three tiles of scores and two accumulators: jobs A0 B0 A1 B1 ..
+// take the scores' places in turn, S of the third job ahead is issued behind a job's own P V, so a group's next scores are there when
+// it has finished with the last ones. (With two CTAs of one tile a group waited 1000 of its 3400 clocks a tile for them.)
+constexpr int TT_PAIR_STAGES = 4;
+constexpr int TT_PAIR_BAR = (2 + 2 * TT_PAIR_STAGES) * TT_SLAB, TT_PAIR_SMEM = TT_PAIR_BAR + 256 + 1024;
+
+__global__ void __launch_bounds__(TT_BWD_THREADS, 1)
+train_forward_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                          const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TtArgs a) {
+  constexpr int NS = TT_PAIR_STAGES;
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  const unsigned base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  unsigned char *base_ptr = smem_raw + (base - smem_u32(smem_raw));
+  const unsigned bars = base + TT_PAIR_BAR;
+  auto k_tile = [&](int s) { return base + (unsigned)((2 + s) * TT_SLAB); };
+  auto v_tile = [&](int s) { return base + (unsigned)((2 + NS + s) * TT_SLAB); };
+  auto k_full = [&](int s) { return bars + 8u * s; };
+  auto k_empty = [&](int s) { return bars + 32u + 8u * s; };
+  auto v_full = [&](int s) { return bars + 64u + 8u * s; };
+  auto v_empty = [&](int s) { return bars + 96u + 8u * s; };
+  auto s_full = [&](int place) { return bars + 128u + 8u * place; };
+  auto p_ready = [&](int place) { return bars + 152u + 8u * place; };
+  auto o_full = [&](int group) { return bars + 176u + 8u * group; };
+  const unsigned q_full = bars + 192;
+  volatile unsigned *tmem_holder = reinterpret_cast<volatile unsigned *>(base_ptr + TT_PAIR_BAR + 208);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(base_ptr + TT_PAIR_BAR + 212);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const TtPlace at = tt_place(a, a.heads, a.span.causal != 0);
+  const int r0 = at.tile * 2 * TT_B, kh = at.head / a.share;
+  const int lo = a.span.lo(r0);
+  auto tiles_of = [&](int group) {
+    const int first = r0 + group * TT_B, last = min(first + TT_B, a.n) - 1;
+    const int end = first < a.n ? a.span.end(last, at.keys) : 0;
+    return end > lo ? (end - lo + TT_B - 1) / TT_B : 0;
+  };
+  // B sees no fewer keys than A, or its rows do not exist: 2 both jobs alternate, the others are of one group
+  const int tiles_a = tiles_of(0), tiles_b = tiles_of(1), both = min(tiles_a, tiles_b), tiles = max(tiles_a, tiles_b);
+  const int jobs = tiles_a + tiles_b;
+  auto tile_of = [&](int job) { return job < 2 * both ? job >> 1 : job - both; };
+  auto group_of = [&](int job) { return job < 2 * both ? job & 1 : tiles_b > tiles_a ? 1 : 0; };
+  auto last_of_tile = [&](int job) { return job >= 2 * both || (job & 1); };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < NS; ++s)
+      for (unsigned bar : {k_full(s), k_empty(s), v_full(s), v_empty(s)}) mbar_init(bar, 1);
+    for (int s = 0; s < 3; ++s) {
+      mbar_init(s_full(s), 1);
+      mbar_init(p_ready(s), 4);
+    }
+    mbar_init(o_full(0), 1);
+    mbar_init(o_full(1), 1);
+    mbar_init(q_full, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) tt_alloc(tmem_holder, 512u);
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const unsigned tmem = *tmem_holder;
+
+  if (warp == 0) {
+    int it = 0;
+    bool ok = true;
+    if (lane == 0 && jobs > 0) {
+      mbar_expect_tx(q_full, 2u * TT_SLAB);
+      tma_load_4d(base, &map_q, 0, at.head, r0, at.stream, q_full);
+      tma_load_4d(base + TT_SLAB, &map_q, 0, at.head, r0 + TT_B, at.stream, q_full);
+    }
+    for (; it < tiles; ++it) {
+      const int st = it % NS, j0 = lo + it * TT_B;
+      ok = mbar_wait_warp(k_empty(st), ((unsigned)(it / NS) & 1u) ^ 1u, abort_flag, nullptr, 61);
+      if (!ok) break;
+      if (lane == 0) {
+        mbar_expect_tx(k_full(st), TT_SLAB);
+        tma_load_4d(k_tile(st), &map_k, 0, kh, j0, at.stream, k_full(st));
+      }
+      __syncwarp();
+      ok = mbar_wait_warp(v_empty(st), ((unsigned)(it / NS) & 1u) ^ 1u, abort_flag, nullptr, 62);
+      if (!ok) {
+        ++it;  // (its keys are on their way)
+        break;
+      }
+      if (lane == 0) {
+        mbar_expect_tx(v_full(st), TT_SLAB);
+        tma_load_4d(v_tile(st), &map_v, 0, kh, j0, at.stream, v_full(st));
+      }
+      __syncwarp();
+    }
+    if (*abort_flag && jobs > 0) {  // copies in flight must land before the shared memory goes away
+      const unsigned long long limit = global_timer() + WAIT_LIMIT_NS;
+      while (!mbar_try_wait(q_full, 0) && global_timer() < limit) {}
+      for (int j = it > NS ? it - NS : 0; j < it; ++j)
+        while (!mbar_try_wait(k_full(j % NS), (unsigned)(j / NS) & 1u) && global_timer() < limit) {}
+      const int v_loads = ok ? it : it - 1;
+      for (int j = v_loads > NS ? v_loads - NS : 0; j < v_loads; ++j)
+        while (!mbar_try_wait(v_full(j % NS), (unsigned)(j / NS) & 1u) && global_timer() < limit) {}
+    }
+  } else if (warp == 1) {
+    const int cols = (a.dim + 15) & ~15;
+    const unsigned long long q_rows = tt_rows(base), k_rows = tt_rows(k_tile(0)), v_cols = tt_cols(v_tile(0));
+    const unsigned idesc_s = umma_idesc_bf16(TT_B), idesc_o = umma_idesc_bf16(cols) | UMMA_B_MN_MAJOR;
+    int keys_seen = 0, values_seen = 0;
+    auto scores = [&](int job) {
+      const int i = tile_of(job), st = i % NS;
+      if (i >= keys_seen) {
+        if (!mbar_wait_warp(k_full(st), (unsigned)(i / NS) & 1u, abort_flag, nullptr, 63)) return false;
+        keys_seen = i + 1;
+      }
+      if (tc_elect()) {
+        tt_mma_rows<64>(tmem + (unsigned)(job % 3 * TT_B), q_rows + (unsigned long long)(group_of(job) * (TT_SLAB >> 4)),
+                        k_rows + (unsigned long long)(st * (TT_SLAB >> 4)), idesc_s);
+        tc_commit(s_full(job % 3));
+        if (last_of_tile(job)) tc_commit(k_empty(st));
+      }
+      __syncwarp();
+      return true;
+    };
+    bool ok = jobs > 0 ? mbar_wait_warp(q_full, 0, abort_flag, nullptr, 64) : true;
+    for (int job = 0; job < 3 && job < jobs && ok; ++job) ok = scores(job);
+    for (int job = 0; job < jobs && ok; ++job) {
+      const int i = tile_of(job), st = i % NS;
+      if (i >= values_seen) {
+        ok = mbar_wait_warp(v_full(st), (unsigned)(i / NS) & 1u, abort_flag, nullptr, 65);
+        if (!ok) break;
+        values_seen = i + 1;
+        const int have = at.keys - (lo + i * TT_B);
+        if (have < TT_B && at.keys < a.m) tt_clear_rows(base_ptr + (v_tile(st) - base), 1, have, lane);
+      }
+      ok = mbar_wait_warp(p_ready(job % 3), (unsigned)(job / 3) & 1u, abort_flag, nullptr, 66);
+      if (!ok) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      if (tc_elect()) {
+        tt_mma_weights<false>(tmem + (unsigned)(3 * TT_B + group_of(job) * 64), tmem + (unsigned)(job % 3 * TT_B),
+                              v_cols + (unsigned long long)(st * (TT_SLAB >> 4)), idesc_o, i > 0);
+        tc_commit(o_full(group_of(job)));
+        if (last_of_tile(job)) tc_commit(v_empty(st));
+      }
+      __syncwarp();
+      if (job + 3 < jobs) ok = scores(job + 3);
+    }
+    if (!ok) {  // a bounded chance for the tensor pipe to finish before tensor memory is freed
+      if (tc_elect()) tc_commit(q_full);
+      __syncwarp();
+      const unsigned long long limit = global_timer() + WAIT_LIMIT_NS;
+      while (!mbar_try_wait(q_full, 1) && global_timer() < limit) {}
+    }
+  } else {
+    const int q = warp & 3, group = (warp - 2) >> 2, mine = group ? tiles_b : tiles_a;
+    const unsigned lanes = (unsigned)(q * 32) << 16, tmem_o = tmem + (unsigned)(3 * TT_B + group * 64) + lanes;
+    const int first = r0 + group * TT_B + q * 32, row = first + lane;
+    const int row_lo = a.span.lo(row), row_end = a.span.end(row, at.keys);
+    const int warp_lo = a.span.lo(first + 31), warp_end = a.span.end(first, at.keys);
+    // a negative factor's sign goes to the scores; zero is small, so that hidden scores of -infinity stay that
+    const float factor = fmaxf(fabsf(a.factor), 1e-30f);
+    float m = TT_NEG, l = 0.f;
+    bool ok = true;
+    for (int i = 0; i < mine && ok; ++i) {
+      const int job = i < both ? 2 * i + group : both + i, place = job % 3, j0 = lo + i * TT_B;
+      ok = mbar_wait_warp(s_full(place), (unsigned)(job / 3) & 1u, abort_flag, nullptr, 67);
+      if (!ok) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const int c_lo = row_lo - j0, c_end = row_end - j0;  // keys j0 + c that this row sees
+      const bool inside = warp_lo <= j0 && warp_end >= j0 + TT_B;
+      const unsigned tmem_s = tmem + (unsigned)(place * TT_B) + lanes;
+      float s[TT_B], keep;
+      {
+        unsigned(&u)[4][32] = reinterpret_cast<unsigned(&)[4][32]>(s);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tc_ld32(tmem_s + (unsigned)(c * 32), u[c]);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+      }
+      const bool grow = tt_reference(s, a, factor, inside, c_lo, c_end, m, l, keep);
+      // the product before is waited for in each tile, so that no wait is ever two phases behind: by a warp that
+      // rescales the accumulator before that, by the others behind the weights
+      const bool rescale = i > 0 && __any_sync(0xffffffffu, grow);
+      if (rescale) {
+        ok = mbar_wait_warp(o_full(group), (unsigned)(i - 1) & 1u, abort_flag, nullptr, 68);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        tt_rescale(tmem_o, a.dim, keep);
+      }
+      tt_weights(s, factor, m, l, tmem_s);
+      if (i > 0 && !rescale) {
+        ok = mbar_wait_warp(o_full(group), (unsigned)(i - 1) & 1u, abort_flag, nullptr, 68);
+        if (!ok) break;
+      }
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_ready(place));
+    }
+    if (ok && mine > 0) ok = mbar_wait_warp(o_full(group), (unsigned)(mine - 1) & 1u, abort_flag, nullptr, 69);
+    ok = __all_sync(0xffffffffu, ok && !*abort_flag);
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const bool live = row < a.n, empty = row_end <= row_lo;
+    bf16 *o = reinterpret_cast<bf16 *>(a.o1.p) + at.stream * a.o1.s + (long long)row * a.o1.r + at.head * a.o1.h;
+    tt_store_row(o, live, a, tmem_o, 0, (a.dim + 15) & ~15, empty ? 0.f : 1.0f / l, mine == 0, ok);
+    if (live)
+      a.lse[((long long)at.stream * a.heads + at.head) * a.n + row] =
+          !ok ? NAN : empty ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+  }
+  __syncwarp();
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == 1) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
   }
 }
 
@@ -555,9 +781,12 @@ train_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
           w[j >> 1] = tt_pack(tt_lo(x), tt_hi(x));
           w[(j >> 1) + 1] = tt_pack(tt_lo(y), tt_hi(y));
         }
-        if (!key_live) {
+        if (!inside) {  // (a weight of zero has no part even where the other factor is not finite)
 #pragma unroll
-          for (int j = 0; j < 16; ++j) w[j] = 0u;
+          for (int j = 0; j < 16; ++j) {
+            const int at_lo = c + 2 * j, at_hi = at_lo + 1;
+            w[j] &= (at_lo < c_lo || at_lo >= c_end ? 0u : 0xffffu) | (at_hi < c_lo || at_hi >= c_end ? 0u : 0xffff0000u);
+          }
         }
         tc_st16(tmem_dp + lanes + (unsigned)(half * 64 + (c >> 1)), w);
       }
@@ -881,6 +1110,19 @@ void forward(const TrainAttention &a, cudaStream_t st) {
   LB_LAUNCH_CHECK();
 }
 
+void forward_pair(const TrainAttention &a, cudaStream_t st) {
+  TtArgs t = tt_args(a, a.n);
+  t.tiles = (a.n + 2 * TT_B - 1) / (2 * TT_B);
+  t.o1 = a.out;
+  t.vec = tt_rows16(a.out);
+  static SharedMemoryOnce once;
+  once.set(train_forward_pair_kernel, TT_PAIR_SMEM);
+  train_forward_pair_kernel<<<tt_grid(t, a.heads), TT_BWD_THREADS, TT_PAIR_SMEM, st>>>(
+      tt_map(a.q, a.streams, a.n, a.heads, a.dim), tt_map(a.k, a.streams, a.m, a.groups, a.dim),
+      tt_map(a.v, a.streams, a.m, a.groups, a.dim), t);
+  LB_LAUNCH_CHECK();
+}
+
 template <int D>
 void backward(const TrainAttention &a, float *delta, cudaStream_t st) {
   const CUtensorMap mq = tt_map(a.q, a.streams, a.n, a.heads, a.dim), mk = tt_map(a.k, a.streams, a.m, a.groups, a.dim),
@@ -913,7 +1155,11 @@ bool train_attention_tc_supports(const TrainAttention &a, bool backward) {
 }
 
 void launch_train_attention_forward_tc(const TrainAttention &a, cudaStream_t st) {
-  if (a.dim <= 64) forward<64>(a, st);
+  // A CTA with two tiles pays off once a row's keys are many: 4096 rows of 16 heads 80 -> 65 us, 8192 rows 228 ->
+  // 203. With 2048 rows (4 streams of 16 heads) 82 and 81 us, and few keys leave its longer start and end bare: 300 rows of 64 x 8 heads 54 -> 64 us.
+  const int seen = a.window > 0 && a.window < a.m ? a.window : a.m;
+  if (a.dim <= 64 && min(a.n, seen) > 2048) forward_pair(a, st);
+  else if (a.dim <= 64) forward<64>(a, st);
   else forward<128>(a, st);
 }
 

@@ -75,6 +75,32 @@ def test_attention_lengths(dtype, dim, opts):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,m,dim,lengths,opts", [
+    (2100, 2100, 64, [2100, 1, 0, 2049], dict()), (2049, 2300, 40, [2300, 129, 1700, 64], dict(causal=False)),
+    (2305, 2177, 64, [2177, 128, 2048, 0], dict(window=2060, causal=False)), (2176, 2400, 8, None, dict(first=200, window=2100)),
+    (1100, 1200, 128, [1200, 65, 0, 1025], dict(first=100))], ids=str)
+def test_attention_long(dtype, n, m, dim, lengths, opts):
+    attention_case(dtype, 4, n, m, 2, 1, dim, lengths=lengths, **opts)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_hidden_lowest_values(dtype, dim):
+    """The type's lowest value in keys and values that the span hides from every row."""
+    g = gen(5)
+    q, dout = (rand(g, 2, 60, 2, dim, dtype=dtype) for _ in range(2))
+    k, v = (rand(g, 2, 100, 2, dim, dtype=dtype) for _ in range(2))
+    results = []
+    for x in (0.0, torch.finfo(dtype).min):
+        k[:, 60:] = x
+        v[:, 60:] = x
+        out, lse = training.attention_forward(q, k, v)
+        results.append((out, lse, *training.attention_backward(dout, q, k, v, out, lse)))
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("what", [math.nan, math.inf, -math.inf, "lowest"])
 def test_attention_padding_is_not_used(dtype, what):
     """What lies behind a stream's length, in keys and values, reaches nothing."""
