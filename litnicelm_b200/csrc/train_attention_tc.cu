@@ -830,8 +830,9 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
   auto a_empty = [&](int s) { return bars + 32u + 8u * s; };
   auto b_full = [&](int s) { return bars + 64u + 8u * s; };
   auto b_empty = [&](int s) { return bars + 96u + 8u * s; };
-  const unsigned q_full = bars + 128, s_full = bars + 136, s_free = bars + 144, dp_full = bars + 152, ds_ready = bars + 160,
-                 done = bars + 168;
+  const unsigned q_full = bars + 128, s_full = bars + 136, s_free = bars + 144, done = bars + 152;
+  auto dp_full = [&](int i) { return bars + 160u + 8u * (i & 1); };
+  auto ds_ready = [&](int i) { return bars + 208u + 8u * (i & 1); };
   auto halves = [&](int q) { return bars + 176u + 8u * q; };  // of the two warps that share 32 rows
   volatile unsigned *tmem_holder = reinterpret_cast<volatile unsigned *>(base_ptr + L::BAR_OFF + 240);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(base_ptr + L::BAR_OFF + 244);
@@ -842,9 +843,10 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
   const int tiles = end > lo ? (end - lo + TT_B - 1) / TT_B : 0;
 
   if (threadIdx.x == 0) {
-    for (unsigned bar : {q_full, s_full, dp_full, done}) mbar_init(bar, 1);
+    for (unsigned bar : {q_full, s_full, dp_full(0), dp_full(1), done}) mbar_init(bar, 1);
     mbar_init(s_free, 8);
-    mbar_init(ds_ready, 8);
+    mbar_init(ds_ready(0), 8);
+    mbar_init(ds_ready(1), 8);
     for (int q = 0; q < 4; ++q) mbar_init(halves(q), 2);
     for (int s = 0; s < L::NA; ++s) {
       mbar_init(a_full(s), 1);
@@ -862,7 +864,7 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  const unsigned tmem_s = *tmem_holder, tmem_dp = tmem_s + 128, tmem_dq = tmem_s + 256;
+  const unsigned tmem_s = *tmem_holder, tmem_dp0 = tmem_s + 128, tmem_dq = tmem_s + 384;
   pdl_wait();
 
   if (warp == 0) {
@@ -921,8 +923,8 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       const int sb = i % L::NB;
       if (!mbar_wait_warp(b_full(sb), (unsigned)(i / L::NB) & 1u, abort_flag, nullptr, 92)) return false;
       if (tc_elect()) {
-        tt_mma_rows<D>(tmem_dp, do_rows, v_rows + stage(sb), idesc_s);
-        tc_commit(dp_full);
+        tt_mma_rows<D>(tmem_dp0 + (unsigned)((i & 1) * 128), do_rows, v_rows + stage(sb), idesc_s);
+        tc_commit(dp_full(i));
         tc_commit(b_empty(sb));
       }
       __syncwarp();
@@ -950,16 +952,17 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
           tc_commit(s_full);
         }
         __syncwarp();
+        ok = upstream(i + 1);  // over dS(i - 1), whose product was issued before
+        if (!ok) break;
       }
-      ok = mbar_wait_warp(ds_ready, (unsigned)i & 1u, abort_flag, nullptr, 95);
+      ok = mbar_wait_warp(ds_ready(i), (unsigned)(i >> 1) & 1u, abort_flag, nullptr, 95);
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       if (tc_elect()) {
-        tt_mma_weights<true>(tmem_dq, tmem_dp, k_cols + stage(sa), idesc_d, i > 0);
+        tt_mma_weights<true>(tmem_dq, tmem_dp0 + (unsigned)((i & 1) * 128), k_cols + stage(sa), idesc_d, i > 0);
         tc_commit(a_empty(sa));
       }
       __syncwarp();
-      if (i + 1 < tiles) ok = upstream(i + 1);
     }
     if (tiles > 0 && tc_elect()) tc_commit(done);
     __syncwarp();
@@ -984,7 +987,7 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
 #pragma unroll
       for (int c = 0; c < 64; c += 32) {
         unsigned u[32];
-        tc_ld32(tmem_dp + lanes + (unsigned)(half * 64 + c), u);
+        tc_ld32(tmem_dp0 + lanes + (unsigned)(half * 64 + c), u);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
         for (int j = 0; j < 32; ++j)
@@ -1002,6 +1005,7 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     bool ok = true;
     for (int i = 0; i < tiles && ok; ++i) {
       const int j0 = lo + i * TT_B + half * 64;
+      const unsigned tmem_dp = tmem_dp0 + (unsigned)((i & 1) * 128);
       const int c_lo = row_lo - j0, c_end = row_end - j0;
       const bool inside = warp_lo <= j0 && warp_end >= j0 + 64;
       ok = mbar_wait_warp(s_full, (unsigned)i & 1u, abort_flag, nullptr, 96);
@@ -1024,7 +1028,7 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         p[j] = tt_lo(t);
         p[j + 1] = tt_hi(t);
       }
-      ok = mbar_wait_warp(dp_full, (unsigned)i & 1u, abort_flag, nullptr, 97);
+      ok = mbar_wait_warp(dp_full(i), (unsigned)(i >> 1) & 1u, abort_flag, nullptr, 97);
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       if (!inside) {
@@ -1058,7 +1062,7 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive(ds_ready);
+      if (lane == 0) mbar_arrive(ds_ready(i));
     }
     if (ok && tiles > 0) ok = mbar_wait_warp(done, 0, abort_flag, nullptr, 98);
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
