@@ -530,11 +530,11 @@ train_forward_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
 template <int D>
 struct TtBwd {
   static constexpr int SLABS = D / 64, TILE = SLABS * TT_SLAB;
-  static constexpr int NA = D == 64 ? 4 : 3, NB = D == 64 ? 4 : 2;
-  static constexpr int A_OFF = 2 * TILE, B_OFF = A_OFF + NA * TILE;
+  static constexpr int NQ = D == 64 ? 2 : 1, NA = D == 64 ? 4 : 3, NB = D == 64 ? 4 : 2;
+  static constexpr int A_OFF = 2 * NQ * TILE, B_OFF = A_OFF + NA * TILE;
   static constexpr int STAT_OFF = B_OFF + NB * TILE;  // [NB][2][128] floats
   static constexpr int BAR_OFF = STAT_OFF + NB * 2 * 128 * 4;
-  static constexpr int TOTAL = BAR_OFF + 256 + 768;
+  static constexpr int TOTAL = BAR_OFF + 384 + 640;
   static_assert(TOTAL <= 227 * 1024, "");
 };
 
@@ -822,7 +822,8 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   const unsigned base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char *base_ptr = smem_raw + (base - smem_u32(smem_raw));
-  const unsigned q_off = base, do_off = base + TILE, bars = base + L::BAR_OFF;
+  const unsigned bars = base + L::BAR_OFF;
+  auto q_tile = [&](int s) { return base + (unsigned)(s * 2 * TILE); };  // and dout's behind it
   auto k_tile = [&](int s) { return base + (unsigned)(L::A_OFF + s * TILE); };
   auto v_tile = [&](int s) { return base + (unsigned)(L::B_OFF + s * TILE); };
   float *stat = reinterpret_cast<float *>(base_ptr + L::STAT_OFF);
@@ -830,24 +831,27 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
   auto a_empty = [&](int s) { return bars + 32u + 8u * s; };
   auto b_full = [&](int s) { return bars + 64u + 8u * s; };
   auto b_empty = [&](int s) { return bars + 96u + 8u * s; };
-  const unsigned q_full = bars + 128, s_full = bars + 136, s_free = bars + 144, done = bars + 152;
-  auto dp_full = [&](int i) { return bars + 160u + 8u * (i & 1); };
-  auto ds_ready = [&](int i) { return bars + 208u + 8u * (i & 1); };
-  auto halves = [&](int q) { return bars + 176u + 8u * q; };  // of the two warps that share 32 rows
-  volatile unsigned *tmem_holder = reinterpret_cast<volatile unsigned *>(base_ptr + L::BAR_OFF + 240);
-  volatile int *abort_flag = reinterpret_cast<volatile int *>(base_ptr + L::BAR_OFF + 244);
+  auto q_full = [&](int s) { return bars + 128u + 8u * s; };
+  auto q_empty = [&](int s) { return bars + 144u + 8u * s; };
+  auto dp_full = [&](int g) { return bars + 160u + 8u * (g & 1); };
+  auto ds_ready = [&](int g) { return bars + 176u + 8u * (g & 1); };
+  auto halves = [&](int q) { return bars + 192u + 8u * q; };  // of the two warps that share 32 rows
+  const unsigned s_full = bars + 224, s_free = bars + 232, done = bars + 240;
+  volatile unsigned *tmem_holder = reinterpret_cast<volatile unsigned *>(base_ptr + L::BAR_OFF + 248);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(base_ptr + L::BAR_OFF + 252);
+  const TtNext next{bars + 256u};
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const TtPlace at = tt_place(a, a.heads, a.span.causal != 0);
-  const int r0 = at.tile * TT_B, r1 = min(r0 + TT_B, a.n), kh = at.head / a.share;
-  const int lo = a.span.lo(r0), end = a.span.end(r1 - 1, at.keys);
-  const int tiles = end > lo ? (end - lo + TT_B - 1) / TT_B : 0;
 
   if (threadIdx.x == 0) {
-    for (unsigned bar : {q_full, s_full, dp_full(0), dp_full(1), done}) mbar_init(bar, 1);
+    for (unsigned bar : {s_full, dp_full(0), dp_full(1), done}) mbar_init(bar, 1);
     mbar_init(s_free, 8);
     mbar_init(ds_ready(0), 8);
     mbar_init(ds_ready(1), 8);
     for (int q = 0; q < 4; ++q) mbar_init(halves(q), 2);
+    for (int s = 0; s < L::NQ; ++s) {
+      mbar_init(q_full(s), 1);
+      mbar_init(q_empty(s), 1);
+    }
     for (int s = 0; s < L::NA; ++s) {
       mbar_init(a_full(s), 1);
       mbar_init(a_empty(s), 1);
@@ -856,6 +860,7 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       mbar_init(b_full(s), 1);
       mbar_init(b_empty(s), 1);
     }
+    next.init(9);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -867,208 +872,267 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
   const unsigned tmem_s = *tmem_holder, tmem_dp0 = tmem_s + 128, tmem_dq = tmem_s + 384;
   pdl_wait();
 
+  struct Item {
+    TtPlace at;
+    int r0, lo, tiles;
+  };
+  auto item = [&](int block) {
+    Item x;
+    x.at = tt_place(a, a.heads, a.span.causal != 0, 1, block);
+    x.r0 = x.at.tile * TT_B;
+    x.lo = a.span.lo(x.r0);
+    const int end = a.span.end(min(x.r0 + TT_B, a.n) - 1, x.at.keys);
+    x.tiles = end > x.lo ? (end - x.lo + TT_B - 1) / TT_B : 0;
+    return x;
+  };
+
   if (warp == 0) {
-    int it = 0;
+    int g = 0, n = 0, a_loads = 0, b_loads = 0;  // tiles of keys so far, items with any, loads issued
     bool ok = true;
-    if (lane == 0 && tiles > 0) {
-      mbar_expect_tx(q_full, 2u * TILE);
-      for (int s = 0; s < SLABS; ++s) {
-        tma_load_4d(q_off + s * TT_SLAB, &map_q, s * 64, at.head, r0, at.stream, q_full);
-        tma_load_4d(do_off + s * TT_SLAB, &map_do, s * 64, at.head, r0, at.stream, q_full);
+    int block = (int)blockIdx.x;
+    for (int w = 0; block >= 0; ++w) {
+      const bool more = next.ask(w, lane);
+      const Item x = item(block);
+      const int kh = x.at.head / a.share, sq = n % L::NQ;
+      if (x.tiles > 0 && ok) {
+        ok = mbar_wait_warp(q_empty(sq), ((unsigned)(n / L::NQ) & 1u) ^ 1u, abort_flag, nullptr, 91);
+        if (ok && lane == 0) {
+          mbar_expect_tx(q_full(sq), 2u * TILE);
+          for (int s = 0; s < SLABS; ++s) {
+            tma_load_4d(q_tile(sq) + s * TT_SLAB, &map_q, s * 64, x.at.head, x.r0, x.at.stream, q_full(sq));
+            tma_load_4d(q_tile(sq) + TILE + s * TT_SLAB, &map_do, s * 64, x.at.head, x.r0, x.at.stream, q_full(sq));
+          }
+        }
+        if (ok) ++n;
+        __syncwarp();
       }
+      for (int i = 0; i < x.tiles && ok; ++i, ++g) {
+        const int sa = g % L::NA, sb = g % L::NB, j0 = x.lo + i * TT_B;
+        ok = mbar_wait_warp(a_empty(sa), ((unsigned)(g / L::NA) & 1u) ^ 1u, abort_flag, nullptr, 91);
+        if (!ok) break;
+        if (lane == 0) {
+          mbar_expect_tx(a_full(sa), (unsigned)TILE);
+          for (int s = 0; s < SLABS; ++s) tma_load_4d(k_tile(sa) + s * TT_SLAB, &map_k, s * 64, kh, j0, x.at.stream, a_full(sa));
+        }
+        ++a_loads;
+        __syncwarp();
+        ok = mbar_wait_warp(b_empty(sb), ((unsigned)(g / L::NB) & 1u) ^ 1u, abort_flag, nullptr, 91);
+        if (!ok) break;
+        if (lane == 0) {
+          mbar_expect_tx(b_full(sb), (unsigned)TILE);
+          for (int s = 0; s < SLABS; ++s) tma_load_4d(v_tile(sb) + s * TT_SLAB, &map_v, s * 64, kh, j0, x.at.stream, b_full(sb));
+        }
+        ++b_loads;
+        __syncwarp();
+      }
+      block = more ? next.take(w, lane, false) : -1;
     }
-    for (; it < tiles; ++it) {
-      const int sa = it % L::NA, sb = it % L::NB, j0 = lo + it * TT_B;
-      ok = mbar_wait_warp(a_empty(sa), ((unsigned)(it / L::NA) & 1u) ^ 1u, abort_flag, nullptr, 91);
-      if (!ok) break;
-      if (lane == 0) {
-        mbar_expect_tx(a_full(sa), (unsigned)TILE);
-        for (int s = 0; s < SLABS; ++s) tma_load_4d(k_tile(sa) + s * TT_SLAB, &map_k, s * 64, kh, j0, at.stream, a_full(sa));
-      }
-      __syncwarp();
-      ok = mbar_wait_warp(b_empty(sb), ((unsigned)(it / L::NB) & 1u) ^ 1u, abort_flag, nullptr, 91);
-      if (!ok) {
-        ++it;  // (its keys are on their way)
-        break;
-      }
-      if (lane == 0) {
-        mbar_expect_tx(b_full(sb), (unsigned)TILE);
-        for (int s = 0; s < SLABS; ++s) tma_load_4d(v_tile(sb) + s * TT_SLAB, &map_v, s * 64, kh, j0, at.stream, b_full(sb));
-      }
-      __syncwarp();
-    }
-    if (*abort_flag && tiles > 0) {  // copies in flight must land before the shared memory goes away
+    if (*abort_flag) {  // copies in flight must land before the shared memory goes away
       const unsigned long long limit = global_timer() + WAIT_LIMIT_NS;
-      while (!mbar_try_wait(q_full, 0) && global_timer() < limit) {}
-      for (int j = it > L::NA ? it - L::NA : 0; j < it; ++j)
+      for (int j = n > L::NQ ? n - L::NQ : 0; j < n; ++j)
+        while (!mbar_try_wait(q_full(j % L::NQ), (unsigned)(j / L::NQ) & 1u) && global_timer() < limit) {}
+      for (int j = a_loads > L::NA ? a_loads - L::NA : 0; j < a_loads; ++j)
         while (!mbar_try_wait(a_full(j % L::NA), (unsigned)(j / L::NA) & 1u) && global_timer() < limit) {}
-      const int b_loads = ok ? it : it - 1;
       for (int j = b_loads > L::NB ? b_loads - L::NB : 0; j < b_loads; ++j)
         while (!mbar_try_wait(b_full(j % L::NB), (unsigned)(j / L::NB) & 1u) && global_timer() < limit) {}
     }
   } else if (warp == 1) {
     const int cols = (a.dim + 15) & ~15;
-    const unsigned long long q_rows = tt_rows(q_off), do_rows = tt_rows(do_off), k_rows = tt_rows(k_tile(0)), v_rows = tt_rows(v_tile(0)),
-                             k_cols = tt_cols(k_tile(0));
+    const unsigned long long q_rows = tt_rows(q_tile(0)), k_rows = tt_rows(k_tile(0)), v_rows = tt_rows(v_tile(0)), k_cols = tt_cols(k_tile(0));
     auto stage = [](int s) { return (unsigned long long)(s * (TILE >> 4)); };
     const unsigned idesc_s = umma_idesc_bf16(TT_B), idesc_d = umma_idesc_bf16(cols) | UMMA_B_MN_MAJOR;
-    // keys behind the stream's length must not meet the zeros of dS as anything but zeros
-    auto arrived = [&](int i) {
-      if (!mbar_wait_warp(a_full(i % L::NA), (unsigned)(i / L::NA) & 1u, abort_flag, nullptr, 92)) return false;
-      const int have = at.keys - (lo + i * TT_B);
-      if (have < TT_B && at.keys < a.m) tt_clear_rows(base_ptr + (k_tile(i % L::NA) - base), SLABS, have, lane);
-      return true;
+    // A tile of an item. S and dP are issued one tile ahead of dQ, into the next item too.
+    struct Job {
+      Item x;
+      int i, g, n;  // tile of the item, of all; item
     };
-    auto upstream = [&](int i) {  // dP of tile i
-      const int sb = i % L::NB;
-      if (!mbar_wait_warp(b_full(sb), (unsigned)(i / L::NB) & 1u, abort_flag, nullptr, 92)) return false;
-      if (tc_elect()) {
-        tt_mma_rows<D>(tmem_dp0 + (unsigned)((i & 1) * 128), do_rows, v_rows + stage(sb), idesc_s);
-        tc_commit(dp_full(i));
-        tc_commit(b_empty(sb));
+    int w = 0;
+    Job lead{item((int)blockIdx.x), -1, -1, -1};
+    auto advance = [&]() {  // the next tile; false: none
+      ++lead.g;
+      if (++lead.i < lead.x.tiles) {
+        if (lead.i == 0) ++lead.n;
+        return true;
       }
-      __syncwarp();
-      return true;
+      while (true) {
+        const int block = next.take(w++, lane, true);
+        if (block < 0) return false;
+        lead.x = item(block);
+        lead.i = 0;
+        if (lead.x.tiles > 0) {
+          ++lead.n;
+          return true;
+        }
+      }
     };
-    bool ok = true;
-    if (tiles > 0) {
-      ok = mbar_wait_warp(q_full, 0, abort_flag, nullptr, 93) && arrived(0);
+    auto issue = [&](const Job &t) {
+      const int sa = t.g % L::NA, sb = t.g % L::NB, sq = t.n % L::NQ;
+      const unsigned long long q_at = q_rows + (unsigned long long)(sq * (2 * TILE >> 4));
+      if (t.i == 0 && !mbar_wait_warp(q_full(sq), (unsigned)(t.n / L::NQ) & 1u, abort_flag, nullptr, 93)) return false;
+      if (!mbar_wait_warp(a_full(sa), (unsigned)(t.g / L::NA) & 1u, abort_flag, nullptr, 92)) return false;
+      // keys behind the stream's length must not meet the zeros of dS as anything but zeros
+      const int have = t.x.at.keys - (t.x.lo + t.i * TT_B);
+      if (have < TT_B && t.x.at.keys < a.m) tt_clear_rows(base_ptr + (k_tile(sa) - base), SLABS, have, lane);
+      if (t.g > 0 && !mbar_wait_warp(s_free, (unsigned)(t.g - 1) & 1u, abort_flag, nullptr, 94)) return false;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      if (ok && tc_elect()) {
-        tt_mma_rows<D>(tmem_s, q_rows, k_rows, idesc_s);
+      if (tc_elect()) {
+        tt_mma_rows<D>(tmem_s, q_at, k_rows + stage(sa), idesc_s);
         tc_commit(s_full);
       }
       __syncwarp();
-      ok = ok && upstream(0);
-    }
-    for (int i = 0; i < tiles && ok; ++i) {
-      const int sa = i % L::NA, na = (i + 1) % L::NA;
-      if (i + 1 < tiles) {
-        ok = arrived(i + 1) && mbar_wait_warp(s_free, (unsigned)i & 1u, abort_flag, nullptr, 94);
-        if (!ok) break;
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        if (tc_elect()) {
-          tt_mma_rows<D>(tmem_s, q_rows, k_rows + stage(na), idesc_s);
-          tc_commit(s_full);
-        }
-        __syncwarp();
-        ok = upstream(i + 1);  // over dS(i - 1), whose product was issued before
-        if (!ok) break;
+      if (!mbar_wait_warp(b_full(sb), (unsigned)(t.g / L::NB) & 1u, abort_flag, nullptr, 92)) return false;
+      if (tc_elect()) {  // over dS of the tile before the last, whose product was issued before
+        tt_mma_rows<D>(tmem_dp0 + (unsigned)((t.g & 1) * 128), q_at + (unsigned long long)(TILE >> 4), v_rows + stage(sb), idesc_s);
+        tc_commit(dp_full(t.g));
+        tc_commit(b_empty(sb));
+        if (t.i + 1 == t.x.tiles) tc_commit(q_empty(sq));
       }
-      ok = mbar_wait_warp(ds_ready(i), (unsigned)(i >> 1) & 1u, abort_flag, nullptr, 95);
+      __syncwarp();
+      return true;
+    };
+    bool more = advance(), ok = !more || issue(lead);
+    while (more && ok) {
+      const Job now = lead;
+      more = advance();
+      ok = !more || issue(lead);
+      if (!ok) break;
+      ok = mbar_wait_warp(ds_ready(now.g), (unsigned)(now.g >> 1) & 1u, abort_flag, nullptr, 95);
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       if (tc_elect()) {
-        tt_mma_weights<true>(tmem_dq, tmem_dp0 + (unsigned)((i & 1) * 128), k_cols + stage(sa), idesc_d, i > 0);
-        tc_commit(a_empty(sa));
+        tt_mma_weights<true>(tmem_dq, tmem_dp0 + (unsigned)((now.g & 1) * 128), k_cols + stage(now.g % L::NA), idesc_d, now.i > 0);
+        tc_commit(a_empty(now.g % L::NA));
+        if (now.i + 1 == now.x.tiles) tc_commit(done);
       }
       __syncwarp();
     }
-    if (tiles > 0 && tc_elect()) tc_commit(done);
-    __syncwarp();
-    if (!ok) {  // a bounded chance for the tensor pipe to finish before tensor memory is freed
+    if (!ok) {  // a bounded chance for the tensor pipe to finish before tensor memory is freed; the items' order goes on
+      while (more) more = next.take(w++, lane, true) >= 0;
+      if (tc_elect()) tc_commit(next.drained());
+      __syncwarp();
       const unsigned long long limit = global_timer() + WAIT_LIMIT_NS;
-      while (!mbar_try_wait(done, 0) && global_timer() < limit) {}
+      while (!mbar_try_wait(next.drained(), 0) && global_timer() < limit) {}
     }
   } else {
     const int q = warp & 3, half = (warp - 2) >> 2;
     const unsigned lanes = (unsigned)(q * 32) << 16;
-    const int row = r0 + q * 32 + lane;
-    const int row_lo = a.span.lo(row), row_end = a.span.end(row, at.keys);
-    const int warp_lo = a.span.lo(r0 + q * 32 + 31), warp_end = a.span.end(r0 + q * 32, at.keys);
-    const long long x = ((long long)at.stream * a.heads + at.head) * a.n + row;
-    const float z = row < a.n ? a.lse[x] : -INFINITY;
-    float delta = row < a.n ? a.delta[x] : 0.f;
-    const float lse = z == -INFINITY ? -INFINITY : -(z * TT_LOG2E);  // to add; a row that sees no key has no weights: 2^(s - infinity)
+    const int cols = (a.dim + 15) & ~15, mid = (cols / 2 + 15) & ~15;  // each half of the warps stores half of the columns
+    int g = 0, n = 0, exact = 0;
+    bool ok = true;
     // dout . out is off by what out was rounded by, which counts in rows of few keys. Where all of a row's keys lie in this one
     // tile, the same sum over keys, p dP, is at hand in 32 bits (the kernel of dk and dv then finds it in place of the other).
-    auto exact_delta = [&](const float (&p)[64], int half, int c_lo, int c_end) {
+    auto exact_delta = [&](const float (&p)[64], unsigned tmem_dp, int c_lo, int c_end) {
       float t = 0.f;
 #pragma unroll
       for (int c = 0; c < 64; c += 32) {
         unsigned u[32];
-        tc_ld32(tmem_dp0 + lanes + (unsigned)(half * 64 + c), u);
+        tc_ld32(tmem_dp + lanes + (unsigned)(half * 64 + c), u);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
         for (int j = 0; j < 32; ++j)
           if (c + j >= c_lo && c + j < c_end) t = fmaf(p[c + j], __uint_as_float(u[j]), t);
       }
-      float *both = stat + q * 32 + lane;
+      // (of two places in turn: the other half has read this one's before it arrives for the next)
+      float *both = stat + (exact & 1) * 256 + q * 32 + lane;
       both[half * 128] = t;
       __syncwarp();
       if (lane == 0) mbar_arrive(halves(q));
-      if (!mbar_wait_warp(halves(q), 0, abort_flag, nullptr, 99)) return NAN;
-      t = both[0] + both[128];
-      if (half == 0 && row < a.n) a.delta[x] = t;
-      return t;
+      const bool met = mbar_wait_warp(halves(q), (unsigned)exact & 1u, abort_flag, nullptr, 99);
+      ++exact;
+      return met ? both[0] + both[128] : NAN;
     };
-    bool ok = true;
-    for (int i = 0; i < tiles && ok; ++i) {
-      const int j0 = lo + i * TT_B + half * 64;
-      const unsigned tmem_dp = tmem_dp0 + (unsigned)((i & 1) * 128);
-      const int c_lo = row_lo - j0, c_end = row_end - j0;
-      const bool inside = warp_lo <= j0 && warp_end >= j0 + 64;
-      ok = mbar_wait_warp(s_full, (unsigned)i & 1u, abort_flag, nullptr, 96);
-      if (!ok) break;
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      float p[64];
-      {
-        unsigned(&u)[2][32] = reinterpret_cast<unsigned(&)[2][32]>(p);
-        tc_ld32(tmem_s + lanes + (unsigned)(half * 64), u[0]);
-        tc_ld32(tmem_s + lanes + (unsigned)(half * 64 + 32), u[1]);
-        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-      }
-      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mbar_arrive(s_free);
-      const unsigned long long f2 = tt_two(a.factor, a.factor), z2 = tt_two(lse, lse);
-#pragma unroll
-      for (int j = 0; j < 64; j += 2) {
-        const unsigned long long t = tt_exp2_two(tt_fma2(tt_two(p[j], p[j + 1]), f2, z2));
-        p[j] = tt_lo(t);
-        p[j + 1] = tt_hi(t);
-      }
-      ok = mbar_wait_warp(dp_full(i), (unsigned)(i >> 1) & 1u, abort_flag, nullptr, 97);
-      if (!ok) break;
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      if (!inside) {
-#pragma unroll
-        for (int j = 0; j < 64; ++j)
-          if (j < c_lo || j >= c_end) p[j] = 0.f;
-      }
-      if (tiles == 1) delta = exact_delta(p, half, c_lo, c_end);
-#pragma unroll
-      for (int c = 0; c < 64; c += 32) {
-        unsigned u[32], w[16];
-        tc_ld32(tmem_dp + lanes + (unsigned)(half * 64 + c), u);
-        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-        const unsigned long long d2 = tt_two(-delta, -delta);
-#pragma unroll
-        for (int j = 0; j < 32; j += 2) {
-          const unsigned long long x = tt_mul2(tt_add2(tt_two(__uint_as_float(u[j]), __uint_as_float(u[j + 1])), d2),
-                                               tt_two(p[c + j], p[c + j + 1]));
-          p[c + j] = tt_lo(x);
-          p[c + j + 1] = tt_hi(x);
+    Item x = item((int)blockIdx.x);
+    auto statistics = [&](float &z, float &delta) {
+      const int row = x.r0 + q * 32 + lane;
+      const long long at = ((long long)x.at.stream * a.heads + x.at.head) * a.n + row;
+      z = row < a.n ? a.lse[at] : -INFINITY;
+      delta = row < a.n ? a.delta[at] : 0.f;
+    };
+    float z, delta;
+    statistics(z, delta);
+    for (int w = 0;; ++w) {
+      const int row = x.r0 + q * 32 + lane;
+      const int row_lo = a.span.lo(row), row_end = a.span.end(row, x.at.keys);
+      const int warp_lo = a.span.lo(x.r0 + q * 32 + 31), warp_end = a.span.end(x.r0 + q * 32, x.at.keys);
+      const float lse = z == -INFINITY ? -INFINITY : -(z * TT_LOG2E);  // to add; a row that sees no key has no weights: 2^(s - infinity)
+      for (int i = 0; i < x.tiles && ok; ++i, ++g) {
+        const int j0 = x.lo + i * TT_B + half * 64;
+        const unsigned tmem_dp = tmem_dp0 + (unsigned)((g & 1) * 128);
+        const int c_lo = row_lo - j0, c_end = row_end - j0;
+        const bool inside = warp_lo <= j0 && warp_end >= j0 + 64;
+        ok = mbar_wait_warp(s_full, (unsigned)g & 1u, abort_flag, nullptr, 96);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        float p[64];
+        {
+          unsigned(&u)[2][32] = reinterpret_cast<unsigned(&)[2][32]>(p);
+          tc_ld32(tmem_s + lanes + (unsigned)(half * 64), u[0]);
+          tc_ld32(tmem_s + lanes + (unsigned)(half * 64 + 32), u[1]);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
         }
-        if (!inside) {  // (a weight of zero has no part even where the other factor is not finite)
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(s_free);
+        const unsigned long long f2 = tt_two(a.factor, a.factor), z2 = tt_two(lse, lse);
 #pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (c + j < c_lo || c + j >= c_end) p[c + j] = 0.f;
+        for (int j = 0; j < 64; j += 2) {
+          const unsigned long long t = tt_exp2_two(tt_fma2(tt_two(p[j], p[j + 1]), f2, z2));
+          p[j] = tt_lo(t);
+          p[j + 1] = tt_hi(t);
+        }
+        ok = mbar_wait_warp(dp_full(g), (unsigned)(g >> 1) & 1u, abort_flag, nullptr, 97);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (!inside) {
+#pragma unroll
+          for (int j = 0; j < 64; ++j)
+            if (j < c_lo || j >= c_end) p[j] = 0.f;
+        }
+        if (x.tiles == 1) {
+          delta = exact_delta(p, tmem_dp, c_lo, c_end);
+          if (half == 0 && row < a.n) a.delta[((long long)x.at.stream * a.heads + x.at.head) * a.n + row] = delta;
         }
 #pragma unroll
-        for (int j = 0; j < 16; ++j) w[j] = tt_pack(p[c + 2 * j], p[c + 2 * j + 1]);
-        tc_st16(tmem_dp + lanes + (unsigned)(half * 64 + (c >> 1)), w);
+        for (int c = 0; c < 64; c += 32) {
+          unsigned u[32], v[16];
+          tc_ld32(tmem_dp + lanes + (unsigned)(half * 64 + c), u);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+          const unsigned long long d2 = tt_two(-delta, -delta);
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            const unsigned long long y = tt_mul2(tt_add2(tt_two(__uint_as_float(u[j]), __uint_as_float(u[j + 1])), d2),
+                                                 tt_two(p[c + j], p[c + j + 1]));
+            p[c + j] = tt_lo(y);
+            p[c + j + 1] = tt_hi(y);
+          }
+          if (!inside) {  // (a weight of zero has no part even where the other factor is not finite)
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (c + j < c_lo || c + j >= c_end) p[c + j] = 0.f;
+          }
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[j] = tt_pack(p[c + 2 * j], p[c + 2 * j + 1]);
+          tc_st16(tmem_dp + lanes + (unsigned)(half * 64 + (c >> 1)), v);
+        }
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(ds_ready(g));
       }
-      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mbar_arrive(ds_ready(i));
+      // the next item's statistics are on their way while this one's rows are stored
+      const Item then = x;
+      const int block = next.take(w, lane, true);
+      if (block >= 0) {
+        x = item(block);
+        statistics(z, delta);
+      }
+      if (ok && then.tiles > 0) ok = mbar_wait_warp(done, (unsigned)n++ & 1u, abort_flag, nullptr, 98);
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      bf16 *o = reinterpret_cast<bf16 *>(a.o1.p) + then.at.stream * a.o1.s + (long long)row * a.o1.r + then.at.head * a.o1.h;
+      ok = __all_sync(0xffffffffu, ok && !*abort_flag);
+      tt_store_row(o, row < a.n, a, tmem_dq + lanes, half ? mid : 0, half ? cols : mid, a.scale, then.tiles == 0, ok);
+      if (block < 0) break;
     }
-    if (ok && tiles > 0) ok = mbar_wait_warp(done, 0, abort_flag, nullptr, 98);
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    bf16 *o = reinterpret_cast<bf16 *>(a.o1.p) + at.stream * a.o1.s + (long long)row * a.o1.r + at.head * a.o1.h;
-    const int cols = (a.dim + 15) & ~15, mid = (cols / 2 + 15) & ~15;  // each half of the warps stores half of the columns
-    tt_store_row(o, row < a.n, a, tmem_dq + lanes, half ? mid : 0, half ? cols : mid, a.scale, tiles == 0, __all_sync(0xffffffffu, ok && !*abort_flag));
   }
   __syncwarp();
   pdl_launch_dependents();

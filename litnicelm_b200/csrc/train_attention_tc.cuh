@@ -70,8 +70,8 @@ struct TtArgs {
 struct TtPlace {
   int tile, head, stream, keys;
 };
-__device__ __forceinline__ TtPlace tt_place(const TtArgs &a, int heads, bool last_first, int ctas = 1) {  // ctas: to a tile
-  const int each = heads * a.streams, b = (int)blockIdx.x / ctas;
+__device__ __forceinline__ TtPlace tt_place(const TtArgs &a, int heads, bool last_first, int ctas, int block) {  // ctas: to a tile
+  const int each = heads * a.streams, b = block / ctas;
   const int t = b / each, rest = b - t * each;
   TtPlace p;
   p.tile = last_first ? a.tiles - 1 - t : t;
@@ -80,6 +80,66 @@ __device__ __forceinline__ TtPlace tt_place(const TtArgs &a, int heads, bool las
   p.keys = a.lengths ? max(0, min(a.m, a.lengths[p.stream])) : a.m;
   return p;
 }
+__device__ __forceinline__ TtPlace tt_place(const TtArgs &a, int heads, bool last_first, int ctas = 1) {
+  return tt_place(a, heads, last_first, ctas, (int)blockIdx.x);
+}
+
+// Blocks that have not started, taken over by running ones (cluster launch control): a block's warps go on with the next tile of
+// rows while its last results are on their way, nothing is set up again, and whoever is free first takes the next. Warp 0 asks one
+// block ahead, `readers` warps and itself take the answers. Two answers' places; 64 bytes of shared memory from `at` on: answers,
+// their barriers, the barrier of a CTA that gave up.
+struct TtNext {
+  unsigned at;
+  __device__ __forceinline__ unsigned full(int w) const { return at + 32u + 8u * (w & 1); }
+  __device__ __forceinline__ unsigned empty(int w) const { return at + 48u + 8u * (w & 1); }
+  __device__ __forceinline__ unsigned drained() const { return at + 64u; }
+  __device__ __forceinline__ void init(int readers) const {
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(full(w), 1);
+      mbar_init(empty(w), readers);
+    }
+    mbar_init(drained(), 1);
+  }
+  // These waits go on in a CTA that gave up on another: each block that it has taken gets its results, if only NaN.
+  static __device__ __forceinline__ bool wait(unsigned bar, unsigned parity) {
+    if (!mbar_try_wait(bar, parity)) {
+      const unsigned long long limit = global_timer() + 16 * WAIT_LIMIT_NS;
+      while (!mbar_try_wait(bar, parity))
+        if (global_timer() > limit) return false;
+    }
+    return true;
+  }
+  // Asks for the block behind the w-th. Not after an answer of none.
+  __device__ __forceinline__ bool ask(int w, int lane) const {
+    if (!__all_sync(0xffffffffu, w < 2 || wait(empty(w), ((unsigned)(w >> 1) & 1u) ^ 1u))) return false;
+    if (lane == 0) {
+      mbar_expect_tx(full(w), 16u);
+      asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(at + 16u * (w & 1)),
+                   "r"(full(w))
+                   : "memory");
+    }
+    __syncwarp();
+    return true;
+  }
+  // The block behind the w-th, or -1.
+  __device__ __forceinline__ int take(int w, int lane, bool reader) const {
+    if (!__all_sync(0xffffffffu, wait(full(w), (unsigned)(w >> 1) & 1u))) return -1;
+    unsigned some, block;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b128 r;\n\t"
+        "ld.shared.b128 r, [%2];\n\t"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n\t}"
+        : "=r"(some), "=r"(block)
+        : "r"(at + 16u * (w & 1))
+        : "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if (reader && lane == 0) mbar_arrive(empty(w));
+    return some ? (int)block : -1;
+  }
+};
 
 __device__ __forceinline__ void tt_alloc(volatile unsigned *holder, unsigned cols) {
   asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void *)holder)), "r"(cols)
