@@ -62,6 +62,14 @@ __device__ __forceinline__ void tt_store_row(bf16 *row, bool live, const TtArgs 
   }
 }
 
+// A tile of 128 rows from r0 on of a head's result, as zeros (by one warp).
+__device__ __forceinline__ void tt_store_zeros(const HeadView &o, const TtArgs &a, const TtPlace &at, int r0, int rows, int lane) {
+  const float none[16] = {};
+  for (int row = r0 + lane; row < min(r0 + TT_B, rows); row += 32)
+    for (int c = 0; c < a.dim; c += 16)
+      tt_store16(reinterpret_cast<bf16 *>(o.p) + at.stream * o.s + (long long)row * o.r + at.head * o.h, a, c, none);
+}
+
 // Rows `from` .. 127 of a tile of slabs, as zeros (by one warp; the tensor cores read them next).
 __device__ __forceinline__ void tt_clear_rows(unsigned char *tile, int slabs, int from, int lane) {
   for (int s = 0; s < slabs; ++s)
@@ -530,6 +538,7 @@ train_forward_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
 template <int D>
 struct TtBwd {
   static constexpr int SLABS = D / 64, TILE = SLABS * TT_SLAB;
+  static constexpr int NP = D == 64 ? 3 : 2;  // tiles of scores and dP in tensor memory, of the kernel for dk and dv
   static constexpr int NQ = D == 64 ? 2 : 1, NA = D == 64 ? 4 : 3, NB = D == 64 ? 4 : 2;
   static constexpr int A_OFF = 2 * NQ * TILE, B_OFF = A_OFF + NA * TILE;
   static constexpr int STAT_OFF = B_OFF + NB * TILE;  // [NB][2][128] floats
@@ -548,7 +557,9 @@ train_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   const unsigned base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char *base_ptr = smem_raw + (base - smem_u32(smem_raw));
-  const unsigned k_off = base, v_off = base + TILE, bars = base + L::BAR_OFF;
+  constexpr int NP = L::NP;
+  const unsigned bars = base + L::BAR_OFF;
+  auto k_tile = [&](int s) { return base + (unsigned)(s * 2 * TILE); };  // and the values' behind it
   auto q_tile = [&](int s) { return base + (unsigned)(L::A_OFF + s * TILE); };
   auto do_tile = [&](int s) { return base + (unsigned)(L::B_OFF + s * TILE); };
   float *stat = reinterpret_cast<float *>(base_ptr + L::STAT_OFF);
@@ -556,25 +567,27 @@ train_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
   auto a_empty = [&](int s) { return bars + 32u + 8u * s; };
   auto b_full = [&](int s) { return bars + 64u + 8u * s; };
   auto b_empty = [&](int s) { return bars + 96u + 8u * s; };
-  const unsigned kv_full = bars + 128, s_full = bars + 136, p_ready = bars + 144, dp_full = bars + 152, ds_ready = bars + 160,
-                 done = bars + 168;
+  auto kv_full = [&](int s) { return bars + 128u + 8u * s; };
+  auto kv_empty = [&](int s) { return bars + 144u + 8u * s; };
+  auto full = [&](int job) { return bars + 160u + 8u * (job % NP); };
+  auto ready = [&](int job) { return bars + 184u + 8u * (job % NP); };
   auto stat_full = [&](int s) { return bars + 208u + 8u * s; };
-  volatile unsigned *tmem_holder = reinterpret_cast<volatile unsigned *>(base_ptr + L::BAR_OFF + 240);
-  volatile int *abort_flag = reinterpret_cast<volatile int *>(base_ptr + L::BAR_OFF + 244);
+  const unsigned done = bars + 240;
+  volatile unsigned *tmem_holder = reinterpret_cast<volatile unsigned *>(base_ptr + L::BAR_OFF + 248);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(base_ptr + L::BAR_OFF + 252);
+  TtNext next{bars + 256u};
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const TtPlace at = tt_place(a, a.groups, false);
-  const int j0 = at.tile * TT_B, j1 = min(j0 + TT_B, at.keys);
-  // rows that see a key of this tile: from lo on, to row_end
-  const int lo = a.span.causal ? max(0, j0 - a.span.first) / TT_B * TT_B : 0;
-  const long long past = a.span.window > 0 ? (long long)j1 - 1 + a.span.window - a.span.first : a.n;
-  const int row_end = past < a.n ? (int)max(past, 0LL) : a.n;
-  const int each = j0 < at.keys && row_end > lo ? (row_end - lo + TT_B - 1) / TT_B : 0;  // tiles per query head
-  const int tiles = each * a.share;
 
   if (threadIdx.x == 0) {
-    for (unsigned bar : {kv_full, s_full, dp_full, done}) mbar_init(bar, 1);
-    mbar_init(p_ready, 8);
-    mbar_init(ds_ready, 8);
+    mbar_init(done, 1);
+    for (int s = 0; s < NP; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(ready(s), 8);
+    }
+    for (int s = 0; s < L::NQ; ++s) {
+      mbar_init(kv_full(s), 1);
+      mbar_init(kv_empty(s), 1);
+    }
     for (int s = 0; s < L::NA; ++s) {
       mbar_init(a_full(s), 1);
       mbar_init(a_empty(s), 1);
@@ -584,6 +597,7 @@ train_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       mbar_init(b_empty(s), 1);
       mbar_init(stat_full(s), 1);
     }
+    next.init(9);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -592,39 +606,77 @@ train_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  const unsigned tmem_s = *tmem_holder, tmem_dp = tmem_s + 128, tmem_dv = tmem_s + 256, tmem_dk = tmem_dv + D;
+  const unsigned tmem = *tmem_holder, tmem_dv = tmem + NP * 128, tmem_dk = tmem_dv + D;
+  auto place = [&](int job) { return tmem + (unsigned)(job % NP * 128); };
   pdl_wait();
 
+  struct Item {
+    TtPlace at;
+    int j0, lo, each, tiles;  // rows that see a key of this tile: `each` tiles of them from lo on, for each query head
+  };
+  auto item = [&](int block) {
+    Item x;
+    x.at = tt_place(a, a.groups, false, 1, block);
+    x.j0 = x.at.tile * TT_B;
+    x.lo = a.span.causal ? max(0, x.j0 - a.span.first) / TT_B * TT_B : 0;
+    const long long past = a.span.window > 0 ? (long long)min(x.j0 + TT_B, x.at.keys) - 1 + a.span.window - a.span.first : a.n;
+    const int row_end = past < a.n ? (int)max(past, 0LL) : a.n;
+    x.each = x.j0 < x.at.keys && row_end > x.lo ? (row_end - x.lo + TT_B - 1) / TT_B : 0;
+    x.tiles = x.each * a.share;
+    return x;
+  };
+
   if (warp == 0) {
-    int it = 0;
+    int g = 0, n = 0, a_loads = 0, b_loads = 0;  // tiles of rows so far, items with any, loads issued
     bool ok = true;
-    if (lane == 0 && tiles > 0) {
-      mbar_expect_tx(kv_full, 2u * TILE);
-      for (int s = 0; s < SLABS; ++s) {
-        tma_load_4d(k_off + s * TT_SLAB, &map_k, s * 64, at.head, j0, at.stream, kv_full);
-        tma_load_4d(v_off + s * TT_SLAB, &map_v, s * 64, at.head, j0, at.stream, kv_full);
+    int block = (int)blockIdx.x;
+    for (int w = 0;; ++w) {
+      Item x = item(max(block, 0));
+      while (block >= 0 && x.tiles == 0) {
+        tt_store_zeros(a.o1, a, x.at, x.j0, a.m, lane);
+        tt_store_zeros(a.o2, a, x.at, x.j0, a.m, lane);
+        next.ask(lane);
+        block = next.answer();
+        x = item(max(block, 0));
       }
-    }
-    for (int h = at.head * a.share; h < (at.head + 1) * a.share && ok; ++h) {
-      const long long stats = ((long long)at.stream * a.heads + h) * a.n;
-      for (int t = 0; t < each; ++t, ++it) {
-        const int sa = it % L::NA, st = it % L::NB, r0 = lo + t * TT_B;
-        ok = mbar_wait_warp(a_empty(sa), ((unsigned)(it / L::NA) & 1u) ^ 1u, abort_flag, nullptr, 80);
+      next.push(w, block, lane);
+      if (block < 0) break;
+      bool asked = false;
+      const int sk = n % L::NQ;
+      if (ok) {
+        ok = mbar_wait_warp(kv_empty(sk), ((unsigned)(n / L::NQ) & 1u) ^ 1u, abort_flag, nullptr, 82);
+        if (ok && lane == 0) {
+          mbar_expect_tx(kv_full(sk), 2u * TILE);
+          for (int s = 0; s < SLABS; ++s) {
+            tma_load_4d(k_tile(sk) + s * TT_SLAB, &map_k, s * 64, x.at.head, x.j0, x.at.stream, kv_full(sk));
+            tma_load_4d(k_tile(sk) + TILE + s * TT_SLAB, &map_v, s * 64, x.at.head, x.j0, x.at.stream, kv_full(sk));
+          }
+        }
+        if (ok) ++n;
+        __syncwarp();
+      }
+      for (int i = 0, h = x.at.head * a.share, t = 0; i < x.tiles && ok; ++i, ++g) {
+        const long long stats = ((long long)x.at.stream * a.heads + h) * a.n;
+        const int sa = g % L::NA, st = g % L::NB, r0 = x.lo + t * TT_B;
+        ok = mbar_wait_warp(a_empty(sa), ((unsigned)(g / L::NA) & 1u) ^ 1u, abort_flag, nullptr, 80);
         if (!ok) break;
         if (lane == 0) {
           mbar_expect_tx(a_full(sa), (unsigned)TILE);
-          for (int s = 0; s < SLABS; ++s) tma_load_4d(q_tile(sa) + s * TT_SLAB, &map_q, s * 64, h, r0, at.stream, a_full(sa));
+          for (int s = 0; s < SLABS; ++s) tma_load_4d(q_tile(sa) + s * TT_SLAB, &map_q, s * 64, h, r0, x.at.stream, a_full(sa));
         }
+        ++a_loads;
         __syncwarp();
-        ok = mbar_wait_warp(b_empty(st), ((unsigned)(it / L::NB) & 1u) ^ 1u, abort_flag, nullptr, 81);
-        if (!ok) {
-          ++it;  // (its rows of q are on their way)
-          break;
+        if (i + 1 == x.tiles) {
+          next.ask(lane);
+          asked = true;
         }
+        ok = mbar_wait_warp(b_empty(st), ((unsigned)(g / L::NB) & 1u) ^ 1u, abort_flag, nullptr, 81);
+        if (!ok) break;
         if (lane == 0) {
           mbar_expect_tx(b_full(st), (unsigned)TILE);
-          for (int s = 0; s < SLABS; ++s) tma_load_4d(do_tile(st) + s * TT_SLAB, &map_do, s * 64, h, r0, at.stream, b_full(st));
+          for (int s = 0; s < SLABS; ++s) tma_load_4d(do_tile(st) + s * TT_SLAB, &map_do, s * 64, h, r0, x.at.stream, b_full(st));
         }
+        ++b_loads;
         // a row that does not exist or sees no key has no weights: 2^(s - infinity)
 #pragma unroll
         for (int e = lane; e < TT_B; e += 32) {
@@ -636,171 +688,211 @@ train_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         __syncwarp();
         if (lane == 0) mbar_arrive(stat_full(st));
         __syncwarp();
+        if (++t == x.each) {
+          t = 0;
+          ++h;
+        }
       }
+      if (!asked) next.ask(lane);
+      block = next.answer();
     }
-    if (*abort_flag && tiles > 0) {  // copies in flight must land before the shared memory goes away
+    if (*abort_flag) {  // copies in flight must land before the shared memory goes away
       const unsigned long long limit = global_timer() + WAIT_LIMIT_NS;
-      while (!mbar_try_wait(kv_full, 0) && global_timer() < limit) {}
-      for (int j = it > L::NA ? it - L::NA : 0; j < it; ++j)
+      for (int j = n > L::NQ ? n - L::NQ : 0; j < n; ++j)
+        while (!mbar_try_wait(kv_full(j % L::NQ), (unsigned)(j / L::NQ) & 1u) && global_timer() < limit) {}
+      for (int j = a_loads > L::NA ? a_loads - L::NA : 0; j < a_loads; ++j)
         while (!mbar_try_wait(a_full(j % L::NA), (unsigned)(j / L::NA) & 1u) && global_timer() < limit) {}
-      const int b_loads = ok ? it : it - 1;
       for (int j = b_loads > L::NB ? b_loads - L::NB : 0; j < b_loads; ++j)
         while (!mbar_try_wait(b_full(j % L::NB), (unsigned)(j / L::NB) & 1u) && global_timer() < limit) {}
     }
   } else if (warp == 1) {
     const int cols = (a.dim + 15) & ~15;
-    const unsigned long long k_rows = tt_rows(k_off), v_rows = tt_rows(v_off), q_rows = tt_rows(q_tile(0)), do_rows = tt_rows(do_tile(0)),
+    const unsigned long long k_rows = tt_rows(k_tile(0)), q_rows = tt_rows(q_tile(0)), do_rows = tt_rows(do_tile(0)),
                              q_cols = tt_cols(q_tile(0)), do_cols = tt_cols(do_tile(0));
     auto stage = [](int s) { return (unsigned long long)(s * (TILE >> 4)); };
     const unsigned idesc_s = umma_idesc_bf16(TT_B), idesc_d = umma_idesc_bf16(cols) | UMMA_B_MN_MAJOR;
-    bool ok = true;
-    if (tiles > 0) {
-      ok = mbar_wait_warp(kv_full, 0, abort_flag, nullptr, 82) && mbar_wait_warp(a_full(0), 0, abort_flag, nullptr, 83);
+    // Jobs: S and dP of each tile in turn, of all items; each takes the next place, and is issued behind the product that read it.
+    int w = 0, i = -1, n = -1, issued = 0, tiles = 0;  // issued: tiles whose S is
+    bool more = true, ok = true;
+    unsigned ends = 0u;  // bit (tile of all) % 4: it is its item's last, % 4 + 4: first
+    auto kv_rows = [&]() { return k_rows + (unsigned long long)(n % L::NQ * (2 * TILE >> 4)); };
+    auto scores = [&]() {
+      if (++i >= tiles) {
+        const int block = next.take(w++, lane);
+        if (block < 0) {
+          more = false;
+          return;
+        }
+        tiles = tt_uniform(item(block).tiles);
+        i = 0;
+        ++n;
+      }
+      const int g = issued, sa = g % L::NA, sk = n % L::NQ;
+      const unsigned bit = 1u << (g & 3);
+      ends = (ends & ~(bit | bit << 4)) | (i + 1 == tiles ? bit : 0u) | (i == 0 ? bit << 4 : 0u);
+      ok = (i > 0 || mbar_wait_warp(kv_full(sk), (unsigned)(n / L::NQ) & 1u, abort_flag, nullptr, 82)) &&
+           mbar_wait_warp(a_full(sa), (unsigned)(g / L::NA) & 1u, abort_flag, nullptr, 83);
+      if (!ok) return;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      if (ok && tc_elect()) {
-        tt_mma_rows<D>(tmem_s, k_rows, q_rows, idesc_s);
-        tc_commit(s_full);
+      if (tc_elect()) {
+        tt_mma_rows<D>(place(2 * g), kv_rows(), q_rows + stage(sa), idesc_s);
+        tc_commit(full(2 * g));
       }
       __syncwarp();
-      ok = ok && mbar_wait_warp(b_full(0), 0, abort_flag, nullptr, 83);
-      if (ok && tc_elect()) {
-        tt_mma_rows<D>(tmem_dp, v_rows, do_rows, idesc_s);
-        tc_commit(dp_full);
+      ++issued;
+    };
+    auto upstream = [&]() {  // dP of the tile whose S was issued last
+      const int g = issued - 1, sb = g % L::NB;
+      ok = mbar_wait_warp(b_full(sb), (unsigned)(g / L::NB) & 1u, abort_flag, nullptr, 85);
+      if (!ok) return;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      if (tc_elect()) {
+        tt_mma_rows<D>(place(2 * g + 1), kv_rows() + (unsigned long long)(TILE >> 4), do_rows + stage(sb), idesc_s);
+        tc_commit(full(2 * g + 1));
+        if (i + 1 == tiles) tc_commit(kv_empty(n % L::NQ));
       }
       __syncwarp();
-    }
-    for (int i = 0; i < tiles && ok; ++i) {
-      const int sa = i % L::NA, sb = i % L::NB, na = (i + 1) % L::NA, nb = (i + 1) % L::NB;
-      ok = mbar_wait_warp(p_ready, (unsigned)i & 1u, abort_flag, nullptr, 84);
+    };
+    scores();
+    if (more && ok) upstream();
+    if (NP == 3 && more && ok) scores();
+    for (int g = 0; g < issued && ok; ++g) {
+      const int sa = g % L::NA, sb = g % L::NB;
+      const unsigned bit = 1u << (g & 3);
+      const bool first = ends & bit << 4, last = ends & bit;
+      ok = mbar_wait_warp(ready(2 * g), (unsigned)(2 * g / NP) & 1u, abort_flag, nullptr, 84);
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      if (tc_elect()) tt_mma_weights<true>(tmem_dv, tmem_s, do_cols + stage(sb), idesc_d, i > 0);
+      if (tc_elect()) tt_mma_weights<true>(tmem_dv, place(2 * g), do_cols + stage(sb), idesc_d, !first);
       __syncwarp();
-      if (i + 1 < tiles) {
-        ok = mbar_wait_warp(a_full(na), (unsigned)((i + 1) / L::NA) & 1u, abort_flag, nullptr, 85);
-        if (!ok) break;
-        if (tc_elect()) {
-          tt_mma_rows<D>(tmem_s, k_rows, q_rows + stage(na), idesc_s);
-          tc_commit(s_full);
-        }
-        __syncwarp();
+      if (more) {
+        if constexpr (NP == 3) upstream();
+        else scores();
       }
-      ok = mbar_wait_warp(ds_ready, (unsigned)i & 1u, abort_flag, nullptr, 86);
+      if (!ok) break;
+      ok = mbar_wait_warp(ready(2 * g + 1), (unsigned)((2 * g + 1) / NP) & 1u, abort_flag, nullptr, 86);
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       if (tc_elect()) {
-        tt_mma_weights<true>(tmem_dk, tmem_dp, q_cols + stage(sa), idesc_d, i > 0);
+        tt_mma_weights<true>(tmem_dk, place(2 * g + 1), q_cols + stage(sa), idesc_d, !first);
         tc_commit(a_empty(sa));
         tc_commit(b_empty(sb));  // (the statistics beside it have been read too)
+        if (last) tc_commit(done);
       }
       __syncwarp();
-      if (i + 1 < tiles) {
-        ok = mbar_wait_warp(b_full(nb), (unsigned)((i + 1) / L::NB) & 1u, abort_flag, nullptr, 85);
-        if (!ok) break;
-        if (tc_elect()) {
-          tt_mma_rows<D>(tmem_dp, v_rows, do_rows + stage(nb), idesc_s);
-          tc_commit(dp_full);
-        }
-        __syncwarp();
+      if (more) {
+        if constexpr (NP == 3) scores();
+        else upstream();
       }
     }
-    if (tiles > 0 && tc_elect()) tc_commit(done);
-    __syncwarp();
-    if (!ok) {  // a bounded chance for the tensor pipe to finish before tensor memory is freed
+    if (!ok) {  // a bounded chance for the tensor pipe to finish before tensor memory is freed; the items' order goes on
+      while (more) more = next.take(w++, lane) >= 0;
+      if (tc_elect()) tc_commit(next.drained());
+      __syncwarp();
       const unsigned long long limit = global_timer() + WAIT_LIMIT_NS;
-      while (!mbar_try_wait(done, 0) && global_timer() < limit) {}
+      while (!mbar_try_wait(next.drained(), 0) && global_timer() < limit) {}
     }
   } else {
     const int q = warp & 3, half = (warp - 2) >> 2;
     const unsigned lanes = (unsigned)(q * 32) << 16;
-    const int key = j0 + q * 32 + lane;
-    const bool key_live = key < at.keys;
+    int g = 0, n = 0;
     bool ok = true;
-    for (int i = 0; i < tiles && ok; ++i) {
-      const int st = i % L::NB, r0 = lo + i % each * TT_B + half * 64;
-      // rows r0 + c that see this key: [c_lo, c_end)
-      const int c_lo = a.span.causal ? key - a.span.first - r0 : 0;
-      const long long pe = a.span.window > 0 ? (long long)key + a.span.window - a.span.first - r0 : 64;
-      const int c_end = !key_live ? 0 : pe < 64 ? (int)max(pe, 0LL) : 64;
-      const bool inside = __all_sync(0xffffffffu, c_lo <= 0 && c_end >= 64);
-      ok = mbar_wait_warp(stat_full(st), (unsigned)(i / L::NB) & 1u, abort_flag, nullptr, 87) &&
-           mbar_wait_warp(s_full, (unsigned)i & 1u, abort_flag, nullptr, 88);
-      if (!ok) break;
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      float p[64];
-      {
-        unsigned(&u)[2][32] = reinterpret_cast<unsigned(&)[2][32]>(p);
-        tc_ld32(tmem_s + lanes + (unsigned)(half * 64), u[0]);
-        tc_ld32(tmem_s + lanes + (unsigned)(half * 64 + 32), u[1]);
-        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-      }
-      const ulonglong2 *z = reinterpret_cast<const ulonglong2 *>(stat + st * 256 + half * 64);
-      const unsigned long long f2 = tt_two(a.factor, a.factor);
-#pragma unroll
-      for (int j = 0; j < 64; j += 4) {
-        const ulonglong2 v = z[j >> 2];
-        const unsigned long long t = tt_exp2_two(tt_fma2(tt_two(p[j], p[j + 1]), f2, v.x));
-        const unsigned long long u = tt_exp2_two(tt_fma2(tt_two(p[j + 2], p[j + 3]), f2, v.y));
-        p[j] = tt_lo(t);
-        p[j + 1] = tt_hi(t);
-        p[j + 2] = tt_lo(u);
-        p[j + 3] = tt_hi(u);
-      }
-      if (!inside) {
-#pragma unroll
-        for (int j = 0; j < 64; ++j)
-          if (j < c_lo || j >= c_end) p[j] = 0.f;
-      }
-#pragma unroll
-      for (int c = 0; c < 64; c += 32) {
-        unsigned w[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) w[j] = tt_pack(p[c + 2 * j], p[c + 2 * j + 1]);
-        tc_st16(tmem_s + lanes + (unsigned)(half * 64 + (c >> 1)), w);
-      }
-      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mbar_arrive(p_ready);
-      ok = mbar_wait_warp(dp_full, (unsigned)i & 1u, abort_flag, nullptr, 89);
-      if (!ok) break;
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const ulonglong2 *de = reinterpret_cast<const ulonglong2 *>(stat + st * 256 + 128 + half * 64);
-#pragma unroll
-      for (int c = 0; c < 64; c += 32) {
-        unsigned u[32], w[16];
-        tc_ld32(tmem_dp + lanes + (unsigned)(half * 64 + c), u);
-        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-        for (int j = 0; j < 32; j += 4) {
-          const ulonglong2 v = de[(c + j) >> 2];
-          const unsigned long long x = tt_mul2(tt_add2(tt_two(__uint_as_float(u[j]), __uint_as_float(u[j + 1])), v.x),
-                                               tt_two(p[c + j], p[c + j + 1]));
-          const unsigned long long y = tt_mul2(tt_add2(tt_two(__uint_as_float(u[j + 2]), __uint_as_float(u[j + 3])), v.y),
-                                               tt_two(p[c + j + 2], p[c + j + 3]));
-          w[j >> 1] = tt_pack(tt_lo(x), tt_hi(x));
-          w[(j >> 1) + 1] = tt_pack(tt_lo(y), tt_hi(y));
+    int block = next.take(0, lane);
+    Item x = item(max(block, 0));
+    for (int w = 1; block >= 0; ++w) {
+      const int key = x.j0 + q * 32 + lane;
+      const bool key_live = key < x.at.keys;
+      for (int i = 0, t = 0; i < x.tiles && ok; ++i, ++g) {
+        const int st = g % L::NB, r0 = x.lo + t * TT_B + half * 64;
+        const unsigned tmem_s = place(2 * g), tmem_dp = place(2 * g + 1);
+        t = t + 1 == x.each ? 0 : t + 1;
+        // rows r0 + c that see this key: [c_lo, c_end)
+        const int c_lo = a.span.causal ? key - a.span.first - r0 : 0;
+        const long long pe = a.span.window > 0 ? (long long)key + a.span.window - a.span.first - r0 : 64;
+        const int c_end = !key_live ? 0 : pe < 64 ? (int)max(pe, 0LL) : 64;
+        const bool inside = __all_sync(0xffffffffu, c_lo <= 0 && c_end >= 64);
+        ok = mbar_wait_warp(stat_full(st), (unsigned)(g / L::NB) & 1u, abort_flag, nullptr, 87) &&
+             mbar_wait_warp(full(2 * g), (unsigned)(2 * g / NP) & 1u, abort_flag, nullptr, 88);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        float p[64];
+        {
+          unsigned(&u)[2][32] = reinterpret_cast<unsigned(&)[2][32]>(p);
+          tc_ld32(tmem_s + lanes + (unsigned)(half * 64), u[0]);
+          tc_ld32(tmem_s + lanes + (unsigned)(half * 64 + 32), u[1]);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
         }
-        if (!inside) {  // (a weight of zero has no part even where the other factor is not finite)
+        const ulonglong2 *z = reinterpret_cast<const ulonglong2 *>(stat + st * 256 + half * 64);
+        const unsigned long long f2 = tt_two(a.factor, a.factor);
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const int at_lo = c + 2 * j, at_hi = at_lo + 1;
-            w[j] &= (at_lo < c_lo || at_lo >= c_end ? 0u : 0xffffu) | (at_hi < c_lo || at_hi >= c_end ? 0u : 0xffff0000u);
+        for (int j = 0; j < 64; j += 4) {
+          const ulonglong2 v = z[j >> 2];
+          const unsigned long long t = tt_exp2_two(tt_fma2(tt_two(p[j], p[j + 1]), f2, v.x));
+          const unsigned long long u = tt_exp2_two(tt_fma2(tt_two(p[j + 2], p[j + 3]), f2, v.y));
+          p[j] = tt_lo(t);
+          p[j + 1] = tt_hi(t);
+          p[j + 2] = tt_lo(u);
+          p[j + 3] = tt_hi(u);
+        }
+        if (!inside) {
+#pragma unroll
+          for (int j = 0; j < 64; ++j)
+            if (j < c_lo || j >= c_end) p[j] = 0.f;
+        }
+#pragma unroll
+        for (int c = 0; c < 64; c += 32) {
+          unsigned w[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) w[j] = tt_pack(p[c + 2 * j], p[c + 2 * j + 1]);
+          tc_st16(tmem_s + lanes + (unsigned)(half * 64 + (c >> 1)), w);
+        }
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(ready(2 * g));
+        ok = mbar_wait_warp(full(2 * g + 1), (unsigned)((2 * g + 1) / NP) & 1u, abort_flag, nullptr, 89);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const ulonglong2 *de = reinterpret_cast<const ulonglong2 *>(stat + st * 256 + 128 + half * 64);
+#pragma unroll
+        for (int c = 0; c < 64; c += 32) {
+          unsigned u[32], w[16];
+          tc_ld32(tmem_dp + lanes + (unsigned)(half * 64 + c), u);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            const ulonglong2 v = de[(c + j) >> 2];
+            const unsigned long long x = tt_mul2(tt_add2(tt_two(__uint_as_float(u[j]), __uint_as_float(u[j + 1])), v.x),
+                                                 tt_two(p[c + j], p[c + j + 1]));
+            const unsigned long long y = tt_mul2(tt_add2(tt_two(__uint_as_float(u[j + 2]), __uint_as_float(u[j + 3])), v.y),
+                                                 tt_two(p[c + j + 2], p[c + j + 3]));
+            w[j >> 1] = tt_pack(tt_lo(x), tt_hi(x));
+            w[(j >> 1) + 1] = tt_pack(tt_lo(y), tt_hi(y));
           }
+          if (!inside) {  // (a weight of zero has no part even where the other factor is not finite)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const int at_lo = c + 2 * j, at_hi = at_lo + 1;
+              w[j] &= (at_lo < c_lo || at_lo >= c_end ? 0u : 0xffffu) | (at_hi < c_lo || at_hi >= c_end ? 0u : 0xffff0000u);
+            }
+          }
+          tc_st16(tmem_dp + lanes + (unsigned)(half * 64 + (c >> 1)), w);
         }
-        tc_st16(tmem_dp + lanes + (unsigned)(half * 64 + (c >> 1)), w);
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(ready(2 * g + 1));
       }
-      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mbar_arrive(ds_ready);
+      const Item then = x;
+      block = next.take(w, lane);
+      if (block >= 0) x = item(block);
+      if (ok) ok = mbar_wait_warp(done, (unsigned)n++ & 1u, abort_flag, nullptr, 90);
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      ok = __all_sync(0xffffffffu, ok && !*abort_flag);
+      const HeadView &o = half ? a.o2 : a.o1;  // one half of the warps stores dk, the other dv
+      bf16 *row = reinterpret_cast<bf16 *>(o.p) + then.at.stream * o.s + (long long)key * o.r + then.at.head * o.h;
+      tt_store_row(row, key < a.m, a, (half ? tmem_dv : tmem_dk) + lanes, 0, (a.dim + 15) & ~15, half ? 1.f : a.scale, false, ok);
     }
-    if (ok && tiles > 0) ok = mbar_wait_warp(done, 0, abort_flag, nullptr, 90);
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const HeadView &o = half ? a.o2 : a.o1;  // one half of the warps stores dk, the other dv
-    bf16 *row = reinterpret_cast<bf16 *>(o.p) + at.stream * o.s + (long long)key * o.r + at.head * o.h;
-    tt_store_row(row, key < a.m, a, (half ? tmem_dv : tmem_dk) + lanes, 0, (a.dim + 15) & ~15, half ? 1.f : a.scale, tiles == 0,
-                 __all_sync(0xffffffffu, ok && !*abort_flag));
   }
   __syncwarp();
   pdl_launch_dependents();
@@ -808,7 +900,7 @@ train_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
   __syncthreads();
   if (warp == 1) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_s), "r"(512u));
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
   }
 }
 
@@ -839,7 +931,7 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
   const unsigned s_full = bars + 224, s_free = bars + 232, done = bars + 240;
   volatile unsigned *tmem_holder = reinterpret_cast<volatile unsigned *>(base_ptr + L::BAR_OFF + 248);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(base_ptr + L::BAR_OFF + 252);
-  const TtNext next{bars + 256u};
+  TtNext next{bars + 256u};
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -890,11 +982,19 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     int g = 0, n = 0, a_loads = 0, b_loads = 0;  // tiles of keys so far, items with any, loads issued
     bool ok = true;
     int block = (int)blockIdx.x;
-    for (int w = 0; block >= 0; ++w) {
-      const bool more = next.ask(w, lane);
-      const Item x = item(block);
+    for (int w = 0;; ++w) {
+      Item x = item(max(block, 0));
+      while (block >= 0 && x.tiles == 0) {
+        tt_store_zeros(a.o1, a, x.at, x.r0, a.n, lane);
+        next.ask(lane);
+        block = next.answer();
+        x = item(max(block, 0));
+      }
+      next.push(w, block, lane);
+      if (block < 0) break;
+      bool asked = false;
       const int kh = x.at.head / a.share, sq = n % L::NQ;
-      if (x.tiles > 0 && ok) {
+      if (ok) {
         ok = mbar_wait_warp(q_empty(sq), ((unsigned)(n / L::NQ) & 1u) ^ 1u, abort_flag, nullptr, 91);
         if (ok && lane == 0) {
           mbar_expect_tx(q_full(sq), 2u * TILE);
@@ -916,6 +1016,10 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         }
         ++a_loads;
         __syncwarp();
+        if (i + 1 == x.tiles) {
+          next.ask(lane);
+          asked = true;
+        }
         ok = mbar_wait_warp(b_empty(sb), ((unsigned)(g / L::NB) & 1u) ^ 1u, abort_flag, nullptr, 91);
         if (!ok) break;
         if (lane == 0) {
@@ -925,7 +1029,8 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         ++b_loads;
         __syncwarp();
       }
-      block = more ? next.take(w, lane, false) : -1;
+      if (!asked) next.ask(lane);
+      block = next.answer();
     }
     if (*abort_flag) {  // copies in flight must land before the shared memory goes away
       const unsigned long long limit = global_timer() + WAIT_LIMIT_NS;
@@ -947,23 +1052,18 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       int i, g, n;  // tile of the item, of all; item
     };
     int w = 0;
-    Job lead{item((int)blockIdx.x), -1, -1, -1};
+    Job lead{};
+    lead.i = lead.g = lead.n = -1;
     auto advance = [&]() {  // the next tile; false: none
       ++lead.g;
-      if (++lead.i < lead.x.tiles) {
-        if (lead.i == 0) ++lead.n;
-        return true;
-      }
-      while (true) {
-        const int block = next.take(w++, lane, true);
-        if (block < 0) return false;
-        lead.x = item(block);
-        lead.i = 0;
-        if (lead.x.tiles > 0) {
-          ++lead.n;
-          return true;
-        }
-      }
+      if (++lead.i < lead.x.tiles) return true;
+      const int block = next.take(w++, lane);
+      if (block < 0) return false;
+      lead.x = item(block);
+      lead.x.tiles = tt_uniform(lead.x.tiles);
+      lead.i = 0;
+      ++lead.n;
+      return true;
     };
     auto issue = [&](const Job &t) {
       const int sa = t.g % L::NA, sb = t.g % L::NB, sq = t.n % L::NQ;
@@ -1007,7 +1107,7 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       __syncwarp();
     }
     if (!ok) {  // a bounded chance for the tensor pipe to finish before tensor memory is freed; the items' order goes on
-      while (more) more = next.take(w++, lane, true) >= 0;
+      while (more) more = next.take(w++, lane) >= 0;
       if (tc_elect()) tc_commit(next.drained());
       __syncwarp();
       const unsigned long long limit = global_timer() + WAIT_LIMIT_NS;
@@ -1041,7 +1141,8 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       ++exact;
       return met ? both[0] + both[128] : NAN;
     };
-    Item x = item((int)blockIdx.x);
+    int block = next.take(0, lane);
+    Item x = item(max(block, 0));
     auto statistics = [&](float &z, float &delta) {
       const int row = x.r0 + q * 32 + lane;
       const long long at = ((long long)x.at.stream * a.heads + x.at.head) * a.n + row;
@@ -1050,7 +1151,7 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     };
     float z, delta;
     statistics(z, delta);
-    for (int w = 0;; ++w) {
+    for (int w = 1; block >= 0; ++w) {
       const int row = x.r0 + q * 32 + lane;
       const int row_lo = a.span.lo(row), row_end = a.span.end(row, x.at.keys);
       const int warp_lo = a.span.lo(x.r0 + q * 32 + 31), warp_end = a.span.end(x.r0 + q * 32, x.at.keys);
@@ -1121,17 +1222,16 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       }
       // the next item's statistics are on their way while this one's rows are stored
       const Item then = x;
-      const int block = next.take(w, lane, true);
+      block = next.take(w, lane);
       if (block >= 0) {
         x = item(block);
         statistics(z, delta);
       }
-      if (ok && then.tiles > 0) ok = mbar_wait_warp(done, (unsigned)n++ & 1u, abort_flag, nullptr, 98);
+      if (ok) ok = mbar_wait_warp(done, (unsigned)n++ & 1u, abort_flag, nullptr, 98);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       bf16 *o = reinterpret_cast<bf16 *>(a.o1.p) + then.at.stream * a.o1.s + (long long)row * a.o1.r + then.at.head * a.o1.h;
       ok = __all_sync(0xffffffffu, ok && !*abort_flag);
-      tt_store_row(o, row < a.n, a, tmem_dq + lanes, half ? mid : 0, half ? cols : mid, a.scale, then.tiles == 0, ok);
-      if (block < 0) break;
+      tt_store_row(o, row < a.n, a, tmem_dq + lanes, half ? mid : 0, half ? cols : mid, a.scale, false, ok);
     }
   }
   __syncwarp();

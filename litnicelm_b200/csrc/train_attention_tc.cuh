@@ -84,46 +84,50 @@ __device__ __forceinline__ TtPlace tt_place(const TtArgs &a, int heads, bool las
   return tt_place(a, heads, last_first, ctas, (int)blockIdx.x);
 }
 
-// Blocks that have not started, taken over by running ones (cluster launch control): a block's warps go on with the next tile of
-// rows while its last results are on their way, nothing is set up again, and whoever is free first takes the next. Warp 0 asks one
-// block ahead, `readers` warps and itself take the answers. Two answers' places; 64 bytes of shared memory from `at` on: answers,
-// their barriers, the barrier of a CTA that gave up.
+// A value that all lanes have, known as such to the compiler: what is computed from it stays in uniform registers.
+__device__ __forceinline__ int tt_uniform(int x) { return __reduce_max_sync(0xffffffffu, x); }
+
+// Blocks that have not started, taken over by running ones (cluster launch control): a block's warps go on with the next tile while
+// its last results are on their way, nothing is set up again, and whoever is free first takes the next. Warp 0 asks, with the last
+// loads of a block (sooner, and others would be free for it first), and passes the blocks that have work on to `readers` warps, in two
+// places in turn; what a block without work leaves it does itself, so a reader that is one or two blocks ahead of the others
+// never waits for them. 72 bytes of shared memory from `at` on.
 struct TtNext {
   unsigned at;
+  int asks = 0;
+  __device__ __forceinline__ unsigned got() const { return at + 24u; }
   __device__ __forceinline__ unsigned full(int w) const { return at + 32u + 8u * (w & 1); }
   __device__ __forceinline__ unsigned empty(int w) const { return at + 48u + 8u * (w & 1); }
-  __device__ __forceinline__ unsigned drained() const { return at + 64u; }
+  __device__ __forceinline__ unsigned drained() const { return at + 64u; }  // of a CTA that gave up
   __device__ __forceinline__ void init(int readers) const {
     for (int w = 0; w < 2; ++w) {
       mbar_init(full(w), 1);
       mbar_init(empty(w), readers);
     }
+    mbar_init(got(), 1);
     mbar_init(drained(), 1);
   }
   // These waits go on in a CTA that gave up on another: each block that it has taken gets its results, if only NaN.
   static __device__ __forceinline__ bool wait(unsigned bar, unsigned parity) {
+    bool ok = true;
     if (!mbar_try_wait(bar, parity)) {
       const unsigned long long limit = global_timer() + 16 * WAIT_LIMIT_NS;
-      while (!mbar_try_wait(bar, parity))
-        if (global_timer() > limit) return false;
+      while (ok && !mbar_try_wait(bar, parity)) ok = global_timer() < limit;
     }
-    return true;
+    return __all_sync(0xffffffffu, ok);
   }
-  // Asks for the block behind the w-th. Not after an answer of none.
-  __device__ __forceinline__ bool ask(int w, int lane) const {
-    if (!__all_sync(0xffffffffu, w < 2 || wait(empty(w), ((unsigned)(w >> 1) & 1u) ^ 1u))) return false;
+  // Not again after an answer of none.
+  __device__ __forceinline__ void ask(int lane) const {
     if (lane == 0) {
-      mbar_expect_tx(full(w), 16u);
-      asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(at + 16u * (w & 1)),
-                   "r"(full(w))
+      mbar_expect_tx(got(), 16u);
+      asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(at), "r"(got())
                    : "memory");
     }
     __syncwarp();
-    return true;
   }
-  // The block behind the w-th, or -1.
-  __device__ __forceinline__ int take(int w, int lane, bool reader) const {
-    if (!__all_sync(0xffffffffu, wait(full(w), (unsigned)(w >> 1) & 1u))) return -1;
+  // The block asked for, or -1.
+  __device__ __forceinline__ int answer() {
+    if (!wait(got(), (unsigned)asks++ & 1u)) return -1;
     unsigned some, block;
     asm volatile(
         "{\n\t.reg .pred p;\n\t.reg .b128 r;\n\t"
@@ -132,12 +136,28 @@ struct TtNext {
         "selp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
         "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n\t}"
         : "=r"(some), "=r"(block)
-        : "r"(at + 16u * (w & 1))
+        : "r"(at)
         : "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
-    if (reader && lane == 0) mbar_arrive(empty(w));
-    return some ? (int)block : -1;
+    return tt_uniform(some ? (int)block : -1);
+  }
+  // The w-th block with work (or -1, the end) for the readers.
+  __device__ __forceinline__ void push(int w, int block, int lane) const {
+    if (!wait(empty(w), ((unsigned)(w >> 1) & 1u) ^ 1u)) return;
+    if (lane == 0) {
+      asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + 16u + 4u * (w & 1)), "r"(block) : "memory");
+      mbar_arrive(full(w));
+    }
+    __syncwarp();
+  }
+  __device__ __forceinline__ int take(int w, int lane) const {
+    if (!wait(full(w), (unsigned)(w >> 1) & 1u)) return -1;
+    int block;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(block) : "r"(at + 16u + 4u * (w & 1)) : "memory");
+    __syncwarp();
+    if (lane == 0) mbar_arrive(empty(w));
+    return tt_uniform(block);
   }
 };
 

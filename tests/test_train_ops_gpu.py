@@ -84,6 +84,20 @@ def test_attention_long(dtype, n, m, dim, lengths, opts):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("dim", [48, 128])
+@pytest.mark.parametrize("opts", [dict(), dict(causal=False), dict(window=60), dict(first=300)], ids=str)
+def test_attention_many_tiles(dtype, dim, opts):
+    """More tiles than a GPU has multiprocessors, many of them without work, in runs and between others."""
+    lengths = [300, 0, 0, 0, 0, 129, 1, 0, 300, 128, 0, 64, 0, 0, 257, 300, 2, 0, 300, 0, 0, 0, 0, 0]
+    attention_case(dtype, 24, 300, 300, 8, 4, dim, lengths=lengths, **opts)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_attention_no_work(dtype):
+    attention_case(dtype, 40, 130, 130, 8, 8, 64, lengths=[0] * 40)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("dim", [64, 128])
 def test_attention_hidden_lowest_values(dtype, dim):
     """The type's lowest value in keys and values that the span hides from every row."""
