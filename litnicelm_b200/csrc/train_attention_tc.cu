@@ -966,7 +966,7 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
 
   struct Item {
     TtPlace at;
-    int r0, lo, tiles;
+    int r0, lo, tiles, ahead;  // ahead: tiles of a first pass, over the same keys
   };
   auto item = [&](int block) {
     Item x;
@@ -975,6 +975,7 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     x.lo = a.span.lo(x.r0);
     const int end = a.span.end(min(x.r0 + TT_B, a.n) - 1, x.at.keys);
     x.tiles = end > x.lo ? (end - x.lo + TT_B - 1) / TT_B : 0;
+    x.ahead = x.tiles == 2 && a.span.window > 0 && a.span.window <= TT_B ? 2 : 0;
     return x;
   };
 
@@ -1006,8 +1007,9 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         if (ok) ++n;
         __syncwarp();
       }
-      for (int i = 0; i < x.tiles && ok; ++i, ++g) {
-        const int sa = g % L::NA, sb = g % L::NB, j0 = x.lo + i * TT_B;
+      const int jobs = x.ahead + x.tiles;
+      for (int i = 0; i < jobs && ok; ++i, ++g) {
+        const int sa = g % L::NA, sb = g % L::NB, j0 = x.lo + (i >= x.ahead ? i - x.ahead : i) * TT_B;
         ok = mbar_wait_warp(a_empty(sa), ((unsigned)(g / L::NA) & 1u) ^ 1u, abort_flag, nullptr, 91);
         if (!ok) break;
         if (lane == 0) {
@@ -1016,7 +1018,7 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         }
         ++a_loads;
         __syncwarp();
-        if (i + 1 == x.tiles) {
+        if (i + 1 == jobs) {
           next.ask(lane);
           asked = true;
         }
@@ -1056,11 +1058,12 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     lead.i = lead.g = lead.n = -1;
     auto advance = [&]() {  // the next tile; false: none
       ++lead.g;
-      if (++lead.i < lead.x.tiles) return true;
+      if (++lead.i < lead.x.tiles + lead.x.ahead) return true;
       const int block = next.take(w++, lane);
       if (block < 0) return false;
       lead.x = item(block);
       lead.x.tiles = tt_uniform(lead.x.tiles);
+      lead.x.ahead = tt_uniform(lead.x.ahead);
       lead.i = 0;
       ++lead.n;
       return true;
@@ -1071,7 +1074,7 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       if (t.i == 0 && !mbar_wait_warp(q_full(sq), (unsigned)(t.n / L::NQ) & 1u, abort_flag, nullptr, 93)) return false;
       if (!mbar_wait_warp(a_full(sa), (unsigned)(t.g / L::NA) & 1u, abort_flag, nullptr, 92)) return false;
       // keys behind the stream's length must not meet the zeros of dS as anything but zeros
-      const int have = t.x.at.keys - (t.x.lo + t.i * TT_B);
+      const int have = t.x.at.keys - (t.x.lo + (t.i >= t.x.ahead ? t.i - t.x.ahead : t.i) * TT_B);
       if (have < TT_B && t.x.at.keys < a.m) tt_clear_rows(base_ptr + (k_tile(sa) - base), SLABS, have, lane);
       if (t.g > 0 && !mbar_wait_warp(s_free, (unsigned)(t.g - 1) & 1u, abort_flag, nullptr, 94)) return false;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -1085,7 +1088,7 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         tt_mma_rows<D>(tmem_dp0 + (unsigned)((t.g & 1) * 128), q_at + (unsigned long long)(TILE >> 4), v_rows + stage(sb), idesc_s);
         tc_commit(dp_full(t.g));
         tc_commit(b_empty(sb));
-        if (t.i + 1 == t.x.tiles) tc_commit(q_empty(sq));
+        if (t.i + 1 == t.x.ahead + t.x.tiles) tc_commit(q_empty(sq));
       }
       __syncwarp();
       return true;
@@ -1100,9 +1103,10 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       if (tc_elect()) {
-        tt_mma_weights<true>(tmem_dq, tmem_dp0 + (unsigned)((now.g & 1) * 128), k_cols + stage(now.g % L::NA), idesc_d, now.i > 0);
+        if (now.i >= now.x.ahead)
+          tt_mma_weights<true>(tmem_dq, tmem_dp0 + (unsigned)((now.g & 1) * 128), k_cols + stage(now.g % L::NA), idesc_d, now.i > now.x.ahead);
         tc_commit(a_empty(now.g % L::NA));
-        if (now.i + 1 == now.x.tiles) tc_commit(done);
+        if (now.i + 1 == now.x.ahead + now.x.tiles) tc_commit(done);
       }
       __syncwarp();
     }
@@ -1119,9 +1123,11 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     const int cols = (a.dim + 15) & ~15, mid = (cols / 2 + 15) & ~15;  // each half of the warps stores half of the columns
     int g = 0, n = 0, exact = 0;
     bool ok = true;
-    // dout . out is off by what out was rounded by, which counts in rows of few keys. Where all of a row's keys lie in this one
-    // tile, the same sum over keys, p dP, is at hand in 32 bits (the kernel of dk and dv then finds it in place of the other).
-    auto exact_delta = [&](const float (&p)[64], unsigned tmem_dp, int c_lo, int c_end) {
+    // dout . out is off by what out was rounded by, which counts in rows of few keys (a window of 12: dq and dk half again as far from
+    // 64 bits as their own rounding leaves them). Where all of a row's keys lie in this one tile, the same sum over keys, p dP, is
+    // at hand in 32 bits; under a narrow window, whose keys lie in two, a first pass over both takes it. (The kernel of dk and dv
+    // then finds it in place of the other.)
+    auto exact_part = [&](const float (&p)[64], unsigned tmem_dp, int c_lo, int c_end) {
       float t = 0.f;
 #pragma unroll
       for (int c = 0; c < 64; c += 32) {
@@ -1132,9 +1138,12 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         for (int j = 0; j < 32; ++j)
           if (c + j >= c_lo && c + j < c_end) t = fmaf(p[c + j], __uint_as_float(u[j]), t);
       }
+      return t;
+    };
+    auto exact_delta = [&](float part) {
       // (of two places in turn: the other half has read this one's before it arrives for the next)
       float *both = stat + (exact & 1) * 256 + q * 32 + lane;
-      both[half * 128] = t;
+      both[half * 128] = part;
       __syncwarp();
       if (lane == 0) mbar_arrive(halves(q));
       const bool met = mbar_wait_warp(halves(q), (unsigned)exact & 1u, abort_flag, nullptr, 99);
@@ -1156,8 +1165,9 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       const int row_lo = a.span.lo(row), row_end = a.span.end(row, x.at.keys);
       const int warp_lo = a.span.lo(x.r0 + q * 32 + 31), warp_end = a.span.end(x.r0 + q * 32, x.at.keys);
       const float lse = z == -INFINITY ? -INFINITY : -(z * TT_LOG2E);  // to add; a row that sees no key has no weights: 2^(s - infinity)
-      for (int i = 0; i < x.tiles && ok; ++i, ++g) {
-        const int j0 = x.lo + i * TT_B + half * 64;
+      float part = 0.f;
+      for (int i = -x.ahead; i < x.tiles && ok; ++i, ++g) {
+        const int j0 = x.lo + (i < 0 ? i + x.ahead : i) * TT_B + half * 64;
         const unsigned tmem_dp = tmem_dp0 + (unsigned)((g & 1) * 128);
         const int c_lo = row_lo - j0, c_end = row_end - j0;
         const bool inside = warp_lo <= j0 && warp_end >= j0 + 64;
@@ -1189,9 +1199,18 @@ train_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
           for (int j = 0; j < 64; ++j)
             if (j < c_lo || j >= c_end) p[j] = 0.f;
         }
-        if (x.tiles == 1) {
-          delta = exact_delta(p, tmem_dp, c_lo, c_end);
-          if (half == 0 && row < a.n) a.delta[((long long)x.at.stream * a.heads + x.at.head) * a.n + row] = delta;
+        if (i < 0 || x.tiles == 1) {
+          part += exact_part(p, tmem_dp, c_lo, c_end);
+          if (i == -1 || x.tiles == 1) {
+            delta = exact_delta(part);
+            if (half == 0 && row < a.n) a.delta[((long long)x.at.stream * a.heads + x.at.head) * a.n + row] = delta;
+          }
+        }
+        if (i < 0) {
+          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) mbar_arrive(ds_ready(g));
+          continue;
         }
 #pragma unroll
         for (int c = 0; c < 64; c += 32) {

@@ -92,6 +92,26 @@ def test_attention_many_tiles(dtype, dim, opts):
     attention_case(dtype, 24, 300, 300, 8, 4, dim, lengths=lengths, **opts)
 
 
+@pytest.mark.parametrize("dim", [40, 64, 128])
+def test_attention_rows_of_one_key(dim):
+    """Their weights are 1 whatever the scores: gradients of q and k are what 32-bit sums leave of nothing, however out was rounded.
+
+    ds = scale p (dp - delta), delta = p dp: sums of dim products in two orders, each off by 2 dim u of the sum of magnitudes,
+    and weights that are off by the score's error, twice (in lse too), and a few u."""
+    g = gen(7)
+    q, k, v = fused(g, 2, 300, 300, 4, 2, dim, BF16)
+    dout = rand(g, 2, 300, 4, dim, dtype=BF16)
+    out, lse = training.attention_forward(q, k, v, window=1)
+    dq, dk, _ = training.attention_backward(dout, q, k, v, out, lse, window=1)
+    u, scale = 2.0 ** -24, dim ** -0.5
+    Q, D, K, V = q.double(), dout.double(), k.double().repeat_interleave(2, 2), v.double().repeat_interleave(2, 2)
+    score, dp = (Q.abs() * K.abs()).sum(-1) * scale, (D.abs() * V.abs()).sum(-1)
+    ds = scale * dp * (2 * 2 * dim * u + 2 * (2 * (dim + 4) * u * score + 16 * u + 8 * u * lse.transpose(1, 2).double().abs()))
+    up = 1 + 2.0 ** -7  # to bfloat16, of ds and of the result
+    assert bool((dq.double().abs() <= ds[..., None] * K.abs() * up + 1e-37).all())
+    assert bool((dk.double().abs() <= (ds[..., None] * Q.abs()).view(2, 300, 2, 2, dim).sum(3) * up + 1e-37).all())
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_attention_no_work(dtype):
     attention_case(dtype, 40, 130, 130, 8, 8, 64, lengths=[0] * 40)
