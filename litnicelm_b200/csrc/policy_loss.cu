@@ -10,8 +10,8 @@
 // written once. A warp takes a row of up to 1024 columns, 128, 256 or 512 threads with 64 elements each take longer ones. Beyond,
 // 512 threads read the row twice, the second time from L2 (two blocks an SM, so that their rows fit there). Row losses are summed in
 // row order in 64 bits, so the loss does not depend on the order in which blocks finish.
-// Bound: HBM, one read of the logits and one write of the gradient. 4096 x 32000 in 32 bits, three in ten rows masked: see the
-// launcher.
+// Bound: HBM, one read of the logits and one write of the gradient. 4096 x 32000 in 32 bits, three in ten rows masked: 151 us for the rows'
+// kernel (6.1 TB/s), 8 us around it; 4093 x 32000 in bfloat16: 87 us.
 #include "train_ops.cuh"
 #include "gemm_tc.cuh"
 #include "tc_ptx.cuh"
@@ -284,7 +284,7 @@ policy_row_kernel(const __grid_constant__ PolicyLoss a, PlWork w, PlForms f) {
 // The same for rows of 8193 to 32768 columns on 16-byte boundaries, by blocks that walk rows and bring the next one into shared memory while
 // they work on one. 32 bits: a block of 1024 threads per SM, 32 exponentials to a thread in registers. bfloat16: two blocks of 512 per SM,
 // whose phases overlap, with 64 elements to a thread as they are (32 registers; the exponentials are taken twice). 4093 x 32000 in bfloat16:
-// 120 us the first way, see the launcher for the second.
+// 120 us the first way, 87 us the second.
 template <typename T>
 struct PlStream;
 template <>

@@ -1,4 +1,5 @@
-// Attention with its backward pass for training in 32 bits on the sm_100a tensor cores. The mathematics is that of train_attention.cu, the division of work that of train_attention_tc.cu.
+// Attention with its backward pass for training in 32 bits on the sm_100a tensor cores. The mathematics is that of train_attention.cu, the
+// division of work that of train_attention_tc.cu.
 //
 // Operands are in three bfloat16 parts, x = x0 + x1 + x2, each the part before it left over: all 24 bits of a finite x. A product
 // is the six of parts whose terms count, smallest first: (0,2) (2,0) (1,1) (0,1) (1,0) (0,0); what is left out is below 2^-23 of a
@@ -11,6 +12,10 @@
 // Heads of more than 64 dimensions (H = 2): a tile's parts are 96 KB, and two tiles of products do not fit beside two resident ones. A
 // CTA then makes 64 of the result's dimensions, and its products' operands come in units of 64 dimensions through four places of shared
 // memory, all four together where a sum runs over all dimensions (small parts first there too).
+//
+// Bound: at the sizes that such models train at, latency: 8 streams of 250 rows, 8 heads of 64 take 67 us forward and backward (split 2 x 9,
+// forward 14, dk and dv 27, dq 27 us) with 128 CTAs of four products' dependent stages each; with 32-bit products on the FMA
+// pipe it was 219 us. 2000 rows of 8 heads of 128: 419 us, 1957 that way; the six products are 100 us of it at the pipe's rate.
 //
 // A CTA: warp 0 issues TMA, warp 1 owns tensor memory and issues the MMAs, eight warps (a thread: a row or key, half of the
 // tile's columns, half of the dimensions of a sum). Every wait is bounded; one that runs out ends the CTA, whose results are then NaN.

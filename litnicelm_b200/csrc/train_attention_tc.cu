@@ -4,13 +4,24 @@
 // forward   one CTA per 128 rows of a head walks the tiles of 128 keys they see: S = Q K^T, four warps (a thread: a row) turn S
 //           into weights 2^(s - m), stored as bfloat16 over the scores' own columns of tensor memory, O += P V from there. The
 //           reference m follows a row's maximum only where that has grown by more than 2^8, so most tiles need no pass over O.
-//           Two CTAs share an SM: one's products run under the other's softmax.
+//           Two CTAs share an SM: one's products run under the other's softmax. Long rows of up to 64 dimensions: one CTA with two
+//           tiles of rows instead.
 // dk, dv    one CTA per 128 keys of a key head walks the tiles of 128 rows that see them, through all query heads that share it:
 //           S^T = K Q^T, dP^T = V dO^T; eight warps (a thread: a key and half of the rows) make P^T and then dS^T = P^T (dP^T -
 //           delta), each over its source's columns; dV += P^T dO and dK += dS^T Q with A from tensor memory and B as it lies in
 //           shared memory, rows of k. While the warps work on P the pipe multiplies for dS of the tile before, and the
-//           other way round: dV(i), S(i+1) | dK(i), dP(i+1).
-// dq        one CTA per 128 rows of a head in the same way: S = Q K^T, dP = dO V^T, dQ += dS K.
+//           other way round: dV(i), S(i+1) | dK(i), dP(i+1); at 64 dimensions a third tile fits into tensor memory, and each product
+//           for the warps is issued one step sooner.
+// dq        one CTA per 128 rows of a head in the same way: S = Q K^T, dP = dO V^T, dQ += dS K, with two places for dP.
+// The two backward kernels stay on their SM: a CTA takes over blocks that have not started (TtNext), so that the next tile's operands
+// and first products arrive under the last one's results.
+//
+// Bound, 4 streams of 2048 rows, 16 heads of 64, causal (forward 75, delta 12, dq 82, dk and dv 108 us): the exponentials, 16 a clock and
+// SM, are 32 us of each kernel, the products 24 us of the forward, 32 of dq, 48 of dk and dv (those into 64 columns take as long as into
+// 128); a tile's stages - product, softmax, product - wait for one another, and what two tiles in flight do not hide is the
+// rest. 8192 rows of 16 heads of 128 on 4 key heads (forward 253, dq 320, dk and dv 450 us): 121 us of exponentials, products of
+// 121, 182 and 242 us; the largest of the 256 blocks for dk and dv holds 256 of the 225 tiles that an SM
+// has on average.
 // The scores are computed once for each, so that no sum depends on the order in which CTAs finish.
 //
 // Rounding to bfloat16: P and dS for their products (the tensor cores take both operands of one type), relative 2^-8 a term,
@@ -320,11 +331,12 @@ train_forward_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
 }
 
 // The same for heads of up to 64 dimensions and more than 128 rows: one CTA per SM takes two tiles of 128 rows, A and B, with four warps
-// each, and walks the tiles of keys once for both. Tensor memory holds three tiles of scores and two accumulators: jobs A0 B0 A1 B1 ..
-// take the scores' places in turn, S of the third job ahead is issued behind a job's own P V, so a group's next scores are there when
-// it has finished with the last ones. (With two CTAs of one tile a group waited 1000 of its 3400 clocks a tile for them.)
+// each, and walks the tiles of keys once for both. Tensor memory holds a tile of scores, its weights and an accumulator for each, so that
+// a group's next scores are made as soon as its warps have the last ones in registers, and are there before it has finished with
+// those. (With two CTAs of one tile, weights over the scores, a group waited 1000 of its 3400 clocks a tile for them; with three
+// places that jobs A0 B0 A1 B1 .. took in turn, each waited for the other's product.) Blocks go on with the next rows (TtNext).
 constexpr int TT_PAIR_STAGES = 4;
-constexpr int TT_PAIR_BAR = (2 + 2 * TT_PAIR_STAGES) * TT_SLAB, TT_PAIR_SMEM = TT_PAIR_BAR + 256 + 1024;
+constexpr int TT_PAIR_BAR = (4 + 2 * TT_PAIR_STAGES) * TT_SLAB, TT_PAIR_SMEM = TT_PAIR_BAR + 384 + 1024;
 
 __global__ void __launch_bounds__(TT_BWD_THREADS, 1)
 train_forward_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -334,44 +346,33 @@ train_forward_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
   const unsigned base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char *base_ptr = smem_raw + (base - smem_u32(smem_raw));
   const unsigned bars = base + TT_PAIR_BAR;
-  auto k_tile = [&](int s) { return base + (unsigned)((2 + s) * TT_SLAB); };
-  auto v_tile = [&](int s) { return base + (unsigned)((2 + NS + s) * TT_SLAB); };
+  auto q_tile = [&](int s) { return base + (unsigned)(s * 2 * TT_SLAB); };  // of A, and of B behind it
+  auto k_tile = [&](int s) { return base + (unsigned)((4 + s) * TT_SLAB); };
+  auto v_tile = [&](int s) { return base + (unsigned)((4 + NS + s) * TT_SLAB); };
   auto k_full = [&](int s) { return bars + 8u * s; };
   auto k_empty = [&](int s) { return bars + 32u + 8u * s; };
   auto v_full = [&](int s) { return bars + 64u + 8u * s; };
   auto v_empty = [&](int s) { return bars + 96u + 8u * s; };
-  auto s_full = [&](int place) { return bars + 128u + 8u * place; };
-  auto p_ready = [&](int place) { return bars + 152u + 8u * place; };
+  auto s_full = [&](int group) { return bars + 128u + 8u * group; };
+  auto s_read = [&](int group) { return bars + 144u + 8u * group; };
+  auto p_ready = [&](int group) { return bars + 160u + 8u * group; };
   auto o_full = [&](int group) { return bars + 176u + 8u * group; };
-  const unsigned q_full = bars + 192;
-  volatile unsigned *tmem_holder = reinterpret_cast<volatile unsigned *>(base_ptr + TT_PAIR_BAR + 208);
-  volatile int *abort_flag = reinterpret_cast<volatile int *>(base_ptr + TT_PAIR_BAR + 212);
+  auto q_full = [&](int s) { return bars + 192u + 8u * s; };
+  auto q_empty = [&](int s) { return bars + 208u + 8u * s; };
+  volatile unsigned *tmem_holder = reinterpret_cast<volatile unsigned *>(base_ptr + TT_PAIR_BAR + 224);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(base_ptr + TT_PAIR_BAR + 228);
+  TtNext next{bars + 256u};
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const TtPlace at = tt_place(a, a.heads, a.span.causal != 0);
-  const int r0 = at.tile * 2 * TT_B, kh = at.head / a.share;
-  const int lo = a.span.lo(r0);
-  auto tiles_of = [&](int group) {
-    const int first = r0 + group * TT_B, last = min(first + TT_B, a.n) - 1;
-    const int end = first < a.n ? a.span.end(last, at.keys) : 0;
-    return end > lo ? (end - lo + TT_B - 1) / TT_B : 0;
-  };
-  // B sees no fewer keys than A, or its rows do not exist: 2 both jobs alternate, the others are of one group
-  const int tiles_a = tiles_of(0), tiles_b = tiles_of(1), both = min(tiles_a, tiles_b), tiles = max(tiles_a, tiles_b);
-  const int jobs = tiles_a + tiles_b;
-  auto tile_of = [&](int job) { return job < 2 * both ? job >> 1 : job - both; };
-  auto group_of = [&](int job) { return job < 2 * both ? job & 1 : tiles_b > tiles_a ? 1 : 0; };
-  auto last_of_tile = [&](int job) { return job >= 2 * both || (job & 1); };
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < NS; ++s)
       for (unsigned bar : {k_full(s), k_empty(s), v_full(s), v_empty(s)}) mbar_init(bar, 1);
-    for (int s = 0; s < 3; ++s) {
-      mbar_init(s_full(s), 1);
+    for (int s = 0; s < 2; ++s) {
+      for (unsigned bar : {s_full(s), o_full(s), q_full(s), q_empty(s)}) mbar_init(bar, 1);
+      mbar_init(s_read(s), 4);
       mbar_init(p_ready(s), 4);
     }
-    mbar_init(o_full(0), 1);
-    mbar_init(o_full(1), 1);
-    mbar_init(q_full, 1);
+    next.init(9);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -382,146 +383,234 @@ train_forward_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const unsigned tmem = *tmem_holder;
 
+  struct Item {
+    TtPlace at;
+    int r0, lo, tiles_a, tiles_b;
+    __device__ int tiles() const { return max(tiles_a, tiles_b); }
+  };
+  auto item = [&](int block) {
+    Item x;
+    x.at = tt_place(a, a.heads, a.span.causal != 0, 1, block);
+    x.r0 = x.at.tile * 2 * TT_B;
+    x.lo = a.span.lo(x.r0);
+    auto tiles_of = [&](int first) {
+      const int end = first < a.n ? a.span.end(min(first + TT_B, a.n) - 1, x.at.keys) : 0;
+      return end > x.lo ? (end - x.lo + TT_B - 1) / TT_B : 0;
+    };
+    x.tiles_a = tiles_of(x.r0);
+    x.tiles_b = tiles_of(x.r0 + TT_B);
+    return x;
+  };
+
   if (warp == 0) {
-    int it = 0;
+    int it = 0, n = 0, k_loads = 0, v_loads = 0;  // tiles of keys so far, items, loads issued
     bool ok = true;
-    if (lane == 0 && jobs > 0) {
-      mbar_expect_tx(q_full, 2u * TT_SLAB);
-      tma_load_4d(base, &map_q, 0, at.head, r0, at.stream, q_full);
-      tma_load_4d(base + TT_SLAB, &map_q, 0, at.head, r0 + TT_B, at.stream, q_full);
+    int block = (int)blockIdx.x;
+    for (int w = 0;; ++w) {
+      Item x = item(max(block, 0));
+      while (block >= 0 && x.tiles() == 0) {
+        for (int half = 0; half < 2; ++half) tt_store_zeros(a.o1, a, x.at, x.r0 + half * TT_B, a.n, lane);
+        for (int row = x.r0 + lane; row < min(x.r0 + 2 * TT_B, a.n); row += 32)
+          a.lse[((long long)x.at.stream * a.heads + x.at.head) * a.n + row] = -INFINITY;
+        next.ask(lane);
+        block = next.answer();
+        x = item(max(block, 0));
+      }
+      next.push(w, block, lane);
+      if (block < 0) break;
+      bool asked = false;
+      const int kh = x.at.head / a.share, sq = n & 1, tiles = x.tiles();
+      if (ok) {
+        ok = mbar_wait_warp(q_empty(sq), ((unsigned)(n >> 1) & 1u) ^ 1u, abort_flag, nullptr, 60);
+        if (ok && lane == 0) {
+          mbar_expect_tx(q_full(sq), 2u * TT_SLAB);
+          tma_load_4d(q_tile(sq), &map_q, 0, x.at.head, x.r0, x.at.stream, q_full(sq));
+          tma_load_4d(q_tile(sq) + TT_SLAB, &map_q, 0, x.at.head, x.r0 + TT_B, x.at.stream, q_full(sq));
+        }
+        if (ok) ++n;
+        __syncwarp();
+      }
+      for (int i = 0; i < tiles && ok; ++i, ++it) {
+        const int st = it % NS, j0 = x.lo + i * TT_B;
+        const unsigned free = ((unsigned)(it / NS) & 1u) ^ 1u;
+        ok = mbar_wait_warp(k_empty(st), free, abort_flag, nullptr, 61);
+        if (!ok) break;
+        if (lane == 0) {
+          mbar_expect_tx(k_full(st), TT_SLAB);
+          tma_load_4d(k_tile(st), &map_k, 0, kh, j0, x.at.stream, k_full(st));
+        }
+        ++k_loads;
+        __syncwarp();
+        if (i + 1 == tiles) {
+          next.ask(lane);
+          asked = true;
+        }
+        ok = mbar_wait_warp(v_empty(st), free, abort_flag, nullptr, 62);
+        if (!ok) break;
+        if (lane == 0) {
+          mbar_expect_tx(v_full(st), TT_SLAB);
+          tma_load_4d(v_tile(st), &map_v, 0, kh, j0, x.at.stream, v_full(st));
+        }
+        ++v_loads;
+        __syncwarp();
+      }
+      if (!asked) next.ask(lane);
+      block = next.answer();
     }
-    for (; it < tiles; ++it) {
-      const int st = it % NS, j0 = lo + it * TT_B;
-      ok = mbar_wait_warp(k_empty(st), ((unsigned)(it / NS) & 1u) ^ 1u, abort_flag, nullptr, 61);
-      if (!ok) break;
-      if (lane == 0) {
-        mbar_expect_tx(k_full(st), TT_SLAB);
-        tma_load_4d(k_tile(st), &map_k, 0, kh, j0, at.stream, k_full(st));
-      }
-      __syncwarp();
-      ok = mbar_wait_warp(v_empty(st), ((unsigned)(it / NS) & 1u) ^ 1u, abort_flag, nullptr, 62);
-      if (!ok) {
-        ++it;  // (its keys are on their way)
-        break;
-      }
-      if (lane == 0) {
-        mbar_expect_tx(v_full(st), TT_SLAB);
-        tma_load_4d(v_tile(st), &map_v, 0, kh, j0, at.stream, v_full(st));
-      }
-      __syncwarp();
-    }
-    if (*abort_flag && jobs > 0) {  // copies in flight must land before the shared memory goes away
+    if (*abort_flag) {  // copies in flight must land before the shared memory goes away
       const unsigned long long limit = global_timer() + WAIT_LIMIT_NS;
-      while (!mbar_try_wait(q_full, 0) && global_timer() < limit) {}
-      for (int j = it > NS ? it - NS : 0; j < it; ++j)
+      for (int j = n > 2 ? n - 2 : 0; j < n; ++j)
+        while (!mbar_try_wait(q_full(j & 1), (unsigned)(j >> 1) & 1u) && global_timer() < limit) {}
+      for (int j = k_loads > NS ? k_loads - NS : 0; j < k_loads; ++j)
         while (!mbar_try_wait(k_full(j % NS), (unsigned)(j / NS) & 1u) && global_timer() < limit) {}
-      const int v_loads = ok ? it : it - 1;
       for (int j = v_loads > NS ? v_loads - NS : 0; j < v_loads; ++j)
         while (!mbar_try_wait(v_full(j % NS), (unsigned)(j / NS) & 1u) && global_timer() < limit) {}
     }
   } else if (warp == 1) {
     const int cols = (a.dim + 15) & ~15;
-    const unsigned long long q_rows = tt_rows(base), k_rows = tt_rows(k_tile(0)), v_cols = tt_cols(v_tile(0));
+    const unsigned long long q_rows = tt_rows(q_tile(0)), k_rows = tt_rows(k_tile(0)), v_cols = tt_cols(v_tile(0));
     const unsigned idesc_s = umma_idesc_bf16(TT_B), idesc_o = umma_idesc_bf16(cols) | UMMA_B_MN_MAJOR;
-    int keys_seen = 0, values_seen = 0;
-    auto scores = [&](int job) {
-      const int i = tile_of(job), st = i % NS;
-      if (i >= keys_seen) {
-        if (!mbar_wait_warp(k_full(st), (unsigned)(i / NS) & 1u, abort_flag, nullptr, 63)) return false;
-        keys_seen = i + 1;
-      }
-      if (tc_elect()) {
-        tt_mma_rows<64>(tmem + (unsigned)(job % 3 * TT_B), q_rows + (unsigned long long)(group_of(job) * (TT_SLAB >> 4)),
-                        k_rows + (unsigned long long)(st * (TT_SLAB >> 4)), idesc_s);
-        tc_commit(s_full(job % 3));
-        if (last_of_tile(job)) tc_commit(k_empty(st));
-      }
-      __syncwarp();
+    // A tile of keys of an item, for both groups. Its S are issued a tile ahead of P V, into the next item too.
+    struct Round {
+      int i, tiles, tiles_a, tiles_b, live, g, n;  // live: keys from the first tile's start on that exist; tile of all; item
+    };
+    Round lead{};
+    lead.i = lead.g = lead.n = -1;
+    int w = 0, sent[2] = {}, added[2] = {};
+    auto advance = [&]() {
+      ++lead.g;
+      if (++lead.i < lead.tiles) return true;
+      const int block = next.take(w++, lane);
+      if (block < 0) return false;
+      const Item x = item(block);
+      lead.tiles_a = tt_uniform(x.tiles_a);
+      lead.tiles_b = tt_uniform(x.tiles_b);
+      lead.tiles = max(lead.tiles_a, lead.tiles_b);
+      lead.live = tt_uniform(x.at.keys < a.m ? x.at.keys - x.lo : 0x7fffffff);
+      lead.i = 0;
+      ++lead.n;
       return true;
     };
-    bool ok = jobs > 0 ? mbar_wait_warp(q_full, 0, abort_flag, nullptr, 64) : true;
-    for (int job = 0; job < 3 && job < jobs && ok; ++job) ok = scores(job);
-    for (int job = 0; job < jobs && ok; ++job) {
-      const int i = tile_of(job), st = i % NS;
-      if (i >= values_seen) {
-        ok = mbar_wait_warp(v_full(st), (unsigned)(i / NS) & 1u, abort_flag, nullptr, 65);
-        if (!ok) break;
-        values_seen = i + 1;
-        const int have = at.keys - (lo + i * TT_B);
-        if (have < TT_B && at.keys < a.m) tt_clear_rows(base_ptr + (v_tile(st) - base), 1, have, lane);
+    auto scores = [&](const Round &t) {
+      const int st = t.g % NS, sq = t.n & 1;
+      if (t.i == 0 && !mbar_wait_warp(q_full(sq), (unsigned)(t.n >> 1) & 1u, abort_flag, nullptr, 64)) return false;
+      if (!mbar_wait_warp(k_full(st), (unsigned)(t.g / NS) & 1u, abort_flag, nullptr, 63)) return false;
+#pragma unroll
+      for (int group = 0; group < 2; ++group) {
+        const bool last = group == 1 || t.i >= t.tiles_b;
+        if (t.i >= (group ? t.tiles_b : t.tiles_a)) continue;
+        if (sent[group] > 0 && !mbar_wait_warp(s_read(group), (unsigned)(sent[group] - 1) & 1u, abort_flag, nullptr, 70)) return false;
+        ++sent[group];
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (tc_elect()) {
+          tt_mma_rows<64>(tmem + (unsigned)(group * TT_B), q_rows + (unsigned long long)((sq * 2 + group) * (TT_SLAB >> 4)),
+                          k_rows + (unsigned long long)(st * (TT_SLAB >> 4)), idesc_s);
+          tc_commit(s_full(group));
+          if (last) tc_commit(k_empty(st));
+          if (last && t.i + 1 == t.tiles) tc_commit(q_empty(sq));
+        }
+        __syncwarp();
       }
-      ok = mbar_wait_warp(p_ready(job % 3), (unsigned)(job / 3) & 1u, abort_flag, nullptr, 66);
-      if (!ok) break;
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      if (tc_elect()) {
-        tt_mma_weights<false>(tmem + (unsigned)(3 * TT_B + group_of(job) * 64), tmem + (unsigned)(job % 3 * TT_B),
-                              v_cols + (unsigned long long)(st * (TT_SLAB >> 4)), idesc_o, i > 0);
-        tc_commit(o_full(group_of(job)));
-        if (last_of_tile(job)) tc_commit(v_empty(st));
+      return true;
+    };
+    auto values = [&](const Round &t) {
+      const int st = t.g % NS, have = t.live - t.i * TT_B;
+      if (!mbar_wait_warp(v_full(st), (unsigned)(t.g / NS) & 1u, abort_flag, nullptr, 65)) return false;
+      if (have < TT_B) tt_clear_rows(base_ptr + (v_tile(st) - base), 1, max(have, 0), lane);
+#pragma unroll
+      for (int group = 0; group < 2; ++group) {
+        const bool last = group == 1 || t.i >= t.tiles_b;
+        if (t.i >= (group ? t.tiles_b : t.tiles_a)) continue;
+        if (!mbar_wait_warp(p_ready(group), (unsigned)added[group]++ & 1u, abort_flag, nullptr, 66)) return false;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (tc_elect()) {
+          tt_mma_weights<false>(tmem + (unsigned)(384 + group * 64), tmem + (unsigned)(256 + group * 64),
+                                v_cols + (unsigned long long)(st * (TT_SLAB >> 4)), idesc_o, t.i > 0);
+          tc_commit(o_full(group));
+          if (last) tc_commit(v_empty(st));
+        }
+        __syncwarp();
       }
-      __syncwarp();
-      if (job + 3 < jobs) ok = scores(job + 3);
+      return true;
+    };
+    bool more = advance(), ok = !more || scores(lead);
+    while (more && ok) {
+      const Round now = lead;
+      more = advance();
+      ok = (!more || scores(lead)) && values(now);
     }
-    if (!ok) {  // a bounded chance for the tensor pipe to finish before tensor memory is freed
-      if (tc_elect()) tc_commit(q_full);
+    if (!ok) {  // a bounded chance for the tensor pipe to finish before tensor memory is freed; the items' order goes on
+      while (more) more = next.take(w++, lane) >= 0;
+      if (tc_elect()) tc_commit(next.drained());
       __syncwarp();
       const unsigned long long limit = global_timer() + WAIT_LIMIT_NS;
-      while (!mbar_try_wait(q_full, 1) && global_timer() < limit) {}
+      while (!mbar_try_wait(next.drained(), 0) && global_timer() < limit) {}
     }
   } else {
-    const int q = warp & 3, group = (warp - 2) >> 2, mine = group ? tiles_b : tiles_a;
-    const unsigned lanes = (unsigned)(q * 32) << 16, tmem_o = tmem + (unsigned)(3 * TT_B + group * 64) + lanes;
-    const int first = r0 + group * TT_B + q * 32, row = first + lane;
-    const int row_lo = a.span.lo(row), row_end = a.span.end(row, at.keys);
-    const int warp_lo = a.span.lo(first + 31), warp_end = a.span.end(first, at.keys);
+    const int q = warp & 3, group = (warp - 2) >> 2;
+    const unsigned lanes = (unsigned)(q * 32) << 16, tmem_s = tmem + (unsigned)(group * TT_B) + lanes,
+                   tmem_p = tmem + (unsigned)(256 + group * 64) + lanes, tmem_o = tmem + (unsigned)(384 + group * 64) + lanes;
     // a negative factor's sign goes to the scores; zero is small, so that hidden scores of -infinity stay that
     const float factor = fmaxf(fabsf(a.factor), 1e-30f);
-    float m = TT_NEG, l = 0.f;
+    int tile = 0, done = 0;  // tiles of this group so far, products of them that it has waited for
     bool ok = true;
-    for (int i = 0; i < mine && ok; ++i) {
-      const int job = i < both ? 2 * i + group : both + i, place = job % 3, j0 = lo + i * TT_B;
-      ok = mbar_wait_warp(s_full(place), (unsigned)(job / 3) & 1u, abort_flag, nullptr, 67);
-      if (!ok) break;
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const int c_lo = row_lo - j0, c_end = row_end - j0;  // keys j0 + c that this row sees
-      const bool inside = warp_lo <= j0 && warp_end >= j0 + TT_B;
-      const unsigned tmem_s = tmem + (unsigned)(place * TT_B) + lanes;
-      float s[TT_B], keep;
+    int block = next.take(0, lane);
+    for (int w = 1; block >= 0; ++w) {
+      int mine, row_lo, row_end, warp_lo, warp_end;  // keys from the first tile's start on
       {
-        unsigned(&u)[4][32] = reinterpret_cast<unsigned(&)[4][32]>(s);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tc_ld32(tmem_s + (unsigned)(c * 32), u[c]);
-        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        const Item x = item(block);
+        const int first = x.r0 + group * TT_B + q * 32;
+        mine = group ? x.tiles_b : x.tiles_a;
+        row_lo = a.span.lo(first + lane) - x.lo;
+        row_end = a.span.end(first + lane, x.at.keys) - x.lo;
+        warp_lo = a.span.lo(first + 31) - x.lo;
+        warp_end = a.span.end(first, x.at.keys) - x.lo;
       }
-      const bool grow = tt_reference(s, a, factor, inside, c_lo, c_end, m, l, keep);
-      // the product before is waited for in each tile, so that no wait is ever two phases behind: by a warp that
-      // rescales the accumulator before that, by the others behind the weights
-      const bool rescale = i > 0 && __any_sync(0xffffffffu, grow);
-      if (rescale) {
-        ok = mbar_wait_warp(o_full(group), (unsigned)(i - 1) & 1u, abort_flag, nullptr, 68);
+      float m = TT_NEG, l = 0.f;
+      for (int i = 0; i < mine && ok; ++i) {
+        const int j0 = i * TT_B;
+        ok = mbar_wait_warp(s_full(group), (unsigned)tile++ & 1u, abort_flag, nullptr, 67);
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        tt_rescale(tmem_o, a.dim, keep);
+        const int c_lo = row_lo - j0, c_end = row_end - j0;  // keys j0 + c that this row sees
+        const bool inside = warp_lo <= j0 && warp_end >= j0 + TT_B;
+        float s[TT_B], keep;
+        {
+          unsigned(&u)[4][32] = reinterpret_cast<unsigned(&)[4][32]>(s);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tc_ld32(tmem_s + (unsigned)(c * 32), u[c]);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(s_read(group));
+        const bool grow = tt_reference(s, a, factor, inside, c_lo, c_end, m, l, keep);
+        if (i > 0) {  // the product before has read the weights' place, and added to what may be rescaled
+          ok = mbar_wait_warp(o_full(group), (unsigned)done++ & 1u, abort_flag, nullptr, 68);
+          if (!ok) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          if (__any_sync(0xffffffffu, grow)) tt_rescale(tmem_o, a.dim, keep);
+        }
+        tt_weights(s, factor, m, l, tmem_p);
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_ready(group));
       }
-      tt_weights(s, factor, m, l, tmem_s);
-      if (i > 0 && !rescale) {
-        ok = mbar_wait_warp(o_full(group), (unsigned)(i - 1) & 1u, abort_flag, nullptr, 68);
-        if (!ok) break;
-      }
-      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mbar_arrive(p_ready(place));
+      asm volatile("" : "+r"(block));  // the block's place once more, instead of in registers through the loop
+      const Item x = item(block);
+      const int row = x.r0 + group * TT_B + q * 32 + lane;
+      block = next.take(w, lane);
+      if (ok && mine > 0) ok = mbar_wait_warp(o_full(group), (unsigned)done++ & 1u, abort_flag, nullptr, 69);
+      ok = __all_sync(0xffffffffu, ok && !*abort_flag);
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const bool live = row < a.n, empty = row_end <= row_lo;
+      bf16 *o = reinterpret_cast<bf16 *>(a.o1.p) + x.at.stream * a.o1.s + (long long)row * a.o1.r + x.at.head * a.o1.h;
+      tt_store_row(o, live, a, tmem_o, 0, (a.dim + 15) & ~15, empty ? 0.f : 1.0f / l, mine == 0, ok);
+      if (live)
+        a.lse[((long long)x.at.stream * a.heads + x.at.head) * a.n + row] =
+            !ok ? NAN : empty ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
     }
-    if (ok && mine > 0) ok = mbar_wait_warp(o_full(group), (unsigned)(mine - 1) & 1u, abort_flag, nullptr, 69);
-    ok = __all_sync(0xffffffffu, ok && !*abort_flag);
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const bool live = row < a.n, empty = row_end <= row_lo;
-    bf16 *o = reinterpret_cast<bf16 *>(a.o1.p) + at.stream * a.o1.s + (long long)row * a.o1.r + at.head * a.o1.h;
-    tt_store_row(o, live, a, tmem_o, 0, (a.dim + 15) & ~15, empty ? 0.f : 1.0f / l, mine == 0, ok);
-    if (live)
-      a.lse[((long long)at.stream * a.heads + at.head) * a.n + row] =
-          !ok ? NAN : empty ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
   }
   __syncwarp();
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -1345,7 +1434,7 @@ void launch_train_attention_forward_tc(const TrainAttention &a, cudaStream_t st)
   // A CTA with two tiles pays off once a row's keys are many: 4096 rows of 16 heads 80 -> 65 us, 8192 rows 228 ->
   // 203. With 2048 rows (4 streams of 16 heads) 82 and 81 us, and few keys leave its longer start and end bare: 300 rows of 64 x 8 heads 54 -> 64 us.
   const int seen = a.window > 0 && a.window < a.m ? a.window : a.m;
-  if (a.dim <= 64 && min(a.n, seen) > 2048) forward_pair(a, st);
+  if (a.dim <= 64 && min(a.n, seen) > TT_B) forward_pair(a, st);
   else if (a.dim <= 64) forward<64>(a, st);
   else forward<128>(a, st);
 }
