@@ -4,8 +4,8 @@
 // forward   one CTA per 128 rows of a head walks the tiles of 128 keys they see: S = Q K^T, four warps (a thread: a row) turn S
 //           into weights 2^(s - m), stored as bfloat16 over the scores' own columns of tensor memory, O += P V from there. The
 //           reference m follows a row's maximum only where that has grown by more than 2^8, so most tiles need no pass over O.
-//           Two CTAs share an SM: one's products run under the other's softmax. Long rows of up to 64 dimensions: one CTA with two
-//           tiles of rows instead.
+//           Two CTAs share an SM: one's products run under the other's softmax. Up to 64 dimensions one CTA with two tiles of rows
+//           and its scores, weights and sums apart in tensor memory instead.
 // dk, dv    one CTA per 128 keys of a key head walks the tiles of 128 rows that see them, through all query heads that share it:
 //           S^T = K Q^T, dP^T = V dO^T; eight warps (a thread: a key and half of the rows) make P^T and then dS^T = P^T (dP^T -
 //           delta), each over its source's columns; dV += P^T dO and dK += dS^T Q with A from tensor memory and B as it lies in
@@ -13,10 +13,10 @@
 //           other way round: dV(i), S(i+1) | dK(i), dP(i+1); at 64 dimensions a third tile fits into tensor memory, and each product
 //           for the warps is issued one step sooner.
 // dq        one CTA per 128 rows of a head in the same way: S = Q K^T, dP = dO V^T, dQ += dS K, with two places for dP.
-// The two backward kernels stay on their SM: a CTA takes over blocks that have not started (TtNext), so that the next tile's operands
-// and first products arrive under the last one's results.
+// These kernels (but the forward of 128 dimensions, whose two CTAs do that for each other) stay on their SM: a CTA takes over blocks that
+// have not started (TtNext), so that the next tile's operands and first products arrive under the last one's results.
 //
-// Bound, 4 streams of 2048 rows, 16 heads of 64, causal (forward 75, delta 12, dq 82, dk and dv 108 us): the exponentials, 16 a clock and
+// Bound, 4 streams of 2048 rows, 16 heads of 64, causal (forward 66, delta 12, dq 83, dk and dv 108 us): the exponentials, 16 a clock and
 // SM, are 32 us of each kernel, the products 24 us of the forward, 32 of dq, 48 of dk and dv (those into 64 columns take as long as into
 // 128); a tile's stages - product, softmax, product - wait for one another, and what two tiles in flight do not hide is the
 // rest. 8192 rows of 16 heads of 128 on 4 key heads (forward 253, dq 320, dk and dv 450 us): 121 us of exponentials, products of
@@ -1431,8 +1431,8 @@ bool train_attention_tc_supports(const TrainAttention &a, bool backward) {
 }
 
 void launch_train_attention_forward_tc(const TrainAttention &a, cudaStream_t st) {
-  // A CTA with two tiles pays off once a row's keys are many: 4096 rows of 16 heads 80 -> 65 us, 8192 rows 228 ->
-  // 203. With 2048 rows (4 streams of 16 heads) 82 and 81 us, and few keys leave its longer start and end bare: 300 rows of 64 x 8 heads 54 -> 64 us.
+  // Two tiles per CTA: 4 streams of 2048 rows of 16 heads 82 -> 70 us, 8192 rows 227 -> 210, 64 streams of 300 rows of 8 heads 54 -> 47,
+  // 129 rows no difference. Rows that see few keys, by a window, leave little to alternate with.
   const int seen = a.window > 0 && a.window < a.m ? a.window : a.m;
   if (a.dim <= 64 && min(a.n, seen) > TT_B) forward_pair(a, st);
   else if (a.dim <= 64) forward<64>(a, st);
