@@ -88,25 +88,28 @@ __device__ __forceinline__ float *element(const MatView &v, long long batch_off,
 }
 
 // Four elements of a row from column c on; `vec`: rows of the view on 16-byte boundaries. What lies behind the row is 0.
+// FLAT: a matrix whose rows follow one another, as one row.
+template <bool FLAT>
 __device__ __forceinline__ void load4(const MatView &v, long long off, long long r, long long c, bool vec, float (&x)[4]) {
-  const float *p = element(v, off, r, c);
-  if (vec && c + 4 <= v.cols) {
+  const float *p = FLAT ? reinterpret_cast<float *>(v.data + off) + c : element(v, off, r, c);
+  if (FLAT || (vec && c + 4 <= v.cols)) {
     const float4 f = *reinterpret_cast<const float4 *>(p);
     x[0] = f.x; x[1] = f.y; x[2] = f.z; x[3] = f.w;
-    return;
-  }
+  } else {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) x[j] = c + j < v.cols ? *reinterpret_cast<const float *>(reinterpret_cast<const char *>(p) + j * v.cs) : 0.f;
+    for (int j = 0; j < 4; ++j) x[j] = c + j < v.cols ? *reinterpret_cast<const float *>(reinterpret_cast<const char *>(p) + j * v.cs) : 0.f;
+  }
 }
+template <bool FLAT>
 __device__ __forceinline__ void store4(const MatView &v, long long off, long long r, long long c, bool vec, const float (&x)[4]) {
-  float *p = element(v, off, r, c);
-  if (vec && c + 4 <= v.cols) {
+  float *p = FLAT ? reinterpret_cast<float *>(v.data + off) + c : element(v, off, r, c);
+  if (FLAT || (vec && c + 4 <= v.cols)) {
     *reinterpret_cast<float4 *>(p) = make_float4(x[0], x[1], x[2], x[3]);
-    return;
-  }
+  } else {
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
-    if (c + j < v.cols) *reinterpret_cast<float *>(reinterpret_cast<char *>(p) + j * v.cs) = x[j];
+    for (int j = 0; j < 4; ++j)
+      if (c + j < v.cols) *reinterpret_cast<float *>(reinterpret_cast<char *>(p) + j * v.cs) = x[j];
+  }
 }
 
 __device__ __forceinline__ double ns_block_sum(double s) {
@@ -127,7 +130,7 @@ enum { VEC_G = 1, VEC_M = 2, VEC_P = 4 };
 // Four groups of four elements at a time and thread, so that their loads are in flight together (with one a step on six matrices of
 // 512 x 2048 took 383 us, with four 375).
 constexpr int NS_AHEAD = 4;
-template <typename F>
+template <bool FLAT, typename F>
 __device__ __forceinline__ void for_quads(long long rows, long long quads, F f) {
   const long long all = rows * quads, step = 256LL * gridDim.x;
   for (long long e0 = blockIdx.x * 256LL + threadIdx.x; e0 < all; e0 += NS_AHEAD * step) {
@@ -136,7 +139,7 @@ __device__ __forceinline__ void for_quads(long long rows, long long quads, F f) 
 #pragma unroll
     for (int i = 0; i < NS_AHEAD; ++i) {
       const long long e = e0 + i * step < all ? e0 + i * step : e0;  // (a group past the end is the first one's again, and not used)
-      r[i] = div_index(e, quads);
+      r[i] = FLAT ? 0 : div_index(e, quads);
       c[i] = (e - r[i] * quads) * 4;
       n += e0 + i * step < all;
     }
@@ -144,18 +147,19 @@ __device__ __forceinline__ void for_quads(long long rows, long long quads, F f) 
   }
 }
 
+template <bool FLAT>
 __global__ void __launch_bounds__(256) muon_begin_kernel(const __grid_constant__ MuonStep g, NsWork w, unsigned vec) {
   pdl_launch_dependents();
   pdl_wait();
   const long long batch = blockIdx.y;
   const long long go = batch_offset(g.grads, batch), mo = g.step ? batch_offset(g.momentum, batch) : 0;
   double sum = 0.0;
-  for_quads(g.grads.rows, (g.grads.cols + 3) / 4, [&](const long long(&r)[NS_AHEAD], const long long(&c)[NS_AHEAD], int n) {
+  for_quads<FLAT>(g.grads.rows, (g.grads.cols + 3) / 4, [&](const long long(&r)[NS_AHEAD], const long long(&c)[NS_AHEAD], int n) {
     float u[NS_AHEAD][4], m[NS_AHEAD][4];
 #pragma unroll
     for (int i = 0; i < NS_AHEAD; ++i) {
-      load4(g.grads, go, r[i], c[i], vec & VEC_G, u[i]);
-      if (g.step) load4(g.momentum, mo, r[i], c[i], vec & VEC_M, m[i]);
+      load4<FLAT>(g.grads, go, r[i], c[i], vec & VEC_G, u[i]);
+      if (g.step) load4<FLAT>(g.momentum, mo, r[i], c[i], vec & VEC_M, m[i]);
     }
 #pragma unroll
     for (int i = 0; i < NS_AHEAD; ++i) {
@@ -166,7 +170,7 @@ __global__ void __launch_bounds__(256) muon_begin_kernel(const __grid_constant__
           m[i][j] = fmaf(g.mu, m[i][j], u[i][j]);
           u[i][j] = g.nesterov ? fmaf(g.mu, m[i][j], u[i][j]) : m[i][j];
         }
-        store4(g.momentum, mo, r[i], c[i], vec & VEC_M, m[i]);
+        store4<FLAT>(g.momentum, mo, r[i], c[i], vec & VEC_M, m[i]);
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) sum += (double)u[i][j] * (double)u[i][j];
@@ -176,6 +180,7 @@ __global__ void __launch_bounds__(256) muon_begin_kernel(const __grid_constant__
   if (threadIdx.x == 0) w.parts[batch * NS_PARTS + blockIdx.x] = sum;
 }
 
+template <bool FLAT>
 __global__ void __launch_bounds__(256) muon_pair_kernel(const __grid_constant__ MuonStep g, NsWork w, unsigned vec, int parts) {
   pdl_launch_dependents();
   pdl_wait();
@@ -185,17 +190,19 @@ __global__ void __launch_bounds__(256) muon_pair_kernel(const __grid_constant__ 
   const double inv = 1.0 / (norm + (double)NS_EPS);
   const float rho = (float)(norm * inv);
   if (blockIdx.x == 0 && threadIdx.x == 0) w.rho[batch] = rho;
+  // x = u scale, by two factors: the second stays in the range of 32 bits whatever the norm
   const double scale = inv * (double)ns_pow2(ns_exp_x(rho, 0));
+  const float first = scale < 1e-30 ? 5.421010862427522e-20f : 1.f, second = (float)(scale / (double)first);  // 2^-64
   __half *hi = w.x[0].hi + batch * g.grads.rows * w.ldx, *lo = w.x[0].lo + batch * g.grads.rows * w.ldx;
-  for_quads(g.grads.rows, w.ldx / 4, [&](const long long(&r)[NS_AHEAD], const long long(&c)[NS_AHEAD], int n) {
+  for_quads<FLAT>(g.grads.rows, w.ldx / 4, [&](const long long(&r)[NS_AHEAD], const long long(&c)[NS_AHEAD], int n) {
     float u[NS_AHEAD][4], m[NS_AHEAD][4];
 #pragma unroll
     for (int i = 0; i < NS_AHEAD; ++i) {
-      const bool in = c[i] < g.grads.cols;
+      const bool in = FLAT || c[i] < g.grads.cols;
 #pragma unroll
       for (int j = 0; j < 4; ++j) u[i][j] = m[i][j] = 0.f;
-      if (in) load4(g.grads, go, r[i], c[i], vec & VEC_G, u[i]);
-      if (in && g.step) load4(g.momentum, mo, r[i], c[i], vec & VEC_M, m[i]);
+      if (in) load4<FLAT>(g.grads, go, r[i], c[i], vec & VEC_G, u[i]);
+      if (in && g.step) load4<FLAT>(g.momentum, mo, r[i], c[i], vec & VEC_M, m[i]);
     }
 #pragma unroll
     for (int i = 0; i < NS_AHEAD; ++i) {
@@ -205,7 +212,7 @@ __global__ void __launch_bounds__(256) muon_pair_kernel(const __grid_constant__ 
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float v = !g.step ? u[i][j] : g.nesterov ? fmaf(g.mu, m[i][j], u[i][j]) : m[i][j];
-        x[j] = (float)((double)v * scale);
+        x[j] = v * first * second;
       }
       ns_split2(x[0], x[1], h[0], l[0]);
       ns_split2(x[2], x[3], h[1], l[1]);
@@ -215,8 +222,9 @@ __global__ void __launch_bounds__(256) muon_pair_kernel(const __grid_constant__ 
   });
 }
 
-__global__ void __launch_bounds__(256) muon_end_kernel(const __grid_constant__ MuonStep g, NsWork w, unsigned vec, float keep,
-                                                       float rate) {
+template <bool FLAT>
+__global__ void __launch_bounds__(256)
+muon_end_kernel(const __grid_constant__ MuonStep g, NsWork w, unsigned vec, float keep, float rate) {
   pdl_launch_dependents();
   pdl_wait();
   const long long batch = blockIdx.y;
@@ -224,14 +232,14 @@ __global__ void __launch_bounds__(256) muon_end_kernel(const __grid_constant__ M
   const Pair x = w.x[g.steps & 1];
   const __half *hi = x.hi + batch * g.grads.rows * w.ldx, *lo = x.lo + batch * g.grads.rows * w.ldx;
   const float scale = ns_pow2(-ns_exp_x(w.rho[batch], g.steps));
-  for_quads(g.grads.rows, (g.grads.cols + 3) / 4, [&](const long long(&r)[NS_AHEAD], const long long(&c)[NS_AHEAD], int n) {
+  for_quads<FLAT>(g.grads.rows, (g.grads.cols + 3) / 4, [&](const long long(&r)[NS_AHEAD], const long long(&c)[NS_AHEAD], int n) {
     uint2 h[NS_AHEAD], l[NS_AHEAD];
     float p[NS_AHEAD][4];
 #pragma unroll
     for (int i = 0; i < NS_AHEAD; ++i) {
       h[i] = *reinterpret_cast<const uint2 *>(hi + r[i] * w.ldx + c[i]);
       l[i] = *reinterpret_cast<const uint2 *>(lo + r[i] * w.ldx + c[i]);
-      if (g.step) load4(g.params, po, r[i], c[i], vec & VEC_P, p[i]);
+      if (g.step) load4<FLAT>(g.params, po, r[i], c[i], vec & VEC_P, p[i]);
     }
 #pragma unroll
     for (int i = 0; i < NS_AHEAD; ++i) {
@@ -243,7 +251,7 @@ __global__ void __launch_bounds__(256) muon_end_kernel(const __grid_constant__ M
         v[j] = ns_value(hh[j], ll[j]) * scale;
         if (g.step) v[j] = fmaf(-rate, v[j], p[i][j] * keep);
       }
-      store4(g.params, po, r[i], c[i], vec & VEC_P, v);
+      store4<FLAT>(g.params, po, r[i], c[i], vec & VEC_P, v);
     }
   });
 }
@@ -797,8 +805,11 @@ void launch_muon(const MuonStep &g, void *workspace, cudaStream_t st) {
   const long long fill = (148 * 8 + count - 1) / count, each = blocks < fill ? blocks : fill;
   const unsigned parts = (unsigned)(each < NS_PARTS ? each : NS_PARTS);
   const dim3 grid(parts, (unsigned)count), wide((unsigned)each, (unsigned)count);
-  launch_pdl(muon_begin_kernel, grid, dim3(256), 0, st, true, g, w, vec);
-  launch_pdl(muon_pair_kernel, wide, dim3(256), 0, st, true, g, w, vec, (int)parts);
+  auto dense = [&](const MatView &v) { return v.cs == 4 && v.rs == 4 * n; };
+  const bool flat = n % 4 == 0 && w.ldx == n && vec == (unsigned)(VEC_G | (g.step ? VEC_M : 0) | VEC_P) && dense(g.grads) &&
+                    dense(g.params) && (!g.step || dense(g.momentum));
+  launch_pdl(flat ? muon_begin_kernel<true> : muon_begin_kernel<false>, grid, dim3(256), 0, st, true, g, w, vec);
+  launch_pdl(flat ? muon_pair_kernel<true> : muon_pair_kernel<false>, wide, dim3(256), 0, st, true, g, w, vec, (int)parts);
   for (int i = 0; i < g.steps; ++i) {
     const Operand x{w.x[i & 1], m, n, w.ldx}, y{w.x[(i + 1) & 1], m, n, w.ldx}, a{w.a, p, p, w.ldp}, b{w.b, p, p, w.ldp};
     if (tall) product<GRAM, true, true>(x, x, a, (int)m, Pair{}, i, w.rho, count, st);
@@ -808,7 +819,8 @@ void launch_muon(const MuonStep &g, void *workspace, cudaStream_t st) {
     else product<APPLY, false, true>(b, x, y, p, x.p, i, w.rho, count, st);
   }
   const float rate = g.lr * sqrtf(m > n ? (float)m / (float)n : 1.f);
-  launch_pdl(muon_end_kernel, wide, dim3(256), 0, st, true, g, w, vec, 1.f - g.lr * g.weight_decay, rate);
+  launch_pdl(flat ? muon_end_kernel<true> : muon_end_kernel<false>, wide, dim3(256), 0, st, true, g, w, vec, 1.f - g.lr * g.weight_decay,
+             rate);
 }
 
 }  // namespace lb
