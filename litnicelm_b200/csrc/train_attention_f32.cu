@@ -14,7 +14,7 @@
 // memory, all four together where a sum runs over all dimensions (small parts first there too).
 //
 // Bound: at the sizes that such models train at, latency: 8 streams of 250 rows, 8 heads of 64 take 67 us forward and backward (split 2 x 9,
-// forward 14, dk and dv 27, dq 27 us) with 128 CTAs of four products' dependent stages each; with 32-bit products on the FMA
+// forward 13, backward 36 us) with 128 CTAs a result of dependent stages of six products each; with 32-bit products on the FMA
 // pipe it was 219 us. 2000 rows of 8 heads of 128: 419 us, 1957 that way; the six products are 100 us of it at the pipe's rate.
 //
 // A CTA: warp 0 issues TMA, warp 1 owns tensor memory and issues the MMAs, eight warps (a thread: a row or key, half of the
@@ -477,10 +477,8 @@ train_forward_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
 // ---- dk and dv ------------------------------------------------------------------------------------------------------------------
 
 template <int H>
-__global__ void __launch_bounds__(TF_THREADS, 1)
-train_dkv_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                     const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do,
-                     const __grid_constant__ TtArgs a) {
+__device__ __forceinline__ void tf_dkv(const CUtensorMap &map_q, const CUtensorMap &map_k, const CUtensorMap &map_v,
+                                       const CUtensorMap &map_do, const TtArgs &a, int block) {
   extern __shared__ unsigned char smem_raw[];
   const unsigned base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char *base_ptr = smem_raw + (base - smem_u32(smem_raw));
@@ -491,8 +489,8 @@ train_dkv_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
   volatile unsigned *tmem_holder = reinterpret_cast<volatile unsigned *>(base_ptr + TF_BAR_OFF + 240);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(base_ptr + TF_BAR_OFF + 244);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int oh = H == 2 ? (int)blockIdx.x & 1 : 0;  // which 64 dimensions of the result
-  const TtPlace at = tt_place(a, a.groups, false, H);
+  const int oh = H == 2 ? block & 1 : 0;  // which 64 dimensions of the result
+  const TtPlace at = tt_place(a, a.groups, false, H, block);
   const int j0 = at.tile * TT_B, j1 = min(j0 + TT_B, at.keys);
   // rows that see a key of this tile: from lo on, to row_end
   const int lo = a.span.causal ? max(0, j0 - a.span.first) / TT_B * TT_B : 0;
@@ -725,10 +723,8 @@ train_dkv_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
 // ---- dq -------------------------------------------------------------------------------------------------------------------------
 
 template <int H>
-__global__ void __launch_bounds__(TF_THREADS, 1)
-train_dq_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                    const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do,
-                    const __grid_constant__ TtArgs a) {
+__device__ __forceinline__ void tf_dq(const CUtensorMap &map_q, const CUtensorMap &map_k, const CUtensorMap &map_v,
+                                      const CUtensorMap &map_do, const TtArgs &a, int block) {
   extern __shared__ unsigned char smem_raw[];
   const unsigned base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char *base_ptr = smem_raw + (base - smem_u32(smem_raw));
@@ -738,8 +734,8 @@ train_dq_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
   volatile unsigned *tmem_holder = reinterpret_cast<volatile unsigned *>(base_ptr + TF_BAR_OFF + 240);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(base_ptr + TF_BAR_OFF + 244);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int oh = H == 2 ? (int)blockIdx.x & 1 : 0;  // which 64 dimensions of the result
-  const TtPlace at = tt_place(a, a.heads, a.span.causal != 0, H);
+  const int oh = H == 2 ? block & 1 : 0;  // which 64 dimensions of the result
+  const TtPlace at = tt_place(a, a.heads, a.span.causal != 0, H, block);
   const int r0 = at.tile * TT_B, r1 = min(r0 + TT_B, a.n), kh = at.head / a.share;
   const int lo = a.span.lo(r0), end = a.span.end(r1 - 1, at.keys);
   const int tiles = end > lo ? (end - lo + TT_B - 1) / TT_B : 0;
@@ -920,6 +916,18 @@ train_dq_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
   }
 }
 
+// Both, in one launch: neither waits for the other, and few rows leave multiprocessors free (4 streams of 64 rows: 14 and 16 us one behind
+// the other).
+template <int H>
+__global__ void __launch_bounds__(TF_THREADS, 1)
+train_backward_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                          const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do,
+                          const __grid_constant__ TtArgs by_keys, const __grid_constant__ TtArgs by_rows, int blocks) {
+  const int block = (int)blockIdx.x;
+  if (block < blocks) tf_dkv<H>(map_q, map_k, map_v, map_do, by_keys, block);
+  else tf_dq<H>(map_q, map_k, map_v, map_do, by_rows, block - blocks);
+}
+
 // ---- host -----------------------------------------------------------------------------------------------------------------------
 
 size_t part_bytes(long long streams, long long heads, long long rows, long long dim) {
@@ -1006,15 +1014,16 @@ void backward(const TrainAttention &a, float *delta, const Parts (&p)[4], cudaSt
   t.o1 = a.dk;
   t.o2 = a.dv;
   t.vec = rows16(a.dk) && rows16(a.dv);
-  static SharedMemoryOnce once_dkv, once_dq;
-  once_dkv.set(train_dkv_f32_kernel<H>, TF_SMEM);
-  launch_pdl(train_dkv_f32_kernel<H>, dim3(tt_grid(t, a.groups, H)), dim3(TF_THREADS), TF_SMEM, st, true, mq, mk, mv, md, t);
-  t = tt_args(a, a.n);
-  t.delta = delta;
-  t.o1 = a.dq;
-  t.vec = rows16(a.dq);
-  once_dq.set(train_dq_f32_kernel<H>, TF_SMEM);
-  launch_pdl(train_dq_f32_kernel<H>, dim3(tt_grid(t, a.heads, H)), dim3(TF_THREADS), TF_SMEM, st, true, mq, mk, mv, md, t);
+  TtArgs u = tt_args(a, a.n);
+  u.delta = delta;
+  u.o1 = a.dq;
+  u.vec = rows16(a.dq);
+  const unsigned by_keys = tt_grid(t, a.groups, H), by_rows = tt_grid(u, a.heads, H);
+  if (by_rows > 0x7fffffffu - by_keys) throw std::invalid_argument("attention: too many rows, heads and streams for one call");
+  static SharedMemoryOnce once;
+  once.set(train_backward_f32_kernel<H>, TF_SMEM);
+  launch_pdl(train_backward_f32_kernel<H>, dim3(by_keys + by_rows), dim3(TF_THREADS), TF_SMEM, st, true, mq, mk, mv, md, t, u,
+             (int)by_keys);
 }
 
 }  // namespace
