@@ -84,6 +84,45 @@ def test_attention_long(dtype, n, m, dim, lengths, opts):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,m,opts", [
+    (300, 300, dict(scale=-0.2)), (300, 300, dict(scale=0.0)), (129, 700, dict(causal=False, scale=1.5)), (300, 500, dict(window=200)),
+    (257, 600, dict(first=340, window=129)), (400, 300, dict(first=5, window=150)), (700, 130, dict(window=129)),
+    (256, 129, dict(causal=False)), (390, 900, dict(first=510)), (700, 2, dict())], ids=str)
+def test_attention_two_row_tiles(dtype, n, m, opts):
+    attention_case(dtype, 3, n, m, 4, 2, 56, lengths=[m, 1, max(1, m - 130)], **opts)
+
+
+@pytest.mark.parametrize("streams,n,opts", [(40, 200, dict()), (24, 300, dict(window=50)), (6, 1500, dict(causal=False))], ids=str)
+def test_attention_calls_at_once(streams, n, opts):
+    """Passes on two streams at the same time, and a captured one replayed beside an eager one, have the results of each by itself."""
+    g = gen(31)
+    lens = torch.randint(0, n + 1, (streams,), generator=g, device="cuda", dtype=torch.int32)
+    sets = [(*fused(g, streams, n, n, 4, 2, 64, BF16), rand(g, streams, n, 4, 64, dtype=BF16)) for _ in range(2)]
+
+    def both(q, k, v, dout):
+        out, lse = training.attention_forward(q, k, v, lengths=lens, **opts)
+        return (out, lse, *training.attention_backward(dout, q, k, v, out, lse, lengths=lens, **opts))
+
+    alone = [both(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams_at_once = [torch.cuda.Stream() for _ in sets]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = both(*sets[0])
+    for _ in range(3):
+        got = []
+        for s, stream in zip(sets, streams_at_once):
+            stream.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(stream):
+                got.append([both(*s) for _ in range(3)][-1])
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(alone + alone[:1], got + [captured]):
+            for x, y in zip(a, b):
+                assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("dim", [48, 128])
 @pytest.mark.parametrize("opts", [dict(), dict(causal=False), dict(window=60), dict(first=300)], ids=str)
 def test_attention_many_tiles(dtype, dim, opts):
