@@ -421,7 +421,8 @@ int litnice_b200_selftest_wait_timeout(int32_t limit_us, int32_t *code, int32_t 
 
 /* Tensors are the table's views (device 1, strides in bytes, any order and overlap for inputs) on the
  * caller's device memory. dtype 0 is f32; these entries also take 2, bfloat16. Outputs may not
- * overlap each other, themselves or inputs unless an entry says so. Every call only enqueues kernels on `stream` (a
+ * overlap each other, themselves or inputs unless an entry says so (those that begin where another
+ * argument does are refused). Every call only enqueues kernels on `stream` (a
  * cudaStream_t of the current device, NULL: the default stream) and allocates nothing: it may be
  * captured into a graph. Where an entry wants a workspace, it is device memory of the size that the
  * _workspace function gives, on a 256-byte boundary, not shared by calls that may overlap on the GPU;

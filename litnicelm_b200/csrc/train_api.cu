@@ -74,6 +74,17 @@ void check_like(LitniceView t, LitniceView u, const char *name, const char *othe
   if (!same) bad(std::string(name) + " differs from " + other + " in shape or type");
 }
 
+// A result that begins where another tensor does would change it under the kernels. (Slices of one buffer may interleave: what
+// begins elsewhere is the caller's care.)
+struct Named {
+  LitniceView t;
+  const char *name;
+};
+void check_apart(Named result, std::initializer_list<Named> others) {
+  for (const Named &o : others)
+    if (result.t->data == o.t->data) bad(std::string(result.name) + " lies on " + o.name);
+}
+
 void check_workspace(const void *workspace, uint64_t have, uint64_t need) {
   if (workspace == nullptr) bad("null workspace");
   if (reinterpret_cast<uintptr_t>(workspace) % 256) bad("the workspace is not on a 256-byte boundary");
@@ -172,6 +183,7 @@ int litnice_b200_attention_forward(LitniceView q, LitniceView k, LitniceView v, 
     check_result(out, "out");
     check_floats(lse, "lse");
     check_workspace(workspace, workspace_bytes, attention_workspace(q, k, false));
+    check_apart({out, "out"}, {{q, "q"}, {k, "k"}, {v, "v"}});
     a.out = head_view(out);
     a.lse = lse;
     launch_train_attention_forward(a, workspace, static_cast<cudaStream_t>(stream));
@@ -218,6 +230,9 @@ int litnice_b200_attention_backward(LitniceView dout, LitniceView q, LitniceView
     check_result(dv, "dv");
     check_floats(lse, "lse");
     check_workspace(workspace, workspace_bytes, attention_workspace(q, k, true));
+    check_apart({dq, "dq"}, {{dout, "dout"}, {q, "q"}, {k, "k"}, {v, "v"}, {out, "out"}, {dk, "dk"}, {dv, "dv"}});
+    check_apart({dk, "dk"}, {{dout, "dout"}, {q, "q"}, {k, "k"}, {v, "v"}, {out, "out"}, {dv, "dv"}});
+    check_apart({dv, "dv"}, {{dout, "dout"}, {q, "q"}, {k, "k"}, {v, "v"}, {out, "out"}});
     a.dout = head_view(dout);
     a.out = head_view(out);
     a.dq = head_view(dq);
@@ -331,6 +346,8 @@ int litnice_b200_muon_step(LitniceView params, LitniceView grads, LitniceView mo
     if (!std::isfinite(options->lr) || !std::isfinite(options->mu) || !std::isfinite(options->weight_decay))
       bad("an option is not finite");
     check_workspace(workspace, workspace_bytes, muon_workspace(grads));
+    check_apart({params, "params"}, {{grads, "grads"}, {momentum, "momentum"}});
+    check_apart({momentum, "momentum"}, {{grads, "grads"}});
     MuonStep g;
     g.step = 1;
     g.grads = make_mat_view(grads, "grads");

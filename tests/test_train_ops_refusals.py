@@ -186,3 +186,31 @@ def test_python_layer_refuses():
         training.muon_step(x, x, x, 0.1)
     with pytest.raises(ValueError, match="not a CUDA tensor"):
         training.policy_loss(x[0, 0], x, x, x)
+
+
+def test_results_on_other_tensors_are_refused(lib):
+    """What begins where an argument does; slices of one buffer that begin elsewhere are taken."""
+    at = [BASE * (i + 1) for i in range(9)]
+    q, k, v = view((2, 8, 4, 16), ptr=at[0]), view((2, 8, 2, 16), ptr=at[1]), view((2, 8, 2, 16), ptr=at[2])
+    for place, name in ((at[0], "q"), (at[1], "k"), (at[2], "v")):
+        assert forward(lib, q=q, k=k, v=v, out=view((2, 8, 4, 16), ptr=place)) == EINVAL
+        assert f"out lies on {name}" in text(lib)
+    opts = training.AttentionOptions(0.25, 1, 0, 0, None)
+    for moved, onto, why in ((2, 0, "dq lies on q"), (3, 1, "dk lies on k"), (4, 3, "dk lies on dv"), (2, 6, "dq lies on out"),
+                             (4, 5, "dv lies on dout")):
+        # q, k, dq, dk, dv, dout, out, v
+        places = list(at)
+        order = [0, 1, 2, 3, 4, 5, 6, 7]
+        order[moved] = onto
+        wide, narrow = (2, 8, 4, 16), (2, 8, 2, 16)
+        shapes = (wide, narrow, wide, narrow, narrow, wide, wide, narrow)
+        tq, tk, tdq, tdk, tdv, tdout, tout, tv = (view(s, ptr=places[o]) for s, o in zip(shapes, order))
+        assert lib.litnice_b200_attention_backward(ref(tdout), ref(tq), ref(tk), ref(tv), ref(tout), BASE * 20, ref(opts), ref(tdq),
+                                                   ref(tdk), ref(tdv), BASE * 30, 1 << 30, None) == EINVAL
+        assert why in text(lib)
+    mo = training.MuonOptions(0.1, 0.9, 0.0, 1, 5)
+    for params, grads, momentum, why in ((0, 0, 1, "params lies on grads"), (0, 1, 0, "params lies on momentum"),
+                                         (0, 1, 1, "momentum lies on grads")):
+        views = [view((80, 96), ptr=at[i]) for i in (params, grads, momentum)]
+        assert lib.litnice_b200_muon_step(*(ref(x) for x in views), ref(mo), BASE * 30, 1 << 30, None) == EINVAL
+        assert why in text(lib)
