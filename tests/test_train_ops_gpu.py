@@ -460,6 +460,19 @@ def test_orthogonalise_scales_and_zeros():
         assert training.orthogonalise(v, out=v) is v and torch.equal(v, got)
 
 
+@pytest.mark.parametrize("shape", [(2, 40, 70), (2, 96, 152), (300, 260), (2, 130, 99)], ids=str)
+@pytest.mark.parametrize("power", [-20, 60, 120])
+def test_orthogonalise_powers_of_two(shape, power):
+    """A power of two changes nothing but what 1e-7 beside the norm is worth (2^-20 of a norm above 50: 2e-3 of a factor, which the
+    iteration forgets no faster than it magnifies it, a factor of 3.4445 a step) and roundings of x, 2^-23 of an element."""
+    u = rand(gen(5), *shape)
+    one, other = training.orthogonalise(u).double(), training.orthogonalise(u * 2.0 ** power).double()
+    norm = torch.linalg.matrix_norm(u.double()).min()
+    part = 1e-7 / float(norm) * max(1.0, 2.0 ** -power) + 4 * 2.0 ** -23
+    off = torch.linalg.matrix_norm(one - other) / torch.linalg.matrix_norm(one)
+    assert bool((off <= 3.4445 ** 5 * part).all()) and bool(torch.isfinite(other).all())
+
+
 def test_orthogonalise_strides():
     g = gen(10)
     big = rand(g, 3, 90, 2, 130)
