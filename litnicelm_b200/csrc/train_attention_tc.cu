@@ -186,7 +186,7 @@ train_forward_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
   unsigned char *base_ptr = smem_raw + (base - smem_u32(smem_raw));
   const unsigned q_off = base, k_off = base + TILE, v_off = base + 2 * TILE, bars = base + 3 * TILE;
   const unsigned q_full = bars, k_full = bars + 8, v_full = bars + 16, k_free = bars + 24, s_full = bars + 32,
-                 p_ready = bars + 40, o_full = bars + 48;
+                 p_ready = bars + 40, o_full = bars + 48, drained = bars + 56;
   volatile unsigned *tmem_holder = reinterpret_cast<volatile unsigned *>(base_ptr + 3 * TILE + 64);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(base_ptr + 3 * TILE + 68);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -196,7 +196,7 @@ train_forward_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
   const int tiles = end > lo ? (end - lo + TT_B - 1) / TT_B : 0;
 
   if (threadIdx.x == 0) {
-    for (unsigned bar : {q_full, k_full, v_full, k_free, s_full, o_full}) mbar_init(bar, 1);
+    for (unsigned bar : {q_full, k_full, v_full, k_free, s_full, o_full, drained}) mbar_init(bar, 1);
     mbar_init(p_ready, 4);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -270,11 +270,11 @@ train_forward_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       }
       __syncwarp();
     }
-    if (!ok) {  // a bounded chance for the tensor pipe to finish before tensor memory is freed
-      if (tc_elect()) tc_commit(o_full);
+    if (!ok) {  // a bounded chance for the tensor pipe to finish before tensor memory is freed (a barrier that no one else waits for)
+      if (tc_elect()) tc_commit(drained);
       __syncwarp();
       const unsigned long long limit = global_timer() + WAIT_LIMIT_NS;
-      while (!mbar_try_wait(o_full, (unsigned)i & 1u) && global_timer() < limit) {}
+      while (!mbar_try_wait(drained, 0) && global_timer() < limit) {}
     }
   } else {
     const int q = warp & 3;
@@ -311,6 +311,7 @@ train_forward_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       if (lane == 0) mbar_arrive(p_ready);
     }
     if (ok && tiles > 0) ok = mbar_wait_warp(o_full, (unsigned)(tiles - 1) & 1u, abort_flag, nullptr, 79);
+    ok = __all_sync(0xffffffffu, ok && !*abort_flag);
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const bool live = row < a.n, empty = row_end <= row_lo;
     bf16 *o = reinterpret_cast<bf16 *>(a.o1.p) + at.stream * a.o1.s + (long long)row * a.o1.r + at.head * a.o1.h;

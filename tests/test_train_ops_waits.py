@@ -1,0 +1,50 @@
+"""What the kernels of the training operators leave after a wait that ran out, read from their sources: no test makes one run out in
+a kernel, and a kernel that gave up must not look like one that has finished."""
+import os
+import re
+
+import pytest
+
+CSRC = os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "litnicelm_b200", "csrc")
+WAIT = r"(?:mbar_wait\w*|TF_WAIT)\("
+AGREED = "ok = __all_sync(0xffffffffu, ok && !*abort_flag);"
+
+
+def source(name):
+    with open(os.path.join(CSRC, name)) as f:
+        text = f.read()
+    return re.sub(r"//[^\n]*", "", text)
+
+
+def body_of(text, name):
+    """What stands between the braces of a function."""
+    m = re.search(r"\b" + name + r"\([^{};]*\)\s*\{", text)
+    assert m, name
+    depth, at = 1, m.end()
+    while depth:
+        depth += {"{": 1, "}": -1}.get(text[at], 0)
+        at += 1
+    return text[m.end():at]
+
+
+@pytest.mark.parametrize("file,store,names", [
+    ("train_attention_tc.cu", "tt_store_row(",
+     ("train_forward_tc_kernel", "train_forward_pair_kernel", "train_dkv_tc_kernel", "train_dq_tc_kernel")),
+    ("train_attention_f32.cu", "tf_store_sums(", ("train_forward_f32_kernel", "tf_dkv", "tf_dq"))],
+    ids=lambda x: x if isinstance(x, str) and x.endswith(".cu") else "")
+def test_attention_stores_behind_the_flag(file, store, names):
+    """Between the last wait and the results every warp asks whether any has given up: a barrier that another role completes while
+    it gives up (the tensor pipe's last) says nothing about the sums."""
+    for name in names:
+        body = body_of(source(file), name)
+        at = body.index(store)
+        waits = [m.start() for m in re.finditer(WAIT, body[:at])]
+        assert waits and AGREED in body[waits[-1]:at], name
+
+
+def test_attention_forward_drains_on_its_own_barrier():
+    body = body_of(source("train_attention_tc.cu"), "train_forward_tc_kernel")
+    drain = body[body.index("if (!ok) {"):]
+    drain = drain[:drain.index("}\n")]
+    (bar,) = re.findall(r"tc_commit\((\w+)\)", drain)
+    assert not re.search(WAIT + bar + r"\b", body), bar
