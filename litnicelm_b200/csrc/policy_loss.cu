@@ -326,13 +326,20 @@ policy_stream_kernel(const __grid_constant__ PolicyLoss a, PlWork w, PlForms f) 
   unsigned phase = 0;
   const float factor = a.inv_temp * PL_LOG2E;
   const double inverse = tid == 0 ? inverse_total(a, w) : 0.0;
+  // A row that did not come in time: it and all after it are NaN (the barrier's phases say nothing any more, the shared memory may hold any
+  // row), and the CTA stays until the copy has landed, within the limit.
+  bool lost = false;
   PlRow next;
   for (int row = blockIdx.x; row < a.rows; row += gridDim.x, r = next) {
     const int after = row + gridDim.x;
     next = row_of(a, after < a.rows ? after : row);
     if (r.fills) {
-      if (tid == 0) fetch(after, next);
+      if (tid == 0 && !lost) fetch(after, next);
       fill_row<T>(a, w, f, row, r.fill, tid, THREADS);
+      continue;
+    }
+    if (lost) {
+      fill_row<T>(a, w, f, row, NAN, tid, THREADS);
       continue;
     }
     const T *x = reinterpret_cast<const T *>(a.logits) + row * a.ld;
@@ -351,7 +358,8 @@ policy_stream_kernel(const __grid_constant__ PolicyLoss a, PlWork w, PlForms f) 
       const unsigned none = HALF ? 0xff80ff80u : 0xff800000u;
       z[i] = c < whole ? *reinterpret_cast<const uint4 *>(sm_row + (size_t)c * sizeof(T)) : make_uint4(none, none, none, none);
     }
-    if (!__syncthreads_and(there)) {  // the row did not come
+    lost = !__syncthreads_and(there);
+    if (lost) {
       fill_row<T>(a, w, f, row, NAN, tid, THREADS);
       continue;
     }
@@ -451,6 +459,10 @@ policy_stream_kernel(const __grid_constant__ PolicyLoss a, PlWork w, PlForms f) 
     if (last < a.vocab) from_float(dx + last, tail * per);
     // the target's own, behind what its thread has stored there
     if (r.target < whole ? tid == r.target / V % THREADS : last == r.target) from_float(dx + r.target, fmaf(out[1], per, slope));
+  }
+  if (lost && tid == 0) {
+    const unsigned long long limit = global_timer() + WAIT_LIMIT_NS;
+    while (!mbar_try_wait(bar, (phase - 1u) & 1u) && global_timer() < limit) {}
   }
 }
 

@@ -48,3 +48,15 @@ def test_attention_forward_drains_on_its_own_barrier():
     drain = drain[:drain.index("}\n")]
     (bar,) = re.findall(r"tc_commit\((\w+)\)", drain)
     assert not re.search(WAIT + bar + r"\b", body), bar
+
+
+def test_policy_rows_behind_a_lost_one():
+    """A row whose copy is late leaves the barrier in a phase of its own: the rows after it must not wait there, nor ask for copies,
+    and the copy must land before the shared memory goes away."""
+    body = body_of(source("policy_loss.cu"), "policy_stream_kernel")
+    loop = body[body.index("for (int row = blockIdx.x"):]
+    wait = re.search(WAIT, loop).start()
+    assert re.search(r"if \(lost\) \{\s*fill_row<T>\(a, w, f, row, NAN, tid, THREADS\);\s*continue;", loop[:wait])
+    assert re.search(r"lost = !__syncthreads_and\(there\);\s*if \(lost\) \{\s*fill_row<T>\(a, w, f, row, NAN, tid, THREADS\);\s*continue;", loop[wait:])
+    assert all("!lost" in loop[loop.rindex("if", 0, m.start()):m.start()] for m in re.finditer(r"fetch\(after", loop[:wait]))
+    assert re.search(r"if \(lost && tid == 0\) \{[^}]*mbar_try_wait\(bar, \(phase - 1u\) & 1u\) && global_timer\(\) < limit", loop[wait:])
