@@ -488,7 +488,7 @@ int litnice_b200_policy_loss(LitniceView logits, const int32_t *targets, const f
 
 /* x, out [..., m, n] f32: every matrix U as X = U / (|U| + 1e-7) (Frobenius) followed by `steps` times
  * X <- 3.4445 X + (-4.7750 A + 2.0315 A A) X, A = X X^T, in the smaller side's space: its singular
- * vectors with values near 1. out may be x. */
+ * vectors with values near 1. out may be x (with the strides of x). */
 uint64_t litnice_b200_orthogonalise_workspace(LitniceView x);
 int litnice_b200_orthogonalise(LitniceView x, LitniceView out, int32_t steps, void *workspace, uint64_t workspace_bytes,
                                void *stream);

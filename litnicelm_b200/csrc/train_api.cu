@@ -322,6 +322,9 @@ int litnice_b200_orthogonalise(LitniceView x, LitniceView out, int32_t steps, vo
     muon_sizes(x);
     if (steps < 0 || steps > 100) bad("steps is out of range");
     check_workspace(workspace, workspace_bytes, muon_workspace(x));
+    // (in place, a matrix is read whole before it is written; another matrix of the call may not have been)
+    for (uint32_t i = 0; out->data == x->data && i < x->rank; ++i)
+      if (x->dims[i] > 1 && out->strides_bytes[i] != x->strides_bytes[i]) bad("out lies on x with another stride");
     MuonStep g;
     g.grads = make_mat_view(x, "x");
     g.params = make_mat_view(out, "out");

@@ -242,7 +242,7 @@ def policy_loss(logits: torch.Tensor, targets: torch.Tensor, old_logp: torch.Ten
 
 def orthogonalise(x: torch.Tensor, *, steps: int = 5, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Every matrix of x [..., m, n] float32 with its singular values driven towards 1: X = x / (|x| + 1e-7), then ``steps`` times
-    X <- 3.4445 X + (-4.7750 A + 2.0315 A A) X with A = X X^T (in the smaller side's space). out may be x."""
+    X <- 3.4445 X + (-4.7750 A + 2.0315 A A) X with A = X X^T (in the smaller side's space). out may be x, with x's strides."""
     _tensor(x, "x")
     out = _like(x) if out is None else out
     (vx, vo), held = _views(("x", "out"), (x, out))
