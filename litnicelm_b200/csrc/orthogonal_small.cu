@@ -20,6 +20,9 @@ namespace {
 constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f, NS_EPS = 1e-7f;
 constexpr int SM_P = 64, SM_LD = SM_P + 4, SM_THREADS = 256, SM_MAX_COLS = 512;
 
+constexpr int small_smem(int ldx) { return (SM_P * ldx + 3 * SM_P * SM_LD) * 4; }
+static_assert(small_smem(SM_MAX_COLS + 4) <= 227 * 1024, "");
+
 struct SmallArgs {
   MuonStep g;
   int p, q, cols, ldx;  // smaller and larger side, columns of a CTA, floats between rows of X
@@ -205,8 +208,9 @@ void launch_muon_small(const MuonStep &g, cudaStream_t st) {
   s.ldx = ((s.cols + 31) & ~31) + 4;
   s.keep = 1.f - g.lr * g.weight_decay;
   s.rate = g.lr * sqrtf(m > n ? (float)m / (float)n : 1.f);
-  const size_t smem = ((size_t)SM_P * s.ldx + 3 * SM_P * SM_LD) * 4;
-  LB_CUDA(cudaFuncSetAttribute(muon_small_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  const size_t smem = small_smem(s.ldx);
+  static SharedMemoryOnce once;  // the largest: the attribute is the kernel's, and calls of other threads want other sizes
+  once.set(muon_small_kernel, small_smem(SM_MAX_COLS + 4));
   launch_pdl_cluster_x(muon_small_kernel, dim3((unsigned)(g.grads.batch * s.ctas)), dim3(SM_THREADS), smem, st, true,
                        (unsigned)s.ctas, s);
 }
