@@ -74,15 +74,17 @@ void check_like(LitniceView t, LitniceView u, const char *name, const char *othe
   if (!same) bad(std::string(name) + " differs from " + other + " in shape or type");
 }
 
-// A result that begins where another tensor does would change it under the kernels. (Slices of one buffer may interleave: what
-// begins elsewhere is the caller's care.)
+// A result (or the workspace) that begins where another argument does would change it under the kernels. (Slices of one buffer may
+// interleave: what begins elsewhere is the caller's care.)
 struct Named {
-  LitniceView t;
+  const void *p;
   const char *name;
+  Named(const void *at, const char *n) : p(at), name(n) {}
+  Named(LitniceView t, const char *n) : p(t ? t->data : nullptr), name(n) {}
 };
 void check_apart(Named result, std::initializer_list<Named> others) {
   for (const Named &o : others)
-    if (result.t->data == o.t->data) bad(std::string(result.name) + " lies on " + o.name);
+    if (o.p != nullptr && result.p == o.p) bad(std::string(result.name) + " lies on " + o.name);
 }
 
 void check_workspace(const void *workspace, uint64_t have, uint64_t need) {
@@ -183,7 +185,10 @@ int litnice_b200_attention_forward(LitniceView q, LitniceView k, LitniceView v, 
     check_result(out, "out");
     check_floats(lse, "lse");
     check_workspace(workspace, workspace_bytes, attention_workspace(q, k, false));
-    check_apart({out, "out"}, {{q, "q"}, {k, "k"}, {v, "v"}});
+    const Named lengths{options->lengths, "lengths"};
+    check_apart({out, "out"}, {{q, "q"}, {k, "k"}, {v, "v"}, lengths});
+    check_apart({lse, "lse"}, {{q, "q"}, {k, "k"}, {v, "v"}, {out, "out"}, lengths});
+    check_apart({workspace, "the workspace"}, {{q, "q"}, {k, "k"}, {v, "v"}, {out, "out"}, {lse, "lse"}, lengths});
     a.out = head_view(out);
     a.lse = lse;
     launch_train_attention_forward(a, workspace, static_cast<cudaStream_t>(stream));
@@ -230,9 +235,12 @@ int litnice_b200_attention_backward(LitniceView dout, LitniceView q, LitniceView
     check_result(dv, "dv");
     check_floats(lse, "lse");
     check_workspace(workspace, workspace_bytes, attention_workspace(q, k, true));
-    check_apart({dq, "dq"}, {{dout, "dout"}, {q, "q"}, {k, "k"}, {v, "v"}, {out, "out"}, {dk, "dk"}, {dv, "dv"}});
-    check_apart({dk, "dk"}, {{dout, "dout"}, {q, "q"}, {k, "k"}, {v, "v"}, {out, "out"}, {dv, "dv"}});
-    check_apart({dv, "dv"}, {{dout, "dout"}, {q, "q"}, {k, "k"}, {v, "v"}, {out, "out"}});
+    const Named lengths{options->lengths, "lengths"}, sums{lse, "lse"};
+    check_apart({dq, "dq"}, {{dout, "dout"}, {q, "q"}, {k, "k"}, {v, "v"}, {out, "out"}, {dk, "dk"}, {dv, "dv"}, sums, lengths});
+    check_apart({dk, "dk"}, {{dout, "dout"}, {q, "q"}, {k, "k"}, {v, "v"}, {out, "out"}, {dv, "dv"}, sums, lengths});
+    check_apart({dv, "dv"}, {{dout, "dout"}, {q, "q"}, {k, "k"}, {v, "v"}, {out, "out"}, sums, lengths});
+    check_apart({workspace, "the workspace"}, {{dout, "dout"}, {q, "q"}, {k, "k"}, {v, "v"}, {out, "out"}, {dq, "dq"}, {dk, "dk"},
+                                               {dv, "dv"}, sums, lengths});
     a.dout = head_view(dout);
     a.out = head_view(out);
     a.dq = head_view(dq);
@@ -287,6 +295,14 @@ int litnice_b200_policy_loss(LitniceView logits, const int32_t *targets, const f
       if (a.dlogits == a.logits && a.dld != a.ld) bad("dlogits lies on logits with another stride");
     }
     check_workspace(workspace, workspace_bytes, policy_loss_workspace_bytes(a.rows));
+    const Named inputs[] = {{targets, "targets"}, {old_logp, "old_logp"}, {advantage, "advantage"}, {ref_logp, "ref_logp"}, {weight, "weight"}};
+    const Named results[] = {{loss, "loss"}, {logp, "logp"}, {dlogits, "dlogits"}, {workspace, "the workspace"}};
+    for (int i = 0; i < 4; ++i) {
+      if (results[i].p == nullptr) continue;
+      for (const Named &input : inputs) check_apart(results[i], {input});
+      if (i != 2) check_apart(results[i], {{logits, "logits"}});  // (the gradient may take its place)
+      for (int j = 0; j < i; ++j) check_apart(results[i], {results[j]});
+    }
     a.targets = targets;
     a.old_logp = old_logp;
     a.advantage = advantage;
@@ -322,6 +338,7 @@ int litnice_b200_orthogonalise(LitniceView x, LitniceView out, int32_t steps, vo
     muon_sizes(x);
     if (steps < 0 || steps > 100) bad("steps is out of range");
     check_workspace(workspace, workspace_bytes, muon_workspace(x));
+    check_apart({workspace, "the workspace"}, {{x, "x"}, {out, "out"}});
     // (in place, a matrix is read whole before it is written; another matrix of the call may not have been)
     for (uint32_t i = 0; out->data == x->data && i < x->rank; ++i)
       if (x->dims[i] > 1 && out->strides_bytes[i] != x->strides_bytes[i]) bad("out lies on x with another stride");
@@ -351,6 +368,7 @@ int litnice_b200_muon_step(LitniceView params, LitniceView grads, LitniceView mo
     check_workspace(workspace, workspace_bytes, muon_workspace(grads));
     check_apart({params, "params"}, {{grads, "grads"}, {momentum, "momentum"}});
     check_apart({momentum, "momentum"}, {{grads, "grads"}});
+    check_apart({workspace, "the workspace"}, {{params, "params"}, {grads, "grads"}, {momentum, "momentum"}});
     MuonStep g;
     g.step = 1;
     g.grads = make_mat_view(grads, "grads");

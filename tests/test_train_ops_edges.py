@@ -44,3 +44,59 @@ def test_orthogonalise_in_place_wants_the_same_strides(lib, shape, turned):
     need = lib.litnice_b200_orthogonalise_workspace(ref(x))
     assert lib.litnice_b200_orthogonalise(ref(x), ref(out), 5, 64 * BASE, need, None) == EINVAL
     assert "out lies on x with another stride" in text(lib)
+
+
+# every address of a call by itself, unless a case puts one onto another
+AT = {name: BASE * (i + 1) for i, name in enumerate(
+    ("q", "k", "v", "out", "lse", "lengths", "dout", "dq", "dk", "dv", "work", "logits", "targets", "old_logp", "advantage",
+     "ref_logp", "weight", "loss", "logp", "dlogits", "x", "params", "grads", "momentum"))}
+WIDE, NARROW = (2, 8, 4, 16), (2, 8, 2, 16)
+
+
+def attention_forward(lib, at):
+    o = training.AttentionOptions(0.25, 1, 0, 0, at["lengths"])
+    tensors = [view(s, ptr=at[n]) for n, s in (("q", WIDE), ("k", NARROW), ("v", NARROW), ("out", WIDE))]
+    q, k, v, out = (ref(t) for t in tensors)
+    return lib.litnice_b200_attention_forward(q, k, v, ref(o), out, at["lse"], at["work"], 1 << 30, None)
+
+
+def attention_backward(lib, at):
+    o = training.AttentionOptions(0.25, 1, 0, 0, at["lengths"])
+    tensors = [view(s, ptr=at[n]) for n, s in (("dout", WIDE), ("q", WIDE), ("k", NARROW), ("v", NARROW), ("out", WIDE), ("dq", WIDE),
+                                               ("dk", NARROW), ("dv", NARROW))]
+    dout, q, k, v, out, dq, dk, dv = (ref(t) for t in tensors)
+    return lib.litnice_b200_attention_backward(dout, q, k, v, out, at["lse"], ref(o), dq, dk, dv, at["work"], 1 << 30, None)
+
+
+def policy_loss(lib, at):
+    o = training.PolicyOptions(1.0, 0.2, 0.2, 0.1)
+    z, d = view((4, 100), ptr=at["logits"]), view((4, 100), ptr=at["dlogits"])
+    return lib.litnice_b200_policy_loss(ref(z), at["targets"], at["old_logp"], at["advantage"], at["ref_logp"], at["weight"], ref(o),
+                                        at["loss"], at["logp"], ref(d), at["work"], 1 << 30, None)
+
+
+def orthogonalise(lib, at):
+    x, out = view((80, 96), ptr=at["x"]), view((80, 96), ptr=at["out"])
+    return lib.litnice_b200_orthogonalise(ref(x), ref(out), 5, at["work"], 1 << 30, None)
+
+
+def muon_step(lib, at):
+    o = training.MuonOptions(0.1, 0.9, 0.0, 1, 5)
+    p, g, m = (view((80, 96), ptr=at[n]) for n in ("params", "grads", "momentum"))
+    return lib.litnice_b200_muon_step(ref(p), ref(g), ref(m), ref(o), at["work"], 1 << 30, None)
+
+
+@pytest.mark.parametrize("call,results,inputs", [
+    (attention_forward, "out lse work", "q k v lengths"),
+    (attention_backward, "dq dk dv work", "dout q k v out lse lengths"),
+    (policy_loss, "loss logp dlogits work", "logits targets old_logp advantage ref_logp weight"),
+    (orthogonalise, "work", "x out"), (muon_step, "work params momentum", "grads")], ids=lambda x: getattr(x, "__name__", ""))
+def test_results_begin_where_nothing_else_does(lib, call, results, inputs):
+    results, inputs = results.split(), inputs.split()
+    pairs = [(r, x) for r in results for x in inputs] + [(a, b) for i, a in enumerate(results) for b in results[:i]]
+    for one, other in pairs:
+        if (one, other) == ("dlogits", "logits"):
+            continue  # in place
+        assert call(lib, {**AT, one: AT[other]}) == EINVAL, (one, other)
+        names = [n.replace("work", "the workspace") for n in (one, other)]
+        assert any(f"{a} lies on {b}" in text(lib) for a, b in (names, names[::-1])), (one, other, text(lib))
