@@ -697,8 +697,7 @@ void launch_product(const Operand &a, const Operand &b, const Operand &out, NsPr
   g.m_tiles = (g.m + T - 1) / T;
   g.n_tiles = (g.n + T - 1) / T;
   const long long per = OP == APPLY ? (long long)g.m_tiles * g.n_tiles : (long long)g.m_tiles * (g.m_tiles + 1) / 2;
-  if (per * count > 0x3fffffffLL) throw std::invalid_argument("too many matrices of this size for one call");
-  g.tiles = (int)(per * count);
+  g.tiles = (int)(per * count);  // (in range: checked before the call's first kernel)
   using L = NsSmem<PAIR>;
   static SharedMemoryOnce once;
   once.set(ns_product_kernel<OP, A_MN, B_MN, PAIR, SPLIT>, L::TOTAL);

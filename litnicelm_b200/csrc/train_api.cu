@@ -164,6 +164,7 @@ void muon_sizes(LitniceView t) {
   for (uint32_t i = 0; i + 2 < t->rank; ++i) count *= t->dims[i];
   if (count > 65535) bad("more than 65535 matrices in one call");
   if ((m < n ? m : n) > 32768 || (m < n ? n : m) > (1 << 22)) bad("a matrix of " + std::to_string(m) + " x " + std::to_string(n));
+  if (count * ((m + 127) / 128) * ((n + 127) / 128) > 0x3fffffff) bad("too many matrices of this size for one call");
 }
 
 uint64_t muon_workspace(LitniceView t) {

@@ -449,9 +449,13 @@ void launch_train_attention_forward(const TrainAttention &a, void *work, cudaStr
 
 void launch_train_attention_backward(const TrainAttention &a, float *delta, void *work, cudaStream_t st) {
   if (!a.bf16) return launch_train_attention_backward_f32(a, delta, work, st);
+  const bool tc = train_attention_tc_supports(a, true);
+  const long long tile = tc ? 128 : TA_B;  // the grids of all three kernels, before the first is launched
+  for (const long long blocks : {(a.n + tile - 1) / tile * a.heads * a.streams, (a.m + tile - 1) / tile * a.groups * a.streams})
+    if (blocks > 0x7fffffffLL) throw std::invalid_argument("attention: too many rows, heads and streams for one call");
   if (a.dim <= 64) launch_delta<8>(a, delta, st);
   else launch_delta<16>(a, delta, st);
-  if (train_attention_tc_supports(a, true)) return launch_train_attention_backward_tc(a, delta, st);
+  if (tc) return launch_train_attention_backward_tc(a, delta, st);
   if (a.dim <= 32) backward<32>(a, delta, st);
   else if (a.dim <= 64) backward<64>(a, delta, st);
   else backward<128>(a, delta, st);

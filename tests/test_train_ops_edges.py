@@ -100,3 +100,21 @@ def test_results_begin_where_nothing_else_does(lib, call, results, inputs):
         assert call(lib, {**AT, one: AT[other]}) == EINVAL, (one, other)
         names = [n.replace("work", "the workspace") for n in (one, other)]
         assert any(f"{a} lies on {b}" in text(lib) for a, b in (names, names[::-1])), (one, other, text(lib))
+
+
+def test_too_many_blocks_are_refused_before_the_first_kernel(lib):
+    """(Without a GPU the first kernel's launch would be an error of the runtime.)"""
+    o = training.AttentionOptions(0.25, 1, 0, 0, None)
+    for columns, m in ((4 * 8, 1), (4 * 9, 1), (4 * 8, 40)):  # rows that TMA can address, and not
+        shape, keys = (1 << 21, 1, 1 << 10, 8), (1 << 21, m, 1 << 10, 8)
+        q = [view(shape, 2, (columns << 10, columns << 10, columns, 2), BASE * (i + 1)) for i in range(4)]
+        k = [view(keys, 2, (m * columns << 10, columns << 10, columns, 2), BASE * (i + 5)) for i in range(4)]
+        assert lib.litnice_b200_attention_backward(ref(q[0]), ref(q[1]), ref(k[0]), ref(k[1]), ref(q[2]), 9 * BASE, ref(o), ref(q[3]),
+                                                   ref(k[2]), ref(k[3]), 10 * BASE, 1 << 62, None) == EINVAL
+        assert "too many rows, heads and streams" in text(lib)
+    x, y, z = (view((60000, 8192, 1 << 22), ptr=BASE * (i + 1)) for i in range(3))
+    assert lib.litnice_b200_orthogonalise_workspace(ref(x)) == 0 and "too many matrices" in text(lib)
+    assert lib.litnice_b200_orthogonalise(ref(x), ref(y), 5, 4 * BASE, 1 << 62, None) == EINVAL and "too many matrices" in text(lib)
+    mo = training.MuonOptions(0.1, 0.9, 0.0, 1, 5)
+    assert lib.litnice_b200_muon_step(ref(x), ref(y), ref(z), ref(mo), 4 * BASE, 1 << 62, None) == EINVAL
+    assert "too many matrices" in text(lib)
