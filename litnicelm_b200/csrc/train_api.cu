@@ -48,7 +48,7 @@ void check_tensor(LitniceView t, const char *name, uint32_t rank, bool bf16_too)
   for (uint32_t i = 0; i < t->rank; ++i) {
     if (t->dims[i] <= 0 || t->dims[i] > MAX_EXTENT) bad(n + " has an extent of " + std::to_string(t->dims[i]));
     if (t->strides_bytes[i] % size) bad(n + " has a stride that is no multiple of its element");
-    if (t->dims[i] > 1 && std::llabs(t->strides_bytes[i]) > (1ll << 50)) bad(n + " has an impossible stride");
+    if (t->dims[i] > 1 && (t->strides_bytes[i] > (1ll << 50) || t->strides_bytes[i] < -(1ll << 50))) bad(n + " has an impossible stride");
   }
 }
 

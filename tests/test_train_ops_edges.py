@@ -118,3 +118,15 @@ def test_too_many_blocks_are_refused_before_the_first_kernel(lib):
     mo = training.MuonOptions(0.1, 0.9, 0.0, 1, 5)
     assert lib.litnice_b200_muon_step(ref(x), ref(y), ref(z), ref(mo), 4 * BASE, 1 << 62, None) == EINVAL
     assert "too many matrices" in text(lib)
+
+
+@pytest.mark.parametrize("stride", [1 << 51, -(1 << 51), -(1 << 63)])
+def test_impossible_strides(lib, stride):
+    at = [BASE * (i + 1) for i in range(6)]
+    q, k, v, out = (view(WIDE if i % 3 == 0 else NARROW, ptr=at[i]) for i in range(4))
+    o = training.AttentionOptions(0.25, 1, 0, 0, None)
+    bad = view(WIDE, strides=(stride, 256, 64, 4), ptr=at[0])
+    assert lib.litnice_b200_attention_forward(ref(bad), ref(k), ref(v), ref(o), ref(out), at[4], at[5], 1 << 30, None) == EINVAL
+    assert "q has an impossible stride" in text(lib)
+    assert lib.litnice_b200_attention_forward(ref(q), ref(k), ref(v), ref(o), ref(bad), at[4], at[5], 1 << 30, None) == EINVAL
+    assert "out has an impossible stride" in text(lib)
