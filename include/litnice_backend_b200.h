@@ -473,7 +473,7 @@ int litnice_b200_attention_backward(LitniceView dout, LitniceView q, LitniceView
  *                           + kl_weight (exp d - d - 1)) / sum_rows weight
  * and dlogits its gradient (NULL: not computed; logits itself: in place). weight NULL: all 1; ref_logp may be
  * NULL if kl_weight is 0. loss: one float, logp [rows]. Rows of weight 0 are not read, their logp and gradient are 0;
- * weights without a sum give loss 0. A target outside the vocabulary in a row of nonzero weight makes
+ * weights whose sum is 0 give loss 0 and gradients of 0. A target outside the vocabulary in a row of nonzero weight makes
  * that row's logp and gradient, and the loss, NaN. */
 typedef struct litnice_b200_policy_options {
   float temp;                /* > 0 */

@@ -160,9 +160,10 @@ __device__ __forceinline__ void fill_row(const PolicyLoss &a, const PlWork &w, c
   }
   for (c += at; c < a.vocab; c += threads) from_float(dx + c, fill);
 }
-// 1 / the weights' sum, once it is there.
+// 1 / the weights' sum, once it is there; 0 for weights without one, all zero or not.
 __device__ __forceinline__ double inverse_total(const PolicyLoss &a, const PlWork &w) {
-  return 1.0 / (a.weight ? *static_cast<volatile double *>(w.total) : (double)a.rows);
+  const double total = a.weight ? *static_cast<volatile double *>(w.total) : (double)a.rows;
+  return total == 0.0 ? 0.0 : 1.0 / total;
 }
 // Loss and slope of a row from its statistics, by one thread: the slope in the logits comes back.
 __device__ __forceinline__ float finish_row(const PolicyLoss &a, const PlWork &w, int row, const PlTerms &t, float share, float z, float top,

@@ -217,8 +217,9 @@ def policy_loss(logits: torch.Tensor, targets: torch.Tensor, old_logp: torch.Ten
 
     With z = logits / temp, logp = log_softmax(z)[target], r = exp(logp - old_logp), d = ref_logp - logp:
     loss = sum weight (-min(r advantage, clip(r, 1 - clip_low, 1 + clip_high) advantage) + kl_weight (exp d - d - 1)) / sum weight.
-    Rows of weight 0 are not read; their logp and gradient are 0. A target outside the vocabulary in another row gives NaN there
-    and in the loss. dlogits may be given, logits itself included; with ``gradient`` false it is None."""
+    Rows of weight 0 are not read; their logp and gradient are 0. Weights whose sum is 0 give loss 0 and gradients of 0. A target
+    outside the vocabulary in another row gives NaN there and in the loss. dlogits may be given, logits itself included; with
+    ``gradient`` false it is None."""
     _tensor(logits, "logits")
     if logits.dim() != 2:
         raise ValueError("logits must be [rows, vocab]")

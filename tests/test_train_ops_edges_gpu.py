@@ -57,3 +57,22 @@ def test_small_matrices_of_two_sizes_from_two_threads():
         for a, results in zip(alone, got):
             assert not isinstance(results, Exception), results
             assert all(torch.equal(a, b) for b in results)
+
+
+# ---- weights that cancel ----------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("vocab", [96, 5001, 32000, 70000])
+def test_policy_loss_weights_that_cancel(dtype, vocab):
+    """Weights without a sum, all zero or not, give loss 0 and gradients of 0; the log probabilities are those of any weight."""
+    g = gen(2)
+    logits = rand(g, 6, vocab, dtype=dtype)
+    targets = torch.randint(0, vocab, (6,), generator=g, device="cuda", dtype=torch.int32)
+    old, adv, ref = (rand(g, 6) - 9 for _ in range(3))
+    more = dict(ref_logp=ref, kl_weight=0.1)
+    want = training.policy_loss(logits, targets, old, adv, **more)[1]
+    weight = torch.tensor([1.0, -2, 0, 3, -1, -1], device="cuda")
+    loss, logp, d = training.policy_loss(logits, targets, old, adv, weight=weight, **more)
+    assert float(loss) == 0 and bool((d == 0).all())
+    assert torch.equal(logp, torch.where(weight != 0, want, torch.zeros_like(want)))
