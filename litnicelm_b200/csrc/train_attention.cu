@@ -344,14 +344,15 @@ train_attention_dkv_kernel(const __grid_constant__ TaArgs g) {
     const int lo = a.causal ? max(0, j0 - a.first) / TA_B * TA_B : 0;
     const long long past = a.window > 0 ? (long long)j1 - 1 + a.window - a.first : a.n;
     const int end = past < a.n ? (int)max(past, 0LL) : a.n;
+    const int live = span.rows_end(a.n, at.keys);  // what rows that see no key hold must not meet their weights of zero
     const float f = a.scale * TA_LOG2E;
     for (int h = at.head * share; h < (at.head + 1) * share; ++h) {
       const long long qb = at.stream * a.q.s + h * a.q.h, db = at.stream * a.dout.s + h * a.dout.h;
       const long long stat = ((long long)at.stream * a.heads + h) * a.n;
       for (int r0 = lo; r0 < end; r0 += TA_B) {
         __syncthreads();
-        load_tile<D>(sq, a.q, qb, r0, a.n, a.dim, g.vec & VQ);
-        load_tile<D>(sdo, a.dout, db, r0, a.n, a.dim, g.vec & VDO);
+        load_tile<D>(sq, a.q, qb, r0, live, a.dim, g.vec & VQ);
+        load_tile<D>(sdo, a.dout, db, r0, live, a.dim, g.vec & VDO);
         __syncthreads();
         float s[8][4];
         tile_dot<D>(sk, sq, s);

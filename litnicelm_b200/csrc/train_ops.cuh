@@ -29,6 +29,11 @@ struct TrainSpan {
   int first, window, causal;
   __host__ __device__ int lo(int i) const { return window > 0 ? (first + i - window + 1 > 0 ? first + i - window + 1 : 0) : 0; }
   __host__ __device__ int end(int i, int keys) const { return causal && first + i + 1 < keys ? first + i + 1 : keys; }
+  // Of n rows, those from here on see no key.
+  __host__ __device__ int rows_end(int n, int keys) const {
+    const long long past = keys <= 0 ? 0 : window > 0 ? (long long)keys - 1 + window - first : n;
+    return past < 0 ? 0 : past < n ? (int)past : n;
+  }
 };
 
 constexpr int TRAIN_MAX_DIM = 128;

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from litnicelm_b200 import training
+from train_ops_util import seen_keys
 
 pytestmark = pytest.mark.gpu
 
@@ -76,3 +77,35 @@ def test_policy_loss_weights_that_cancel(dtype, vocab):
     loss, logp, d = training.policy_loss(logits, targets, old, adv, weight=weight, **more)
     assert float(loss) == 0 and bool((d == 0).all())
     assert torch.equal(logp, torch.where(weight != 0, want, torch.zeros_like(want)))
+
+
+# ---- rows that see no key ---------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("dim", [64, 128, 33])
+@pytest.mark.parametrize("m,lengths,opts", [
+    (300, [100, 33, 0, 256], dict(window=40)), (300, [130, 1, 200, 255], dict(window=3)), (90, None, dict(window=40)),
+    (300, [77, 128, 0, 290], dict(window=100, causal=False)), (200, [60, 150, 5, 0], dict(first=30, window=25)),
+    (100, None, dict(first=400, window=7))], ids=str)
+@pytest.mark.parametrize("fill", [math.nan, math.inf])
+def test_rows_that_see_no_key_reach_nothing(dtype, dim, m, lengths, opts, fill):
+    """Whatever their queries and upstream gradients hold."""
+    g = gen(3)
+    streams, n, heads = 4, 300, 4
+    q, dout = (rand(g, streams, n, heads, dim, dtype=dtype) for _ in range(2))
+    k, v = (rand(g, streams, m, 2, dim, dtype=dtype) for _ in range(2))
+    lens = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    seen = seen_keys(n, m, opts.get("causal", True), opts.get("first", 0), opts["window"], lens, streams, "cuda")
+    empty = ~seen.any(3).expand(streams, 1, n)[:, 0]
+    assert bool(empty.any())
+    results = []
+    for x in (0.0, fill):
+        q[empty], dout[empty] = x, x
+        out, lse = training.attention_forward(q, k, v, lengths=lens, **opts)
+        results.append((out, lse, *training.attention_backward(dout, q, k, v, out, lse, lengths=lens, **opts)))
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+    out, lse, dq = results[1][:3]
+    assert bool((out[empty] == 0).all()) and bool((dq[empty] == 0).all())
+    assert bool((lse.transpose(1, 2)[empty] == -math.inf).all())
