@@ -803,10 +803,16 @@ train_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     const unsigned idesc_s = umma_idesc_bf16(TT_B), idesc_d = umma_idesc_bf16(cols) | UMMA_B_MN_MAJOR;
     // Jobs: S and dP of each tile in turn, of all items; each takes the next place, and is issued behind the product that read it.
     int w = 0, i = -1, n = -1, issued = 0, tiles = 0;  // issued: tiles whose S is
-    int lo = 0, each = 0, t = 0, live = 0, have = TT_B;  // rows of the item; have: of the tile whose S was issued last, those that see a key
+    int each = 1, live = 0x7fffffff;  // live: rows from the item's first on that see a key, where others follow
     bool more = true, ok = true;
     unsigned ends = 0u;  // bit (tile of all) % 4: it is its item's last, % 4 + 4: first
     auto kv_rows = [&]() { return k_rows + (unsigned long long)(n % L::NQ * (2 * TILE >> 4)); };
+    // What rows that see no key hold must not meet their weights of zero (rows behind the last are zeros already).
+    auto clear = [&](unsigned tile) {
+      if (live == 0x7fffffff) return;
+      const int have = live - i % each * TT_B;
+      if (have < TT_B) tt_clear_rows(base_ptr + (tile - base), SLABS, max(have, 0), lane);
+    };
     auto scores = [&]() {
       if (++i >= tiles) {
         const int block = next.take(w++, lane);
@@ -816,23 +822,19 @@ train_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         }
         const Item x = item(block);
         tiles = tt_uniform(x.tiles);
-        lo = tt_uniform(x.lo);
-        each = tt_uniform(x.each);
-        live = tt_uniform(a.span.rows_end(a.n, x.at.keys));
-        i = t = 0;
+        each = tt_uniform(max(x.each, 1));
+        const int rows = a.span.rows_end(a.n, x.at.keys);
+        live = tt_uniform(rows < a.n ? rows - x.lo : 0x7fffffff);
+        i = 0;
         ++n;
-      } else if (++t == each) {
-        t = 0;
       }
-      // what rows that see no key hold must not meet their weights of zero (rows behind the last are zeros already)
-      have = live < a.n ? live - (lo + t * TT_B) : TT_B;
       const int g = issued, sa = g % L::NA, sk = n % L::NQ;
       const unsigned bit = 1u << (g & 3);
       ends = (ends & ~(bit | bit << 4)) | (i + 1 == tiles ? bit : 0u) | (i == 0 ? bit << 4 : 0u);
       ok = (i > 0 || mbar_wait_warp(kv_full(sk), (unsigned)(n / L::NQ) & 1u, abort_flag, nullptr, 82)) &&
            mbar_wait_warp(a_full(sa), (unsigned)(g / L::NA) & 1u, abort_flag, nullptr, 83);
       if (!ok) return;
-      if (have < TT_B) tt_clear_rows(base_ptr + (q_tile(sa) - base), SLABS, have, lane);
+      clear(q_tile(sa));
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       if (tc_elect()) {
         tt_mma_rows<D>(place(2 * g), kv_rows(), q_rows + stage(sa), idesc_s);
@@ -845,7 +847,7 @@ train_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       const int g = issued - 1, sb = g % L::NB;
       ok = mbar_wait_warp(b_full(sb), (unsigned)(g / L::NB) & 1u, abort_flag, nullptr, 85);
       if (!ok) return;
-      if (have < TT_B) tt_clear_rows(base_ptr + (do_tile(sb) - base), SLABS, have, lane);
+      clear(do_tile(sb));
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       if (tc_elect()) {
         tt_mma_rows<D>(place(2 * g + 1), kv_rows() + (unsigned long long)(TILE >> 4), do_rows + stage(sb), idesc_s);
