@@ -463,7 +463,9 @@ int litnice_b200_attention_forward(LitniceView q, LitniceView k, LitniceView v,
                                    const litnice_b200_attention_options *options, LitniceView out, float *lse,
                                    void *workspace, uint64_t workspace_bytes, void *stream);
 /* Gradients of sum(out * dout) from what the forward call left in out and lse. dout and dq like q, dk and dv like k.
- * Weights and their gradients are rounded to bfloat16 for their products where the forward call's are. */
+ * Weights and their gradients are rounded to bfloat16 for their products where the forward call's are. Weights are
+ * taken from lse, whose 32 bits leave them off by |lse| 2^-24 of themselves and more: scores of thousands cost
+ * the gradients accuracy, from about 2^20 on nothing is left of it (the forward call bears any that 32 bits hold). */
 uint64_t litnice_b200_attention_backward_workspace(LitniceView q, LitniceView k);
 int litnice_b200_attention_backward(LitniceView dout, LitniceView q, LitniceView k, LitniceView v, LitniceView out,
                                     const float *lse, const litnice_b200_attention_options *options, LitniceView dq,

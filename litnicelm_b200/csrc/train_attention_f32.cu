@@ -416,7 +416,7 @@ train_forward_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       if (!inside) {
 #pragma unroll
         for (int j = 0; j < 64; ++j)
-          if (j >= c_end || j < c_lo) s[j] = 2.f * TT_NEG;  // weight zero against any reference
+          if (j >= c_end || j < c_lo) s[j] = -INFINITY;  // weight zero against any reference
       }
       float mq[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll

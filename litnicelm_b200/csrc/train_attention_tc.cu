@@ -146,7 +146,13 @@ __device__ __forceinline__ bool tt_reference(float (&s)[TT_B], const TtArgs &a, 
   return grow;
 }
 // The weights 2^(factor s - m), summed into l, as bfloat16 over the scores' own columns, which this warp has read.
-__device__ __forceinline__ void tt_weights(const float (&s)[TT_B], float factor, float m, float &l, unsigned tmem) {
+__device__ __forceinline__ void tt_weights(float (&s)[TT_B], float factor, float m, float &l, unsigned tmem) {
+  // m is rounded, factor s - m is not until it is an exponent: common to a row's weights, but far from zero more than 32 bits hold
+  if (__any_sync(0xffffffffu, fabsf(m) > TT_FAR)) {
+#pragma unroll
+    for (int j = 0; j < TT_B; ++j) s[j] *= factor;
+    factor = 1.f;
+  }
   unsigned long long lq[4] = {0ull, 0ull, 0ull, 0ull};
   const unsigned long long f2 = tt_two(factor, factor), m2 = tt_two(-m, -m);
 #pragma unroll

@@ -16,7 +16,8 @@ typedef __nv_bfloat16 bf16;
 
 constexpr int TT_B = 128;
 constexpr int TT_SLAB = 128 * 128;  // 128 rows of 64 elements
-constexpr float TT_NEG = -1.0e30f, TT_SLACK = 8.f, TT_LOG2E = 1.4426950408889634f;
+constexpr float TT_NEG = -3.0e38f, TT_SLACK = 8.f, TT_LOG2E = 1.4426950408889634f;  // TT_NEG: below every score
+constexpr float TT_FAR = 268435456.f;  // 2^28: half a step of a score there is 2^3 to 2^4, of an exponent
 
 __device__ __forceinline__ float tt_exp2(float x) {
   float y;

@@ -190,7 +190,8 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
                        dk: Optional[torch.Tensor] = None,
                        dv: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(dq, dk, dv): gradients of sum(out * dout), from what ``attention_forward`` with the same options returned. Key heads
-    shared by query heads receive the sum over those. dq, dk and dv may be given, slices of one buffer for instance."""
+    shared by query heads receive the sum over those. dq, dk and dv may be given, slices of one buffer for instance. Weights come
+    from lse, so they are off by |lse| 2^-24 of themselves: scores far beyond thousands leave the gradients no accuracy."""
     for t, name in ((q, "q"), (k, "k"), (v, "v"), (lse, "lse")):
         _tensor(t, name)
     dq = _like(q) if dq is None else dq

@@ -109,3 +109,52 @@ def test_rows_that_see_no_key_reach_nothing(dtype, dim, m, lengths, opts, fill):
     out, lse, dq = results[1][:3]
     assert bool((out[empty] == 0).all()) and bool((dq[empty] == 0).all())
     assert bool((lse.transpose(1, 2)[empty] == -math.inf).all())
+
+
+# ---- scores far from zero ---------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("dim,n", [(64, 100), (64, 300), (128, 150), (33, 90)])
+@pytest.mark.parametrize("size", [1e4, 1e10, 1e16])
+def test_forward_all_scores_far_below_zero(dtype, dim, n, size, factor=-1.0):
+    """Equal scores, however low: the mean of the values. The weights are 1 exactly, their sum a whole number; a product over n keys is
+    off by 2 n u of the sum of magnitudes, its rounding by half a step."""
+    g = gen(4)
+    q = torch.full((1, n, 2, dim), size, device="cuda").to(dtype)
+    k, v = (factor * q), rand(g, 1, n, 2, dim, dtype=dtype)
+    out, lse = training.attention_forward(q, k, v)
+    count = torch.arange(1, n + 1, device="cuda", dtype=torch.float64)
+    V = v.double()
+    want, mean = V.cumsum(1) / count[:, None, None], V.abs().cumsum(1) / count[:, None, None]
+    h = torch.finfo(dtype).eps / 2
+    bound = (2 * n + 8) * 2.0 ** -24 * mean
+    assert bool(((out.double() - want).abs() <= bound + h * (want.abs() + bound)).all())
+    score = factor * float(q.flatten()[0]) ** 2 * dim * dim ** -0.5
+    # a sum of dim equal products and the scale; the log of the count
+    assert bool(((lse.double() - (score + count.log())).abs() <= (2 * dim + 16) * 2.0 ** -24 * (abs(score) + count.log() + 1)).all())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("dim,n", [(64, 100), (64, 300), (128, 150), (33, 90)])
+@pytest.mark.parametrize("size", [1e2, 1e4, 1e6, 1e12])
+def test_forward_weight_on_one_key(dtype, dim, n, size):
+    """Scores whose largest is ahead of the others by more than they are off by: the row is that key's value, rounded once more at most."""
+    g = gen(5)
+    q, k = ((rand(g, 1, n, 2, dim) * size).to(dtype) for _ in range(2))
+    v = rand(g, 1, n, 2, dim, dtype=dtype)
+    out, lse = training.attention_forward(q, k, v)
+    Q, K = (x.double().transpose(1, 2) for x in (q, k))
+    s = Q @ K.mT * dim ** -0.5
+    off = ((dim + 8) * 2 * 2.0 ** -24 * (Q.abs() @ K.abs().mT) * dim ** -0.5).amax(3)
+    s = torch.where(seen_keys(n, n, True, 0, 0, None, 1, "cuda"), s, torch.full_like(s, -math.inf))
+    top = s.topk(2, 3)
+    alone = top.values[..., 0] - top.values[..., 1] > 2 * off + 60  # the others' weights are below 2^-80
+    assert bool(alone[:, :, 1:].any())
+    at = top.indices[..., 0]
+    want = v.transpose(1, 2).gather(2, at[..., None].expand(-1, -1, -1, dim)).double()
+    got = out.transpose(1, 2).double()
+    # the weight and the sum that divides by it are the same number, in bfloat16's product rounded once
+    h = (torch.finfo(dtype).eps if dtype == BF16 else 8 * 2.0 ** -24)
+    assert bool(((got - want).abs() <= h * want.abs() + 1e-20)[alone].all())
+    assert bool(((lse.double() - top.values[..., 0]).abs() <= off + 8 * 2.0 ** -24 * top.values[..., 0].abs() + 1e-6)[alone].all())
