@@ -11,7 +11,8 @@ stream of that device, nothing is synchronised, and calls may be captured into a
 for the call. Tensors that another stream uses need its ordering, as everywhere in torch.
 
 The gradients are explicit, as in the table: nothing here joins torch's autograd, and tensors that would need it are refused
-while it records. There is no fallback: without the library or without a GPU every call raises.
+while it records; so are tensors with a tangent of forward mode, and views whose values lie negated in memory (``x.conj().imag``).
+There is no fallback: without the library or without a GPU every call raises.
 """
 from __future__ import annotations
 
@@ -22,6 +23,7 @@ import struct
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from .plugin import NativeError, load_library
 
@@ -81,6 +83,14 @@ def _tensor(t, name: str):
         raise TypeError(f"{name} is not a tensor")
 
 
+def _plain(t: torch.Tensor, name: str):
+    """That the tensor's memory is all there is to it."""
+    if t.dtype is torch.float32 and t.is_neg():  # (only views of complex tensors are)
+        raise ValueError(f"{name} is a view of negated values: use resolve_neg()")
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError(f"{name} has a tangent: the operators here have no forward-mode derivative")
+
+
 @functools.lru_cache(maxsize=4096)
 def _view_head(dtype, shape, strides, name) -> bytes:
     """A view without its address."""
@@ -101,6 +111,7 @@ def _views(names, tensors):
     for name, t in zip(names, tensors):
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name} is not a tensor")
+        _plain(t, name)
         if t.device != device:
             if device is not None:
                 raise ValueError(f"{name} is on {t.device}, not on {device}")
@@ -146,6 +157,7 @@ def _vector(t: Optional[torch.Tensor], name: str, count: int, dtype, device) -> 
     if t is None:
         return None
     _tensor(t, name)
+    _plain(t, name)
     if t.dtype != dtype or t.shape != (count,) or (count > 1 and t.stride(0) != 1):
         raise ValueError(f"{name} must be a dense {dtype} vector of {count} elements")
     if t.device != device:
@@ -194,6 +206,7 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
     from lse, so they are off by |lse| 2^-24 of themselves: scores far beyond thousands leave the gradients no accuracy."""
     for t, name in ((q, "q"), (k, "k"), (v, "v"), (lse, "lse")):
         _tensor(t, name)
+    _plain(lse, "lse")
     dq = _like(q) if dq is None else dq
     dk = _like(k) if dk is None else dk
     dv = _like(v) if dv is None else dv

@@ -2,8 +2,11 @@
 import ctypes as C
 
 import pytest
+import torch
+from torch.autograd import forward_ad
 
 from litnicelm_b200 import plugin, training
+from train_ops_calls import calls_with
 
 BASE = 1 << 20  # an address that nothing dereferences
 EINVAL, ECUDA = -1, -2
@@ -130,3 +133,26 @@ def test_impossible_strides(lib, stride):
     assert "q has an impossible stride" in text(lib)
     assert lib.litnice_b200_attention_forward(ref(q), ref(k), ref(v), ref(o), ref(bad), at[4], at[5], 1 << 30, None) == EINVAL
     assert "out has an impossible stride" in text(lib)
+
+
+@pytest.mark.parametrize("shape", [(1, 4, 2, 8), (2, 8)])
+def test_views_of_negated_values_are_refused(shape):
+    x = torch.zeros(*shape, dtype=torch.complex64).conj().imag
+    assert x.dtype == torch.float32 and x.is_neg()
+    for call in calls_with(x, x):
+        with pytest.raises(ValueError, match="negated"):
+            call()
+
+
+@pytest.mark.parametrize("shape", [(1, 4, 2, 8), (2, 8)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_tangents_are_refused(shape, dtype):
+    x = torch.zeros(*shape, dtype=dtype)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in calls_with(dual, dual):
+            with pytest.raises(ValueError, match="tangent"):
+                call()
+        for call in calls_with(x, x):  # those without one get as far as the device
+            with pytest.raises(ValueError, match="not a CUDA tensor"):
+                call()

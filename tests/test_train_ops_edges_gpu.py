@@ -4,8 +4,10 @@ import threading
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from litnicelm_b200 import training
+from train_ops_calls import calls_with
 from train_ops_util import seen_keys
 
 pytestmark = pytest.mark.gpu
@@ -158,3 +160,37 @@ def test_forward_weight_on_one_key(dtype, dim, n, size):
     h = (torch.finfo(dtype).eps if dtype == BF16 else 8 * 2.0 ** -24)
     assert bool(((got - want).abs() <= h * want.abs() + 1e-20)[alone].all())
     assert bool(((lse.double() - top.values[..., 0]).abs() <= off + 8 * 2.0 ** -24 * top.values[..., 0].abs() + 1e-6)[alone].all())
+
+
+# ---- tensors that are more than their memory ----------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("shape", [(1, 4, 2, 8), (2, 8)])
+def test_memory_that_is_not_all_of_a_tensor(shape):
+    """In any place of a call: refused, and nothing written."""
+    other = rand(gen(8), *shape)
+    vectors = torch.zeros(2, dtype=torch.complex64, device="cuda").conj().imag
+    if len(shape) == 2:
+        ids, n = torch.zeros(2, dtype=torch.int32, device="cuda"), torch.zeros(2, device="cuda")
+        for more in (dict(old_logp=vectors), dict(advantage=vectors), dict(ref_logp=vectors), dict(weight=vectors)):
+            with pytest.raises(ValueError, match="negated"):
+                training.policy_loss(other, ids, **{"old_logp": n, "advantage": n, **more})
+    x = torch.ones(*shape, dtype=torch.complex64, device="cuda").conj().imag
+    for call in calls_with(x, other):
+        with pytest.raises(ValueError, match="negated"):
+            call()
+    assert bool((x == 0).all())
+    with forward_ad.dual_level():
+        y = torch.ones(*shape, device="cuda")
+        for call in calls_with(forward_ad.make_dual(y, torch.ones_like(y)), other):
+            with pytest.raises(ValueError, match="tangent"):
+                call()
+        assert bool((y == 1).all())
+
+
+@pytest.mark.parametrize("shape", [(1, 4, 2, 8), (2, 8)])
+def test_gradients_that_autograd_would_want(shape):
+    other, x = rand(gen(9), *shape), rand(gen(10), *shape).requires_grad_()
+    for call in calls_with(x, other):
+        with pytest.raises(ValueError, match="requires a gradient"):
+            call()
