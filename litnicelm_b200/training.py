@@ -12,7 +12,7 @@ for the call. Tensors that another stream uses need its ordering, as everywhere 
 
 The gradients are explicit, as in the table: nothing here joins torch's autograd, and tensors that would need it are refused
 while it records; so are tensors with a tangent of forward mode, and views whose values lie negated in memory (``x.conj().imag``).
-There is no fallback: without the library or without a GPU every call raises.
+Results that are given count as changed in place, as autograd's checks of saved tensors want. There is no fallback: without the library or without a GPU every call raises.
 """
 from __future__ import annotations
 
@@ -89,6 +89,13 @@ def _plain(t: torch.Tensor, name: str):
         raise ValueError(f"{name} is a view of negated values: use resolve_neg()")
     if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
         raise ValueError(f"{name} has a tangent: the operators here have no forward-mode derivative")
+
+
+def _changed(*results):
+    """Memory that the caller has given was written."""
+    given = [t for t in results if t is not None]
+    if given:
+        torch.autograd.graph.increment_version(given)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -185,7 +192,7 @@ def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scal
     Row i stands at position first + i and sees key j if j < m, j < lengths[stream], with ``causal`` j <= first + i, with a
     ``window`` j > first + i - window. A row that sees no key has out 0 and lse -inf. scale: 1 / sqrt(dim) if None."""
     _tensor(q, "q")
-    out = _like(q) if out is None else out
+    given, out = out, _like(q) if out is None else out
     (vq, vk, vv, vo), held = _views(("q", "k", "v", "out"), (q, k, v, out))
     o = _options(q, scale, causal, first, window, lengths)
     streams, n, heads = q.shape[:3]
@@ -193,6 +200,7 @@ def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scal
     lib = _library()
     work = _workspace(lib.litnice_b200_attention_forward_workspace(vq, vk), q.device)
     _run(q.device, lib.litnice_b200_attention_forward, vq, vk, vv, C.addressof(o), vo, lse.data_ptr(), work.data_ptr(), work.numel())
+    _changed(given)
     return out, lse
 
 
@@ -207,6 +215,7 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
     for t, name in ((q, "q"), (k, "k"), (v, "v"), (lse, "lse")):
         _tensor(t, name)
     _plain(lse, "lse")
+    given = dq, dk, dv
     dq = _like(q) if dq is None else dq
     dk = _like(k) if dk is None else dk
     dv = _like(v) if dv is None else dv
@@ -219,6 +228,7 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
     work = _workspace(lib.litnice_b200_attention_backward_workspace(vq, vk), q.device)
     _run(q.device, lib.litnice_b200_attention_backward, vd, vq, vk, vv, vo, lse.data_ptr(), C.addressof(o), wq, wk, wv,
          work.data_ptr(), work.numel())
+    _changed(*given)
     return dq, dk, dv
 
 
@@ -237,7 +247,7 @@ def policy_loss(logits: torch.Tensor, targets: torch.Tensor, old_logp: torch.Ten
     _tensor(logits, "logits")
     if logits.dim() != 2:
         raise ValueError("logits must be [rows, vocab]")
-    rows, dev = logits.shape[0], logits.device
+    rows, dev, given = logits.shape[0], logits.device, dlogits if gradient else None
     if gradient:
         dlogits = _like(logits) if dlogits is None else dlogits
         (vz, vd), held = _views(("logits", "dlogits"), (logits, dlogits))
@@ -252,6 +262,7 @@ def policy_loss(logits: torch.Tensor, targets: torch.Tensor, old_logp: torch.Ten
          _vector(old_logp, "old_logp", rows, torch.float32, dev), _vector(advantage, "advantage", rows, torch.float32, dev),
          _vector(ref_logp, "ref_logp", rows, torch.float32, dev), _vector(weight, "weight", rows, torch.float32, dev),
          C.addressof(o), loss.data_ptr(), logp.data_ptr(), vd, work.data_ptr(), work.numel())
+    _changed(given)
     return loss, logp, dlogits
 
 
@@ -259,11 +270,12 @@ def orthogonalise(x: torch.Tensor, *, steps: int = 5, out: Optional[torch.Tensor
     """Every matrix of x [..., m, n] float32 with its singular values driven towards 1: X = x / (|x| + 1e-7), then ``steps`` times
     X <- 3.4445 X + (-4.7750 A + 2.0315 A A) X with A = X X^T (in the smaller side's space). out may be x, with x's strides."""
     _tensor(x, "x")
-    out = _like(x) if out is None else out
+    given, out = out, _like(x) if out is None else out
     (vx, vo), held = _views(("x", "out"), (x, out))
     lib = _library()
     work = _workspace(lib.litnice_b200_orthogonalise_workspace(vx), x.device)
     _run(x.device, lib.litnice_b200_orthogonalise, vx, vo, steps, work.data_ptr(), work.numel())
+    _changed(given)
     return out
 
 
@@ -276,3 +288,4 @@ def muon_step(params: torch.Tensor, grads: torch.Tensor, momentum: torch.Tensor,
     lib = _library()
     work = _workspace(lib.litnice_b200_orthogonalise_workspace(vg), grads.device)
     _run(grads.device, lib.litnice_b200_muon_step, vp, vg, vm, C.addressof(o), work.data_ptr(), work.numel())
+    _changed(params, momentum)

@@ -162,6 +162,41 @@ def test_forward_weight_on_one_key(dtype, dim, n, size):
     assert bool(((lse.double() - top.values[..., 0]).abs() <= off + 8 * 2.0 ** -24 * top.values[..., 0].abs() + 1e-6)[alone].all())
 
 
+# ---- results in memory that the caller gives --------------------------------------------------------------------------------------
+
+
+def test_given_results_count_as_changed():
+    g = gen(6)
+    q, k, v = (rand(g, 1, 20, 2, 16) for _ in range(3))
+    given = {n: torch.empty_like(q) for n in ("out", "dq", "dk", "dv")}
+    z, x, u = rand(g, 4, 30), rand(g, 8, 12), rand(g, 8, 12)
+    targets, old, adv = torch.zeros(4, dtype=torch.int32, device="cuda"), rand(g, 4), rand(g, 4)
+    p, m = rand(g, 8, 12), rand(g, 8, 12)
+    before = {n: t._version for n, t in {**given, "z": z, "u": u, "x": x, "p": p, "m": m, "q": q, "k": k, "v": v}.items()}
+    out, lse = training.attention_forward(q, k, v, out=given["out"])
+    training.attention_backward(q, q, k, v, out, lse, dq=given["dq"], dv=given["dv"])
+    training.policy_loss(z, targets, old, adv, dlogits=z)
+    training.orthogonalise(x, out=u)
+    training.muon_step(p, x, m, 0.1)
+    after = {n: t._version for n, t in {**given, "z": z, "u": u, "x": x, "p": p, "m": m, "q": q, "k": k, "v": v}.items()}
+    changed = {n for n in before if after[n] != before[n]}
+    assert changed == {"out", "dq", "dv", "z", "u", "p", "m"}
+
+
+def test_autograd_sees_that_a_step_changed_what_it_saved():
+    g = gen(7)
+    p = rand(g, 8, 12).requires_grad_()
+    loss = (p * p).sum()
+    with torch.no_grad():
+        training.muon_step(p, rand(g, 8, 12), torch.zeros(8, 12, device="cuda"), 0.1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():  # tensors without a version
+        a, b, c = (torch.ones(8, 12, device="cuda") for _ in range(3))
+        training.muon_step(a, b, c, 0.1)
+        assert bool((c == 1.95).all())
+
+
 # ---- tensors that are more than their memory ----------------------------------------------------------------------------------------
 
 
