@@ -174,6 +174,12 @@ def _vector(t: Optional[torch.Tensor], name: str, count: int, dtype, device) -> 
     return t.data_ptr()
 
 
+def _steps(steps: int) -> int:
+    if not 0 <= steps <= 100:  # (before ctypes takes its lowest 32 bits)
+        raise ValueError("steps is out of range")
+    return steps
+
+
 def _options(q: torch.Tensor, scale, causal, first, window, lengths) -> AttentionOptions:
     if q.dim() != 4:
         raise ValueError("q must be [streams, rows, heads, dim]")
@@ -271,6 +277,7 @@ def orthogonalise(x: torch.Tensor, *, steps: int = 5, out: Optional[torch.Tensor
     X <- 3.4445 X + (-4.7750 A + 2.0315 A A) X with A = X X^T (in the smaller side's space). out may be x, with x's strides."""
     _tensor(x, "x")
     given, out = out, _like(x) if out is None else out
+    _steps(steps)
     (vx, vo), held = _views(("x", "out"), (x, out))
     lib = _library()
     work = _workspace(lib.litnice_b200_orthogonalise_workspace(vx), x.device)
@@ -283,8 +290,8 @@ def muon_step(params: torch.Tensor, grads: torch.Tensor, momentum: torch.Tensor,
               weight_decay: float = 0.0, nesterov: bool = True, steps: int = 5) -> None:
     """One optimiser step on matrices [..., m, n] float32, in place: momentum <- mu momentum + grads, U = grads + mu momentum (or
     momentum without ``nesterov``), params <- (1 - lr weight_decay) params - lr sqrt(max(1, m / n)) orthogonalise(U)."""
+    o = MuonOptions(lr, mu, weight_decay, 1 if nesterov else 0, _steps(steps))
     (vp, vg, vm), held = _views(("params", "grads", "momentum"), (params, grads, momentum))
-    o = MuonOptions(lr, mu, weight_decay, 1 if nesterov else 0, steps)
     lib = _library()
     work = _workspace(lib.litnice_b200_orthogonalise_workspace(vg), grads.device)
     _run(grads.device, lib.litnice_b200_muon_step, vp, vg, vm, C.addressof(o), work.data_ptr(), work.numel())

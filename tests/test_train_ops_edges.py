@@ -156,3 +156,13 @@ def test_tangents_are_refused(shape, dtype):
         for call in calls_with(x, x):  # those without one get as far as the device
             with pytest.raises(ValueError, match="not a CUDA tensor"):
                 call()
+
+
+@pytest.mark.parametrize("steps", [-1, 101, (1 << 32) + 5, -(1 << 32)])
+def test_steps_beyond_32_bits(steps):
+    """(An integer of ctypes takes the lowest bits of what it is given.)"""
+    x = torch.zeros(2, 8)
+    with pytest.raises(ValueError, match="steps is out of range"):
+        training.orthogonalise(x, steps=steps)
+    with pytest.raises(ValueError, match="steps is out of range"):
+        training.muon_step(x, x, x, 0.1, steps=steps)
