@@ -8,7 +8,7 @@ from torch.autograd import forward_ad
 
 from litnicelm_b200 import training
 from train_ops_calls import calls_with
-from train_ops_util import seen_keys
+from train_ops_util import check, loss_reference, seen_keys
 
 pytestmark = pytest.mark.gpu
 
@@ -229,3 +229,60 @@ def test_gradients_that_autograd_would_want(shape):
     for call in calls_with(x, other):
         with pytest.raises(ValueError, match="requires a gradient"):
             call()
+
+
+# ---- policy loss: rows of every length and boundary ----------------------------------------------------------------------------------
+
+
+def wide_loss(dtype, rows, vocab, ld, dld, in_place):
+    """Rows of logits `ld` elements apart and of the gradient `dld`; the last column is one row's target, the first another's. What lies
+    between the gradient's rows stays."""
+    g = gen(vocab + ld)
+    buffer = rand(g, rows, ld, dtype=dtype) * 2
+    logits = buffer[:, :vocab]
+    targets = torch.randint(0, vocab, (rows,), generator=g, device="cuda", dtype=torch.int32)
+    targets[0], targets[1] = vocab - 1, 0
+    now = torch.log_softmax(logits.double(), 1).gather(1, targets.long()[:, None])[:, 0]
+    old, refp = ((now + s * rand(g, rows).double()).float() for s in (0.3, 0.4))
+    adv, weight = rand(g, rows), torch.ones(rows, device="cuda")
+    weight[2] = 0
+    ref = loss_reference(logits, targets, old, adv, ref=refp, weight=weight, kl=0.1)
+    out = buffer if in_place else torch.full((rows, dld), 7.0, dtype=dtype, device="cuda")
+    before = out[:, vocab:].clone()
+    loss, logp, d = training.policy_loss(logits, targets, old, adv, ref_logp=refp, weight=weight, kl_weight=0.1, dlogits=out[:, :vocab])
+    check("loss", loss, ref["loss"])
+    check("logp", logp, ref["logp"])
+    keep = ~ref["near"]
+    check("dlogits", d[keep], tuple(x[keep] for x in ref["dlogits"]))
+    assert torch.equal(out[:, vocab:], before)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("vocab", [1021, 1025, 8191, 8193, 12001, 16383, 16385, 20003, 32001, 32767, 32769])
+def test_policy_loss_rows_off_16_bytes(dtype, vocab):
+    wide_loss(dtype, 5, vocab, vocab, vocab, False)
+    wide_loss(dtype, 5, vocab, vocab + 2, (vocab + 15) // 8 * 8, False)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("vocab", [1021, 8193, 10001, 16389, 32001, 32767, 32768, 40001])
+@pytest.mark.parametrize("rows", [5, 300])
+def test_policy_loss_rows_with_a_tail(dtype, vocab, rows):
+    """On 16-byte boundaries, of columns that vectors do not divide."""
+    ld = (vocab + 15) // 8 * 8
+    wide_loss(dtype, rows, vocab, ld, vocab, False)
+    wide_loss(dtype, rows, vocab, ld, ld + 8, False)
+    wide_loss(dtype, rows, vocab, ld, ld, True)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("vocab", [90, 8193, 32001, 50001])
+def test_policy_loss_without_gradient(dtype, vocab):
+    g = gen(12)
+    for ld in (vocab, (vocab + 7) // 8 * 8):
+        logits = rand(g, 7, ld, dtype=dtype)[:, :vocab]
+        targets = torch.randint(0, vocab, (7,), generator=g, device="cuda", dtype=torch.int32)
+        old, adv = -9 + rand(g, 7), rand(g, 7)
+        a = training.policy_loss(logits, targets, old, adv, gradient=False)
+        b = training.policy_loss(logits, targets, old, adv)
+        assert a[2] is None and torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
