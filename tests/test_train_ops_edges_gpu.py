@@ -286,3 +286,75 @@ def test_policy_loss_without_gradient(dtype, vocab):
         a = training.policy_loss(logits, targets, old, adv, gradient=False)
         b = training.policy_loss(logits, targets, old, adv)
         assert a[2] is None and torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+# ---- several operators at once, captured and not --------------------------------------------------------------------------------------
+
+
+def passes():
+    """Calls that share kernels in other forms: types, head dimensions, sizes of matrices, lengths of rows."""
+    g = gen(20)
+
+    def attention(dtype, n, dim, **more):
+        q, dout = (rand(g, 3, n, 4, dim, dtype=dtype) for _ in range(2))
+        k, v = (rand(g, 3, n, 2, dim, dtype=dtype) for _ in range(2))
+        lens = torch.tensor([n, n // 2, 0], dtype=torch.int32, device="cuda")
+
+        def run():
+            out, lse = training.attention_forward(q, k, v, lengths=lens, **more)
+            return (out, lse, *training.attention_backward(dout, q, k, v, out, lse, lengths=lens, **more))
+        return run
+
+    def loss(dtype, rows, vocab):
+        z = rand(g, rows, vocab, dtype=dtype)
+        t = torch.randint(0, vocab, (rows,), generator=g, device="cuda", dtype=torch.int32)
+        old, adv, w = -9 + rand(g, rows), rand(g, rows), (rand(g, rows) > 0).float()
+        return lambda: training.policy_loss(z, t, old, adv, weight=w)
+
+    def step(*shape):
+        p, d, m = (rand(g, *shape) for _ in range(3))
+
+        def run():
+            a, b = p.clone(), m.clone()
+            training.muon_step(a, d, b, 0.02)
+            return a, b
+        return run
+
+    return [attention(F32, 200, 64), attention(F32, 150, 128, window=30), attention(BF16, 300, 64), attention(BF16, 300, 128),
+            attention(BF16, 120, 33), loss(F32, 300, 9000), loss(BF16, 40, 32000), loss(F32, 50, 40000), step(2, 64, 256), step(5, 300),
+            step(3, 200, 150), step(1024, 300)]
+
+
+def test_operators_from_several_threads():
+    calls = passes()
+    alone = [call() for call in calls]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        got = at_once(*(lambda call=call: [call() for _ in range(20)] for call in calls))
+        for a, results in zip(alone, got):
+            assert not isinstance(results, Exception), results
+            for b in results:
+                assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_operators_captured_beside_eager_ones():
+    """One graph of all, replayed while the same calls run on another stream."""
+    calls = passes()
+    alone = [call() for call in calls]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = [call() for call in calls]
+    side = torch.cuda.Stream()
+    for _ in range(5):
+        for results in captured:
+            for x in results:
+                x.fill_(float("nan"))
+        side.wait_stream(torch.cuda.current_stream())
+        graph.replay()
+        with torch.cuda.stream(side):
+            eager = [call() for call in calls]
+        torch.cuda.synchronize()
+        for a, b, c in zip(alone, captured, eager):
+            assert all(torch.equal(x, y) and torch.equal(x, z) for x, y, z in zip(a, b, c))
+    del captured, graph  # before the process ends
