@@ -428,7 +428,8 @@ int litnice_b200_selftest_wait_timeout(int32_t limit_us, int32_t *code, int32_t 
  * _workspace function gives, on a 256-byte boundary, not shared by calls that may overlap on the GPU;
  * what it holds before and after does not matter. Return 0 or a negative code, with text in
  * litnice_b200_last_error(NULL) of the same thread; a refused call has enqueued nothing. No result
- * depends on the order in which blocks finish. */
+ * depends on the order in which blocks finish. Waits inside kernels are bounded (a second and more); what
+ * a kernel that gave up on one leaves is NaN. */
 #define LITNICE_B200_VIEW_F32 0u
 #define LITNICE_B200_VIEW_BF16 2u
 
@@ -441,9 +442,9 @@ int litnice_b200_backend_stream(void *backend, void **stream);
  * j <= first + i, with window > 0 j > first + i - window. A row that sees no key has out 0 and lse
  * -infinity and takes no part in any gradient, whatever its q and dout hold. Other rows count, those
  * at and behind lengths[stream] too, which see the keys below it: their q and dout are taken to be
- * finite, and a dout of zero leaves one out of the gradients. Keys and values at and behind lengths[stream] are not
- * used, whatever they hold, and get gradients of zero. Rows of keys and values below it are taken to
- * be finite: one that is not may reach rows that do not see it. */
+ * finite, and a dout of zero leaves one out of the gradients. Keys and values at and behind
+ * lengths[stream] are not used, whatever they hold, and get gradients of zero. Rows of keys and values
+ * below it are taken to be finite: one that is not may reach rows that do not see it. */
 typedef struct litnice_b200_attention_options {
   float scale;            /* of the scores, finite */
   int32_t causal;
@@ -455,17 +456,20 @@ typedef struct litnice_b200_attention_options {
 /* q [streams, n, heads, dim], k and v [streams, m, groups, dim], out like q: one dtype, dim 1 .. 128,
  * heads a multiple of groups (head h uses key head h * groups / heads). lse [streams, heads, n] f32
  * dense: log of the sum of exp(scores). Scores, weights and sums in 32 bits. bfloat16 operands
- * whose columns are contiguous and whose rows lie on 16-byte boundaries run on the tensor cores, weights
- * rounded to bfloat16 for their product with the values, other bfloat16 operands with 32-bit products;
+ * with dim a multiple of 8, contiguous columns, and streams, rows and heads on 16-byte boundaries a positive
+ * distance apart run on the tensor cores, weights rounded to bfloat16 for their product with the values; other
+ * bfloat16 operands run with 32-bit products, 9 to 15 times slower;
  * f32 operands run on the tensor cores in three bfloat16 parts, which keep their 24 bits. */
 uint64_t litnice_b200_attention_forward_workspace(LitniceView q, LitniceView k);
 int litnice_b200_attention_forward(LitniceView q, LitniceView k, LitniceView v,
                                    const litnice_b200_attention_options *options, LitniceView out, float *lse,
                                    void *workspace, uint64_t workspace_bytes, void *stream);
 /* Gradients of sum(out * dout) from what the forward call left in out and lse. dout and dq like q, dk and dv like k.
- * Weights and their gradients are rounded to bfloat16 for their products where the forward call's are. Weights are
- * taken from lse, whose 32 bits leave them off by |lse| 2^-24 of themselves and more: scores of thousands cost
- * the gradients accuracy, from about 2^20 on nothing is left of it (the forward call bears any that 32 bits hold). */
+ * Weights and their gradients are rounded to bfloat16 for their products where the forward call's are. Weights
+ * are taken from lse, whose 32 bits leave them off by |lse| 2^-24 of themselves and more: scores of
+ * thousands cost the gradients accuracy, from about 2^20 on nothing is left of it. (The forward call bears
+ * any that 32 bits hold; on the tensor cores in bfloat16 it computes rows with scores beyond 2^28 a second
+ * time, slowly.) */
 uint64_t litnice_b200_attention_backward_workspace(LitniceView q, LitniceView k);
 int litnice_b200_attention_backward(LitniceView dout, LitniceView q, LitniceView k, LitniceView v, LitniceView out,
                                     const float *lse, const litnice_b200_attention_options *options, LitniceView dq,
@@ -492,7 +496,9 @@ int litnice_b200_policy_loss(LitniceView logits, const int32_t *targets, const f
 
 /* x, out [..., m, n] f32: every matrix U as X = U / (|U| + 1e-7) (Frobenius) followed by `steps` times
  * X <- 3.4445 X + (-4.7750 A + 2.0315 A A) X, A = X X^T, in the smaller side's space: its singular
- * vectors with values near 1. out may be x (with the strides of x). */
+ * vectors with values near 1. out may be x (with the strides of x). But for matrices with one side of at
+ * most 64 and the other of at most 4096, X, A and their polynomial are held in 22 bits (pairs of fp16 values)
+ * between products summed in 32. */
 uint64_t litnice_b200_orthogonalise_workspace(LitniceView x);
 int litnice_b200_orthogonalise(LitniceView x, LitniceView out, int32_t steps, void *workspace, uint64_t workspace_bytes,
                                void *stream);

@@ -207,7 +207,7 @@ train_attention_forward_kernel(const __grid_constant__ TaArgs g) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int key = j0 + j * 16 + tx;
-        s[i][j] = key >= first && key < last ? s[i][j] * f : -INFINITY;
+        s[i][j] = key >= first && key < last ? __fmul_rn(s[i][j], f) : -INFINITY;  // (rounded, or the difference from m is not)
         top = fmaxf(top, s[i][j]);
       }
       top = fmaxf(m[i], row_max16(top));

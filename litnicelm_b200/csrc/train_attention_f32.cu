@@ -14,11 +14,12 @@
 // memory, all four together where a sum runs over all dimensions (small parts first there too).
 //
 // Bound: at the sizes that such models train at, latency: 8 streams of 250 rows, 8 heads of 64 take 67 us forward and backward (split 2 x 9,
-// forward 13, backward 36 us) with 128 CTAs a result of dependent stages of six products each; with 32-bit products on the FMA
+// forward 13, backward 35 us) with 128 CTAs a result of dependent stages of six products each; with 32-bit products on the FMA
 // pipe it was 219 us. 2000 rows of 8 heads of 128: 419 us, 1957 that way; the six products are 100 us of it at the pipe's rate.
 //
 // A CTA: warp 0 issues TMA, warp 1 owns tensor memory and issues the MMAs, eight warps (a thread: a row or key, half of the
-// tile's columns, half of the dimensions of a sum). Every wait is bounded; one that runs out ends the CTA, whose results are then NaN.
+// tile's columns, half of the dimensions of a sum; with both sums and the parts in the making dk and dv's spill 500 bytes at H = 1, 372
+// at H = 2). Every wait is bounded; one that runs out ends the CTA, whose results are then NaN.
 #include "train_attention_tc.cuh"
 
 namespace lb {
@@ -108,8 +109,6 @@ __global__ void __launch_bounds__(256) train_split_kernel(const __grid_constant_
 }
 
 // ---- helpers of the three kernels ----------------------------------------------------------------------------------------------
-
-// Parts of the two operands of a product, in the order of their size.
 
 // The product of rows of a and rows of b over 64 dimensions, smallest parts first. (Descriptors differ by constants: see tt_mma_rows in
 // train_attention_tc.cu.)
@@ -412,7 +411,7 @@ train_forward_f32_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
       }
 #pragma unroll
-      for (int j = 0; j < 64; ++j) s[j] *= a.factor;
+      for (int j = 0; j < 64; ++j) s[j] = __fmul_rn(s[j], a.factor);  // (rounded, or the difference from m is not)
       if (!inside) {
 #pragma unroll
         for (int j = 0; j < 64; ++j)

@@ -16,12 +16,12 @@
 // These kernels (but the forward of 128 dimensions, whose two CTAs do that for each other) stay on their SM: a CTA takes over blocks that
 // have not started (TtNext), so that the next tile's operands and first products arrive under the last one's results.
 //
-// Bound, 4 streams of 2048 rows, 16 heads of 64, causal (forward 66, delta 12, dq 83, dk and dv 108 us): the exponentials, 16 a clock and
+// Bound, 4 streams of 2048 rows, 16 heads of 64, causal (forward 65, delta 12, dq 81, dk and dv 103 us): the exponentials, 16 a clock and
 // SM, are 32 us of each kernel, the products 24 us of the forward, 32 of dq, 48 of dk and dv (those into 64 columns take as long as into
 // 128); a tile's stages - product, softmax, product - wait for one another, and what two tiles in flight do not hide is the
-// rest. 8192 rows of 16 heads of 128 on 4 key heads (forward 253, dq 320, dk and dv 450 us): 121 us of exponentials, products of
-// 121, 182 and 242 us; the largest of the 256 blocks for dk and dv holds 256 of the 225 tiles that an SM
-// has on average.
+// rest. 8192 rows of 16 heads of 128 on 4 key heads (forward 253, delta 21, dq 323, dk and dv 455 us in the
+// first passes, together 1.05 ms; from about the hundredth in a row on 287, 23, 363 and 494): 121 us of exponentials, products of 121, 182
+// and 242 us; the largest of the 256 blocks for dk and dv holds 256 of the 225 tiles that an SM has on average.
 // The scores are computed once for each, so that no sum depends on the order in which CTAs finish.
 //
 // Rounding to bfloat16: P and dS for their products (the tensor cores take both operands of one type), relative 2^-8 a term,
@@ -142,17 +142,12 @@ __device__ __forceinline__ bool tt_reference(float (&s)[TT_B], const TtArgs &a, 
   const bool grow = mx > m + TT_SLACK;
   keep = grow ? tt_exp2(m - mx) : 1.f;
   if (grow) m = mx;
-  l = l * keep + (mx - mx) + (top != top ? top : 0.f);  // a score that is no number, or infinite, shows in the sum
+  if (top != top) m = top;  // a score that is no number, or infinite, shows in the reference, and so in the sum
+  l *= keep;
   return grow;
 }
 // The weights 2^(factor s - m), summed into l, as bfloat16 over the scores' own columns, which this warp has read.
-__device__ __forceinline__ void tt_weights(float (&s)[TT_B], float factor, float m, float &l, unsigned tmem) {
-  // m is rounded, factor s - m is not until it is an exponent: common to a row's weights, but far from zero more than 32 bits hold
-  if (__any_sync(0xffffffffu, fabsf(m) > TT_FAR)) {
-#pragma unroll
-    for (int j = 0; j < TT_B; ++j) s[j] *= factor;
-    factor = 1.f;
-  }
+__device__ __forceinline__ void tt_weights(const float (&s)[TT_B], float factor, float m, float &l, unsigned tmem) {
   unsigned long long lq[4] = {0ull, 0ull, 0ull, 0ull};
   const unsigned long long f2 = tt_two(factor, factor), m2 = tt_two(-m, -m);
 #pragma unroll
@@ -169,6 +164,63 @@ __device__ __forceinline__ void tt_weights(float (&s)[TT_B], float factor, float
   lq[0] = tt_add2(tt_add2(lq[0], lq[1]), tt_add2(lq[2], lq[3]));
   l += tt_lo(lq[0]) + tt_hi(lq[0]);
 }
+// m is rounded, factor s - m is not until it is an exponent: a factor of 2^(|m| 2^-25) common to a row's weights, which cancels, but far
+// from zero is more than 32 bits hold. Such a row is computed again when its tiles are done, by one warp, a lane a key, in 32-bit
+// arithmetic with rounded scores. (With the scores of a tile rounded first where a reference is far, the branch alone took the forward
+// of 4 x 2048 rows from 63.6 to 67.5 us.)
+__device__ __forceinline__ bool tt_far(float m, float l) {
+  return fabsf(m) < INFINITY && (fabsf(m) > TT_FAR || !(l > 0.f && l < INFINITY));
+}
+__device__ __noinline__ void tt_row_again(const TtArgs &a, int stream, int head, int row, int lo, int end, int lane) {
+  const int kh = head / a.share;
+  const bf16 *q = reinterpret_cast<const bf16 *>(a.q.p) + stream * a.q.s + (long long)row * a.q.r + head * a.q.h;
+  const bf16 *k = reinterpret_cast<const bf16 *>(a.k.p) + stream * a.k.s + kh * a.k.h;
+  const bf16 *v = reinterpret_cast<const bf16 *>(a.v.p) + stream * a.v.s + kh * a.v.h;
+  auto score = [&](int j) {
+    const bf16 *x = k + (long long)j * a.k.r;
+    float s = 0.f;
+    for (int c = 0; c < a.dim; c += 8) {  // (what TMA can address: dim a multiple of 8, rows on 16-byte boundaries)
+      const uint4 u = *reinterpret_cast<const uint4 *>(q + c), w = *reinterpret_cast<const uint4 *>(x + c);
+      const __nv_bfloat162 *y = reinterpret_cast<const __nv_bfloat162 *>(&u), *z = reinterpret_cast<const __nv_bfloat162 *>(&w);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = __bfloat1622float2(y[i]), g = __bfloat1622float2(z[i]);
+        s = fmaf(f.x, g.x, fmaf(f.y, g.y, s));
+      }
+    }
+    return __fmul_rn(s, a.factor);  // (rounded, or the difference from m is not)
+  };
+  float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int j = lo + lane; j < end; j += 32) m = fmaxf(m, score(j));
+  for (int i = 16; i > 0; i >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, i));
+  for (int j0 = lo; j0 < end; j0 += 32) {
+    const float p = j0 + lane < end ? tt_exp2(score(j0 + lane) - m) : 0.f;
+    l += p;
+#pragma unroll 4
+    for (int t = 0; t < min(32, end - j0); ++t) {
+      const float w = __shfl_sync(0xffffffffu, p, t);
+      const bf16 *x = v + (long long)(j0 + t) * a.v.r;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (lane + 32 * e < a.dim) o[e] = fmaf(w, __bfloat162float(x[lane + 32 * e]), o[e]);
+    }
+  }
+  for (int i = 16; i > 0; i >>= 1) l += __shfl_xor_sync(0xffffffffu, l, i);
+  bf16 *out = reinterpret_cast<bf16 *>(a.o1.p) + stream * a.o1.s + (long long)row * a.o1.r + head * a.o1.h;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (lane + 32 * e < a.dim) out[lane + 32 * e] = __float2bfloat16_rn(o[e] / l);
+  if (lane == 0) a.lse[((long long)stream * a.heads + head) * a.n + row] = (m + log2f(l)) * 0.6931471805599453f;
+}
+// Those of a warp's 32 rows from row0 on, behind what the tiles have left of them.
+__device__ __forceinline__ void tt_rows_again(const TtArgs &a, const TtPlace &at, int row0, unsigned which, int lane) {
+  __syncwarp();
+  for (; which != 0u; which &= which - 1u) {
+    const int row = row0 + __ffs((int)which) - 1;
+    tt_row_again(a, at.stream, at.head, row, a.span.lo(row), a.span.end(row, at.keys), lane);
+  }
+}
+
 // This lane's accumulator row times keep.
 __device__ __forceinline__ void tt_rescale(unsigned tmem, int dim, float keep) {
 #pragma unroll 1
@@ -327,6 +379,8 @@ train_forward_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     if (live)
       a.lse[((long long)at.stream * a.heads + at.head) * a.n + row] =
           !ok ? NAN : empty ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+    const unsigned far = __ballot_sync(0xffffffffu, ok && live && !empty && tt_far(m, l));
+    if (far != 0u) tt_rows_again(a, at, r0 + q * 32, far, lane);
   }
   __syncwarp();
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -617,6 +671,8 @@ train_forward_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
       if (live)
         a.lse[((long long)x.at.stream * a.heads + x.at.head) * a.n + row] =
             !ok ? NAN : empty ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+      const unsigned far = __ballot_sync(0xffffffffu, ok && live && !empty && tt_far(m, l));
+      if (far != 0u) tt_rows_again(a, x.at, x.r0 + group * TT_B + q * 32, far, lane);
     }
   }
   __syncwarp();
@@ -809,16 +865,9 @@ train_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     const unsigned idesc_s = umma_idesc_bf16(TT_B), idesc_d = umma_idesc_bf16(cols) | UMMA_B_MN_MAJOR;
     // Jobs: S and dP of each tile in turn, of all items; each takes the next place, and is issued behind the product that read it.
     int w = 0, i = -1, n = -1, issued = 0, tiles = 0;  // issued: tiles whose S is
-    int each = 1, live = 0x7fffffff;  // live: rows from the item's first on that see a key, where others follow
     bool more = true, ok = true;
     unsigned ends = 0u;  // bit (tile of all) % 4: it is its item's last, % 4 + 4: first
     auto kv_rows = [&]() { return k_rows + (unsigned long long)(n % L::NQ * (2 * TILE >> 4)); };
-    // What rows that see no key hold must not meet their weights of zero (rows behind the last are zeros already).
-    auto clear = [&](unsigned tile) {
-      if (live == 0x7fffffff) return;
-      const int have = live - i % each * TT_B;
-      if (have < TT_B) tt_clear_rows(base_ptr + (tile - base), SLABS, max(have, 0), lane);
-    };
     auto scores = [&]() {
       if (++i >= tiles) {
         const int block = next.take(w++, lane);
@@ -826,11 +875,7 @@ train_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
           more = false;
           return;
         }
-        const Item x = item(block);
-        tiles = tt_uniform(x.tiles);
-        each = tt_uniform(max(x.each, 1));
-        const int rows = a.span.rows_end(a.n, x.at.keys);
-        live = tt_uniform(rows < a.n ? rows - x.lo : 0x7fffffff);
+        tiles = tt_uniform(item(block).tiles);
         i = 0;
         ++n;
       }
@@ -840,7 +885,6 @@ train_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       ok = (i > 0 || mbar_wait_warp(kv_full(sk), (unsigned)(n / L::NQ) & 1u, abort_flag, nullptr, 82)) &&
            mbar_wait_warp(a_full(sa), (unsigned)(g / L::NA) & 1u, abort_flag, nullptr, 83);
       if (!ok) return;
-      clear(q_tile(sa));
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       if (tc_elect()) {
         tt_mma_rows<D>(place(2 * g), kv_rows(), q_rows + stage(sa), idesc_s);
@@ -853,7 +897,6 @@ train_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       const int g = issued - 1, sb = g % L::NB;
       ok = mbar_wait_warp(b_full(sb), (unsigned)(g / L::NB) & 1u, abort_flag, nullptr, 85);
       if (!ok) return;
-      clear(do_tile(sb));
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       if (tc_elect()) {
         tt_mma_rows<D>(place(2 * g + 1), kv_rows() + (unsigned long long)(TILE >> 4), do_rows + stage(sb), idesc_s);
@@ -947,6 +990,21 @@ train_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 #pragma unroll
           for (int j = 0; j < 64; ++j)
             if (j < c_lo || j >= c_end) p[j] = 0.f;
+          // What rows that see no key hold must not meet their weights of zero in dV and dK: this half's four warps clear them in both
+          // tiles (S is done with q's; dP reads dout's meanwhile, into columns that count for nothing). Rows behind the last are
+          // zeros already.
+          const int keys = a.lengths ? max(0, min(a.m, a.lengths[x.at.stream])) : a.m, live = a.span.rows_end(a.n, keys);
+          if (live < a.n && live < r0 + 64) {
+            if (!(ok = mbar_wait_warp(b_full(st), (unsigned)(g / L::NB) & 1u, abort_flag, nullptr, 85))) break;
+            const int from = max(live - r0, 0);
+            for (int s = 0; s < SLABS; ++s)
+              for (int e = from * 8 + q * 32 + lane; e < 64 * 8; e += 128) {
+                const int to = s * TT_SLAB + half * 64 * 128 + e * 16;
+                *reinterpret_cast<uint4 *>(base_ptr + (q_tile(g % L::NA) - base) + to) = make_uint4(0u, 0u, 0u, 0u);
+                *reinterpret_cast<uint4 *>(base_ptr + (do_tile(st) - base) + to) = make_uint4(0u, 0u, 0u, 0u);
+              }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          }
         }
 #pragma unroll
         for (int c = 0; c < 64; c += 32) {
@@ -1396,6 +1454,9 @@ template <int D>
 void forward(const TrainAttention &a, cudaStream_t st) {
   TtArgs t = tt_args(a, a.n);
   t.o1 = a.out;
+  t.q = a.q;
+  t.k = a.k;
+  t.v = a.v;
   t.vec = tt_rows16(a.out);
   const size_t smem = 3 * (size_t)(D / 64) * TT_SLAB + 128 + 1024;
   static SharedMemoryOnce once;
@@ -1410,6 +1471,9 @@ void forward_pair(const TrainAttention &a, cudaStream_t st) {
   TtArgs t = tt_args(a, a.n);
   t.tiles = (a.n + 2 * TT_B - 1) / (2 * TT_B);
   t.o1 = a.out;
+  t.q = a.q;
+  t.k = a.k;
+  t.v = a.v;
   t.vec = tt_rows16(a.out);
   static SharedMemoryOnce once;
   once.set(train_forward_pair_kernel, TT_PAIR_SMEM);

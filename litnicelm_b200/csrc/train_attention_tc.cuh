@@ -65,6 +65,7 @@ struct TtArgs {
   float *lse;
   float *delta;
   HeadView o1, o2;       // out | dq | dk, dv
+  HeadView q, k, v;      // of the bfloat16 forward kernels (tt_row_again)
   int vec;               // results' rows on 16-byte boundaries
 };
 
