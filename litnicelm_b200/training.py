@@ -85,7 +85,7 @@ def _tensor(t, name: str):
 
 def _plain(t: torch.Tensor, name: str):
     """That the tensor's memory is all there is to it."""
-    if t.dtype is torch.float32 and t.is_neg():  # (only views of complex tensors are)
+    if t.is_neg():
         raise ValueError(f"{name} is a view of negated values: use resolve_neg()")
     if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
         raise ValueError(f"{name} has a tangent: the operators here have no forward-mode derivative")
@@ -114,11 +114,12 @@ def _view_head(dtype, shape, strides, name) -> bytes:
 def _views(names, tensors):
     """(addresses of the tensors' views, the memory that holds them), checked to be CUDA tensors of one device that autograd does
     not record."""
-    recording, device, heads, at = torch.is_grad_enabled(), None, [], 8
+    recording, device, heads, at, dual = torch.is_grad_enabled(), None, [], 8, forward_ad._current_level >= 0
     for name, t in zip(names, tensors):
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name} is not a tensor")
-        _plain(t, name)
+        if dual or t.is_neg():
+            _plain(t, name)
         if t.device != device:
             if device is not None:
                 raise ValueError(f"{name} is on {t.device}, not on {device}")
@@ -164,7 +165,8 @@ def _vector(t: Optional[torch.Tensor], name: str, count: int, dtype, device) -> 
     if t is None:
         return None
     _tensor(t, name)
-    _plain(t, name)
+    if forward_ad._current_level >= 0 or t.is_neg():
+        _plain(t, name)
     if t.dtype != dtype or t.shape != (count,) or (count > 1 and t.stride(0) != 1):
         raise ValueError(f"{name} must be a dense {dtype} vector of {count} elements")
     if t.device != device:
@@ -274,7 +276,8 @@ def policy_loss(logits: torch.Tensor, targets: torch.Tensor, old_logp: torch.Ten
 
 def orthogonalise(x: torch.Tensor, *, steps: int = 5, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Every matrix of x [..., m, n] float32 with its singular values driven towards 1: X = x / (|x| + 1e-7), then ``steps`` times
-    X <- 3.4445 X + (-4.7750 A + 2.0315 A A) X with A = X X^T (in the smaller side's space). out may be x, with x's strides."""
+    X <- 3.4445 X + (-4.7750 A + 2.0315 A A) X with A = X X^T (in the smaller side's space). out may be x, with x's strides. But for
+    matrices with one side of at most 64 and the other of at most 4096, X and A are held in 22 bits between products summed in 32."""
     _tensor(x, "x")
     given, out = out, _like(x) if out is None else out
     _steps(steps)
