@@ -1,7 +1,8 @@
 // Orthogonalised momentum: the update of a weight matrix by the polynomial iteration
 //   X = U / (|U| + 1e-7),  X <- a X + (b A + c A^2) X,  A = X X^T,  (a, b, c) = (3.4445, -4.7750, 2.0315)
 // in the space of the matrix's smaller side (X <- X (b A + c A^2) + a X with A = X^T X for a tall one), which drives its singular
-// values towards 1; and the optimiser step with it,
+// values towards 1 (a Newton-Schulz iteration; the quintic's coefficients as K. Jordan published them with this optimiser in 2024);
+// and the optimiser step with it,
 //   momentum <- mu momentum + grad,  U = grad + mu momentum or momentum,
 //   params <- (1 - lr decay) params - lr sqrt(max(1, m / n)) X.
 // All matrices of a call have one shape and go through each product together.
@@ -19,7 +20,7 @@
 //
 // One persistent kernel for the three products of a step, tiles of 128 x 128: warp 0 issues TMA (stages of 64 k: four tiles of 16
 // KB), warp 1 owns tensor memory and issues the MMAs, eight warps add finished chains (a thread: a row and half of the columns) and
-// store through patches of shared memory that TMA carries out. Nothing is transposed in memory: an operand whose rows run along k
+// store through patches of shared memory that TMA carries out (a pair's threads, with 128 columns, spill 116 to 176 bytes). Nothing is transposed in memory: an operand whose rows run along k
 // is read as it lies (M or N contiguous). A and B are symmetric: tiles up to the diagonal are multiplied, and stored on both
 // sides of it.
 // Every wait is bounded; one that runs out ends the CTA, whose results are then NaN. Pairs of CTAs share a tile of 256 rows where there are tiles for all SMs, clusters of up
@@ -271,7 +272,6 @@ struct NsProduct {
   const float *rho;
 };
 
-template <bool PAIR>
 struct NsSmem {
   static constexpr int STAGES = 3, TILE = 16384, STAGE = 4 * TILE;
   static constexpr int PATCH_OFF = STAGES * STAGE, PATCH = 4096;  // 32 x 32 elements of hi and of lo, per storing warp
@@ -327,8 +327,8 @@ ns_product_kernel(const __grid_constant__ CUtensorMap map_ah, const __grid_const
                   const __grid_constant__ CUtensorMap map_bh, const __grid_constant__ CUtensorMap map_bl,
                   const __grid_constant__ CUtensorMap map_oh, const __grid_constant__ CUtensorMap map_ol,
                   const __grid_constant__ NsProduct g) {
-  using L = NsSmem<PAIR>;
-  constexpr int S = L::STAGES, CTAS = PAIR ? 2 : 1, T = 128 * CTAS;  // tiles of T x T by CTAS CTAs, each 128 rows in HALVES pieces
+  using L = NsSmem;
+  constexpr int S = L::STAGES, CTAS = PAIR ? 2 : 1, T = 128 * CTAS;  // tiles of T x T by CTAS CTAs, 128 rows each
   constexpr int CHAINS = 4 / CTAS, COLS = 64 * CTAS;  // chains in flight, T columns of tensor memory each; columns of a thread
   constexpr bool SYM = OP != APPLY;
   static_assert(!(PAIR && SPLIT), "");
@@ -698,7 +698,7 @@ void launch_product(const Operand &a, const Operand &b, const Operand &out, NsPr
   g.n_tiles = (g.n + T - 1) / T;
   const long long per = OP == APPLY ? (long long)g.m_tiles * g.n_tiles : (long long)g.m_tiles * (g.m_tiles + 1) / 2;
   g.tiles = (int)(per * count);  // (in range: checked before the call's first kernel)
-  using L = NsSmem<PAIR>;
+  using L = NsSmem;
   static SharedMemoryOnce once;
   once.set(ns_product_kernel<OP, A_MN, B_MN, PAIR, SPLIT>, L::TOTAL);
   const int per_tile = SPLIT ? g.splits : CTAS, ctas = SPLIT || g.tiles < 148 / CTAS ? g.tiles : 148 / CTAS;
