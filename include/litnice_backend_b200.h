@@ -443,8 +443,8 @@ int litnice_b200_backend_stream(void *backend, void **stream);
  * -infinity and takes no part in any gradient, whatever its q and dout hold. Other rows count, those
  * at and behind lengths[stream] too, which see the keys below it: their q and dout are taken to be
  * finite, and a dout of zero leaves one out of the gradients. Keys and values at and behind
- * lengths[stream] are not used, whatever they hold, and get gradients of zero. Rows of keys and values
- * below it are taken to be finite: one that is not may reach rows that do not see it. */
+ * lengths[stream], and those that no row sees, are not used, whatever they hold, and get gradients of
+ * zero. The others are taken to be finite: one that is not may reach rows that do not see it. */
 typedef struct litnice_b200_attention_options {
   float scale;            /* of the scores, finite */
   int32_t causal;

@@ -141,6 +141,7 @@ TrainAttention attention_args(LitniceView q, LitniceView k, LitniceView v, const
   a.causal = o->causal != 0;
   a.first = o->first;
   a.window = o->window;
+  a.seen = a.causal && a.first + a.n < a.m ? a.first + a.n : a.m;
   a.bf16 = q->dtype == LITNICE_B200_VIEW_BF16;
   if ((__int128)a.streams * a.heads * a.n > (__int128)1 << 40 || (__int128)a.streams * a.groups * a.m > (__int128)1 << 40)
     bad("too many rows, heads and streams for one call");

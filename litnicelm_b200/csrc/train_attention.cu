@@ -49,16 +49,16 @@ struct TaArgs {
 };
 enum { VQ = 1, VK = 2, VV = 4, VDO = 8, VO = 16 };
 
-// Rows r0 .. r0 + 63 of a head into shared memory, those from `end` on and the columns behind dim as zeros.
+// Rows r0 .. r0 + 63 of a head into shared memory, those from `end` on, or before `begin`, and the columns behind dim as zeros.
 template <int D>
-__device__ __forceinline__ void load_tile(float *to, const HeadView &x, long long base, int r0, int end, int dim, bool vec) {
+__device__ __forceinline__ void load_tile(float *to, const HeadView &x, long long base, int r0, int end, int dim, bool vec, int begin = 0) {
   constexpr int LD = D + 4, Q = D / 4;
   const bf16 *p = reinterpret_cast<const bf16 *>(x.p) + base;
 #pragma unroll 4
   for (int e = threadIdx.x; e < TA_B * Q; e += TA_THREADS) {
     const int r = e / Q, c = e % Q * 4;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (r0 + r < end) v = load4(p + (long long)(r0 + r) * x.r + c * x.c, x.c, dim - c, vec);
+    if (r0 + r >= begin && r0 + r < end) v = load4(p + (long long)(r0 + r) * x.r + c * x.c, x.c, dim - c, vec);
     *reinterpret_cast<float4 *>(to + r * LD + c) = v;
   }
 }
@@ -164,8 +164,8 @@ __device__ __forceinline__ TaPlace ta_place(const TaArgs &g, int heads, bool las
   p.tile = last_first ? g.tiles - 1 - t : t;
   p.stream = rest / heads;
   p.head = rest - p.stream * heads;
-  p.keys = g.a.m;
-  if (g.a.lengths) p.keys = max(0, min(g.a.m, g.a.lengths[p.stream]));
+  p.keys = g.a.seen;
+  if (g.a.lengths) p.keys = max(0, min(g.a.seen, g.a.lengths[p.stream]));
   return p;
 }
 
@@ -195,8 +195,8 @@ train_attention_forward_kernel(const __grid_constant__ TaArgs g) {
   const float f = a.scale * TA_LOG2E;
   for (int j0 = lo; j0 < end; j0 += TA_B) {
     __syncthreads();
-    load_tile<D>(sk, a.k, kb, j0, at.keys, a.dim, g.vec & VK);
-    load_tile<D>(sv, a.v, vb, j0, at.keys, a.dim, g.vec & VV);
+    load_tile<D>(sk, a.k, kb, j0, at.keys, a.dim, g.vec & VK, span.lo(r0));
+    load_tile<D>(sv, a.v, vb, j0, at.keys, a.dim, g.vec & VV, span.lo(r0));
     __syncthreads();
     float s[8][4];
     tile_dot<D>(sq, sk, s);
@@ -294,8 +294,8 @@ train_attention_dq_kernel(const __grid_constant__ TaArgs g) {
   const float f = a.scale * TA_LOG2E;
   for (int j0 = lo; j0 < end; j0 += TA_B) {
     __syncthreads();
-    load_tile<D>(sk, a.k, kb, j0, at.keys, a.dim, g.vec & VK);
-    load_tile<D>(sv, a.v, vb, j0, at.keys, a.dim, g.vec & VV);
+    load_tile<D>(sk, a.k, kb, j0, at.keys, a.dim, g.vec & VK, span.lo(r0));
+    load_tile<D>(sv, a.v, vb, j0, at.keys, a.dim, g.vec & VV, span.lo(r0));
     __syncthreads();
     float s[8][4], dp[8][4];
     tile_dot<D>(sq, sk, s);

@@ -5,7 +5,7 @@
 // is the six of parts whose terms count, smallest first: (0,2) (2,0) (1,1) (0,1) (1,0) (0,0); what is left out is below 2^-23 of a
 // term. The tensor pipe truncates when it adds, so an accumulator in tensor memory holds one tile's product and is added to a
 // sum in registers, rounded to nearest. Queries, keys, values and upstream gradients are split once by a kernel in front
-// (which also clears keys behind a stream's length and rows that see no key, and sums dout . out), weights and their gradients in registers on their way
+// (which also clears keys behind a stream's length or every row, and rows that see no key, and sums dout . out), weights and their gradients in registers on their way
 // to tensor memory: of the 128 columns that a tile's scores took, each half of the warps writes the first two parts over its own
 // 64, and the third behind them.
 //
@@ -39,7 +39,7 @@ struct TfTensor {
 struct TfSplit {
   TfTensor t[4];
   int count, streams, dim, chunks;  // chunks: of eight elements, 8 H to a row
-  int m;
+  int seen;
   TrainSpan span;
   const int *lengths;
   HeadView out;           // with delta: of the last tensor, dout
@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(256) train_split_kernel(const __grid_constant_
   const int head_at = b / per, s = head_at / t.heads, h = head_at - s * t.heads;
   const int row = (b - head_at * per) * each_block + (int)threadIdx.x / g.chunks, c = (int)threadIdx.x % g.chunks * 8;
   const bool in = row < t.rows;
-  const int keys = g.lengths ? max(0, min(g.m, g.lengths[s])) : g.m, live = t.keys ? keys : g.span.rows_end(t.rows, keys);
+  const int keys = g.lengths ? max(0, min(g.seen, g.lengths[s])) : g.seen, live = t.keys ? keys : g.span.rows_end(t.rows, keys);
   float x[8] = {};
   const long long off = (long long)s * t.x.s + (long long)row * t.x.r + (long long)h * t.x.h + (long long)c * t.x.c;
   if (row < live) {
@@ -960,7 +960,7 @@ void split(const TrainAttention &a, char *work, float *delta, Parts (&parts)[4],
   g.streams = a.streams;
   g.dim = a.dim;
   g.chunks = a.dim > 64 ? 16 : 8;
-  g.m = a.m;
+  g.seen = a.seen;
   g.span = TrainSpan{a.first, a.window, a.causal};
   g.lengths = a.lengths;
   g.out = a.out;

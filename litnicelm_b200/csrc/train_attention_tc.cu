@@ -28,7 +28,7 @@
 // of independent sign, as much as the operands themselves have been rounded by; the results.
 //
 // Warp 0 issues TMA, warp 1 owns tensor memory and issues the MMAs. Rows outside the tensors load as zeros; keys behind a
-// stream's length, and rows that see no key, are cleared in shared memory where a product would multiply them by a weight of
+// stream's length or every row, and rows that see no key, are cleared in shared memory where a product would multiply them by a weight of
 // zero. Every wait is bounded; one that runs out ends the CTA, whose results are then NaN. No clusters, no multicast.
 #include "train_attention_tc.cuh"
 
@@ -993,7 +993,7 @@ train_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
           // What rows that see no key hold must not meet their weights of zero in dV and dK: this half's four warps clear them in both
           // tiles (S is done with q's; dP reads dout's meanwhile, into columns that count for nothing). Rows behind the last are
           // zeros already.
-          const int keys = a.lengths ? max(0, min(a.m, a.lengths[x.at.stream])) : a.m, live = a.span.rows_end(a.n, keys);
+          const int keys = a.lengths ? max(0, min(a.seen, a.lengths[x.at.stream])) : a.seen, live = a.span.rows_end(a.n, keys);
           if (live < a.n && live < r0 + 64) {
             if (!(ok = mbar_wait_warp(b_full(st), (unsigned)(g / L::NB) & 1u, abort_flag, nullptr, 85))) break;
             const int from = max(live - r0, 0);

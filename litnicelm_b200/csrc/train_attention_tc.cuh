@@ -60,6 +60,7 @@ __device__ __forceinline__ float tt_max3(float a, float b, float c) {
 struct TtArgs {
   int n, m, heads, groups, share, streams, dim, tiles;
   TrainSpan span;
+  int seen;
   const int *lengths;
   float scale, factor;   // factor = scale * log2(e)
   float *lse;
@@ -79,7 +80,7 @@ __device__ __forceinline__ TtPlace tt_place(const TtArgs &a, int heads, bool las
   p.tile = last_first ? a.tiles - 1 - t : t;
   p.stream = rest / heads;
   p.head = rest - p.stream * heads;
-  p.keys = a.lengths ? max(0, min(a.m, a.lengths[p.stream])) : a.m;
+  p.keys = a.lengths ? max(0, min(a.seen, a.lengths[p.stream])) : a.seen;
   return p;
 }
 __device__ __forceinline__ TtPlace tt_place(const TtArgs &a, int heads, bool last_first, int ctas = 1) {
@@ -181,6 +182,7 @@ TtArgs tt_args(const TrainAttention &a, int rows) {
   t.dim = a.dim;
   t.tiles = (rows + TT_B - 1) / TT_B;
   t.span = TrainSpan{a.first, a.window, a.causal};
+  t.seen = a.seen;
   t.lengths = a.lengths;
   t.scale = a.scale;
   t.factor = a.scale * TT_LOG2E;

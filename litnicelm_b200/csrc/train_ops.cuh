@@ -20,6 +20,7 @@ struct TrainAttention {
   int streams = 0, n = 0, m = 0, heads = 0, groups = 0, dim = 0;
   float scale = 1.f;
   int causal = 0, first = 0, window = 0;
+  int seen = 0;                    // keys from here on are behind every row, as those from a stream's length on
   int bf16 = 0;
 };
 

@@ -358,3 +358,32 @@ def test_operators_captured_beside_eager_ones():
         for a, b, c in zip(alone, captured, eager):
             assert all(torch.equal(x, y) and torch.equal(x, z) for x, y, z in zip(a, b, c))
     del captured, graph  # before the process ends
+
+
+# ---- keys that no row sees ----------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("dim", [64, 128, 33])
+@pytest.mark.parametrize("n,m,lengths,opts", [
+    (100, 300, None, dict()), (300, 500, None, dict(window=50)), (1, 200, None, dict(first=70)), (130, 400, [400, 200, 100, 0], dict(first=60)),
+    (70, 200, None, dict(first=100, window=10)), (200, 300, [250, 300, 1, 190], dict(window=1))], ids=str)
+@pytest.mark.parametrize("fill", [math.nan, -math.inf])
+def test_keys_that_no_row_sees_reach_nothing(dtype, dim, n, m, lengths, opts, fill):
+    """The unused end of a cache, and what lies before every row's window, may hold anything."""
+    g = gen(13)
+    streams, heads = 4, 4
+    q, dout = (rand(g, streams, n, heads, dim, dtype=dtype) for _ in range(2))
+    k, v = (rand(g, streams, m, 2, dim, dtype=dtype) for _ in range(2))
+    lens = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    seen = seen_keys(n, m, True, opts.get("first", 0), opts.get("window", 0), lens, streams, "cuda")
+    unseen = ~seen.any(2).expand(streams, 1, m)[:, 0]
+    assert bool(unseen.any())
+    results = []
+    for x in (0.0, fill):
+        k[unseen], v[unseen] = x, x
+        out, lse = training.attention_forward(q, k, v, lengths=lens, **opts)
+        results.append((out, lse, *training.attention_backward(dout, q, k, v, out, lse, lengths=lens, **opts)))
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+    assert bool((results[1][3][unseen] == 0).all()) and bool((results[1][4][unseen] == 0).all())
