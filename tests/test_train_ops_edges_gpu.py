@@ -1,5 +1,8 @@
 """The training operators where calls come close to what they were not made for, through litnicelm_b200.training."""
 import math
+import os
+import subprocess
+import sys
 import threading
 
 import pytest
@@ -387,3 +390,117 @@ def test_keys_that_no_row_sees_reach_nothing(dtype, dim, n, m, lengths, opts, fi
     for a, b in zip(*results):
         assert torch.equal(a, b)
     assert bool((results[1][3][unseen] == 0).all()) and bool((results[1][4][unseen] == 0).all())
+
+
+# ---- far apart, and in any order ----------------------------------------------------------------------------------------------------
+
+
+def far(rows, *shape, dtype=F32):
+    """`rows` blocks of zeros, each as far from the next as 2^31 elements and some leave them."""
+    size = math.prod(shape)
+    step = ((1 << 31) // (rows - 1) + 8192) // 8 * 8
+    buffer = torch.empty((rows - 1) * step + size, dtype=dtype, device="cuda")
+    strides = [math.prod(shape[i + 1:]) for i in range(len(shape))]
+    out = torch.as_strided(buffer, (rows, *shape), (step, *strides))
+    out.zero_()
+    return out
+
+
+@pytest.mark.parametrize("dtype,dim", [(F32, 40), (BF16, 64), (BF16, 128), (BF16, 33)])
+def test_attention_streams_far_apart(dtype, dim):
+    g = gen(14)
+    near = [rand(g, 2, 140, h, dim, dtype=dtype) for h in (4, 2, 2, 4)]
+    out, lse = training.attention_forward(*near[:3])
+    want = (out, *training.attention_backward(near[3], *near[:3], out, lse))
+    for place in range(4):  # one operand at a time
+        x = far(2, 140, near[place].shape[2], dim, dtype=dtype)
+        x.copy_(near[place])
+        args = [x if i == place else t for i, t in enumerate(near)]
+        result = torch.empty_like(out)
+        o, s = training.attention_forward(*args[:3], out=result)
+        got = (o, *training.attention_backward(args[3], *args[:3], o, s))
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+        del x, args
+    for place in range(4):  # and one result
+        x = far(2, 140, want[place].shape[2], dim, dtype=dtype)
+        if place == 0:
+            training.attention_forward(*near[:3], out=x)
+        else:
+            training.attention_backward(near[3], *near[:3], out, lse, **{("dq", "dk", "dv")[place - 1]: x})
+        assert torch.equal(x, want[place])
+        del x
+
+
+@pytest.mark.parametrize("vocab", [96, 5000, 20001, 32000, 40000])
+def test_policy_loss_rows_far_apart(vocab):
+    g = gen(15)
+    z = rand(g, 4, vocab, dtype=BF16)
+    targets = torch.randint(0, vocab, (4,), generator=g, device="cuda", dtype=torch.int32)
+    old, adv = -9 + rand(g, 4), rand(g, 4)
+    want = training.policy_loss(z, targets, old, adv)
+    x = far(4, vocab, dtype=BF16)
+    x.copy_(z)
+    got = training.policy_loss(x, targets, old, adv)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    training.policy_loss(x, targets, old, adv, dlogits=x)
+    assert torch.equal(x, want[2])
+
+
+@pytest.mark.parametrize("shape", [(40, 70), (200, 300), (300, 200)])
+def test_matrices_far_apart_and_turned(shape):
+    """Weights, gradients and momentum each in their own order of memory."""
+    g = gen(16)
+    p, d, m = (rand(g, 2, *shape) for _ in range(3))
+    a, b = p.clone(), m.clone()
+    training.muon_step(a, d, b, 0.03, weight_decay=0.1)
+    for place in range(3):
+        for form in ("far", "turned", "apart"):
+            if form == "far":
+                x = far(2, *shape)
+            elif form == "turned":
+                x = torch.empty(2, shape[1], shape[0], device="cuda").mT
+            else:
+                x = torch.empty(2, shape[0], 2, shape[1], 3, device="cuda")[:, :, 1, :, 1]
+            args = [p.clone(), d, m.clone()]
+            x.copy_(args[place])
+            args[place] = x
+            training.muon_step(*args[:2], args[2], 0.03, weight_decay=0.1)
+            assert torch.equal(args[0], a) and torch.equal(args[2], b) and torch.equal(args[1], d)
+            del x, args
+    e = torch.zeros(1, *shape, device="cuda").expand(2, -1, -1)  # a broadcast gradient
+    p2, m2 = p.clone(), m.clone()
+    training.muon_step(p2, e, m2, 0.03)
+    p3, m3 = p.clone(), m.clone()
+    training.muon_step(p3, e.contiguous(), m3, 0.03)
+    assert torch.equal(p2, p3) and torch.equal(m2, m3)
+
+
+def test_first_calls_of_a_process_inside_a_capture():
+    code = """
+import torch
+from litnicelm_b200 import training
+g = torch.Generator(device="cuda").manual_seed(1)
+x = [torch.randn(2, 300, 4, 64, generator=g, device="cuda") for _ in range(4)]
+y = [t.bfloat16() for t in x]
+w = torch.randn(2, 300, 200, generator=g, device="cuda")
+z, ids, n = torch.randn(5, 32000, generator=g, device="cuda"), torch.zeros(5, dtype=torch.int32, device="cuda"), torch.zeros(5, device="cuda")
+def run():
+    r = []
+    for q, k, v, d in (x, y):
+        out, lse = training.attention_forward(q, k, v)
+        r += [out, lse, *training.attention_backward(d, q, k, v, out, lse)]
+    return r + [training.orthogonalise(w), training.orthogonalise(w[:, :40]), *training.policy_loss(z, ids, n, n)]
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = run()
+graph.replay()
+want = run()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, want))
+del got, graph
+print("done")
+"""
+    root = os.path.join(os.path.dirname(os.path.abspath(__file__)), "..")
+    p = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=120)
+    assert p.returncode == 0 and "done" in p.stdout, p.stdout + p.stderr
