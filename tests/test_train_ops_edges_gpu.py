@@ -504,3 +504,26 @@ print("done")
     root = os.path.join(os.path.dirname(os.path.abspath(__file__)), "..")
     p = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=120)
     assert p.returncode == 0 and "done" in p.stdout, p.stdout + p.stderr
+
+
+# ---- scores that are no numbers -------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("dim", [64, 128, 33])
+@pytest.mark.parametrize("n", [90, 300])
+@pytest.mark.parametrize("what", [math.nan, math.inf])
+def test_scores_that_are_no_numbers_stay_in_their_rows(dtype, dim, n, what):
+    """A query's reach its own row, a key's the rows that see it (an infinite score leaves a row no finite sum either)."""
+    g = gen(17)
+    q, k, v = (rand(g, 2, n, 2, dim, dtype=dtype) for _ in range(3))
+    out, lse = training.attention_forward(q, k, v)
+    hit = torch.zeros(2, n, 2, dtype=torch.bool, device="cuda")
+    q[0, 40, 1], k[1, n - 20, 0, 0] = what, what
+    hit[0, 40, 1], hit[1, n - 20:, 0] = True, True
+    if what == math.inf:
+        q[1, n - 20:, 0, 0] = q[1, n - 20:, 0, 0].abs() + 1  # a score of +infinity in the rows that see it
+        out, lse = training.attention_forward(q, torch.where(torch.isfinite(k), k, torch.ones_like(k)), v)
+    got, sums = training.attention_forward(q, k, v)
+    assert bool(got[hit].isnan().all()) and bool(sums.transpose(1, 2)[hit].isnan().all())
+    assert torch.equal(got[~hit], out[~hit]) and torch.equal(sums.transpose(1, 2)[~hit], lse.transpose(1, 2)[~hit])
